@@ -42,6 +42,53 @@ struct sg_attn_spill {
   int total;
 };
 
+// One sg_block_norm call (k_block_norm.hip): strides in elements; off null: every
+// row, and gate [cols]; otherwise gate [n_seq][cols].
+struct sg_block_norm_args {
+  void* xn;
+  void* sum;
+  const void* x;
+  const void* h;
+  int64_t ldxn, lds, ldx, ldh;
+  const float* w_post;
+  const float* w_pre;
+  const float* gate;
+  const int32_t* off;
+  float eps, scale;
+  int rows, cols, n_seq;
+};
+
+// One sg_attention_masked call (k_attn_masked.hip); strides in elements.
+struct sg_attn_masked_args {
+  void* out;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t ldo, ldq, ldk, ldv;
+  const int32_t* off;
+  const float* slopes;
+  const int32_t* docs;
+  const int32_t* prefix;
+  float scale, softcap;
+  int rows, n_seq, heads, kv_heads, hd, causal, window;
+};
+
+// One sg_adapters_apply call (k_adapters.hip): the bank's packed weights, strides
+// in elements; u: [ksplit][rows][rank_pad] floats.
+struct sg_adapters_args {
+  void* dst;
+  const void* base;
+  const void* x;
+  int64_t ldd, ldb, ldx;
+  const void* wa;
+  const void* wb;
+  const float* scales;
+  const int32_t* off;
+  const int32_t* ids;
+  float* u;
+  int rows, n_seq, n_adapters, in_dim, out_dim, rank_pad;
+};
+
 namespace sgk {
 
 // GEMM operands are block-major int8 [K/32][rows][32]; activation buffers hold
@@ -258,6 +305,21 @@ size_t attention_exact_scratch(int T, int H, int max_len);
 hipError_t attention_exact(const float* q, int ldq, const float* k, const float* v, int ldkv, float* out, int ldo,
                            const int32_t* seq_off, const int32_t* row_seq, int n_seq, int T, int H, int HKV, int hd,
                            float scale, int max_len, float* P, float* amax, hipStream_t s);
+
+// ---- operators over device-resident offsets; dtype: SG_F32 / SG_F16 / SG_BF16 ----
+constexpr int kBlockNormCols = 8192;  // longest row
+hipError_t block_norm(const sg_block_norm_args& a, int dtype, hipStream_t s);
+hipError_t attention_masked(const sg_attn_masked_args& a, int dtype, hipStream_t s);
+// Adapter weights, one after another: a [n][rank][in], b [n][out][rank] (contiguous)
+// into the fragment order of k_adapters.hip, rank and in_dim padded with zeros.
+constexpr int kAdapterMaxRank = 256;
+inline int adapters_rank_pad(int rank) { return (rank + 15) / 16 * 16; }
+size_t adapters_a_bytes(int dtype, int n, int rank, int in_dim);
+size_t adapters_b_bytes(int dtype, int n, int rank, int out_dim);
+hipError_t adapters_pack(int dtype, const void* a, const void* b, int n, int rank, int in_dim, int out_dim, void* wa,
+                         void* wb, hipStream_t s);
+size_t adapters_work_bytes(int dtype, int rows, int in_dim, int rank_pad);
+hipError_t adapters_apply(const sg_adapters_args& a, int dtype, hipStream_t s);
 
 // ---- brute-force search (k_search.hip) ----
 // Storage modes, the values of brute.QuantizationMode (search/brute/quant.go:8-15).

@@ -22,6 +22,7 @@ SG_ERR_DEVICE = -6
 SG_ERR_NOMEM = -7
 
 SG_ATTN_FAST, SG_ATTN_EXACT = 0, 1
+SG_F32, SG_F16, SG_BF16 = 0, 1, 2
 
 _ERR_NAMES = {
     SG_ERR_EMPTY: "EMPTY",
@@ -89,7 +90,13 @@ class Profile(ctypes.Structure):
                 ("launches", ctypes.c_int64 * SG_K_CLASSES)]
 
 
+class AttnMask(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("slopes", _vp), ("doc_ids", _vp),
+                ("prefix", _vp), ("causal", ctypes.c_int32), ("window", ctypes.c_int32)]
+
+
 _i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
 _f32 = ctypes.c_float
 _pp = ctypes.POINTER(ctypes.c_void_p)
 
@@ -132,6 +139,15 @@ _PROTOS = {
     "sg_gelu_quick_mul": (ctypes.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),
     "sg_embed_tokens": (ctypes.c_int, [_vp, _vp, _vp, _i32, _vp]),
     "sg_pool_l2": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _vp, _i32, _vp]),
+    "sg_attention_masked": (ctypes.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32,
+                                           _i32, _vp, _i32, ctypes.POINTER(AttnMask), _vp]),
+    "sg_block_norm": (ctypes.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _f32,
+                                     _vp, _f32, _vp, _i32, _vp]),
+    "sg_adapter_bank_create": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _pp]),
+    "sg_adapter_bank_free": (None, [_vp]),
+    "sg_adapters_work_bytes": (ctypes.c_int, [_vp, _i32, ctypes.POINTER(ctypes.c_size_t)]),
+    "sg_adapters_apply": (ctypes.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _vp,
+                                         ctypes.c_size_t, _vp]),
     "sg_index_build": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _i32, _pp]),
     "sg_index_build_device": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, ctypes.c_int64, _i32, _vp, _pp]),
     "sg_index_deserialize": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _pp]),

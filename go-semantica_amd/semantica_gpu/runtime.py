@@ -57,6 +57,7 @@ class Context:
         h = ctypes.c_void_p()
         _lib.check(self.lib.sg_init(device, ctypes.byref(h)))
         self.handle = h
+        self.device = device
 
     def close(self):
         if self.handle:

@@ -330,6 +330,95 @@ int sg_embed_tokens(sg_model *model, float *dst, const int32_t *d_tokens, int32_
 int sg_pool_l2(sg_ctx *ctx, float *out, const float *x, int32_t ldx, int32_t out_dim,
                const int32_t *seq_offsets, int32_t n_seq, void *stream);
 
+/* ---- layer operators of sibling models (device pointers, work on `stream`) ----
+ * No counterpart in the reference, which runs one architecture with one set of
+ * weights: what a layer of another decoder-derived embedder, or a fine-tuned one,
+ * needs beside the products above.  All of them take a packed batch whose CSR
+ * offsets d_seq_offsets[n_seq + 1] are in device memory (sequence i is rows
+ * d_seq_offsets[i] .. d_seq_offsets[i+1] - 1; ascending; empty sequences are
+ * allowed), return once their work is enqueued, allocate nothing and wait for
+ * nothing, so they may be captured into a HIP graph and called from several
+ * threads or on several streams at once.  Rows of no sequence (before the first
+ * or behind the last) are left as they were.  The contents of device arrays are
+ * not checked; offsets outside 0 .. rows and ids that name nothing are never
+ * followed out of the tensors.  Element types: */
+#define SG_F32 0
+#define SG_F16 1
+#define SG_BF16 2
+
+/* How a score becomes a weight in sg_attention_masked.  i and j: positions of a
+ * query and a key in their sequence.  All pointers are device memory. */
+typedef struct sg_attn_mask {
+  float scale;            /* of q . k; 0: 1/sqrt(head_dim) */
+  float softcap;          /* > 0: scores become softcap * tanh(score / softcap); 0: they stay */
+  const float *slopes;    /* [n_heads]: slopes[h] * |i - j| is subtracted after the cap; NULL: nothing */
+  const int32_t *doc_ids; /* [rows]: keys of the query's own document are visible, and none if its id is
+                             negative (padding); NULL: the whole sequence is one document */
+  const int32_t *prefix;  /* [n_seq]: with causal, a sequence's first prefix[i] keys are visible to all of
+                             its queries; NULL: none */
+  int32_t causal;         /* keys behind the query are hidden */
+  int32_t window;         /* > 0: keys with |i - j| >= window are hidden, prefix or not; 0: none */
+} sg_attn_mask;
+
+/* Attention of every sequence with itself: out_i = sum_j softmax_j(score_ij) v_j
+ * over the visible keys; zeros for a query that sees none.  Hidden keys do not
+ * touch the result, whatever they hold (infinities and NaN included).  q
+ * [rows][ldq] and out [rows][ldo] hold n_heads heads of head_dim side by side, k
+ * [rows][ldk] and v [rows][ldv] n_kv_heads (a divisor of n_heads) of them, all of
+ * type dtype; strides in elements.  Sums and softmax statistics are float32.
+ * float32 products keep 22 bits of each operand (2^-37 of its row's largest value
+ * at worst), 16-bit types round the weights to their type.  head_dim: a multiple of 8 up to 256;
+ * pointers 16-byte aligned, strides whole 16 bytes (k's and v's up to 2^22
+ * elements); out apart from q, k and v.
+ * mask NULL: scale 1/sqrt(head_dim), nothing hidden. */
+int sg_attention_masked(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int64_t ldq, const void *k, int64_t ldk,
+                        const void *v, int64_t ldv, int32_t dtype, int32_t n_heads, int32_t n_kv_heads,
+                        int32_t head_dim, int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq,
+                        const sg_attn_mask *mask, void *stream);
+
+/* What stands between two blocks of a layer, in one pass:
+ *   y   = x * rsqrt(mean(x^2) + eps) * w_post      (w_post NULL: y = x)
+ *   sum = h + scale * gate * y                     (gate NULL: 1)
+ *   xn  = sum * rsqrt(mean(sum^2) + eps) * w_pre   (from sum before it is rounded; xn NULL: not wanted)
+ * x, h, sum, xn: [rows][cols] of type dtype with row strides in elements; w_post,
+ * w_pre [cols] and gate float32.  d_seq_offsets NULL (n_seq 0): every row, one
+ * gate [cols] for all.  Otherwise gate is [n_seq][cols], one for each sequence.
+ * cols 1 .. 8192, rows and strides of any alignment (whole 16 bytes are
+ * faster).  sum and xn may each be x or h (same pointer and stride); otherwise no
+ * output overlaps another tensor. */
+int sg_block_norm(sg_ctx *ctx, void *xn, int64_t ldxn, void *sum, int64_t lds, const void *x, int64_t ldx,
+                  const void *h, int64_t ldh, int32_t dtype, int32_t rows, int32_t cols, const float *w_post,
+                  const float *w_pre, float eps, const float *gate, float scale, const int32_t *d_seq_offsets,
+                  int32_t n_seq, void *stream);
+
+/* Low-rank adapters of one projection, laid out for the GPU once.  d_a
+ * [n_adapters][rank][in_dim] and d_b [n_adapters][out_dim][rank] (device memory,
+ * contiguous, type dtype; an adapter of a smaller rank is padded with zeros),
+ * d_scales [n_adapters] float32.  rank 1 .. 256, in_dim and out_dim multiples of
+ * 8.  The arrays are read on the context's stream after what `stream` holds, and
+ * may be freed after return.  Freeing the bank waits for the device. */
+typedef struct sg_adapter_bank sg_adapter_bank;
+int sg_adapter_bank_create(sg_ctx *ctx, const void *d_a, const void *d_b, const float *d_scales, int32_t dtype,
+                           int32_t n_adapters, int32_t rank, int32_t in_dim, int32_t out_dim, void *stream,
+                           sg_adapter_bank **out);
+void sg_adapter_bank_free(sg_adapter_bank *bank);
+
+/* Bytes of workspace that sg_adapters_apply needs for `rows` rows. */
+int sg_adapters_work_bytes(const sg_adapter_bank *bank, int32_t rows, size_t *bytes);
+
+/* dst_t = base_t + scale_a * B_a (A_a x_t) for every row t, a = d_adapter_ids[i] of
+ * the sequence i that holds it; dst_t = base_t where a names no adapter (-1).
+ * base: the shared projection's output (sg_matmul_q8_0_int8's, for one); dst may
+ * be base.  x [rows][ldx], base and dst [rows][ldb / ldd] of the bank's type,
+ * strides in elements, pointers 16-byte aligned, strides whole 16 bytes.  work:
+ * sg_adapters_work_bytes of device memory, 16-byte aligned, in use until the
+ * call's work on `stream` is done (one for each stream or graph that runs at the
+ * same time).  dst does not overlap x, or base unless it is base.  The sums are
+ * float32 and in the same order every time. */
+int sg_adapters_apply(sg_ctx *ctx, void *dst, int64_t ldd, const void *base, int64_t ldb, const sg_adapter_bank *bank,
+                      const void *x, int64_t ldx, int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq,
+                      const int32_t *d_adapter_ids, void *work, size_t work_bytes, void *stream);
+
 /* ---- tokenizer (internal/tokenizer) -------------------------------------
  * The reference's SentencePiece-style BPE tokenizer on the host: text ->
  * the token IDs sg_forward takes.  Same normalization (NFKC / accents /

@@ -51,13 +51,12 @@ using sgp::bf16x8_t;
 using sgp::chunk;
 using sgp::elem;
 
-constexpr int kWaves = 4, kNT = kWaves * SG_WAVE;
-constexpr int kSub = 32;  // keys and queries of a matrix core tile
+constexpr int kSub = 32;  // keys of a block: one or two matrix core tiles
 constexpr float kLog2e = 1.44269504088896340736f;
 // A row's maximum is raised (and its sums rescaled) only when a score passes it by
 // this many powers of two, so most tiles rescale nothing; weights stay below 2^8.
 constexpr float kSlack = 8.0f;
-constexpr int kScanTiles = 32;  // tiles of one look at the document ids
+constexpr int kScanWords = 64;  // 32 tiles each: one look at the document ids
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
@@ -82,18 +81,40 @@ struct mul<float> {
   static constexpr float shift = 5.0f;
 };
 
-template <typename M>
-__device__ __forceinline__ f32x16_t mfma32(s16x8_t a, s16x8_t b, f32x16_t c) {
-  if constexpr (__is_same(M, bf16_t))
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
-}
+// The matrix core tile of QT queries: accumulator type, and one step of M's type.
+template <int QT>
+struct core;
+template <>
+struct core<32> {
+  typedef f32x16_t acc;
+  static constexpr int REGS = 16;
+  template <typename M>
+  static __device__ __forceinline__ acc step(s16x8_t a, s16x8_t b, acc c) {
+    if constexpr (__is_same(M, bf16_t))
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct core<16> {
+  typedef f32x4_t acc;
+  static constexpr int REGS = 4;
+  template <typename M>
+  static __device__ __forceinline__ acc step(s16x8_t a, s16x8_t b, acc c) {
+    if constexpr (__is_same(M, bf16_t))
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+  }
+};
 
-template <int D>
-__device__ __forceinline__ int swz_k(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
-template <int D>
-__device__ __forceinline__ int swz_v(int row) { return D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
+// What a row's piece index is xor-ed by.  An LDS cycle serves 128 bytes: eight lanes
+// of a K load (eight rows, one piece: three bits spread them), or the 16 lanes of a
+// transposing V load (four rows, two pieces each: two bits above the lowest).  Only
+// a piece's low three bits change, so most of an address is an immediate.
+__device__ __forceinline__ constexpr int swz_k(int row) { return row & 7; }
+__device__ __forceinline__ constexpr int swz_v(int row) { return (row & 3) << 1; }
 
 constexpr int kTop = 13;  // rows are brought to 2^13 .. 2^14 before they are halved
 constexpr int kLim = 110;
@@ -114,6 +135,7 @@ __device__ __forceinline__ float finite_top(const float* x) {
 #pragma unroll
   for (int i = 0; i < N; i++) top = fmaxf(top, fabsf(x[i]));
   if (__ballot(top == INFINITY)) {
+    asm volatile("");  // (a branch, not sixteen selects for everyone)
     top = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; i++) top = fmaxf(top, fabsf(x[i]) < INFINITY ? fabsf(x[i]) : 0.0f);
@@ -121,28 +143,54 @@ __device__ __forceinline__ float finite_top(const float* x) {
   return top;
 }
 
-// Eight values times by, as fp16 halves.
+// Eight values times `by` (a power of two), as fp16 halves: hi = fp16(x by) and lo =
+// fp16(x by - hi), each rounded once, two instructions a value.
 __device__ __forceinline__ void halves(const float* x, float by, s16x8_t& hi, s16x8_t& lo) {
-  half8_t h, l;
+  typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+  u32x4_t h, l;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const hl16 s = split_f16(x[i] * by);
-    h[i] = s.hi;
-    l[i] = s.lo;
+  for (int i = 0; i < 4; i++) {
+    uint32_t hh, ll;
+    asm("v_fma_mixlo_f16 %0, %2, %4, 0\n\t"
+        "v_fma_mixhi_f16 %0, %3, %4, 0\n\t"
+        "v_fma_mixlo_f16 %1, %2, %4, -%0 op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %1, %3, %4, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]"
+        : "=&v"(hh), "=&v"(ll)
+        : "v"(x[2 * i]), "v"(x[2 * i + 1]), "v"(by));
+    h[i] = hh;
+    l[i] = ll;
   }
   hi = __builtin_bit_cast(s16x8_t, h);
   lo = __builtin_bit_cast(s16x8_t, l);
 }
 
-// tanh.  ACCURATE: Lambert's continued fraction to seven levels below 1.5 (relative
-// error 5e-8 at its end), and 1 - 2 / (e^2x + 1) above, where the second term's
-// rounding no longer shows; the plain form is off by 1e-7 absolute, which a cap of
-// 50 turns into 5e-6 of a weight: nothing beside 16-bit weights.
-template <bool ACCURATE>
-__device__ __forceinline__ float tanh_of(float x) {
+// The sum of the eight 16-bit values of p, added to l.
+template <typename M>
+__device__ __forceinline__ float add_up(s16x8_t p, float l) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (__is_same(M, bf16_t)) {
+      typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+      const b2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+      const short two[2] = {p[2 * i], p[2 * i + 1]};
+      l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, two), ones, l, false);
+    } else {
+      typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+      const h2 ones = {(_Float16)1, (_Float16)1};
+      const short two[2] = {p[2 * i], p[2 * i + 1]};
+      l = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, two), ones, l, false);
+    }
+  }
+  return l;
+}
+
+// tanh for float32 scores: Lambert's continued fraction to seven levels below 1.5
+// (relative error 5e-8 at its end), and 1 - 2 / (e^2x + 1) above, where the second
+// term's rounding no longer shows.  (The second form alone, off by 1e-7 absolute
+// which a cap of 50 turns into 5e-6 of a weight, serves the 16-bit types.)
+__device__ __forceinline__ float tanh_f32(float x) {
   const float e = __builtin_amdgcn_exp2f(x * (2.0f * kLog2e));
   const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
-  if constexpr (!ACCURATE) return far;
   const float z = x * x;
   const float num = x * __builtin_fmaf(__builtin_fmaf(z + 378.0f, z, 17325.0f), z, 135135.0f);
   const float den = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(28.0f, z, 3150.0f), z, 62370.0f), z, 135135.0f);
@@ -151,20 +199,27 @@ __device__ __forceinline__ float tanh_of(float x) {
   return fabsf(x) < 1.5f ? near : far;
 }
 
-template <typename T, int D_, int RW_, int KW_>
+// A form: QT queries a wave, RW groups of them and KW shares of each tile's keys.
+template <typename T, int D_, int QT_, int RW_, int KW_>
 struct form {
-  static constexpr int D = D_, RW = RW_, KW = KW_;
+  static constexpr int D = D_, QT = QT_, RW = RW_, KW = KW_;
+  static constexpr int NW = RW * KW, NT = NW * SG_WAVE;
   static constexpr bool F32 = __is_same(T, float);
   static constexpr int PARTS = mul<T>::parts;
   static constexpr int NSUB = KW > 1 || D == 256 || (F32 && D == 128) ? 1 : 2;  // 32-key blocks a wave takes of a tile
-  static constexpr int BK = kSub * KW * NSUB, BM = kSub * RW;
+  static constexpr int BK = kSub * KW * NSUB, BM = QT * RW;
   static constexpr int HALF = BK * D * 2;             // bytes of one tile's K (or V), one part
   static constexpr int TILE = 2 * PARTS * HALF;       // K and V
   static constexpr int STAGES = !F32 && 2 * TILE <= (128 << 10) ? 2 : 1;
   static constexpr int KEYS = F32 ? 3 * BK * 4 : 0;   // per-key powers of a float32 tile
-  static constexpr int JOIN = KW > 1 ? kWaves * kSub * D * 4 : 0;
+  static constexpr int JOIN = KW > 1 ? NW * QT * D * 4 : 0;
   static constexpr int LDS = (STAGES * TILE + KEYS) > JOIN ? (STAGES * TILE + KEYS) : JOIN;
-  static_assert(RW * KW == kWaves, "four waves");
+  static constexpr int WAVES = (QT == 32 && D == 256) || (NW == 4 && KW > 1) ? 1 : 2;  // a SIMD has registers for
+  // Lane (n, g): query n; of a 32-key block, register r is key KSTR (r / 4) + 4 g + r % 4.
+  static constexpr int G = SG_WAVE / QT, KSTR = 4 * G;
+  static constexpr int SR = kSub / G;          // a lane's scores of a block
+  static constexpr int KDIM = 8 * G;           // dims of a score step; keys of an output step
+  static constexpr int KS = D / KDIM, DB = D / QT, PS = kSub / KDIM;
 };
 
 // One query's view of the keys.
@@ -177,7 +232,7 @@ struct view {
 template <typename T>
 __device__ __forceinline__ float score_of(const sg_attn_masked_args& a, float dot, float slope, int gap) {
   float s = dot * a.scale;
-  if (a.softcap > 0.0f) s = a.softcap * tanh_of<true>(s / a.softcap);
+  if (a.softcap > 0.0f) s = a.softcap * tanh_f32(s / a.softcap);
   return (s - slope * fabsf((float)gap)) * kLog2e;
 }
 
@@ -220,13 +275,6 @@ __device__ __forceinline__ void careful_row(const sg_attn_masked_args& a, int ro
   }
 }
 
-struct yes {
-  static constexpr bool value = true;
-};
-struct no {
-  static constexpr bool value = false;
-};
-
 // Every wave's copies have landed and its LDS reads are done, in all waves.
 __device__ __forceinline__ void publish() {
   sg_wait_vmcnt<0>();
@@ -234,42 +282,71 @@ __device__ __forceinline__ void publish() {
   asm volatile("" ::: "memory");
 }
 
-template <typename T, int D, int RW, int KW>
-__global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_masked_args a,
-                                                                                                  int row_tiles) {
-  typedef form<T, D, RW, KW> F;
+template <typename T, int D, int QT, int RW, int KW>
+__global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES)) void k_attn_masked(
+    sg_attn_masked_args a, int row_tiles) {
+  typedef form<T, D, QT, RW, KW> F;
+  typedef core<QT> X;
+  typedef typename X::acc acc_t;
   typedef typename mul<T>::type M;
   typedef __attribute__((address_space(3))) void* lds_ptr;
   typedef __attribute__((address_space(3))) s16x4_t* lds_s4;
   constexpr int C = D / 8;      // 16-byte pieces of an LDS row
-  constexpr int KS = D / 16;    // k-steps of a score
-  constexpr int DB = D / kSub;  // 32-dim blocks of an output
+  constexpr int kNT = F::NT, kWaves = F::NW, G = F::G, KS = F::KS, DB = F::DB, SR = F::SR, R = X::REGS;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   __shared__ int range[kWaves][4];
-  __shared__ uint32_t scan;
+  __shared__ uint32_t scan[kScanWords];
   __shared__ int first_e;
-  __shared__ float ml[kWaves][2][kSub];
+  __shared__ float ml[kWaves][2][QT];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = w % RW, kw = w / RW;
-  const int n = lane & 31, g = lane >> 5;
+  const int n = lane % QT, g = lane / QT;
   const int h = blockIdx.x % a.heads, tile_i = (int)(blockIdx.x / a.heads);
   const int row0 = (a.causal ? row_tiles - 1 - tile_i : tile_i) * F::BM;  // causal: the long rows first
   const int kvh = h / (a.heads / a.kv_heads);
-  const int row = row0 + kSub * rw + n, rc = min(row, a.rows - 1);
+  const int row = row0 + QT * rw + n, rc = min(row, a.rows - 1);
+
+  // ---- Q's loads go out first: lane (n, g), step ks: dims KDIM ks + 8 g .. + 7 of the row ----
+  const T* const qp = static_cast<const T*>(a.q) + (int64_t)rc * a.ldq + h * a.hd + 8 * g;
+  constexpr int QV = F::F32 ? 2 : 1;  // 16-byte loads of eight values
+  f32x4_t qx[KS][QV];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+    for (int i = 0; i < QV; i++)
+      qx[ks][i] = F::KDIM * ks + 8 * g < a.hd ? *reinterpret_cast<const f32x4_t*>(qp + F::KDIM * ks + 4 * i) : f32x4_t{0, 0, 0, 0};
 
   // ---- the row's keys ----
   view me;
   {
     const int last = min(row0 + F::BM, a.rows) - 1;
-    const int i0 = sgp::find_seq(a.off, a.n_seq, row0, lane), i1 = sgp::find_seq(a.off, a.n_seq, last, lane);
-    int lo = max(i0, 0), hi = max(i1, lo);
-    while (lo < hi) {
-      const int mid = lo + (hi - lo + 1) / 2;
-      if (a.off[mid] <= rc) lo = mid;
-      else hi = mid - 1;
+    int lo, hi, s0, s1;
+    if (a.n_seq < SG_WAVE) {  // one load for all offsets
+      const int off = a.off[min(lane, a.n_seq)];
+      lo = max((int)__popcll(__ballot(lane < a.n_seq && off <= row0)) - 1, 0);
+      hi = max((int)__popcll(__ballot(lane < a.n_seq && off <= last)) - 1, lo);
+      while (__ballot(lo < hi)) {
+        const int mid = lo + (hi - lo + 1) / 2;
+        if (__shfl(off, mid) <= rc) lo = mid;
+        else hi = mid - 1;
+        hi = max(hi, lo);
+      }
+      s0 = __shfl(off, lo);
+      s1 = __shfl(off, lo + 1);
+    } else {
+      lo = max(sgp::find_seq(a.off, a.n_seq, row0, lane), 0);
+      hi = max(sgp::find_seq(a.off, a.n_seq, last, lane), lo);
+      while (lo < hi) {
+        const int mid = lo + (hi - lo + 1) / 2;
+        if (a.off[mid] <= rc) lo = mid;
+        else hi = mid - 1;
+      }
+      s0 = a.off[lo];
+      s1 = a.off[lo + 1];
     }
-    const int s0 = sgp::clamp_row(a.off[lo], a.rows), s1 = sgp::clamp_row(a.off[lo + 1], a.rows);
+    s0 = sgp::clamp_row(s0, a.rows);
+    s1 = sgp::clamp_row(s1, a.rows);
     me.live = row < a.rows && s0 <= row && row < s1;
     me.lo = s0;
     me.hi = s1;
@@ -291,7 +368,7 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_m
   {
     int v[4] = {me.lo, -me.hi, me.hi ? me.doc : INT32_MAX, me.hi ? -me.doc : INT32_MAX};
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1)
+    for (int o = QT / 2; o >= 1; o >>= 1)
 #pragma unroll
       for (int i = 0; i < 4; i++) v[i] = min(v[i], __shfl_xor(v[i], o));
     if (lane == 0)
@@ -302,69 +379,93 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_m
   __syncthreads();
   int all[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-    all[i] = __builtin_amdgcn_readfirstlane(min(min(range[0][i], range[1][i]), min(range[2][i], range[3][i])));
+  for (int i = 0; i < 4; i++) {
+    all[i] = range[0][i];
+#pragma unroll
+    for (int v = 1; v < kWaves; v++) all[i] = min(all[i], range[v][i]);
+    all[i] = __builtin_amdgcn_readfirstlane(all[i]);
+  }
   const int kend = -all[1];
   const int kbeg = all[0] < kend ? all[0] & ~(kSub - 1) : 0;
   const int nt = all[0] < kend ? (kend - kbeg + F::BK - 1) / F::BK : 0;
 
-  // ---- Q as the B operand: lane (n, g), step ks: dims 16 ks + 8 g .. + 7 of the row ----
+  // ---- Q as the B operand, its sign turned where the scale is negative ----
   s16x8_t q[F::PARTS][KS];
-  float qf = a.scale;  // a score's factor
+  float qf = fabsf(a.scale);  // a score's factor
   {
-    const T* qp = static_cast<const T*>(a.q) + (int64_t)rc * a.ldq + h * a.hd + 8 * g;
     if constexpr (F::F32) {
-      float x[KS][8];
+      float top = finite_top<8 * KS>(reinterpret_cast<const float*>(&qx[0][0]));
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        const bool on = 16 * ks + 8 * g < a.hd;
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-          *reinterpret_cast<f32x4_t*>(&x[ks][4 * i]) =
-              on ? *reinterpret_cast<const f32x4_t*>(qp + 16 * ks + 4 * i) : f32x4_t{0, 0, 0, 0};
-      }
-      float top = finite_top<8 * KS>(&x[0][0]);
-      top = fmaxf(top, __shfl_xor(top, 32));
+      for (int o = QT; o < SG_WAVE; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
       const int e = row_exp(top);
+      const float by = a.scale < 0.0f ? -pow2(kTop - e) : pow2(kTop - e);
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) halves(x[ks], pow2(kTop - e), q[0][ks], q[F::PARTS - 1][ks]);
+      for (int ks = 0; ks < KS; ks++) halves(reinterpret_cast<const float*>(&qx[ks][0]), by, q[0][ks], q[F::PARTS - 1][ks]);
       qf *= pow2(e - kTop);
     } else {
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++)
-        q[0][ks] = 16 * ks + 8 * g < a.hd ? *reinterpret_cast<const s16x8_t*>(qp + 16 * ks) : s16x8_t{};
+      for (int ks = 0; ks < KS; ks++) {
+        q[0][ks] = __builtin_bit_cast(s16x8_t, qx[ks][0]);
+        if (a.scale < 0.0f) q[0][ks] ^= (short)0x8000;
+      }
     }
   }
+  // A score in powers of two is t = x ca + cb of what the matrix core gives, x = s
+  // times the row's power, or, under a cap, x = -1 / (e^2s/cap + 1).
   const bool capped = a.softcap > 0.0f;
-  const float before = capped ? qf / a.softcap : qf * kLog2e;
-  const float after = a.softcap * kLog2e;
+  const float cs = capped ? qf / a.softcap * (F::F32 ? 1.0f : 2.0f * kLog2e) : qf * kLog2e;
+  const float cap2 = a.softcap * kLog2e;
   const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
 
   // ---- tiles ----
   // The first tile from t on that may hold a key of a document of this
-  // workgroup's rows (nt: none).
-  uint32_t mask = 0;
+  // workgroup's rows (nt: none).  A look covers kScanWords * 32 tiles, four ids a
+  // thread and load.
   int scan0 = 0, scan1 = 0;
   auto next = [&](int t) {
     if (!a.docs) return t;
     while (t < nt) {
       if (t >= scan1) {
         scan0 = t;
-        scan1 = t + kScanTiles;
+        scan1 = t + kScanWords * 32;
         __syncthreads();
-        if (tid == 0) scan = 0;
+        if (tid < kScanWords) scan[tid] = 0;
         __syncthreads();
-        const int end = min(kend, kbeg + scan1 * F::BK);
-        for (int j = kbeg + scan0 * F::BK + tid; j < end; j += kNT) {
-          const int d = a.docs[j];
-          if (d >= all[2] && -d >= all[3]) atomicOr(&scan, 1u << ((j - kbeg) / F::BK - scan0));
+        const int first = kbeg + scan0 * F::BK, count = min(kend - first, (scan1 - scan0) * F::BK);
+        const int32_t* ids = a.docs + first;
+        const bool whole = (reinterpret_cast<uintptr_t>(ids) & 15) == 0;
+        constexpr int U = 4;  // loads in flight
+        for (int j0 = 0; j0 < count; j0 += 4 * kNT * U) {
+          i32x4_t d[U];
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            const int j = j0 + 4 * (u * kNT + tid);
+            d[u] = i32x4_t{-1, -1, -1, -1};
+            if (whole && j + 4 <= count) {
+              d[u] = *reinterpret_cast<const i32x4_t*>(ids + j);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                if (j + i < count) d[u][i] = ids[j + i];
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            const int tile = (j0 + 4 * (u * kNT + tid)) / F::BK;
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 4; i++) any |= d[u][i] >= all[2] && -d[u][i] >= all[3];
+            // A tile's BK / 4 lanes lie together; the first of them speaks for all.
+            constexpr int L = F::BK / 4;
+            const uint64_t b = __ballot(any) >> (lane & ~(L - 1));
+            if ((lane & (L - 1)) == 0 && (b & ((1ull << L) - 1))) atomicOr(&scan[tile >> 5], 1u << (tile & 31));
+          }
         }
         __syncthreads();
-        mask = __builtin_amdgcn_readfirstlane(scan);
       }
-      const uint32_t left = mask >> (t - scan0);
+      const uint32_t left = __builtin_amdgcn_readfirstlane(scan[(t - scan0) >> 5]) >> ((t - scan0) & 31);
       if (left) return t + __builtin_ctz(left);
-      t = scan1;
+      t += 32 - ((t - scan0) & 31);
     }
     return nt;
   };
@@ -374,144 +475,206 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_m
   // that are not stored.
   float* const key_mul = reinterpret_cast<float*>(lds + F::STAGES * F::TILE);  // [3][BK]: K's power, V's exponent, V's power
   int e_ref = INT32_MIN;  // float32: the largest exponent of the first 32 keys' V
-  auto stage = [&](int st, int t) {
+  // 16-bit types: a copy is 64 pieces, RPC rows of the tile.  Row r of a tile is row
+  // (w COPIES + i) RPC + lane / C; its piece index is xor-ed by swz(r), which is the
+  // xor of the two terms' (their bits are apart), so all but an xor of a copy's
+  // address is one lane offset and scalars.
+  constexpr int COPIES = F::HALF / 1024 / kWaves, RPC = SG_WAVE / C;
+  const uint32_t row_k = (uint32_t)(lane / C) * (uint32_t)a.ldk * 2u, row_v = (uint32_t)(lane / C) * (uint32_t)a.ldv * 2u;
+  const uint32_t piece_k = (uint32_t)((lane % C) ^ swz_k(lane / C)) * 16u;
+  const uint32_t piece_v = (uint32_t)((lane % C) ^ swz_v(lane / C)) * 16u;
+  auto copy = [&](int st, int t) {
     const int k0 = kbeg + t * F::BK;
-    if constexpr (!F::F32) {
-      constexpr int COPIES = F::HALF / 1024 / kWaves;
-      const uint32_t base = (uint32_t)(uintptr_t)(lds_ptr)(lds + st * F::TILE);
-      const i32x4_t rk = sg_raw_rsrc(static_cast<const T*>(a.k) + (int64_t)k0 * a.ldk + kvh * a.hd);
-      const i32x4_t rv = sg_raw_rsrc(static_cast<const T*>(a.v) + (int64_t)k0 * a.ldv + kvh * a.hd);
+    const uint32_t base = (uint32_t)(uintptr_t)(lds_ptr)(lds + st * F::TILE) + (uint32_t)(w * COPIES) * 1024u;
+    const i32x4_t rk = sg_raw_rsrc(static_cast<const T*>(a.k) + (int64_t)k0 * a.ldk + kvh * a.hd);
+    const i32x4_t rv = sg_raw_rsrc(static_cast<const T*>(a.v) + (int64_t)k0 * a.ldv + kvh * a.hd);
+    if (a.hd == D && k0 + F::BK <= a.rows) {
 #pragma unroll
       for (int i = 0; i < COPIES; i++) {
-        const int at = (w * COPIES + i) * 64 + lane, r = at / C, s = at % C;
-        const int from = min(r, a.rows - 1 - k0);
-        const int ck = min(s ^ swz_k<D>(r), a.hd / 8 - 1), cv = min(s ^ swz_v<D>(r), a.hd / 8 - 1);
-        const uint32_t dst = base + (uint32_t)(w * COPIES + i) * 1024u;
-        sg_lds_copy16(dst, (uint32_t)(from * (int)a.ldk + ck * 8) * 2u, rk, 0);
-        sg_lds_copy16(dst + F::HALF, (uint32_t)(from * (int)a.ldv + cv * 8) * 2u, rv, 0);
+        const int r = (w * COPIES + i) * RPC;
+        sg_lds_copy16(base + 1024u * i, row_k + (piece_k ^ (uint32_t)(swz_k(r) * 16)), rk, (uint32_t)r * (uint32_t)a.ldk * 2u);
+        sg_lds_copy16(base + F::HALF + 1024u * i, row_v + (piece_v ^ (uint32_t)(swz_v(r) * 16)), rv,
+                      (uint32_t)r * (uint32_t)a.ldv * 2u);
       }
     } else {
-      constexpr int CL = C / 8;  // pieces of eight values a thread takes of a row, eight threads a row
-      const int j = tid & 7;
+#pragma unroll 1
+      for (int i = 0; i < COPIES; i++) {
+        const int r = (w * COPIES + i) * RPC + lane / C;
+        const uint32_t from = (uint32_t)min(r, a.rows - 1 - k0);
+        const int ck = min((lane % C) ^ swz_k(r), a.hd / 8 - 1), cv = min((lane % C) ^ swz_v(r), a.hd / 8 - 1);
+        sg_lds_copy16(base + 1024u * i, (from * (uint32_t)a.ldk + ck * 8) * 2u, rk, 0);
+        sg_lds_copy16(base + F::HALF + 1024u * i, (from * (uint32_t)a.ldv + cv * 8) * 2u, rv, 0);
+      }
+    }
+  };
+
+  // float32: a tile's rows through registers, TPR threads a row, CL pieces of eight
+  // values a thread and round.  AHEAD: loaded while the tile before is computed.
+  constexpr int TPR = kNT / F::BK > 8 ? kNT / F::BK : 8;
+  constexpr int CL = F::F32 ? C / TPR : 1, ROUNDS = F::F32 ? F::BK * TPR / kNT : 1;
+  constexpr bool AHEAD = KW == 1 && CL * ROUNDS <= 2;
+  f32x4_t held[F::F32 ? 2 : 1][ROUNDS][CL][2];
+  const int jt = tid % TPR;
+  auto load = [&](int t) {
+    const int k0 = kbeg + t * F::BK;
 #pragma unroll
-      for (int p = 0; p < F::BK / (kNT / 8); p++) {
-        const int r = p * (kNT / 8) + tid / 8;
-        const int64_t from = min(k0 + r, a.rows - 1);
+    for (int p = 0; p < ROUNDS; p++) {
+      const int64_t from = min(k0 + p * (kNT / TPR) + tid / TPR, a.rows - 1);
 #pragma unroll
-        for (int v = 0; v < 2; v++) {
-          const T* src = v ? static_cast<const T*>(a.v) + from * a.ldv : static_cast<const T*>(a.k) + from * a.ldk;
-          float x[CL][8];
+      for (int v = 0; v < 2; v++) {
+        const T* src = v ? static_cast<const T*>(a.v) + from * a.ldv : static_cast<const T*>(a.k) + from * a.ldk;
 #pragma unroll
-          for (int i = 0; i < CL; i++) {
-            const int c = j + 8 * i;
-            const bool on = c < a.hd / 8;
+        for (int i = 0; i < CL; i++)
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-              *reinterpret_cast<f32x4_t*>(&x[i][4 * u]) =
-                  on ? *reinterpret_cast<const f32x4_t*>(src + kvh * a.hd + 8 * c + 4 * u) : f32x4_t{0, 0, 0, 0};
+          for (int u = 0; u < 2; u++)
+            held[v][p][i][u] = jt + TPR * i < a.hd / 8
+                                   ? *reinterpret_cast<const f32x4_t*>(src + kvh * a.hd + 8 * (jt + TPR * i) + 4 * u)
+                                   : f32x4_t{0, 0, 0, 0};
+      }
+    }
+  };
+  auto put = [&]() {
+#pragma unroll
+    for (int p = 0; p < ROUNDS; p++) {
+      const int r = p * (kNT / TPR) + tid / TPR;
+#pragma unroll
+      for (int v = 0; v < 2; v++) {
+        float top = finite_top<8 * CL>(reinterpret_cast<const float*>(&held[v][p][0][0]));
+#pragma unroll
+        for (int o = TPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        int e = row_exp(top);
+        if (v) {
+          if (e_ref == INT32_MIN) {
+            if (jt == 0 && top > 0.0f) atomicMax(&first_e, e);
+            __syncthreads();
+            e_ref = __builtin_amdgcn_readfirstlane(first_e);
+            if (e_ref == INT32_MIN) e_ref = 0;
           }
-          float top = finite_top<8 * CL>(&x[0][0]);
+          e = min(max(e, max(e_ref - kSpan, -kLim)), min(e_ref + kSpan, kLim));
+        }
 #pragma unroll
-          for (int o = 4; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-          int e = row_exp(top);
+        for (int i = 0; i < CL; i++) {
+          const int c = jt + TPR * i;
+          s16x8_t hi, lo;
+          halves(reinterpret_cast<const float*>(&held[v][p][i][0]), pow2(kTop - e), hi, lo);
+          unsigned char* dst = lds + v * F::PARTS * F::HALF + (r * C + (c ^ (v ? swz_v(r) : swz_k(r)))) * 16;
+          *reinterpret_cast<s16x8_t*>(dst) = hi;
+          *reinterpret_cast<s16x8_t*>(dst + F::HALF) = lo;
+        }
+        if (jt == 0) {
           if (v) {
-            if (e_ref == INT32_MIN) {
-              if (j == 0 && top > 0.0f) atomicMax(&first_e, e);
-              __syncthreads();
-              e_ref = __builtin_amdgcn_readfirstlane(first_e);
-              if (e_ref == INT32_MIN) e_ref = 0;
-            }
-            e = min(max(e, max(e_ref - kSpan, -kLim)), min(e_ref + kSpan, kLim));
-          }
-#pragma unroll
-          for (int i = 0; i < CL; i++) {
-            const int c = j + 8 * i;
-            s16x8_t hi, lo;
-            halves(x[i], pow2(kTop - e), hi, lo);
-            unsigned char* dst =
-                lds + v * F::PARTS * F::HALF + (r * C + (c ^ (v ? swz_v<D>(r) : swz_k<D>(r)))) * 16;
-            *reinterpret_cast<s16x8_t*>(dst) = hi;
-            *reinterpret_cast<s16x8_t*>(dst + F::HALF) = lo;
-          }
-          if (j == 0) {
-            if (v) {
-              key_mul[F::BK + r] = (float)(e - e_ref);
-              key_mul[2 * F::BK + r] = pow2(e_ref - e);
-            } else {
-              key_mul[r] = pow2(e - kTop);
-            }
+            key_mul[F::BK + r] = (float)(e - e_ref);
+            key_mul[2 * F::BK + r] = pow2(e_ref - e);
+          } else {
+            key_mul[r] = pow2(e - kTop);
           }
         }
       }
     }
   };
 
-  f32x16_t o[DB] = {};
+  acc_t o[DB] = {};
   float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
 
-  // The scores of 32 keys from k on, at row kr of the LDS tile, and their part of o.
-  auto block = [&](const unsigned char* tile, int k, int kr, auto masked) {
-    constexpr bool MASKED = decltype(masked)::value;
-    f32x16_t s = {};
-    const unsigned char* kt = tile + (kr + n) * (D * 2);
-    const int sk = swz_k<D>(kr + n);
+  // Addresses within a tile: K, lane n's row, for the steps that differ in a piece's
+  // low three bits; V, the transposing load's row and piece.
+  constexpr int KVAR = 8 / G, VVAR = QT == 32 ? 2 : 4;
+  uint32_t k_at[KVAR], v_at[VVAR];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)(lds);
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-      const unsigned char* p = kt + (((2 * ks + g) ^ sk) << 4);
-      const s16x8_t kh = *reinterpret_cast<const s16x8_t*>(p);
-      if constexpr (F::F32) {
-        const s16x8_t kl = *reinterpret_cast<const s16x8_t*>(p + F::HALF);
-        s = mfma32<M>(kl, q[0][ks], s);
-        s = mfma32<M>(kh, q[F::PARTS - 1][ks], s);
+  for (int i = 0; i < KVAR; i++) k_at[i] = lds0 + (uint32_t)(n * (D * 2) + (((G * i + g) ^ swz_k(n)) << 4));
+  {
+    // The transposing load takes from lane i of 16 row i / 4's dims 4 (i % 4) .. + 3.
+    const int r = 4 * g + ((lane & 15) >> 2), c = (QT == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
+#pragma unroll
+    for (int i = 0; i < VVAR; i++)
+      v_at[i] = lds0 + (uint32_t)(F::PARTS * F::HALF + r * (D * 2) + (((QT / 8 * i + c) ^ swz_v(r)) << 4) + (lane & 1) * 8);
+  }
+  typedef __attribute__((address_space(3))) const s16x8_t* lds_s8;
+
+  // The scores of 32 keys from k on, at byte `at` of the LDS tile's rows (key_mul:
+  // row kr), and their part of o.  masked: this lane sees keys [lo, hi), and if
+  // `mixed` those of them whose document (of key k + lane % 32: ids) is its own.
+  auto block = [&](uint32_t at, int k, int kr, bool masked, int lo, int hi, bool mixed, int ids) {
+    float s[SR];
+#pragma unroll
+    for (int sub = 0; sub < kSub / QT; sub++) {
+      acc_t c = {};
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        // Step ks: piece G ks + g, the low three bits in k_at.
+        const uint32_t p = k_at[ks % KVAR] + at + (uint32_t)(sub * QT * D * 2 + ks / KVAR * 128);
+        const s16x8_t kh = *(lds_s8)(uintptr_t)p;
+        if constexpr (F::F32) {
+          const s16x8_t kl = *(lds_s8)(uintptr_t)(p + F::HALF);
+          c = X::template step<M>(kl, q[0][ks], c);
+          c = X::template step<M>(kh, q[F::PARTS - 1][ks], c);
+        }
+        c = X::template step<M>(kh, q[0][ks], c);
       }
-      s = mfma32<M>(kh, q[0][ks], s);
+#pragma unroll
+      for (int r = 0; r < R; r++) s[sub * R + r] = c[r];
     }
-    // Register r: key 8 (r / 4) + 4 g + r % 4.
-    float pv[16];
+    // Register r: key KSTR (r / 4) + 4 g + r % 4.  t = s ca + cb.
+    float ca = 1.0f, cb = 0.0f;
     if constexpr (F::F32) {
 #pragma unroll
-      for (int b = 0; b < 4; b++) {
-        const f32x4_t km = *reinterpret_cast<const f32x4_t*>(key_mul + kr + 8 * b + 4 * g);
+      for (int b = 0; b < SR / 4; b++) {
+        const f32x4_t km = *reinterpret_cast<const f32x4_t*>(key_mul + kr + F::KSTR * b + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[4 * b + i] *= km[i];
       }
     }
-#pragma unroll
-    for (int r = 0; r < 16; r++) s[r] *= before;
     if (capped) {
 #pragma unroll
-      for (int r = 0; r < 16; r++) s[r] = tanh_of<F::F32>(s[r]) * after;
+      for (int r = 0; r < SR; r++) {
+        if constexpr (F::F32) {
+          s[r] = tanh_f32(s[r] * cs) * cap2;
+        } else {
+          s[r] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[r] * cs));
+        }
+      }
+      if constexpr (!F::F32) {
+        ca = 2.0f * cap2;
+        cb = cap2;
+      }
+    } else {
+      ca = cs;
     }
     if (a.slopes) {
       const float far = (float)(row - k - 4 * g);
 #pragma unroll
-      for (int r = 0; r < 16; r++) s[r] = __builtin_fmaf(-slope, fabsf(far - (float)(8 * (r >> 2) + (r & 3))), s[r]);
+      for (int r = 0; r < SR; r++)
+        s[r] = __builtin_fmaf(-slope, fabsf(far - (float)(F::KSTR * (r >> 2) + (r & 3))), __builtin_fmaf(s[r], ca, cb));
+      ca = 1.0f;
+      cb = 0.0f;
     }
     if constexpr (F::F32) {
 #pragma unroll
-      for (int b = 0; b < 4; b++) {
-        const f32x4_t ve = *reinterpret_cast<const f32x4_t*>(key_mul + F::BK + kr + 8 * b + 4 * g);
+      for (int b = 0; b < SR / 4; b++) {
+        const f32x4_t ve = *reinterpret_cast<const f32x4_t*>(key_mul + F::BK + kr + F::KSTR * b + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[4 * b + i] += ve[i];
+        for (int i = 0; i < 4; i++) s[4 * b + i] = __builtin_fmaf(s[4 * b + i], ca, ve[i]);
       }
+      ca = 1.0f;
     }
-    if constexpr (MASKED) {
-      const int lo = me.lo - k - 4 * g, hi = me.hi - k - 4 * g;
+    if (masked) {
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int c = 8 * (r >> 2) + (r & 3);
-        s[r] = c >= lo && c < hi ? s[r] : -INFINITY;
+      for (int r = 0; r < SR; r++) {
+        const int c = F::KSTR * (r >> 2) + 4 * g + (r & 3);
+        s[r] = c >= lo - k && c < hi - k ? s[r] : -INFINITY;
       }
-      if (a.docs) {
-        const int d = a.docs[min(k + n, a.rows - 1)];
+      if (mixed) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) s[r] = __shfl(d, 8 * (r >> 2) + 4 * g + (r & 3)) == me.doc ? s[r] : -INFINITY;
+        for (int r = 0; r < SR; r++) s[r] = __shfl(ids, F::KSTR * (r >> 2) + 4 * g + (r & 3)) == me.doc ? s[r] : -INFINITY;
       }
     }
     float top = s[0];
 #pragma unroll
-    for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
-    top = fmaxf(top, __shfl_xor(top, 32));
+    for (int r = 1; r < SR; r++) top = fmaxf(top, s[r]);
+#pragma unroll
+    for (int x = QT; x < SG_WAVE; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    if constexpr (!F::F32) top = __builtin_fmaf(top, ca, cb);
     if (__ballot(top > m + kSlack)) {  // (-inf + 8 is -inf: a row's first visible key raises it)
       const float to = fmaxf(m, top);
       const float by = to > m ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
@@ -520,84 +683,112 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_m
 #pragma unroll
       for (int d = 0; d < DB; d++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) o[d][r] *= by;
+        for (int r = 0; r < R; r++) o[d][r] *= by;
     }
-    const float from = (m == -INFINITY ? 0.0f : m) - mul<T>::shift;
+    const float from = cb - (m == -INFINITY ? 0.0f : m) + mul<T>::shift;
+    // P^T, KDIM keys a step: the lane's registers 8 st .. + 7.
+    s16x8_t p[F::PARTS][F::PS];
 #pragma unroll
-    for (int r = 0; r < 16; r++) pv[r] = __builtin_amdgcn_exp2f(s[r] - from);
-    if constexpr (F::F32) {
+    for (int st = 0; st < F::PS; st++) {
+      float pv[8];
 #pragma unroll
-      for (int b = 0; b < 4; b++) {
-        const f32x4_t vw = *reinterpret_cast<const f32x4_t*>(key_mul + 2 * F::BK + kr + 8 * b + 4 * g);
-#pragma unroll
-        for (int i = 0; i < 4; i++) l = __builtin_fmaf(pv[4 * b + i], vw[i], l);
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; r++) l += pv[r];
-    }
-    // P^T, 16 keys a step: the lane's registers 8 st .. + 7.
-    s16x8_t p[F::PARTS][2];
-#pragma unroll
-    for (int st = 0; st < 2; st++) {
+      for (int i = 0; i < 8; i++)
+        pv[i] = __builtin_amdgcn_exp2f(F::F32 ? s[8 * st + i] + from : __builtin_fmaf(s[8 * st + i], ca, from));
       if constexpr (F::F32) {
-        halves(pv + 8 * st, 1.0f, p[0][st], p[F::PARTS - 1][st]);
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const f32x4_t vw = *reinterpret_cast<const f32x4_t*>(key_mul + 2 * F::BK + kr + F::KSTR * (2 * st + b) + 4 * g);
+#pragma unroll
+          for (int i = 0; i < 4; i++) l = __builtin_fmaf(pv[4 * b + i], vw[i], l);
+        }
+        halves(pv, 1.0f, p[0][st], p[F::PARTS - 1][st]);
       } else {
         chunk<M> c;
 #pragma unroll
-        for (int i = 0; i < 8; i++) c.v[i] = elem<M>::from(pv[8 * st + i]);
+        for (int i = 0; i < 8; i++) c.v[i] = elem<M>::from(pv[i]);
         p[0][st] = __builtin_bit_cast(s16x8_t, c);
+        l = add_up<M>(p[0][st], l);  // the weights as they are multiplied
       }
     }
-    // V^T: lane dim 32 d + n, keys 16 st + 4 g + 0..3 and + 8; the transposing load
-    // takes from lane i of 16 the row i / 4's dims 4 (i % 4) .. + 3.
-    const int vr = kr + 4 * g + ((lane & 15) >> 2);
-    const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vb = (lane & 1) * 8;
-    const unsigned char* vt = tile + F::PARTS * F::HALF;
+    // V^T: lane dim QT d + n, its eight keys those of the lane's p.
 #pragma unroll
     for (int d = 0; d < DB; d++) {
 #pragma unroll
-      for (int st = 0; st < 2; st++) {
+      for (int st = 0; st < F::PS; st++) {
         s16x8_t vf[F::PARTS];
 #pragma unroll
         for (int part = 0; part < F::PARTS; part++) {
           s16x4_t half[2];
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-            const int r = vr + 16 * st + 8 * u;
-            const unsigned char* at = vt + part * F::HALF + r * (D * 2) + (((4 * d + vc) ^ swz_v<D>(r)) << 4) + vb;
-            half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at));
-          }
+          for (int u = 0; u < 2; u++)
+            half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s4)(uintptr_t)(v_at[d % VVAR] + at + (uint32_t)(part * F::HALF + F::KSTR * (2 * st + u) * D * 2 + d / VVAR * 128)));
           vf[part] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
         }
         if constexpr (F::F32) {
-          o[d] = mfma32<M>(vf[F::PARTS - 1], p[0][st], o[d]);
-          o[d] = mfma32<M>(vf[0], p[F::PARTS - 1][st], o[d]);
+          o[d] = X::template step<M>(vf[F::PARTS - 1], p[0][st], o[d]);
+          o[d] = X::template step<M>(vf[0], p[F::PARTS - 1][st], o[d]);
         }
-        o[d] = mfma32<M>(vf[0], p[0][st], o[d]);
+        o[d] = X::template step<M>(vf[0], p[0][st], o[d]);
       }
     }
   };
-  auto compute = [&](int st, int t) {
-    const unsigned char* tile = lds + st * F::TILE;
+
+  // The ids of a tile's keys, loaded with the tile: lane l has key l % 32's of its blocks.
+  int ids[F::NSUB] = {};
+  auto load_ids = [&](int t, int(&to)[F::NSUB]) {
+    if (a.docs)
 #pragma unroll
+      for (int i = 0; i < F::NSUB; i++) to[i] = a.docs[min(kbeg + t * F::BK + (kw + KW * i) * kSub + (lane & 31), a.rows - 1)];
+  };
+  auto compute = [&](int st, int t) {
+    // (One copy of the code for both blocks: two made the compiler copy o between them.)
+#pragma unroll 1
     for (int i = 0; i < F::NSUB; i++) {
       const int kr = (kw + KW * i) * kSub, k = kbeg + t * F::BK + kr;
-      if (!__ballot(me.lo < k + kSub && me.hi > k)) continue;
-      if (!a.docs && !__ballot(me.live && (me.lo > k || me.hi < k + kSub)))
-        block(tile, k, kr, no{});
-      else
-        block(tile, k, kr, yes{});
+      int lo = me.lo, hi = me.hi, id = 0;
+      bool mixed = false;
+      if (a.docs) {
+        id = i ? ids[F::NSUB - 1] : ids[0];
+        const int one = __builtin_amdgcn_readfirstlane(id);
+        mixed = __ballot(id != one) != 0;
+        if (!mixed && me.doc != one) hi = 0;  // one document's keys, and not this row's
+      }
+      if (!__ballot(lo < k + kSub && hi > k)) continue;
+      const bool masked = mixed || __ballot(me.live && (lo > k || hi < k + kSub)) != 0;
+      block((uint32_t)(st * F::TILE + kr * (D * 2)), k, kr, masked, lo, hi, mixed, id);
     }
   };
 
-  if constexpr (F::STAGES == 2) {
-    int t = next(0), st = 0;
-    if (t < nt) stage(0, t);
+  if constexpr (F::F32) {
+    int t = next(0);
+    if (AHEAD && t < nt) load(t);
+    while (t < nt) {
+      load_ids(t, ids);
+      const int tn = next(t + 1);
+      if (!AHEAD) load(t);
+      __syncthreads();  // the previous tile is done with
+      put();
+      __syncthreads();
+      if (AHEAD && tn < nt) load(tn);
+      compute(0, t);
+      t = tn;
+    }
+  } else if constexpr (F::STAGES == 2) {
+    int t = next(0), st = 0, ahead[F::NSUB] = {};
+    if (t < nt) {
+      copy(0, t);
+      load_ids(t, ahead);
+    }
     while (t < nt) {
       const int tn = next(t + 1);
       publish();
-      if (tn < nt) stage(st ^ 1, tn);
+#pragma unroll
+      for (int i = 0; i < F::NSUB; i++) ids[i] = ahead[i];
+      if (tn < nt) {
+        copy(st ^ 1, tn);
+        load_ids(tn, ahead);
+      }
       compute(st, t);
       st ^= 1;
       t = tn;
@@ -605,13 +796,14 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_m
   } else {
     for (int t = next(0); t < nt; t = next(t + 1)) {
       __syncthreads();
-      stage(0, t);
-      if constexpr (F::F32) __syncthreads();
-      else publish();
+      copy(0, t);
+      load_ids(t, ids);
+      publish();
       compute(0, t);
     }
   }
-  l += __shfl_xor(l, 32);
+#pragma unroll
+  for (int x = QT; x < SG_WAVE; x *= 2) l += __shfl_xor(l, x);
 
   // ---- the waves that shared these rows ----
   int db0 = 0, db1 = DB;
@@ -629,11 +821,11 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_m
 #pragma unroll
     for (int i = 0; i < KW; i++) l += ml[i * RW + rw][1][n] * __builtin_amdgcn_exp2f(ml[i * RW + rw][0][n] - from);
     const float by = __builtin_amdgcn_exp2f(m - from);
-    float* mine = reinterpret_cast<float*>(lds) + w * (kSub * D) + lane;
+    float* mine = reinterpret_cast<float*>(lds) + w * (QT * D) + lane;
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) mine[(d * 16 + r) * 64] = o[d][r] * by;
+      for (int r = 0; r < R; r++) mine[(d * R + r) * 64] = o[d][r] * by;
     __syncthreads();
     constexpr int EACH = (DB + KW - 1) / KW;
     db0 = min(DB, kw * EACH);
@@ -642,12 +834,12 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_m
     for (int d = 0; d < EACH; d++) {
       if (db0 + d >= db1) continue;
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const float* from0 = reinterpret_cast<const float*>(lds) + ((db0 + d) * 16 + r) * 64 + lane;
-        float s = from0[rw * (kSub * D)];
+      for (int r = 0; r < R; r++) {
+        const float* from0 = reinterpret_cast<const float*>(lds) + ((db0 + d) * R + r) * 64 + lane;
+        float sum = from0[rw * (QT * D)];
 #pragma unroll
-        for (int i = 1; i < KW; i++) s += from0[(i * RW + rw) * (kSub * D)];
-        o[d][r] = s;
+        for (int i = 1; i < KW; i++) sum += from0[(i * RW + rw) * (QT * D)];
+        o[d][r] = sum;
       }
     }
   }
@@ -663,8 +855,8 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_m
   for (int d = 0; d < KEEP; d++) {
     if (db0 + d >= db1) continue;
 #pragma unroll
-    for (int b = 0; b < 4; b++) {
-      const int at = (db0 + d) * kSub + 8 * b + 4 * g;
+    for (int b = 0; b < R / 4; b++) {
+      const int at = (db0 + d) * QT + 8 * b + 4 * g;
       if (at >= a.hd) continue;
       struct alignas(4 * sizeof(T)) { T v[4]; } piece;
 #pragma unroll
@@ -677,30 +869,34 @@ __global__ __launch_bounds__(kNT, D == 256 ? 1 : 2) void k_attn_masked(sg_attn_m
     }
   }
   uint64_t again = __ballot(bad && me.live);
-  again = (again | (again >> 32)) & 0xffffffffu;
+#pragma unroll
+  for (int x = 32; x >= QT; x /= 2) again |= again >> x;
+  again &= (1ull << QT) - 1;
   while (again) {
     const int i = __builtin_ctzll(again);
     again &= again - 1;
-    careful_row<T, D>(a, row0 + kSub * rw + i, h, __builtin_amdgcn_readlane(me.lo, i), __builtin_amdgcn_readlane(me.hi, i),
-                      __builtin_amdgcn_readlane(me.doc, i), db0 * kSub, min(a.hd, db1 * kSub), lane);
+    careful_row<T, D>(a, row0 + QT * rw + i, h, __builtin_amdgcn_readlane(me.lo, i), __builtin_amdgcn_readlane(me.hi, i),
+                      __builtin_amdgcn_readlane(me.doc, i), db0 * QT, min(a.hd, db1 * QT), lane);
   }
 }
 
-template <typename T, int D, int RW, int KW>
+template <typename T, int D, int QT, int RW, int KW>
 hipError_t launch(const sg_attn_masked_args& a, hipStream_t s) {
-  typedef form<T, D, RW, KW> F;
+  typedef form<T, D, QT, RW, KW> F;
   const int64_t tiles = ((int64_t)a.rows + F::BM - 1) / F::BM;
   if (tiles * a.heads > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_attn_masked<T, D, RW, KW>), dim3((unsigned)(tiles * a.heads)), dim3(kNT), F::LDS, s, a, (int)tiles);
+  hipLaunchKernelGGL((k_attn_masked<T, D, QT, RW, KW>), dim3((unsigned)(tiles * a.heads)), dim3(F::NT), F::LDS, s, a,
+                     (int)tiles);
   return hipGetLastError();
 }
 
 template <typename T, int D>
 hipError_t by_form(const sg_attn_masked_args& a, hipStream_t s) {
   const int64_t wide = ((int64_t)a.rows + 127) / 128 * a.heads;
-  if (wide >= 512) return launch<T, D, 4, 1>(a, s);
-  if constexpr (__is_same(T, float) && D == 256) return launch<T, D, 2, 2>(a, s);
-  else return launch<T, D, 1, 4>(a, s);
+  if constexpr (__is_same(T, float) && D == 256)
+    return wide >= 512 ? launch<T, D, 16, 8, 1>(a, s) : launch<T, D, 16, 2, 2>(a, s);
+  else
+    return wide >= 512 ? launch<T, D, 32, 4, 1>(a, s) : launch<T, D, 32, 1, 4>(a, s);
 }
 
 template <typename T>

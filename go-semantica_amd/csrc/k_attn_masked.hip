@@ -109,12 +109,14 @@ struct core<16> {
   }
 };
 
-// What a row's piece index is xor-ed by.  An LDS cycle serves 128 bytes: eight lanes
-// of a K load (eight rows, one piece: three bits spread them), or the 16 lanes of a
-// transposing V load (four rows, two pieces each: two bits above the lowest).  Only
-// a piece's low three bits change, so most of an address is an immediate.
-__device__ __forceinline__ constexpr int swz_k(int row) { return row & 7; }
-__device__ __forceinline__ constexpr int swz_v(int row) { return (row & 3) << 1; }
+// What a row's piece index is xor-ed by.  An LDS cycle serves 256 bytes: 16 lanes of a
+// K load (16 rows, one piece), or 32 lanes of a transposing V load (four rows, four
+// pieces each).  Rows of 64 dims are 128 bytes, two to a cycle's banks.  (An xor of
+// three bits, for cycles of 128 bytes, doubled the LDS time.)
+template <int D>
+__device__ __forceinline__ constexpr int swz_k(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+template <int D>
+__device__ __forceinline__ constexpr int swz_v(int row) { return D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
 
 constexpr int kTop = 13;  // rows are brought to 2^13 .. 2^14 before they are halved
 constexpr int kLim = 110;
@@ -481,8 +483,8 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   // address is one lane offset and scalars.
   constexpr int COPIES = F::HALF / 1024 / kWaves, RPC = SG_WAVE / C;
   const uint32_t row_k = (uint32_t)(lane / C) * (uint32_t)a.ldk * 2u, row_v = (uint32_t)(lane / C) * (uint32_t)a.ldv * 2u;
-  const uint32_t piece_k = (uint32_t)((lane % C) ^ swz_k(lane / C)) * 16u;
-  const uint32_t piece_v = (uint32_t)((lane % C) ^ swz_v(lane / C)) * 16u;
+  const uint32_t piece_k = (uint32_t)((lane % C) ^ swz_k<D>(lane / C)) * 16u;
+  const uint32_t piece_v = (uint32_t)((lane % C) ^ swz_v<D>(lane / C)) * 16u;
   auto copy = [&](int st, int t) {
     const int k0 = kbeg + t * F::BK;
     const uint32_t base = (uint32_t)(uintptr_t)(lds_ptr)(lds + st * F::TILE) + (uint32_t)(w * COPIES) * 1024u;
@@ -492,8 +494,8 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
 #pragma unroll
       for (int i = 0; i < COPIES; i++) {
         const int r = (w * COPIES + i) * RPC;
-        sg_lds_copy16(base + 1024u * i, row_k + (piece_k ^ (uint32_t)(swz_k(r) * 16)), rk, (uint32_t)r * (uint32_t)a.ldk * 2u);
-        sg_lds_copy16(base + F::HALF + 1024u * i, row_v + (piece_v ^ (uint32_t)(swz_v(r) * 16)), rv,
+        sg_lds_copy16(base + 1024u * i, row_k + (piece_k ^ (uint32_t)(swz_k<D>(r) * 16)), rk, (uint32_t)r * (uint32_t)a.ldk * 2u);
+        sg_lds_copy16(base + F::HALF + 1024u * i, row_v + (piece_v ^ (uint32_t)(swz_v<D>(r) * 16)), rv,
                       (uint32_t)r * (uint32_t)a.ldv * 2u);
       }
     } else {
@@ -501,7 +503,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       for (int i = 0; i < COPIES; i++) {
         const int r = (w * COPIES + i) * RPC + lane / C;
         const uint32_t from = (uint32_t)min(r, a.rows - 1 - k0);
-        const int ck = min((lane % C) ^ swz_k(r), a.hd / 8 - 1), cv = min((lane % C) ^ swz_v(r), a.hd / 8 - 1);
+        const int ck = min((lane % C) ^ swz_k<D>(r), a.hd / 8 - 1), cv = min((lane % C) ^ swz_v<D>(r), a.hd / 8 - 1);
         sg_lds_copy16(base + 1024u * i, (from * (uint32_t)a.ldk + ck * 8) * 2u, rk, 0);
         sg_lds_copy16(base + F::HALF + 1024u * i, (from * (uint32_t)a.ldv + cv * 8) * 2u, rv, 0);
       }
@@ -557,7 +559,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
           const int c = jt + TPR * i;
           s16x8_t hi, lo;
           halves(reinterpret_cast<const float*>(&held[v][p][i][0]), pow2(kTop - e), hi, lo);
-          unsigned char* dst = lds + v * F::PARTS * F::HALF + (r * C + (c ^ (v ? swz_v(r) : swz_k(r)))) * 16;
+          unsigned char* dst = lds + v * F::PARTS * F::HALF + (r * C + (c ^ (v ? swz_v<D>(r) : swz_k<D>(r)))) * 16;
           *reinterpret_cast<s16x8_t*>(dst) = hi;
           *reinterpret_cast<s16x8_t*>(dst + F::HALF) = lo;
         }
@@ -576,19 +578,21 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   acc_t o[DB] = {};
   float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
 
-  // Addresses within a tile: K, lane n's row, for the steps that differ in a piece's
-  // low three bits; V, the transposing load's row and piece.
-  constexpr int KVAR = 8 / G, VVAR = QT == 32 ? 2 : 4;
+  // Addresses within a tile: K, lane n's row; V, the transposing load's row and
+  // piece.  The xor reaches a piece's low four bits: a variant for each of their
+  // values (of 32-query tiles' V: 4 d + 0..3; of 16-query tiles': 2 d + 0..1, whose
+  // lowest d bit it leaves alone), immediates for the rest.
+  constexpr int KVAR = KS < 16 / G ? KS : 16 / G, VLOW = QT == 32 ? 1 : 2, VVAR = DB / VLOW < 4 ? DB / VLOW : 4;
   uint32_t k_at[KVAR], v_at[VVAR];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)(lds);
 #pragma unroll
-  for (int i = 0; i < KVAR; i++) k_at[i] = lds0 + (uint32_t)(n * (D * 2) + (((G * i + g) ^ swz_k(n)) << 4));
+  for (int i = 0; i < KVAR; i++) k_at[i] = lds0 + (uint32_t)(n * (D * 2) + (((G * i + g) ^ swz_k<D>(n)) << 4));
   {
     // The transposing load takes from lane i of 16 row i / 4's dims 4 (i % 4) .. + 3.
     const int r = 4 * g + ((lane & 15) >> 2), c = (QT == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
 #pragma unroll
     for (int i = 0; i < VVAR; i++)
-      v_at[i] = lds0 + (uint32_t)(F::PARTS * F::HALF + r * (D * 2) + (((QT / 8 * i + c) ^ swz_v(r)) << 4) + (lane & 1) * 8);
+      v_at[i] = lds0 + (uint32_t)(F::PARTS * F::HALF + r * (D * 2) + (((4 * i + c) ^ swz_v<D>(r)) << 4) + (lane & 1) * 8);
   }
   typedef __attribute__((address_space(3))) const s16x8_t* lds_s8;
 
@@ -602,8 +606,8 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       acc_t c = {};
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
-        // Step ks: piece G ks + g, the low three bits in k_at.
-        const uint32_t p = k_at[ks % KVAR] + at + (uint32_t)(sub * QT * D * 2 + ks / KVAR * 128);
+        // Step ks: piece G ks + g, the low four bits in k_at.
+        const uint32_t p = k_at[ks % KVAR] + at + (uint32_t)(sub * QT * D * 2 + ks / KVAR * 256);
         const s16x8_t kh = *(lds_s8)(uintptr_t)p;
         if constexpr (F::F32) {
           const s16x8_t kl = *(lds_s8)(uintptr_t)(p + F::HALF);
@@ -722,7 +726,8 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
 #pragma unroll
           for (int u = 0; u < 2; u++)
             half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s4)(uintptr_t)(v_at[d % VVAR] + at + (uint32_t)(part * F::HALF + F::KSTR * (2 * st + u) * D * 2 + d / VVAR * 128)));
+                (lds_s4)(uintptr_t)(v_at[d / VLOW % VVAR] + at + (uint32_t)(part * F::HALF + F::KSTR * (2 * st + u) * D * 2 + d % VLOW * 32 +
+                                                                    d / VLOW / VVAR * 256)));
           vf[part] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
         }
         if constexpr (F::F32) {

@@ -186,10 +186,31 @@ __device__ __forceinline__ float add_up(s16x8_t p, float l) {
   return l;
 }
 
-// tanh for float32 scores: Lambert's continued fraction to seven levels below 1.5
-// (relative error 5e-8 at its end), and 1 - 2 / (e^2x + 1) above, where the second
-// term's rounding no longer shows.  (The second form alone, off by 1e-7 absolute
-// which a cap of 50 turns into 5e-6 of a weight, serves the 16-bit types.)
+// tanh of the scores of a block.  Below kNear (a cap of 50: scores to 25) an odd
+// polynomial, Chebyshev's of degree 3 (16-bit types: 6e-7 relative) or 5 (float32:
+// 9e-8) in x^2: no exponential, which costs six multiplications' time each and was
+// two thirds of a capped block's vector time.  A block with a larger score takes the
+// exact forms.
+constexpr float kNear = 0.5f;
+template <bool F32>
+__device__ __forceinline__ float tanh_near(float x, float by) {  // by tanh(x)
+  const float z = x * x;
+  float p;
+  if constexpr (F32) {
+    p = __builtin_fmaf(z, -0.00661201408f, 0.021273822f);
+    p = __builtin_fmaf(z, p, -0.0538932246f);
+    p = __builtin_fmaf(z, p, 0.133329003f);
+    p = __builtin_fmaf(z, p, -0.333333241f);
+    p = __builtin_fmaf(z, p, 1.0f);
+  } else {
+    p = __builtin_fmaf(z, -0.0443927384f, 0.131899394f);
+    p = __builtin_fmaf(z, p, -0.333262842f);
+    p = __builtin_fmaf(z, p, 0.999999451f);
+  }
+  return x * by * p;
+}
+// Lambert's continued fraction to seven levels below 1.5 (relative error 5e-8 at its
+// end), and 1 - 2 / (e^2x + 1) above, where the second term's rounding no longer shows.
 __device__ __forceinline__ float tanh_f32(float x) {
   const float e = __builtin_amdgcn_exp2f(x * (2.0f * kLog2e));
   const float far = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
@@ -201,6 +222,17 @@ __device__ __forceinline__ float tanh_f32(float x) {
   return fabsf(x) < 1.5f ? near : far;
 }
 
+// The largest over the lanes of a query (lanes n, n + QT, ...).
+template <int QT>
+__device__ __forceinline__ float query_max(float v) {
+  if constexpr (QT == 16) {
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  }
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+
 // A form: QT queries a wave, RW groups of them and KW shares of each tile's keys.
 template <typename T, int D_, int QT_, int RW_, int KW_>
 struct form {
@@ -209,19 +241,20 @@ struct form {
   static constexpr bool F32 = __is_same(T, float);
   static constexpr int PARTS = mul<T>::parts;
   static constexpr int NSUB = KW > 1 || D == 256 || (F32 && D == 128) ? 1 : 2;  // 32-key blocks a wave takes of a tile
+  static constexpr int KB = kSub * NSUB;  // which are adjacent, and taken together
   static constexpr int BK = kSub * KW * NSUB, BM = QT * RW;
   static constexpr int HALF = BK * D * 2;             // bytes of one tile's K (or V), one part
   static constexpr int TILE = 2 * PARTS * HALF;       // K and V
-  static constexpr int STAGES = !F32 && 2 * TILE <= (128 << 10) ? 2 : 1;
-  static constexpr int KEYS = F32 ? 3 * BK * 4 : 0;   // per-key powers of a float32 tile
+  static constexpr int STAGES = (!F32 || KW == 1) && 2 * TILE <= (128 << 10) ? 2 : 1;
+  static constexpr int KEYS = F32 ? STAGES * 3 * BK * 4 : 0;  // per-key powers of a float32 tile
   static constexpr int JOIN = KW > 1 ? NW * QT * D * 4 : 0;
   static constexpr int LDS = (STAGES * TILE + KEYS) > JOIN ? (STAGES * TILE + KEYS) : JOIN;
   static constexpr int WAVES = (QT == 32 && D == 256) || (NW == 4 && KW > 1) ? 1 : 2;  // a SIMD has registers for
   // Lane (n, g): query n; of a 32-key block, register r is key KSTR (r / 4) + 4 g + r % 4.
   static constexpr int G = SG_WAVE / QT, KSTR = 4 * G;
-  static constexpr int SR = kSub / G;          // a lane's scores of a block
+  static constexpr int SR = KB / G;            // a lane's scores of its keys of a tile
   static constexpr int KDIM = 8 * G;           // dims of a score step; keys of an output step
-  static constexpr int KS = D / KDIM, DB = D / QT, PS = kSub / KDIM;
+  static constexpr int KS = D / KDIM, DB = D / QT, PS = KB / KDIM;
 };
 
 // One query's view of the keys.
@@ -310,14 +343,20 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   const int row = row0 + QT * rw + n, rc = min(row, a.rows - 1);
 
   // ---- Q's loads go out first: lane (n, g), step ks: dims KDIM ks + 8 g .. + 7 of the row ----
-  const T* const qp = static_cast<const T*>(a.q) + (int64_t)rc * a.ldq + h * a.hd + 8 * g;
+  const T* const qp = static_cast<const T*>(a.q) + (int64_t)rc * a.ldq + h * a.hd;
   constexpr int QV = F::F32 ? 2 : 1;  // 16-byte loads of eight values
   f32x4_t qx[KS][QV];
 #pragma unroll
   for (int ks = 0; ks < KS; ks++)
 #pragma unroll
     for (int i = 0; i < QV; i++)
-      qx[ks][i] = F::KDIM * ks + 8 * g < a.hd ? *reinterpret_cast<const f32x4_t*>(qp + F::KDIM * ks + 4 * i) : f32x4_t{0, 0, 0, 0};
+      qx[ks][i] = *reinterpret_cast<const f32x4_t*>(qp + min(F::KDIM * ks + 8 * g, a.hd - 8) + 4 * i);
+  if (a.hd != D)
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int i = 0; i < QV; i++)
+        if (F::KDIM * ks + 8 * g >= a.hd) qx[ks][i] = f32x4_t{0, 0, 0, 0};
 
   // ---- the row's keys ----
   view me;
@@ -412,10 +451,10 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       }
     }
   }
-  // A score in powers of two is t = x ca + cb of what the matrix core gives, x = s
-  // times the row's power, or, under a cap, x = -1 / (e^2s/cap + 1).
+  // A score in powers of two is what the matrix core gives times cs, or, under a
+  // cap, cap2 times the tanh of that.
   const bool capped = a.softcap > 0.0f;
-  const float cs = capped ? qf / a.softcap * (F::F32 ? 1.0f : 2.0f * kLog2e) : qf * kLog2e;
+  const float cs = capped ? qf / a.softcap : qf * kLog2e;
   const float cap2 = a.softcap * kLog2e;
   const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
 
@@ -475,7 +514,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   // Tile t's K and V into LDS.  Keys past the tensors' end repeat the last row,
   // pieces past head_dim the last piece: they meet zeros of Q, or make outputs
   // that are not stored.
-  float* const key_mul = reinterpret_cast<float*>(lds + F::STAGES * F::TILE);  // [3][BK]: K's power, V's exponent, V's power
+  float* const key_muls = reinterpret_cast<float*>(lds + F::STAGES * F::TILE);  // [stage][3][BK]: K's power, V's exponent, V's power
   int e_ref = INT32_MIN;  // float32: the largest exponent of the first 32 keys' V
   // 16-bit types: a copy is 64 pieces, RPC rows of the tile.  Row r of a tile is row
   // (w COPIES + i) RPC + lane / C; its piece index is xor-ed by swz(r), which is the
@@ -511,10 +550,9 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   };
 
   // float32: a tile's rows through registers, TPR threads a row, CL pieces of eight
-  // values a thread and round.  AHEAD: loaded while the tile before is computed.
+  // values a thread and round.
   constexpr int TPR = kNT / F::BK > 8 ? kNT / F::BK : 8;
   constexpr int CL = F::F32 ? C / TPR : 1, ROUNDS = F::F32 ? F::BK * TPR / kNT : 1;
-  constexpr bool AHEAD = KW == 1 && CL * ROUNDS <= 2;
   f32x4_t held[F::F32 ? 2 : 1][ROUNDS][CL][2];
   const int jt = tid % TPR;
   auto load = [&](int t) {
@@ -529,13 +567,13 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
         for (int i = 0; i < CL; i++)
 #pragma unroll
           for (int u = 0; u < 2; u++)
-            held[v][p][i][u] = jt + TPR * i < a.hd / 8
-                                   ? *reinterpret_cast<const f32x4_t*>(src + kvh * a.hd + 8 * (jt + TPR * i) + 4 * u)
-                                   : f32x4_t{0, 0, 0, 0};
+            held[v][p][i][u] =
+                *reinterpret_cast<const f32x4_t*>(src + kvh * a.hd + 8 * min(jt + TPR * i, a.hd / 8 - 1) + 4 * u);
       }
     }
   };
-  auto put = [&]() {
+  auto put = [&](int st) {
+    float* const key_mul = key_muls + st * 3 * F::BK;
 #pragma unroll
     for (int p = 0; p < ROUNDS; p++) {
       const int r = p * (kNT / TPR) + tid / TPR;
@@ -559,7 +597,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
           const int c = jt + TPR * i;
           s16x8_t hi, lo;
           halves(reinterpret_cast<const float*>(&held[v][p][i][0]), pow2(kTop - e), hi, lo);
-          unsigned char* dst = lds + v * F::PARTS * F::HALF + (r * C + (c ^ (v ? swz_v<D>(r) : swz_k<D>(r)))) * 16;
+          unsigned char* dst = lds + st * F::TILE + v * F::PARTS * F::HALF + (r * C + (c ^ (v ? swz_v<D>(r) : swz_k<D>(r)))) * 16;
           *reinterpret_cast<s16x8_t*>(dst) = hi;
           *reinterpret_cast<s16x8_t*>(dst + F::HALF) = lo;
         }
@@ -596,77 +634,93 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   }
   typedef __attribute__((address_space(3))) const s16x8_t* lds_s8;
 
-  // The scores of 32 keys from k on, at byte `at` of the LDS tile's rows (key_mul:
-  // row kr), and their part of o.  masked: this lane sees keys [lo, hi), and if
-  // `mixed` those of them whose document (of key k + lane % 32: ids) is its own.
-  auto block = [&](uint32_t at, int k, int kr, bool masked, int lo, int hi, bool mixed, int ids) {
+  // The scores of this wave's KB keys of a tile, from k on, at row kr of LDS stage
+  // st, and their part of o.  masked: this lane sees keys [lo, hi), and if `mixed`
+  // those of them whose document (of key k + lane % KB: ids) is its own.
+  auto block = [&](int st, int k, int kr, bool masked, int lo, int hi, bool mixed, int ids) {
+    const uint32_t at = (uint32_t)(st * F::TILE + kr * (D * 2));
+    const float* const key_mul = key_muls + st * 3 * F::BK + kr;
+    // A step's products go to different accumulators one after another: a matrix
+    // instruction that adds to the last one's result waits for it.
+    constexpr int NS = F::KB / QT, CH = F::F32 ? 3 : 1;
+    acc_t c[NS][CH] = {};
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+      // Step ks: piece G ks + g, the low four bits in k_at.
+      const lds_s8 p = (lds_s8)(uintptr_t)(k_at[ks % KVAR] + at) + ks / KVAR * 16;
+      s16x8_t kf[NS][F::PARTS];
+#pragma unroll
+      for (int sub = 0; sub < NS; sub++)
+#pragma unroll
+        for (int part = 0; part < F::PARTS; part++) kf[sub][part] = p[(sub * QT * D * 2 + part * F::HALF) / 16];
+#pragma unroll
+      for (int sub = 0; sub < NS; sub++) c[sub][0] = X::template step<M>(kf[sub][0], q[0][ks], c[sub][0]);
+      if constexpr (F::F32) {
+#pragma unroll
+        for (int sub = 0; sub < NS; sub++) c[sub][1] = X::template step<M>(kf[sub][0], q[F::PARTS - 1][ks], c[sub][1]);
+#pragma unroll
+        for (int sub = 0; sub < NS; sub++) c[sub][CH - 1] = X::template step<M>(kf[sub][F::PARTS - 1], q[0][ks], c[sub][CH - 1]);
+      }
+    }
     float s[SR];
 #pragma unroll
-    for (int sub = 0; sub < kSub / QT; sub++) {
-      acc_t c = {};
+    for (int sub = 0; sub < NS; sub++)
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        // Step ks: piece G ks + g, the low four bits in k_at.
-        const uint32_t p = k_at[ks % KVAR] + at + (uint32_t)(sub * QT * D * 2 + ks / KVAR * 256);
-        const s16x8_t kh = *(lds_s8)(uintptr_t)p;
-        if constexpr (F::F32) {
-          const s16x8_t kl = *(lds_s8)(uintptr_t)(p + F::HALF);
-          c = X::template step<M>(kl, q[0][ks], c);
-          c = X::template step<M>(kh, q[F::PARTS - 1][ks], c);
-        }
-        c = X::template step<M>(kh, q[0][ks], c);
-      }
-#pragma unroll
-      for (int r = 0; r < R; r++) s[sub * R + r] = c[r];
-    }
-    // Register r: key KSTR (r / 4) + 4 g + r % 4.  t = s ca + cb.
-    float ca = 1.0f, cb = 0.0f;
+      for (int r = 0; r < R; r++) s[sub * R + r] = F::F32 ? c[sub][0][r] + (c[sub][CH / 2][r] + c[sub][CH - 1][r]) : c[sub][0][r];
+    // Register r: key KSTR (r / 4) + 4 g + r % 4.  The score is s ca.
+    float ca = cs;
     if constexpr (F::F32) {
 #pragma unroll
       for (int b = 0; b < SR / 4; b++) {
-        const f32x4_t km = *reinterpret_cast<const f32x4_t*>(key_mul + kr + F::KSTR * b + 4 * g);
+        const f32x4_t km = *reinterpret_cast<const f32x4_t*>(key_mul + F::KSTR * b + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[4 * b + i] *= km[i];
       }
     }
     if (capped) {
+      float most = 0.0f;
 #pragma unroll
       for (int r = 0; r < SR; r++) {
-        if constexpr (F::F32) {
-          s[r] = tanh_f32(s[r] * cs) * cap2;
-        } else {
-          s[r] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[r] * cs));
-        }
+        s[r] *= cs;
+        most = fmaxf(most, fabsf(s[r]));
       }
-      if constexpr (!F::F32) {
-        ca = 2.0f * cap2;
-        cb = cap2;
+      if (__ballot(most > kNear)) {
+        // (Through an empty asm: the compiler would compute this side for both.)
+#pragma unroll
+        for (int r = 0; r < SR; r++) asm volatile("" : "+v"(s[r]));
+#pragma unroll
+        for (int r = 0; r < SR; r++)
+          s[r] = F::F32 ? tanh_f32(s[r]) * cap2
+                        : __builtin_fmaf(-2.0f * cap2,
+                                         __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * (2.0f * kLog2e)) + 1.0f), cap2);
+      } else {
+#pragma unroll
+        for (int r = 0; r < SR; r++) s[r] = tanh_near<F::F32>(s[r], cap2);
       }
-    } else {
-      ca = cs;
+      ca = 1.0f;
     }
     if (a.slopes) {
       const float far = (float)(row - k - 4 * g);
 #pragma unroll
       for (int r = 0; r < SR; r++)
-        s[r] = __builtin_fmaf(-slope, fabsf(far - (float)(F::KSTR * (r >> 2) + (r & 3))), __builtin_fmaf(s[r], ca, cb));
+        s[r] = __builtin_fmaf(-slope, fabsf(far - (float)(F::KSTR * (r >> 2) + (r & 3))), s[r] * ca);
       ca = 1.0f;
-      cb = 0.0f;
     }
     if constexpr (F::F32) {
 #pragma unroll
       for (int b = 0; b < SR / 4; b++) {
-        const f32x4_t ve = *reinterpret_cast<const f32x4_t*>(key_mul + F::BK + kr + F::KSTR * b + 4 * g);
+        const f32x4_t ve = *reinterpret_cast<const f32x4_t*>(key_mul + F::BK + F::KSTR * b + 4 * g);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[4 * b + i] = __builtin_fmaf(s[4 * b + i], ca, ve[i]);
       }
       ca = 1.0f;
     }
     if (masked) {
+      const int c0 = lo - k - 4 * g, c1 = hi - k - 4 * g;
 #pragma unroll
       for (int r = 0; r < SR; r++) {
-        const int c = F::KSTR * (r >> 2) + 4 * g + (r & 3);
-        s[r] = c >= lo - k && c < hi - k ? s[r] : -INFINITY;
+        const int c = F::KSTR * (r >> 2) + (r & 3);
+        s[r] = c >= c0 && c < c1 ? s[r] : -INFINITY;
       }
       if (mixed) {
 #pragma unroll
@@ -676,9 +730,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < SR; r++) top = fmaxf(top, s[r]);
-#pragma unroll
-    for (int x = QT; x < SG_WAVE; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-    if constexpr (!F::F32) top = __builtin_fmaf(top, ca, cb);
+    top = query_max<QT>(top) * ca;
     if (__ballot(top > m + kSlack)) {  // (-inf + 8 is -inf: a row's first visible key raises it)
       const float to = fmaxf(m, top);
       const float by = to > m ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
@@ -689,122 +741,120 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
 #pragma unroll
         for (int r = 0; r < R; r++) o[d][r] *= by;
     }
-    const float from = cb - (m == -INFINITY ? 0.0f : m) + mul<T>::shift;
+    const float from = mul<T>::shift - (m == -INFINITY ? 0.0f : m);
     // P^T, KDIM keys a step: the lane's registers 8 st .. + 7.
     s16x8_t p[F::PARTS][F::PS];
 #pragma unroll
-    for (int st = 0; st < F::PS; st++) {
+    for (int ps = 0; ps < F::PS; ps++) {
       float pv[8];
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        pv[i] = __builtin_amdgcn_exp2f(F::F32 ? s[8 * st + i] + from : __builtin_fmaf(s[8 * st + i], ca, from));
+        pv[i] = __builtin_amdgcn_exp2f(F::F32 ? s[8 * ps + i] + from : __builtin_fmaf(s[8 * ps + i], ca, from));
       if constexpr (F::F32) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-          const f32x4_t vw = *reinterpret_cast<const f32x4_t*>(key_mul + 2 * F::BK + kr + F::KSTR * (2 * st + b) + 4 * g);
+          const f32x4_t vw = *reinterpret_cast<const f32x4_t*>(key_mul + 2 * F::BK + F::KSTR * (2 * ps + b) + 4 * g);
 #pragma unroll
           for (int i = 0; i < 4; i++) l = __builtin_fmaf(pv[4 * b + i], vw[i], l);
         }
-        halves(pv, 1.0f, p[0][st], p[F::PARTS - 1][st]);
+        halves(pv, 1.0f, p[0][ps], p[F::PARTS - 1][ps]);
       } else {
         chunk<M> c;
 #pragma unroll
         for (int i = 0; i < 8; i++) c.v[i] = elem<M>::from(pv[i]);
-        p[0][st] = __builtin_bit_cast(s16x8_t, c);
-        l = add_up<M>(p[0][st], l);  // the weights as they are multiplied
+        p[0][ps] = __builtin_bit_cast(s16x8_t, c);
+        l = add_up<M>(p[0][ps], l);  // the weights as they are multiplied
       }
     }
-    // V^T: lane dim QT d + n, its eight keys those of the lane's p.
+    // V^T: lane dim QT d + n, its eight keys those of the lane's p; DG blocks of dims
+    // in turn (as above).
+    constexpr int DG = F::F32 ? (QT == 16 ? 4 : 2) : (DB < 4 ? DB : 4);
 #pragma unroll
-    for (int d = 0; d < DB; d++) {
+    for (int d0 = 0; d0 < DB; d0 += DG) {
 #pragma unroll
-      for (int st = 0; st < F::PS; st++) {
-        s16x8_t vf[F::PARTS];
+      for (int ps = 0; ps < F::PS; ps++) {
+        s16x8_t vf[DG][F::PARTS];
 #pragma unroll
-        for (int part = 0; part < F::PARTS; part++) {
-          s16x4_t half[2];
+        for (int i = 0; i < DG; i++) {
+          const int d = d0 + i;
 #pragma unroll
-          for (int u = 0; u < 2; u++)
-            half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s4)(uintptr_t)(v_at[d / VLOW % VVAR] + at + (uint32_t)(part * F::HALF + F::KSTR * (2 * st + u) * D * 2 + d % VLOW * 32 +
-                                                                    d / VLOW / VVAR * 256)));
-          vf[part] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          for (int part = 0; part < F::PARTS; part++) {
+            s16x4_t half[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+              half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds_s4)(uintptr_t)(v_at[d / VLOW % VVAR] + at) +
+                  (part * F::HALF + F::KSTR * (2 * ps + u) * D * 2 + d % VLOW * 32 + d / VLOW / VVAR * 256) / 8);
+            vf[i][part] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          }
         }
+#pragma unroll
+        for (int i = 0; i < DG; i++) o[d0 + i] = X::template step<M>(vf[i][0], p[0][ps], o[d0 + i]);
         if constexpr (F::F32) {
-          o[d] = X::template step<M>(vf[F::PARTS - 1], p[0][st], o[d]);
-          o[d] = X::template step<M>(vf[0], p[F::PARTS - 1][st], o[d]);
+#pragma unroll
+          for (int i = 0; i < DG; i++) o[d0 + i] = X::template step<M>(vf[i][0], p[F::PARTS - 1][ps], o[d0 + i]);
+#pragma unroll
+          for (int i = 0; i < DG; i++) o[d0 + i] = X::template step<M>(vf[i][F::PARTS - 1], p[0][ps], o[d0 + i]);
         }
-        o[d] = X::template step<M>(vf[0], p[0][st], o[d]);
       }
     }
   };
 
-  // The ids of a tile's keys, loaded with the tile: lane l has key l % 32's of its blocks.
-  int ids[F::NSUB] = {};
-  auto load_ids = [&](int t, int(&to)[F::NSUB]) {
-    if (a.docs)
-#pragma unroll
-      for (int i = 0; i < F::NSUB; i++) to[i] = a.docs[min(kbeg + t * F::BK + (kw + KW * i) * kSub + (lane & 31), a.rows - 1)];
-  };
-  auto compute = [&](int st, int t) {
-    // (One copy of the code for both blocks: two made the compiler copy o between them.)
-#pragma unroll 1
-    for (int i = 0; i < F::NSUB; i++) {
-      const int kr = (kw + KW * i) * kSub, k = kbeg + t * F::BK + kr;
-      int lo = me.lo, hi = me.hi, id = 0;
-      bool mixed = false;
-      if (a.docs) {
-        id = i ? ids[F::NSUB - 1] : ids[0];
-        const int one = __builtin_amdgcn_readfirstlane(id);
-        mixed = __ballot(id != one) != 0;
-        if (!mixed && me.doc != one) hi = 0;  // one document's keys, and not this row's
-      }
-      if (!__ballot(lo < k + kSub && hi > k)) continue;
-      const bool masked = mixed || __ballot(me.live && (lo > k || hi < k + kSub)) != 0;
-      block((uint32_t)(st * F::TILE + kr * (D * 2)), k, kr, masked, lo, hi, mixed, id);
+  // The document of key l % KB of this wave's in lane l, loaded with the tile.
+  const int kr = kw * F::KB;
+  auto load_ids = [&](int t) { return a.docs ? a.docs[min(kbeg + t * F::BK + kr + lane % F::KB, a.rows - 1)] : 0; };
+  auto compute = [&](int st, int t, int ids) {
+    const int k = kbeg + t * F::BK + kr;
+    int lo = me.lo, hi = me.hi;
+    bool mixed = false;
+    if (a.docs) {
+      const int one = __builtin_amdgcn_readfirstlane(ids);
+      mixed = __ballot(ids != one) != 0;
+      if (!mixed && me.doc != one) hi = 0;  // one document's keys, and not this row's
     }
+    if (!__ballot(lo < k + F::KB && hi > k)) return;
+    const bool masked = mixed || __ballot(me.live && (lo > k || hi < k + F::KB)) != 0;
+    block(st, k, kr, masked, lo, hi, mixed, ids);
   };
 
-  if constexpr (F::F32) {
-    int t = next(0);
-    if (AHEAD && t < nt) load(t);
-    while (t < nt) {
-      load_ids(t, ids);
-      const int tn = next(t + 1);
-      if (!AHEAD) load(t);
-      __syncthreads();  // the previous tile is done with
-      put();
-      __syncthreads();
-      if (AHEAD && tn < nt) load(tn);
-      compute(0, t);
-      t = tn;
-    }
-  } else if constexpr (F::STAGES == 2) {
-    int t = next(0), st = 0, ahead[F::NSUB] = {};
+  int t = next(0);
+  if constexpr (F::STAGES == 2) {
+    // A tile ahead: 16-bit types' copies are in flight while the tile before is
+    // computed, float32 rows are loaded before it and halved behind it.
+    int st = 0, ids = 0;
     if (t < nt) {
-      copy(0, t);
-      load_ids(t, ahead);
+      if constexpr (F::F32) {
+        load(t);
+        put(0);
+      } else {
+        copy(0, t);
+      }
+      ids = load_ids(t);
     }
     while (t < nt) {
       const int tn = next(t + 1);
+      int ahead = 0;
       publish();
-#pragma unroll
-      for (int i = 0; i < F::NSUB; i++) ids[i] = ahead[i];
       if (tn < nt) {
-        copy(st ^ 1, tn);
-        load_ids(tn, ahead);
+        if constexpr (F::F32) load(tn);
+        else copy(st ^ 1, tn);
+        ahead = load_ids(tn);
       }
-      compute(st, t);
+      compute(st, t, ids);
       st ^= 1;
+      if (F::F32 && tn < nt) put(st);
       t = tn;
+      ids = ahead;
     }
   } else {
-    for (int t = next(0); t < nt; t = next(t + 1)) {
-      __syncthreads();
-      copy(0, t);
-      load_ids(t, ids);
+    for (; t < nt; t = next(t + 1)) {
+      if constexpr (F::F32) load(t);
+      __syncthreads();  // the previous tile is done with
+      if constexpr (F::F32) put(0);
+      else copy(0, t);
+      const int ids = load_ids(t);
       publish();
-      compute(0, t);
+      compute(0, t, ids);
     }
   }
 #pragma unroll

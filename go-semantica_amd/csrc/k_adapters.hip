@@ -71,117 +71,54 @@ __device__ __forceinline__ f32x4_t mfma<float>(const chunk<float>& a, const chun
 
 // The adapters of a workgroup's ROWS rows: own[r] in LDS (kNone: its sequence has
 // none; kNoRow: a row of no sequence, which is left as it was), and their distinct
-// ids in rising order of first row.
+// ids in rising order of first row, each with the 16-row tiles that hold it (bits).
 constexpr int kNone = -1, kNoRow = -2;
 template <int ROWS>
 struct tile_ids {
-  int own[ROWS], list[ROWS], count;
+  int own[ROWS], list[ROWS], tiles[ROWS], count;
 };
 
+// From each row's id in lane 0 .. ROWS - 1 of the first wave.
+template <int ROWS>
+__device__ __forceinline__ void list_ids(int id, tile_ids<ROWS>& t, int lane) {
+  if (lane < ROWS) t.own[lane] = id;
+  int n = 0;
+  uint64_t left = __ballot(lane < ROWS && id >= 0);
+  while (left) {
+    const int pick = __builtin_amdgcn_readfirstlane(__shfl(id, __builtin_ctzll(left)));
+    const uint64_t its = __ballot(lane < ROWS && id == pick);
+    int bits = 0;
+#pragma unroll
+    for (int r = 0; r < ROWS / kTile; r++) bits |= ((its >> (r * kTile)) & 0xffff) ? 1 << r : 0;
+    if (lane == 0) {
+      t.list[n] = pick;
+      t.tiles[n] = bits;
+    }
+    n++;
+    left &= ~its;
+  }
+  if (lane == 0) t.count = n;
+}
+
+// The same from the offsets, by every thread of the workgroup.
 template <int ROWS>
 __device__ __forceinline__ void find_ids(const sg_adapters_args& a, int row0, tile_ids<ROWS>& t, int tid) {
   static_assert(ROWS <= SG_WAVE, "a lane per row");
   if (tid < SG_WAVE) {
-    const int lane = tid, last = min(row0 + ROWS, a.rows) - 1;
-    const int i0 = sgp::find_seq(a.off, a.n_seq, row0, lane), i1 = sgp::find_seq(a.off, a.n_seq, last, lane);
-    const int row = min(row0 + lane, last);
-    int lo = max(i0, 0), hi = max(i1, lo);  // the row's sequence lies between the first and the last row's
-    while (lo < hi) {
-      const int mid = lo + (hi - lo + 1) / 2;
-      if (a.off[mid] <= row) lo = mid;
-      else hi = mid - 1;
-    }
+    const int lane = tid, last = min(row0 + ROWS, a.rows) - 1, row = min(row0 + lane, last);
+    int seq, s0, s1;
+    sgp::row_seq(a.off, a.n_seq, row0, last, row, lane, seq, s0, s1);
     int id = kNoRow;
-    if (lane < ROWS && row0 + lane <= last && a.off[lo] <= row && row < a.off[lo + 1]) {
-      id = a.ids[lo];
+    if (lane < ROWS && row0 + lane <= last && s0 <= row && row < s1) {
+      id = a.ids[seq];
       if (id < 0 || id >= a.n_adapters) id = kNone;
     }
-    if (lane < ROWS) t.own[lane] = id;
-    int n = 0;
-    uint64_t left = __ballot(id >= 0);
-    while (left) {
-      const int pick = __builtin_amdgcn_readfirstlane(__shfl(id, __builtin_ctzll(left)));
-      if (lane == 0) t.list[n] = pick;
-      n++;
-      left &= ~__ballot(id == pick);
-    }
-    if (lane == 0) t.count = n;
+    list_ids<ROWS>(id, t, lane);
   }
   __syncthreads();
 }
 
-// ---- down: u[part][row][rank] ------------------------------------------------
-// A workgroup: RT tiles of 16 rows, one part of in_dim, NRB blocks of 16 ranks.
-// Its four waves take a quarter of the part's steps each and add up through LDS.
-template <typename T, int RT, int NRB>
-__global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int parts, int steps_each) {
-  constexpr int V = elem<T>::vec, STEP = step_of<T>(), ROWS = RT * kTile;
-  __shared__ tile_ids<ROWS> ids;
-  __shared__ float sums[kWaves][ROWS][NRB * 16 + 4];  // + 4: rows on different banks
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 15, g = lane >> 4;
-  const int part = blockIdx.x % parts, row0 = (int)(blockIdx.x / parts) * ROWS;
-  const int rb0 = blockIdx.y * NRB, rbs = a.rank_pad / 16;
-  find_ids<ROWS>(a, row0, ids, tid);
-  const int steps = (a.in_dim + STEP - 1) / STEP;
-  const int p0 = part * steps_each, p1 = min(steps, p0 + steps_each);
-  const int each = (p1 - p0 + kWaves - 1) / kWaves;
-  const int k0 = min(p1, p0 + w * each), k1 = min(p1, k0 + each);
-  const T* x[RT];
-#pragma unroll
-  for (int r = 0; r < RT; r++)
-    x[r] = static_cast<const T*>(a.x) + (int64_t)min(row0 + r * kTile + n, a.rows - 1) * a.ldx + g * V;
-
-  for (int i = 0; i < ids.count; i++) {
-    const int id = __builtin_amdgcn_readfirstlane(ids.list[i]);
-    const chunk<T>* wa = static_cast<const chunk<T>*>(a.wa) + ((int64_t)id * rbs + rb0) * steps * 64 + lane;
-    f32x4_t acc[RT][NRB] = {};
-    // U steps' loads go out before their products (the compiler does not unroll
-    // loops with matrix instructions); a step past the wave's last is zeros.
-    constexpr int U = RT * NRB <= 2 ? 8 : RT * NRB <= 4 ? 4 : 2;
-    for (int k = k0; k < k1; k += U) {
-      chunk<T> xf[U][RT], af[U][NRB];
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        const bool on = k + u < k1;
-#pragma unroll
-        for (int b = 0; b < NRB; b++)
-          af[u][b] = on && rb0 + b < rbs ? wa[((int64_t)b * steps + k + u) * 64] : chunk<T>{};
-#pragma unroll
-        for (int r = 0; r < RT; r++)
-          xf[u][r] = on && (k + u) * STEP + g * V < a.in_dim
-                         ? *reinterpret_cast<const chunk<T>*>(x[r] + (int64_t)(k + u) * STEP)
-                         : chunk<T>{};
-      }
-#pragma unroll
-      for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int b = 0; b < NRB; b++)
-#pragma unroll
-          for (int r = 0; r < RT; r++) acc[r][b] = mfma<T>(af[u][b], xf[u][r], acc[r][b]);
-    }
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-      if (ids.own[r * kTile + n] == id) {
-#pragma unroll
-        for (int b = 0; b < NRB; b++)
-          *reinterpret_cast<f32x4_t*>(&sums[w][r * kTile + n][16 * b + 4 * g]) = acc[r][b];
-      }
-  }
-  __syncthreads();
-  const int width = min(NRB, rbs - rb0) * 4;  // float4 a row
-  for (int i = tid; i < ROWS * width; i += kNT) {
-    const int r = i / width, c = (i % width) * 4;
-    if (ids.own[r] < 0) continue;  // (rows past the end have none)
-    f32x4_t s = *reinterpret_cast<const f32x4_t*>(&sums[0][r][c]);
-#pragma unroll
-    for (int v = 1; v < kWaves; v++) s += *reinterpret_cast<const f32x4_t*>(&sums[v][r][c]);
-    *reinterpret_cast<f32x4_t*>(a.u + ((int64_t)part * a.rows + row0 + r) * a.rank_pad + rb0 * 16 + c) = s;
-  }
-}
-
-// ---- up: dst = base + scale B u ------------------------------------------------
-// u's operand of one 16-rank block in LDS, ready to load: 16-bit types, lane (n, g)
+// u's operand of one 16-rank block, ready to load: 16-bit types, lane (n, g)
 // 8 values: ranks 8 (g & 1) .. + 7 of row n, upper halves for g < 2, what they
 // leave for g >= 2; float32, lane (n, g) ranks 4 g .. + 3.
 template <typename T>
@@ -199,48 +136,194 @@ __device__ __forceinline__ void put_u<float>(chunk<float>* at, int n, int r4, co
   *reinterpret_cast<f32x4_t*>(&at[16 * (r4 >> 2) + n]) = u;
 }
 
-// A workgroup: RT tiles of 16 rows and `cols` columns (a multiple of 32), the
-// 32-column pairs dealt over its waves.
-template <typename T, int RT>
-__global__ __launch_bounds__(kNT) void k_adapter_up(sg_adapters_args a, int parts, int cols, int slices) {
+// A row's u, four values in each of TPR lanes side by side, is multiplied by the
+// power of two that brings its largest value to 2^10 .. 2^11 (exact, and undone by
+// `back`): fp16 then holds every u that float32 holds, and its second half stays
+// clear of the subnormals.
+template <int TPR>
+__device__ __forceinline__ float to_range(const f32x4_t& s, float& back, float top = 0.0f) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(s[i]));
+#pragma unroll
+  for (int o = TPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 11), 254);
+  const float up = __uint_as_float((uint32_t)min(264 - e, 254) << 23);
+  back = 1.0f / up;
+  return up;
+}
+
+// ---- down: u[part][row][rank], times the adapter's scale, and the rows' ids ----------
+// A workgroup: RT tiles of 16 rows, one part of in_dim, NRB blocks of 16 ranks, and
+// every gridDim.z-th of the rows' adapters.  Its four waves take a quarter of the
+// part's steps each and add up through LDS.
+template <typename T, int RT, int NRB>
+__global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int parts, int steps_each) {
+  constexpr int V = elem<T>::vec, STEP = step_of<T>(), ROWS = RT * kTile;
+  __shared__ tile_ids<ROWS> ids;
+  __shared__ float sums[kWaves][ROWS][NRB * 16 + 4];  // + 4: rows on different banks
+  __shared__ float scale[ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int part = blockIdx.x % parts, row0 = (int)(blockIdx.x / parts) * ROWS;
+  const int rb0 = blockIdx.y * NRB, rbs = a.rank_pad / 16;
+  const int steps = (a.in_dim + STEP - 1) / STEP;
+  const int p0 = part * steps_each, p1 = min(steps, p0 + steps_each);
+  const int each = (p1 - p0 + kWaves - 1) / kWaves;
+  const int k0 = min(p1, p0 + w * each), k1 = min(p1, k0 + each);
+  const T* x[RT];
+#pragma unroll
+  for (int r = 0; r < RT; r++)
+    x[r] = static_cast<const T*>(a.x) + (int64_t)min(row0 + r * kTile + n, a.rows - 1) * a.ldx + g * V;
+  // U steps' loads go out before their products (the compiler does not unroll loops
+  // with matrix instructions); a step past the wave's last is zeros.  The first of
+  // x go out before the rows' adapters are known.
+  constexpr int U = RT * NRB <= 2 ? 8 : RT * NRB <= 4 ? 4 : 2;
+  chunk<T> xf[U][RT];
+  auto load_x = [&](int k, int tiles) {
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int r = 0; r < RT; r++)
+        xf[u][r] = k + u < k1 && (tiles >> r & 1) && (k + u) * STEP + g * V < a.in_dim
+                       ? *reinterpret_cast<const chunk<T>*>(x[r] + (int64_t)(k + u) * STEP)
+                       : chunk<T>{};
+  };
+  load_x(k0, (1 << RT) - 1);
+  find_ids<ROWS>(a, row0, ids, tid);
+  if (tid < ROWS) scale[tid] = ids.own[tid] >= 0 ? a.scales[ids.own[tid]] : 0.0f;  // read behind the loop's barrier
+
+  for (int i = blockIdx.z; i < ids.count; i += gridDim.z) {
+    const int id = __builtin_amdgcn_readfirstlane(ids.list[i]), tiles = __builtin_amdgcn_readfirstlane(ids.tiles[i]);
+    const chunk<T>* wa = static_cast<const chunk<T>*>(a.wa) + ((int64_t)id * rbs + rb0) * steps * 64 + lane;
+    f32x4_t acc[RT][NRB] = {};
+    for (int k = k0; k < k1; k += U) {
+      chunk<T> af[U][NRB];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int b = 0; b < NRB; b++)
+          af[u][b] = k + u < k1 && rb0 + b < rbs ? wa[((int64_t)b * steps + k + u) * 64] : chunk<T>{};
+      if (k > k0 || i != (int)blockIdx.z) load_x(k, tiles);
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int b = 0; b < NRB; b++)
+#pragma unroll
+          for (int r = 0; r < RT; r++)
+            if (RT == 1 || (tiles >> r & 1)) acc[r][b] = mfma<T>(af[u][b], xf[u][r], acc[r][b]);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+      if (ids.own[r * kTile + n] == id) {
+#pragma unroll
+        for (int b = 0; b < NRB; b++)
+          *reinterpret_cast<f32x4_t*>(&sums[w][r * kTile + n][16 * b + 4 * g]) = acc[r][b];
+      }
+  }
+  __syncthreads();
+  constexpr int WIDTH = NRB * 4;  // float4 a row
+  for (int i = tid; i < ROWS * WIDTH; i += kNT) {
+    const int r = i / WIDTH, c = (i % WIDTH) * 4;
+    if (a.ready) {
+      // One part and all the ranks: u as up's operand.
+      f32x4_t s = {0, 0, 0, 0};
+      if (ids.own[r] >= 0) {
+#pragma unroll
+        for (int v = 0; v < kWaves; v++) s += *reinterpret_cast<const f32x4_t*>(&sums[v][r][c]);
+        s *= scale[r];
+      }
+      float by;
+      const float up = to_range<WIDTH>(s, by);
+      bool mine = ids.own[r] < 0 && blockIdx.z == 0;  // (zeros) or of an adapter that this workgroup took
+      for (int j = blockIdx.z; j < ids.count; j += gridDim.z) mine |= ids.own[r] == ids.list[j];
+      if (row0 + r >= a.rows || !mine) continue;
+      if (c < a.rank_pad)
+        put_u<T>(static_cast<chunk<T>*>(a.ready) + ((int64_t)(row0 + r) / kTile * rbs + c / 16) * 64, (row0 + r) % kTile, c & 15,
+                 s * up);
+      if (c == 0) a.back[row0 + r] = by;
+      continue;
+    }
+    if (c >= (rbs - rb0) * 16) continue;
+    // Rows of the adapters that this workgroup took (rows past the end have none).
+    bool mine = false;
+    for (int j = blockIdx.z; j < ids.count; j += gridDim.z) mine |= ids.own[r] == ids.list[j];
+    if (!mine) continue;
+    f32x4_t s = *reinterpret_cast<const f32x4_t*>(&sums[0][r][c]);
+#pragma unroll
+    for (int v = 1; v < kWaves; v++) s += *reinterpret_cast<const f32x4_t*>(&sums[v][r][c]);
+    *reinterpret_cast<f32x4_t*>(a.u + ((int64_t)part * a.rows + row0 + r) * a.rank_pad + rb0 * 16 + c) = s * scale[r];
+  }
+  if (part == 0 && blockIdx.y == 0 && blockIdx.z == 0 && tid < ROWS && row0 + tid < a.rows) a.row_ids[row0 + tid] = ids.own[tid];
+}
+
+// ---- up: dst = base + scale B u ------------------------------------------------
+// A workgroup: RT tiles of 16 rows and CW = 128 PAIRS columns, a wave PAIRS of their
+// 32-column pairs.  The products go through LDS so that base and dst are read and
+// written in rows of CW columns.  (A loop over tiles that loads the next one's base
+// and u ahead took the registers of a third of the waves, 207 us for 190 at the bf16
+// sizes below; a workgroup of 1024 columns in turn, 197.)
+template <typename T, int RT, int PAIRS>
+__global__ __launch_bounds__(kNT) void k_adapter_up(sg_adapters_args a, int parts, int slices) {
   constexpr int V = elem<T>::vec, ROWS = RT * kTile, BL = V == 4 ? 64 : 32;  // lanes that a B fragment holds
+  constexpr int CW = 128 * PAIRS, LD = CW + 4, PIECES = ROWS * CW / V / kNT;  // 16-byte pieces a thread
   extern __shared__ char smem[];
   __shared__ tile_ids<ROWS> ids;
   __shared__ float back[ROWS];
   chunk<T>* us = reinterpret_cast<chunk<T>*>(smem);  // [RT][rank_pad / 16][64]
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int slice = blockIdx.x % slices, row0 = (int)(blockIdx.x / slices) * ROWS;
-  const int rbs = a.rank_pad / 16;
-  find_ids<ROWS>(a, row0, ids, tid);
-  {
-    // TPR threads a row, up to kHeld pieces of four ranks each.  A row's u times
-    // its adapter's scale is multiplied by the power of two that brings its
-    // largest value to 2^10 .. 2^11 (exact; undone below): fp16 then holds every
-    // u that float32 holds, and its second half stays clear of the subnormals.
-    constexpr int TPR = kNT / ROWS, kHeld = sgk::kAdapterMaxRank / 4 / (kNT / kTile);
-    static_assert(kHeld * TPR * 4 * RT >= sgk::kAdapterMaxRank, "row_tiles keeps RT * rank within 256");
-    const int r = tid / TPR;
-    const int id = ids.own[r];
-    const float* u = a.u + (int64_t)(row0 + r) * a.rank_pad;
-    f32x4_t s[kHeld];
-    float top = 0.0f;
+  const int slice = blockIdx.x % slices, rbs = a.rank_pad / 16, pairs = (a.out_dim + 31) / 32;
+  float* const delta = reinterpret_cast<float*>(us + RT * rbs * 64);  // [ROWS][LD]
+  // Piece i of this thread: row r0 + i RSTEP of a tile, columns col .. .
+  constexpr int RSTEP = kNT / (CW / V);
+  const int r0 = tid / (CW / V), cc = tid % (CW / V) * V, col = slice * CW + cc;
+  const bool in = col < a.out_dim;
+  // TPR threads a row of u, up to kHeld pieces of four ranks each.
+  constexpr int TPR = kNT / ROWS, kHeld = sgk::kAdapterMaxRank / 4 / (kNT / kTile);
+  static_assert(kHeld * TPR * 4 * RT >= sgk::kAdapterMaxRank, "row_tiles keeps RT * rank within 256");
+  // The wave's pairs.  (One past the last is the last again; it is not stored.)
+  const chunk<T>* wb[PAIRS];
+#pragma unroll
+  for (int p = 0; p < PAIRS; p++)
+    wb[p] = static_cast<const chunk<T>*>(a.wb) + (int64_t)min(slice * (CW / 32) + w * PAIRS + p, pairs - 1) * 2 * rbs * BL +
+            (lane & (BL - 1));
+
+  chunk<T> bv[PIECES];
+  f32x4_t s[kHeld];
+  int rid = kNoRow;
+  auto load = [&](int row0) {
+    if (in)
+#pragma unroll
+      for (int i = 0; i < PIECES; i++)
+        if (row0 + r0 + i * RSTEP < a.rows)
+          bv[i] = *reinterpret_cast<const chunk<T>*>(static_cast<const T*>(a.base) + (int64_t)(row0 + r0 + i * RSTEP) * a.ldb + col);
+    const float* u = a.u + (int64_t)min(row0 + tid / TPR, a.rows - 1) * a.rank_pad;
 #pragma unroll
     for (int k = 0; k < kHeld; k++) {
       const int c = (tid % TPR + k * TPR) * 4;
       s[k] = f32x4_t{0, 0, 0, 0};
-      if (id >= 0 && c < a.rank_pad) {
+      if (c < a.rank_pad)
         for (int p = 0; p < parts; p++) s[k] += *reinterpret_cast<const f32x4_t*>(u + (int64_t)p * a.rows * a.rank_pad + c);
-        s[k] *= a.scales[id];
-      }
+    }
+    rid = tid < ROWS && row0 + tid < a.rows ? a.row_ids[row0 + tid] : kNoRow;
+  };
+  const int row0 = (int)(blockIdx.x / slices) * ROWS;
+  load(row0);
+  if (tid < SG_WAVE) list_ids<ROWS>(rid, ids, lane);
+  __syncthreads();
+  {
+    // A row without an adapter has no u: what down left there goes no further.
+    const int r = tid / TPR;
+    const bool has = ids.own[r] >= 0;
+    float top = 0.0f, by;
+#pragma unroll
+    for (int k = 0; k < kHeld; k++) {
+      s[k] = has ? s[k] : f32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(s[k][i]));
     }
-#pragma unroll
-    for (int o = TPR / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const int e = min(max((int)(__float_as_uint(top) >> 23), 11), 254);
-    const float up = __uint_as_float((uint32_t)min(264 - e, 254) << 23);
-    if (tid % TPR == 0) back[r] = 1.0f / up;
+    const float up = to_range<TPR>(s[0], by, top);
+    if (tid % TPR == 0) back[r] = by;
 #pragma unroll
     for (int k = 0; k < kHeld; k++) {
       const int c = (tid % TPR + k * TPR) * 4;
@@ -248,74 +331,202 @@ __global__ __launch_bounds__(kNT) void k_adapter_up(sg_adapters_args a, int part
     }
   }
   __syncthreads();
-  int own[RT];
-  float by[RT];
+  int own[RT], owner[PIECES];
 #pragma unroll
-  for (int r = 0; r < RT; r++) {
-    own[r] = ids.own[r * kTile + n];
-    by[r] = back[r * kTile + n];
+  for (int r = 0; r < RT; r++) own[r] = ids.own[r * kTile + n];
+#pragma unroll
+  for (int i = 0; i < PIECES; i++) owner[i] = ids.own[r0 + i * RSTEP];
+  const int turns = ids.count * rbs;
+  f32x4_t sum[PAIRS][RT][2] = {}, acc[PAIRS][RT][2] = {};
+  // The adapters' rank blocks one after another, U of them loaded at a time.
+  constexpr int U = 4 / PAIRS;
+  int li = 0, lrb = 0, ci = 0, crb = 0;
+  for (int e = 0; e < turns; e += U) {
+    chunk<T> wf[U][PAIRS][2];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (e + u < turns) {
+        const int64_t first = (int64_t)__builtin_amdgcn_readfirstlane(ids.list[li]) * pairs * 2 * rbs * BL + lrb * BL;
+#pragma unroll
+        for (int p = 0; p < PAIRS; p++) {
+          wf[u][p][0] = wb[p][first];
+          wf[u][p][1] = wb[p][first + rbs * BL];
+        }
+        if (++lrb == rbs) {
+          lrb = 0;
+          li++;
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (e + u < turns) {
+        const int tiles = __builtin_amdgcn_readfirstlane(ids.tiles[ci]);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+          if (RT > 1 && !(tiles >> r & 1)) continue;
+          const chunk<T> uf = us[(r * rbs + crb) * 64 + lane];
+#pragma unroll
+          for (int p = 0; p < PAIRS; p++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) acc[p][r][j] = mfma<T>(wf[u][p][j], uf, acc[p][r][j]);
+        }
+        if (++crb == rbs) {
+          // The other adapters' rows are dropped, not multiplied by zero: a weight
+          // that is no number stays with its own requests.
+          const int id = __builtin_amdgcn_readfirstlane(ids.list[ci]);
+          crb = 0;
+          ci++;
+          if (ids.count > 1) {
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+              for (int p = 0; p < PAIRS; p++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                  sum[p][r][j] = own[r] == id ? acc[p][r][j] : sum[p][r][j];
+                  acc[p][r][j] = f32x4_t{0, 0, 0, 0};
+                }
+          } else {  // (a row without an adapter ignores its sum)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+#pragma unroll
+              for (int p = 0; p < PAIRS; p++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) sum[p][r][j] = acc[p][r][j];
+          }
+        }
+      }
   }
-  const int pairs = (a.out_dim + 31) / 32;
-  const int c1 = min(a.out_dim, (slice + 1) * cols);
-  const T* base = static_cast<const T*>(a.base);
-  T* dst = static_cast<T*>(a.dst);
-  for (int col0 = slice * cols + 32 * w; col0 < c1; col0 += 32 * kWaves) {
-    const int col = col0 + 8 * g;
-    chunk<T> bv[RT][8 / V];
+#pragma unroll
+  for (int p = 0; p < PAIRS; p++)
 #pragma unroll
     for (int r = 0; r < RT; r++)
 #pragma unroll
-      for (int h = 0; h < 8 / V; h++)
-        if (own[r] != kNoRow && col < a.out_dim)
-          bv[r][h] = *reinterpret_cast<const chunk<T>*>(base + (int64_t)(row0 + r * kTile + n) * a.ldb + col + h * V);
-    f32x4_t sum[RT][2] = {};
-    for (int i = 0; i < ids.count; i++) {
-      const int id = __builtin_amdgcn_readfirstlane(ids.list[i]);
-      const chunk<T>* wb =
-          static_cast<const chunk<T>*>(a.wb) + ((int64_t)id * pairs + col0 / 32) * 2 * rbs * BL + (lane & (BL - 1));
-      f32x4_t acc[RT][2] = {};
-      constexpr int U = RT <= 2 ? 4 : 2;
-      for (int b = 0; b < rbs; b += U) {
-        chunk<T> wf[U][2];
+      for (int j = 0; j < 2; j++)
+        *reinterpret_cast<f32x4_t*>(delta + (r * kTile + n) * LD + (w * PAIRS + p) * 32 + 8 * g + 4 * j) = sum[p][r][j];
+  __syncthreads();
+  if (in) {
 #pragma unroll
-        for (int u = 0; u < U; u++)
-          if (b + u < rbs) {
-            wf[u][0] = wb[(b + u) * BL];
-            wf[u][1] = wb[(rbs + b + u) * BL];
-          }
+    for (int i = 0; i < PIECES; i++) {
+      if (owner[i] == kNoRow) continue;
+      chunk<T> o = bv[i];
+      const int r = r0 + i * RSTEP;
+      if (owner[i] >= 0) {
+        const float f = back[r];
 #pragma unroll
-        for (int u = 0; u < U; u++)
-          if (b + u < rbs) {
+        for (int q = 0; q < V; q += 4) {
+          const f32x4_t d = *reinterpret_cast<const f32x4_t*>(delta + r * LD + cc + q);
 #pragma unroll
-            for (int r = 0; r < RT; r++) {
-              const chunk<T> uf = us[(r * rbs + b + u) * 64 + lane];
-              acc[r][0] = mfma<T>(wf[u][0], uf, acc[r][0]);
-              acc[r][1] = mfma<T>(wf[u][1], uf, acc[r][1]);
-            }
-          }
+          for (int k = 0; k < 4; k++) o.v[q + k] = elem<T>::from(__builtin_fmaf(d[k], f, elem<T>::to(o.v[q + k])));
+        }
       }
-      // The other adapters' rows are dropped, not multiplied by zero: a weight
-      // that is no number stays with its own requests.
+      *reinterpret_cast<chunk<T>*>(static_cast<T*>(a.dst) + (int64_t)(row0 + r) * a.ldd + col) = o;
+    }
+  }
+}
+
+// The same from operands that down left ready (one part of in_dim, at most 64 ranks:
+// batches of many rows): u's fragments come straight from memory into registers, so
+// that nothing of a tile is prepared once for each of its slices, which was half of
+// up's vector instructions (both kernels at the sizes below: 115 / 190 us so, 111 /
+// 162 now; the bytes take 82 / 123 at a copy's rate).
+template <typename T, int RT, int PAIRS, int NRB>
+__global__ __launch_bounds__(kNT) void k_adapter_up_ready(sg_adapters_args a, int slices) {
+  constexpr int V = elem<T>::vec, ROWS = RT * kTile, BL = V == 4 ? 64 : 32;
+  constexpr int CW = 128 * PAIRS, LD = CW + 4, PIECES = ROWS * CW / V / kNT;
+  __shared__ float delta[ROWS][LD];
+  __shared__ tile_ids<ROWS> ids;
+  __shared__ float back[ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int slice = blockIdx.x % slices, row0 = (int)(blockIdx.x / slices) * ROWS;
+  const int rbs = a.rank_pad / 16, pairs = (a.out_dim + 31) / 32;
+  constexpr int RSTEP = kNT / (CW / V);
+  const int r0 = tid / (CW / V), cc = tid % (CW / V) * V, col = slice * CW + cc;
+  const bool in = col < a.out_dim;
+  int rid = kNoRow;
+  if (tid < ROWS && row0 + tid < a.rows) {
+    rid = a.row_ids[row0 + tid];
+    back[tid] = a.back[row0 + tid];
+  }
+  chunk<T> bv[PIECES];
+  const T* const bp = static_cast<const T*>(a.base) + (int64_t)(row0 + r0) * a.ldb + col;
+#pragma unroll
+  for (int i = 0; i < PIECES; i++)
+    if (in && row0 + r0 + i * RSTEP < a.rows) bv[i] = *reinterpret_cast<const chunk<T>*>(bp + i * RSTEP * a.ldb);
+  chunk<T> uf[RT][NRB];
+#pragma unroll
+  for (int r = 0; r < RT; r++)
+#pragma unroll
+    for (int b = 0; b < NRB; b++) {
+      const int64_t tile = min(row0 / kTile + r, (a.rows - 1) / kTile);
+      uf[r][b] = b < rbs ? static_cast<const chunk<T>*>(a.ready)[(tile * rbs + b) * 64 + lane] : chunk<T>{};
+    }
+  if (tid < SG_WAVE) list_ids<ROWS>(rid, ids, lane);
+  __syncthreads();
+  int own[RT], owner[PIECES];
+#pragma unroll
+  for (int r = 0; r < RT; r++) own[r] = ids.own[r * kTile + n];
+#pragma unroll
+  for (int i = 0; i < PIECES; i++) owner[i] = ids.own[r0 + i * RSTEP];
+  const chunk<T>* wb[PAIRS];
+#pragma unroll
+  for (int p = 0; p < PAIRS; p++)
+    wb[p] = static_cast<const chunk<T>*>(a.wb) + (int64_t)min(slice * (CW / 32) + w * PAIRS + p, pairs - 1) * 2 * rbs * BL +
+            (lane & (BL - 1));
+  f32x4_t sum[PAIRS][RT][2];
+  const int count = ids.count;
+  for (int i = 0; i < count; i++) {
+    const int id = __builtin_amdgcn_readfirstlane(ids.list[i]);
+    const int64_t first = (int64_t)id * pairs * 2 * rbs * BL;
+    f32x4_t acc[PAIRS][RT][2] = {};
+#pragma unroll
+    for (int p = 0; p < PAIRS; p++) {
+      chunk<T> wf[NRB][2];
+#pragma unroll
+      for (int b = 0; b < NRB; b++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) wf[b][j] = b < rbs ? wb[p][first + (j * rbs + b) * BL] : chunk<T>{};
+#pragma unroll
+      for (int b = 0; b < NRB; b++)
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) acc[p][r][j] = mfma<T>(wf[b][j], uf[r][b], acc[p][r][j]);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; r++)
+#pragma unroll
+      for (int p = 0; p < PAIRS; p++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) sum[p][r][j] = i == 0 || own[r] == id ? acc[p][r][j] : sum[p][r][j];
+  }
+  if (count > 0)
+#pragma unroll
+    for (int p = 0; p < PAIRS; p++)
 #pragma unroll
       for (int r = 0; r < RT; r++)
 #pragma unroll
-        for (int j = 0; j < 2; j++) sum[r][j] = own[r] == id ? acc[r][j] : sum[r][j];
-    }
+        for (int j = 0; j < 2; j++)
+          *reinterpret_cast<f32x4_t*>(&delta[r * kTile + n][(w * PAIRS + p) * 32 + 8 * g + 4 * j]) = sum[p][r][j];
+  __syncthreads();
+  if (!in) return;
+  T* const dp = static_cast<T*>(a.dst) + (int64_t)(row0 + r0) * a.ldd + col;
 #pragma unroll
-    for (int r = 0; r < RT; r++) {
-      if (own[r] == kNoRow || col >= a.out_dim) continue;
+  for (int i = 0; i < PIECES; i++) {
+    if (owner[i] == kNoRow) continue;
+    chunk<T> o = bv[i];
+    if (owner[i] >= 0) {
+      const int r = r0 + i * RSTEP;
+      const float f = back[r];
 #pragma unroll
-      for (int h = 0; h < 8 / V; h++) {
-        chunk<T> o;
+      for (int q = 0; q < V; q += 4) {
+        const f32x4_t d = *reinterpret_cast<const f32x4_t*>(&delta[r][cc + q]);
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-          const int e = h * V + i;
-          o.v[i] = own[r] >= 0 ? elem<T>::from(__builtin_fmaf(sum[r][e >> 2][e & 3], by[r], elem<T>::to(bv[r][h].v[i])))
-                               : bv[r][h].v[i];
-        }
-        *reinterpret_cast<chunk<T>*>(dst + (int64_t)(row0 + r * kTile + n) * a.ldd + col + h * V) = o;
+        for (int k = 0; k < 4; k++) o.v[q + k] = elem<T>::from(__builtin_fmaf(d[k], f, elem<T>::to(o.v[q + k])));
       }
     }
+    *reinterpret_cast<chunk<T>*>(dp + i * RSTEP * a.ldd) = o;
   }
 }
 
@@ -377,50 +588,88 @@ hipError_t pack(const void* a, const void* b, int n, int rank, int in_dim, int o
 }
 
 // ---- launches ----------------------------------------------------------------------
-// Tiles a workgroup takes: more rows share its weight loads, as long as that
-// leaves a workgroup for every CU.
-int row_tiles(int rows, int rank_pad) {
+// Tiles a workgroup takes: more rows share its weight loads, as long as that leaves
+// `least` workgroups.
+int row_tiles(int rows, int rank_pad, int least) {
   for (int rt = 4; rt > 1; rt /= 2)
-    if (rt * rank_pad <= 256 && (rows + rt * kTile - 1) / (rt * kTile) >= kCus) return rt;
+    if (rt * rank_pad <= 256 && (rows + rt * kTile - 1) / (rt * kTile) >= least) return rt;
   return 1;
 }
+// Two workgroups a CU at least.  Both sides, us for 30725 float32 rows of 768 (rank
+// 16, 1280 columns) / 16384 bf16 rows of 2048 (rank 64, 8192 columns): up with one
+// tile 107 / 198, two 111 / 162, four (an earlier form) 126 / 192 for two's 115 / 190.
+int down_tiles(int rows, int rank_pad) { return row_tiles(rows, rank_pad, 2 * kCus); }
+int up_tiles(int rows, int rank_pad) { return std::min(2, row_tiles(rows, rank_pad, 2 * kCus)); }
 
 // Parts of down's sum: enough workgroups for the CUs, four steps of each wave at least.
 template <typename T>
 int parts_of(int rows, int in_dim, int rank_pad) {
-  const int rt = row_tiles(rows, rank_pad);
+  const int rt = down_tiles(rows, rank_pad);
   const int wgs = (rows + rt * kTile - 1) / (rt * kTile), steps = (in_dim + step_of<T>() - 1) / step_of<T>();
   const int most = std::min(kMostSplit, std::max(1, steps / (4 * kWaves)));
   return std::max(1, std::min(most, kCus / std::max(1, wgs)));
 }
 
 template <typename T, int RT>
-hipError_t apply_rt(const sg_adapters_args& a, hipStream_t s) {
-  const int parts = parts_of<T>(a.rows, a.in_dim, a.rank_pad);
+hipError_t down(const sg_adapters_args& a, int parts, hipStream_t s) {
   const int tiles = (a.rows + RT * kTile - 1) / (RT * kTile), rbs = a.rank_pad / 16;
   const int steps = (a.in_dim + step_of<T>() - 1) / step_of<T>(), each = (steps + parts - 1) / parts;
+  // Adapters that a workgroup's rows are likely to have, over as many workgroups
+  // while those are few (64 single tokens with 48 adapters: 6.8 us, 16.4 one after
+  // another).
+  const int64_t likely = std::min<int64_t>(std::min(a.n_adapters, a.n_seq), ((int64_t)RT * kTile * a.n_seq + a.rows - 1) / a.rows);
+  const int z = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(likely, RT * kTile), 4 * kCus / ((int64_t)tiles * parts)));
+  const dim3 grid((unsigned)(tiles * parts), rbs <= 2 ? 1 : (rbs + 3) / 4, z);
   if (rbs == 1)
-    hipLaunchKernelGGL((k_adapter_down<T, RT, 1>), dim3((unsigned)tiles * parts, 1), dim3(kNT), 0, s, a, parts, each);
+    hipLaunchKernelGGL((k_adapter_down<T, RT, 1>), grid, dim3(kNT), 0, s, a, parts, each);
   else if (rbs == 2)
-    hipLaunchKernelGGL((k_adapter_down<T, RT, 2>), dim3((unsigned)tiles * parts, 1), dim3(kNT), 0, s, a, parts, each);
+    hipLaunchKernelGGL((k_adapter_down<T, RT, 2>), grid, dim3(kNT), 0, s, a, parts, each);
   else
-    hipLaunchKernelGGL((k_adapter_down<T, RT, 4>), dim3((unsigned)tiles * parts, (rbs + 3) / 4), dim3(kNT), 0, s, a, parts, each);
-  // Columns a workgroup takes: a pair for every wave at least, more while the
-  // grid keeps four workgroups a CU.  The slice is the fast index of the grid
-  // (and workgroup i runs on XCD i % 8): with eight slices or a multiple, an
-  // XCD's L2 holds its own slice of the adapters' B and no other.
-  int cols = 32 * kWaves;
-  while (cols < 1024 && (int64_t)tiles * ((a.out_dim + 2 * cols - 1) / (2 * cols)) >= 4 * kCus) cols *= 2;
-  const int slices = (a.out_dim + cols - 1) / cols;
-  hipLaunchKernelGGL((k_adapter_up<T, RT>), dim3((unsigned)tiles * slices), dim3(kNT), (size_t)RT * rbs * 64 * 16, s, a, parts,
-                     cols, slices);
+    hipLaunchKernelGGL((k_adapter_down<T, RT, 4>), grid, dim3(kNT), 0, s, a, parts, each);
   return hipGetLastError();
 }
 
+template <typename T, int RT, int PAIRS>
+hipError_t up(const sg_adapters_args& a, int parts, hipStream_t s) {
+  constexpr int CW = 128 * PAIRS;
+  const int tiles = (a.rows + RT * kTile - 1) / (RT * kTile), slices = (a.out_dim + CW - 1) / CW;
+  const dim3 grid((unsigned)tiles * slices);
+  if (a.ready) {
+    if (a.rank_pad == 16)
+      hipLaunchKernelGGL((k_adapter_up_ready<T, RT, PAIRS, 1>), grid, dim3(kNT), 0, s, a, slices);
+    else if (a.rank_pad == 32)
+      hipLaunchKernelGGL((k_adapter_up_ready<T, RT, PAIRS, 2>), grid, dim3(kNT), 0, s, a, slices);
+    else
+      hipLaunchKernelGGL((k_adapter_up_ready<T, RT, PAIRS, 4>), grid, dim3(kNT), 0, s, a, slices);
+    return hipGetLastError();
+  }
+  const size_t lds = (size_t)RT * a.rank_pad / 16 * 64 * 16 + sizeof(float) * RT * kTile * (CW + 4);
+  hipLaunchKernelGGL((k_adapter_up<T, RT, PAIRS>), grid, dim3(kNT), lds, s, a, parts, slices);
+  return hipGetLastError();
+}
+
+template <typename T, int RT>
+hipError_t up(const sg_adapters_args& a, int parts, hipStream_t s) {
+  // Columns a workgroup takes: 256 while that leaves eight workgroups a CU, else 128
+  // (always 128: 110 / 183 us at the sizes above).  The slice is the fast index of
+  // the grid (and workgroup i runs on XCD i % 8): with eight slices or a multiple, an
+  // XCD's L2 holds its own slices of the adapters' B and no other.
+  const int64_t tiles = (a.rows + RT * kTile - 1) / (RT * kTile);
+  return tiles * ((a.out_dim + 255) / 256) >= 8 * kCus ? up<T, RT, 2>(a, parts, s) : up<T, RT, 1>(a, parts, s);
+}
+
 template <typename T>
-hipError_t apply(const sg_adapters_args& a, hipStream_t s) {
-  const int rt = row_tiles(a.rows, a.rank_pad);
-  return rt == 4 ? apply_rt<T, 4>(a, s) : rt == 2 ? apply_rt<T, 2>(a, s) : apply_rt<T, 1>(a, s);
+hipError_t apply(sg_adapters_args a, hipStream_t s) {
+  const int parts = parts_of<T>(a.rows, a.in_dim, a.rank_pad);
+  // The workspace: u (or its operands, of whole tiles), then an id and a factor a row.
+  const size_t tiled = (size_t)(a.rows + kTile - 1) / kTile * kTile;
+  a.row_ids = reinterpret_cast<int32_t*>(a.u + (parts > 1 ? parts * (size_t)a.rows : tiled) * a.rank_pad);
+  a.back = reinterpret_cast<float*>(a.row_ids + a.rows);
+  a.ready = parts == 1 && a.rank_pad <= 64 ? a.u : nullptr;
+  const int d = down_tiles(a.rows, a.rank_pad), u = up_tiles(a.rows, a.rank_pad);
+  const hipError_t e = d == 4 ? down<T, 4>(a, parts, s) : d == 2 ? down<T, 2>(a, parts, s) : down<T, 1>(a, parts, s);
+  if (e != hipSuccess) return e;
+  return u == 2 ? up<T, 2>(a, parts, s) : up<T, 1>(a, parts, s);
 }
 
 }  // namespace
@@ -441,7 +690,8 @@ hipError_t adapters_pack(int dtype, const void* a, const void* b, int n, int ran
 }
 size_t adapters_work_bytes(int dtype, int rows, int in_dim, int rank_pad) {
   const int parts = dtype == SG_F32 ? parts_of<float>(rows, in_dim, rank_pad) : parts_of<_Float16>(rows, in_dim, rank_pad);
-  return sizeof(float) * (size_t)parts * rows * rank_pad;
+  const size_t tiled = (size_t)(rows + kTile - 1) / kTile * kTile;
+  return sizeof(float) * ((parts > 1 ? parts * (size_t)rows : tiled) * rank_pad + 2 * (size_t)rows);
 }
 hipError_t adapters_apply(const sg_adapters_args& a, int dtype, hipStream_t s) {
   if (dtype == SG_F32) return apply<float>(a, s);

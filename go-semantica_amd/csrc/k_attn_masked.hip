@@ -186,29 +186,26 @@ __device__ __forceinline__ float add_up(s16x8_t p, float l) {
   return l;
 }
 
-// tanh of the scores of a block.  Below kNear (a cap of 50: scores to 25) an odd
-// polynomial, Chebyshev's of degree 3 (16-bit types: 6e-7 relative) or 5 (float32:
-// 9e-8) in x^2: no exponential, which costs six multiplications' time each and was
-// two thirds of a capped block's vector time.  A block with a larger score takes the
-// exact forms.
-constexpr float kNear = 0.5f;
-template <bool F32>
-__device__ __forceinline__ float tanh_near(float x, float by) {  // by tanh(x)
+// tanh of the scores of a block.  Below a limit an odd polynomial, Chebyshev's in x^2:
+// degree 2 below 0.35 (16-bit types: 3e-6 relative, under a cap of 50 scores to 17
+// within 5e-5), degree 5 below 0.5 (float32: 9e-8); no exponential or reciprocal,
+// each of which costs six multiplications' time.  A block with a larger score takes
+// the exact forms.
+constexpr float kNear16 = 0.35f, kNear32 = 0.5f;
+constexpr float kTanh16[3] = {0.999997118f, -0.332908736f, 0.123943759f};
+__device__ __forceinline__ float tanh_near32(float x) {
   const float z = x * x;
-  float p;
-  if constexpr (F32) {
-    p = __builtin_fmaf(z, -0.00661201408f, 0.021273822f);
-    p = __builtin_fmaf(z, p, -0.0538932246f);
-    p = __builtin_fmaf(z, p, 0.133329003f);
-    p = __builtin_fmaf(z, p, -0.333333241f);
-    p = __builtin_fmaf(z, p, 1.0f);
-  } else {
-    p = __builtin_fmaf(z, -0.0443927384f, 0.131899394f);
-    p = __builtin_fmaf(z, p, -0.333262842f);
-    p = __builtin_fmaf(z, p, 0.999999451f);
-  }
-  return x * by * p;
+  float p = __builtin_fmaf(z, -0.00661201408f, 0.021273822f);
+  p = __builtin_fmaf(z, p, -0.0538932246f);
+  p = __builtin_fmaf(z, p, 0.133329003f);
+  p = __builtin_fmaf(z, p, -0.333333241f);
+  p = __builtin_fmaf(z, p, 1.0f);
+  return x * p;
 }
+// bf16 has float32's exponents, so under a cap its weights need no running maximum:
+// 2^+-kMostCap2 and sums of them times values below 2^40 are in range (a value that
+// overflows the sum makes an output that is not finite, and careful_row takes it).
+constexpr float kMostCap2 = 80.0f;
 // Lambert's continued fraction to seven levels below 1.5 (relative error 5e-8 at its
 // end), and 1 - 2 / (e^2x + 1) above, where the second term's rounding no longer shows.
 __device__ __forceinline__ float tanh_f32(float x) {
@@ -249,7 +246,7 @@ struct form {
   static constexpr int KEYS = F32 ? STAGES * 3 * BK * 4 : 0;  // per-key powers of a float32 tile
   static constexpr int JOIN = KW > 1 ? NW * QT * D * 4 : 0;
   static constexpr int LDS = (STAGES * TILE + KEYS) > JOIN ? (STAGES * TILE + KEYS) : JOIN;
-  static constexpr int WAVES = (QT == 32 && D == 256) || (NW == 4 && KW > 1) ? 1 : 2;  // a SIMD has registers for
+  static constexpr int WAVES = (QT == 32 && D == 256) || (NW == 4 && KW > 1) ? 1 : D == 64 && !F32 ? 3 : 2;  // a SIMD has registers for
   // Lane (n, g): query n; of a 32-key block, register r is key KSTR (r / 4) + 4 g + r % 4.
   static constexpr int G = SG_WAVE / QT, KSTR = 4 * G;
   static constexpr int SR = KB / G;            // a lane's scores of its keys of a tile
@@ -361,31 +358,8 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   // ---- the row's keys ----
   view me;
   {
-    const int last = min(row0 + F::BM, a.rows) - 1;
-    int lo, hi, s0, s1;
-    if (a.n_seq < SG_WAVE) {  // one load for all offsets
-      const int off = a.off[min(lane, a.n_seq)];
-      lo = max((int)__popcll(__ballot(lane < a.n_seq && off <= row0)) - 1, 0);
-      hi = max((int)__popcll(__ballot(lane < a.n_seq && off <= last)) - 1, lo);
-      while (__ballot(lo < hi)) {
-        const int mid = lo + (hi - lo + 1) / 2;
-        if (__shfl(off, mid) <= rc) lo = mid;
-        else hi = mid - 1;
-        hi = max(hi, lo);
-      }
-      s0 = __shfl(off, lo);
-      s1 = __shfl(off, lo + 1);
-    } else {
-      lo = max(sgp::find_seq(a.off, a.n_seq, row0, lane), 0);
-      hi = max(sgp::find_seq(a.off, a.n_seq, last, lane), lo);
-      while (lo < hi) {
-        const int mid = lo + (hi - lo + 1) / 2;
-        if (a.off[mid] <= rc) lo = mid;
-        else hi = mid - 1;
-      }
-      s0 = a.off[lo];
-      s1 = a.off[lo + 1];
-    }
+    int lo, s0, s1;
+    sgp::row_seq(a.off, a.n_seq, row0, min(row0 + F::BM, a.rows) - 1, rc, lane, lo, s0, s1);
     s0 = sgp::clamp_row(s0, a.rows);
     s1 = sgp::clamp_row(s1, a.rows);
     me.live = row < a.rows && s0 <= row && row < s1;
@@ -457,6 +431,11 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   const float cs = capped ? qf / a.softcap : qf * kLog2e;
   const float cap2 = a.softcap * kLog2e;
   const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+  // 16-bit types: cap2 tanh(s cs) = s (t0 + s^2 (t1 + s^2 t2)) where |s| <= near.
+  const float t0 = cap2 * cs * kTanh16[0], t1 = cap2 * cs * cs * cs * kTanh16[1];
+  const float t2 = cap2 * cs * cs * (cs * cs) * cs * kTanh16[2];
+  const float near = F::F32 ? kNear32 : cs > 1e-6f && cs < 1e6f ? kNear16 / cs : -1.0f;
+  const bool fixed = __is_same(T, bf16_t) && capped && cap2 <= kMostCap2;
 
   // ---- tiles ----
   // The first tile from t on that may hold a key of a document of this
@@ -614,7 +593,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   };
 
   acc_t o[DB] = {};
-  float m = -INFINITY, l = 0.0f;  // l: this lane's keys only
+  float m = fixed ? 0.0f : -INFINITY, l = 0.0f;  // l: this lane's keys only
 
   // Addresses within a tile: K, lane n's row; V, the transposing load's row and
   // piece.  The xor reaches a piece's low four bits: a variant for each of their
@@ -681,10 +660,10 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       float most = 0.0f;
 #pragma unroll
       for (int r = 0; r < SR; r++) {
-        s[r] *= cs;
+        if constexpr (F::F32) s[r] *= cs;
         most = fmaxf(most, fabsf(s[r]));
       }
-      if (__ballot(most > kNear)) {
+      if (__ballot(most > near)) {
         // (Through an empty asm: the compiler would compute this side for both.)
 #pragma unroll
         for (int r = 0; r < SR; r++) asm volatile("" : "+v"(s[r]));
@@ -692,10 +671,13 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
         for (int r = 0; r < SR; r++)
           s[r] = F::F32 ? tanh_f32(s[r]) * cap2
                         : __builtin_fmaf(-2.0f * cap2,
-                                         __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * (2.0f * kLog2e)) + 1.0f), cap2);
+                                         __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * cs * (2.0f * kLog2e)) + 1.0f), cap2);
       } else {
 #pragma unroll
-        for (int r = 0; r < SR; r++) s[r] = tanh_near<F::F32>(s[r], cap2);
+        for (int r = 0; r < SR; r++) {
+          const float z = s[r] * s[r];
+          s[r] = F::F32 ? tanh_near32(s[r]) * cap2 : s[r] * __builtin_fmaf(z, __builtin_fmaf(z, t2, t1), t0);
+        }
       }
       ca = 1.0f;
     }
@@ -727,19 +709,21 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
         for (int r = 0; r < SR; r++) s[r] = __shfl(ids, F::KSTR * (r >> 2) + 4 * g + (r & 3)) == me.doc ? s[r] : -INFINITY;
       }
     }
-    float top = s[0];
+    if (!fixed) {
+      float top = s[0];
 #pragma unroll
-    for (int r = 1; r < SR; r++) top = fmaxf(top, s[r]);
-    top = query_max<QT>(top) * ca;
-    if (__ballot(top > m + kSlack)) {  // (-inf + 8 is -inf: a row's first visible key raises it)
-      const float to = fmaxf(m, top);
-      const float by = to > m ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
-      m = to;
-      l *= by;
+      for (int r = 1; r < SR; r++) top = fmaxf(top, s[r]);
+      top = query_max<QT>(top) * ca;
+      if (__ballot(top > m + kSlack)) {  // (-inf + 8 is -inf: a row's first visible key raises it)
+        const float to = fmaxf(m, top);
+        const float by = to > m ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+        m = to;
+        l *= by;
 #pragma unroll
-      for (int d = 0; d < DB; d++)
+        for (int d = 0; d < DB; d++)
 #pragma unroll
-        for (int r = 0; r < R; r++) o[d][r] *= by;
+          for (int r = 0; r < R; r++) o[d][r] *= by;
+      }
     }
     const float from = mul<T>::shift - (m == -INFINITY ? 0.0f : m);
     // P^T, KDIM keys a step: the lane's registers 8 st .. + 7.
@@ -749,7 +733,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       float pv[8];
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        pv[i] = __builtin_amdgcn_exp2f(F::F32 ? s[8 * ps + i] + from : __builtin_fmaf(s[8 * ps + i], ca, from));
+        pv[i] = __builtin_amdgcn_exp2f(F::F32 ? s[8 * ps + i] + from : fixed ? s[8 * ps + i] : __builtin_fmaf(s[8 * ps + i], ca, from));
       if constexpr (F::F32) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {

@@ -74,7 +74,7 @@ struct sg_attn_masked_args {
 };
 
 // One sg_adapters_apply call (k_adapters.hip): the bank's packed weights, strides
-// in elements; u: [ksplit][rows][rank_pad] floats.
+// in elements; u: adapters_work_bytes (the launcher places the rest in it).
 struct sg_adapters_args {
   void* dst;
   const void* base;
@@ -86,6 +86,9 @@ struct sg_adapters_args {
   const int32_t* off;
   const int32_t* ids;
   float* u;
+  int32_t* row_ids;
+  float* back;
+  void* ready;
   int rows, n_seq, n_adapters, in_dim, out_dim, rank_pad;
 };
 

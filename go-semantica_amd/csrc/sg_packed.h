@@ -60,6 +60,51 @@ __device__ __forceinline__ int find_seq(const int32_t* __restrict__ off, int n, 
   }
 }
 
+// The sequence of each lane's row, the wave's rows being row0 .. last: an index in
+// [0, n) and its offsets, whatever the offsets hold; a row of no sequence gets one
+// that does not contain it.  A step narrows both ends 64-fold, and one more load
+// serves all lanes unless 63 sequences or more share the rows: the dependent loads
+// are what this costs (a lane's own bisection of 256 offsets is eight of them).
+__device__ __forceinline__ void row_seq(const int32_t* __restrict__ off, int n, int row0, int last, int row, int lane,
+                                        int& seq, int& s0, int& s1) {
+  int i0 = 0, i1 = 0, span = n;  // row0's is in [i0, i0 + span), last's in [i1, i1 + span)
+  while (span >= SG_WAVE) {
+    const int step = (span + 63) >> 6, at = lane * step;
+    const bool le0 = at < span && i0 + at < n && off[min(i0 + at, n)] <= row0;
+    const bool le1 = at < span && i1 + at < n && off[min(i1 + at, n)] <= last;
+    i0 += max((int)__popcll(__ballot(le0)) - 1, 0) * step;
+    i1 += max((int)__popcll(__ballot(le1)) - 1, 0) * step;
+    span = step;
+  }
+  const int count = max(min(n - i0, i1 - i0 + span), 1);  // candidates from i0 on
+  if (count < SG_WAVE) {
+    const int o = off[min(i0 + lane, n)];
+    int lo = max((int)__popcll(__ballot(lane < count && o <= row0)) - 1, 0);
+    int hi = max((int)__popcll(__ballot(lane < count && o <= last)) - 1, lo);
+    while (__ballot(lo < hi)) {
+      const int mid = lo + (hi - lo + 1) / 2;
+      const int v = __shfl(o, mid);
+      if (lo < hi) {
+        if (v <= row) lo = mid;
+        else hi = mid - 1;
+      }
+    }
+    s0 = __shfl(o, lo);
+    s1 = __shfl(o, lo + 1);
+    seq = i0 + lo;
+    return;
+  }
+  int hi = i0 + count - 1;
+  seq = i0;
+  while (seq < hi) {
+    const int mid = seq + (hi - seq + 1) / 2;
+    if (off[mid] <= row) seq = mid;
+    else hi = mid - 1;
+  }
+  s0 = off[seq];
+  s1 = off[seq + 1];
+}
+
 __device__ __forceinline__ float wave_sum(float a) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) a += __shfl_xor(a, o);

@@ -104,7 +104,11 @@ def attention_tol(dtype, hd, out, mean, size, softcap=0.0):
     score = products * size + 16 * F * (size + 1) + softcap * 2.0 ** -22
     # The weights' rounding to the type, the values' halves, the sums over the keys.
     weights = {"f32": 2.0 ** -20, "f16": U["f16"], "bf16": U["bf16"]}[dtype] + 2048 * F
-    return U[dtype] * out.abs() + (2 * score + weights) * mean + TINY[dtype]
+    # 16-bit weights are summed as they are multiplied, p_j (1 + d_j) with |d_j| <= u, so the
+    # result is off by sum_j p_j d_j (v_j - o) / sum_j p_j (1 + d_j), at most
+    # u (mean |v| + |o|) / (1 - u): the sum's own share is the u |o|.
+    total = 0.0 if dtype == "f32" else U[dtype] * (1 + 2 * U[dtype])
+    return (U[dtype] + total) * out.abs() + (2 * score + weights * (1 + 2 * U[dtype])) * mean + TINY[dtype]
 
 
 def run_attention(ctx, q, k, v, off, heads, kv_heads, fill=7.0, **kw):

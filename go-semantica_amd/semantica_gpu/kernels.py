@@ -185,13 +185,24 @@ def pool_l2(ctx, out, x, out_dim, offsets, stream=None):
                                   _stream(stream)))
 
 
+# The checks below are on the path of every call, which for a short query takes the
+# GPU no longer than it takes Python: they read each property once and tell what is
+# wrong only when something is.
+_TORCH = None
 _DTYPES = {}
 
 
-def _dtype(t):
-    if not _DTYPES:
+def _torch():
+    global _TORCH
+    if _TORCH is None:
         import torch
         _DTYPES.update({torch.float32: _lib.SG_F32, torch.float16: _lib.SG_F16, torch.bfloat16: _lib.SG_BF16})
+        _TORCH = torch
+    return _TORCH
+
+
+def _dtype(t):
+    _torch()
     d = _DTYPES.get(t.dtype)
     if d is None:
         raise ValueError(f"{t.dtype}: float32, float16 or bfloat16 is needed")
@@ -200,39 +211,43 @@ def _dtype(t):
 
 def _rows_of(ctx, name, t, rows, cols, dtype):
     """The pointer and row stride of a [rows][cols] tensor whose rows are contiguous."""
-    if not t.is_cuda or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         raise ValueError(f"{name} must lie on the context's device")
     if t.dtype != dtype:
         raise ValueError(f"{name}: {t.dtype} beside {dtype}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+    if t.shape != (rows, cols):
         raise ValueError(f"{name}: shape {tuple(t.shape)} where ({rows}, {cols}) is needed")
     ld, inner = t.stride()
-    if cols > 1 and inner != 1:
+    if inner != 1 and cols > 1:
         raise ValueError(f"{name}: its rows must be contiguous")
-    return ctypes.c_void_p(t.data_ptr()), ld if rows > 1 else max(ld, _whole(cols, t.element_size()))
-
-
-def _whole(cols, size):
-    """A stride for a single row, whose own torch leaves open: whole 16 bytes."""
-    return -(-cols * size // 16) * 16 // size
+    if rows <= 1:  # torch leaves a single row's stride open: whole 16 bytes
+        size = t.element_size()
+        ld = max(ld, -(-cols * size // 16) * 16 // size)
+    return t.data_ptr(), ld
 
 
 def _vec(ctx, name, t, n, dtype):
-    """The pointer of an optional contiguous vector of n values; n None: any number."""
+    """The pointer of an optional contiguous array of n values; n None: any number."""
     if t is None:
         return None
-    if not t.is_cuda or t.device.index != ctx.device or not t.is_contiguous():
+    if t.get_device() != ctx.device or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous on the context's device")
-    if str(t.dtype) != dtype or (n is not None and t.numel() != n):
-        raise ValueError(f"{name}: {n} values of {dtype} are needed")
-    return ctypes.c_void_p(t.data_ptr())
+    if t.dtype != dtype or (n is not None and t.numel() != n):
+        raise ValueError(f"{name}: {n if n is not None else 'any number of'} values of {dtype} are needed")
+    return t.data_ptr()
+
+
+def _offsets(ctx, t):
+    """The pointer of the CSR offsets and the number of sequences."""
+    return _vec(ctx, "offsets", t, None, _torch().int32), t.numel() - 1
 
 
 def _stream_of(ctx, stream):
-    if stream is None:
-        import torch
-        return ctypes.c_void_p(torch.cuda.current_stream(ctx.device).cuda_stream)
-    return ctypes.c_void_p(stream)
+    if stream is not None:
+        return stream
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # current_stream() builds an object: 1 us
+    return raw(ctx.device) if raw else torch.cuda.current_stream(ctx.device).cuda_stream
 
 
 def attention_masked(ctx, out, q, k, v, n_heads, n_kv_heads, offsets, *, scale=0.0, softcap=0.0, slopes=None,
@@ -241,21 +256,22 @@ def attention_masked(ctx, out, q, k, v, n_heads, n_kv_heads, offsets, *, scale=0
 
     q, out [rows, n_heads * hd], k, v [rows, n_kv_heads * hd]; offsets int32 [n_seq + 1];
     slopes float32 [n_heads]; doc_ids int32 [rows]; prefix int32 [n_seq]."""
+    torch = _torch()
     rows, qd = q.shape
     hd = qd // max(n_heads, 1)
     if hd * n_heads != qd:
         raise ValueError(f"q: {qd} columns for {n_heads} heads")
-    o, ldo = _rows_of(ctx, "out", out, rows, qd, q.dtype)
-    qp, ldq = _rows_of(ctx, "q", q, rows, qd, q.dtype)
-    kp, ldk = _rows_of(ctx, "k", k, rows, n_kv_heads * hd, q.dtype)
-    vp, ldv = _rows_of(ctx, "v", v, rows, n_kv_heads * hd, q.dtype)
-    n_seq = offsets.numel() - 1
-    mask = _lib.AttnMask(scale, softcap, _vec(ctx, "slopes", slopes, n_heads, "torch.float32"),
-                         _vec(ctx, "doc_ids", doc_ids, rows, "torch.int32"),
-                         _vec(ctx, "prefix", prefix, n_seq, "torch.int32"), int(causal), window)
+    dtype = q.dtype
+    qp, ldq = _rows_of(ctx, "q", q, rows, qd, dtype)
+    o, ldo = _rows_of(ctx, "out", out, rows, qd, dtype)
+    kp, ldk = _rows_of(ctx, "k", k, rows, n_kv_heads * hd, dtype)
+    vp, ldv = _rows_of(ctx, "v", v, rows, n_kv_heads * hd, dtype)
+    off, n_seq = _offsets(ctx, offsets)
+    mask = _lib.AttnMask(scale, softcap, _vec(ctx, "slopes", slopes, n_heads, torch.float32),
+                         _vec(ctx, "doc_ids", doc_ids, rows, torch.int32),
+                         _vec(ctx, "prefix", prefix, n_seq, torch.int32), causal, window)
     _lib.check(ctx.lib.sg_attention_masked(ctx.handle, o, ldo, qp, ldq, kp, ldk, vp, ldv, _dtype(q), n_heads, n_kv_heads,
-                                           hd, rows, _vec(ctx, "offsets", offsets, None, "torch.int32"), n_seq,
-                                           ctypes.byref(mask), _stream_of(ctx, stream)))
+                                           hd, rows, off, n_seq, mask, _stream_of(ctx, stream)))
 
 
 def block_norm(ctx, xn, sum, x, h, w_post, w_pre, eps, *, gate=None, scale=1.0, offsets=None, stream=None):
@@ -263,19 +279,18 @@ def block_norm(ctx, xn, sum, x, h, w_post, w_pre, eps, *, gate=None, scale=1.0, 
 
     sum, xn, x, h [rows, cols]; w_post (or None), w_pre (None with xn None), float32 [cols];
     gate float32 [cols], or [n_seq, cols] with offsets."""
+    f32 = _torch().float32
     rows, cols = x.shape
-    s, lds = _rows_of(ctx, "sum", sum, rows, cols, x.dtype)
-    xp, ldx = _rows_of(ctx, "x", x, rows, cols, x.dtype)
-    hp, ldh = _rows_of(ctx, "h", h, rows, cols, x.dtype)
-    np_, ldn = _rows_of(ctx, "xn", xn, rows, cols, x.dtype) if xn is not None else (None, 0)
-    n_seq = offsets.numel() - 1 if offsets is not None else 0
-    _lib.check(ctx.lib.sg_block_norm(ctx.handle, np_, ldn, s, lds, xp, ldx, hp, ldh, _dtype(x), rows, cols,
-                                     _vec(ctx, "w_post", w_post, cols, "torch.float32"),
-                                     _vec(ctx, "w_pre", w_pre, cols, "torch.float32"), eps,
-                                     _vec(ctx, "gate", gate, cols * max(n_seq, 1) if offsets is not None else cols,
-                                          "torch.float32"),
-                                     scale, _vec(ctx, "offsets", offsets, None, "torch.int32"), n_seq,
-                                     _stream_of(ctx, stream)))
+    dtype = x.dtype
+    xp, ldx = _rows_of(ctx, "x", x, rows, cols, dtype)
+    hp, ldh = _rows_of(ctx, "h", h, rows, cols, dtype)
+    s, lds = _rows_of(ctx, "sum", sum, rows, cols, dtype)
+    n, ldn = _rows_of(ctx, "xn", xn, rows, cols, dtype) if xn is not None else (None, 0)
+    off, n_seq = _offsets(ctx, offsets) if offsets is not None else (None, 0)
+    _lib.check(ctx.lib.sg_block_norm(ctx.handle, n, ldn, s, lds, xp, ldx, hp, ldh, _dtype(x), rows, cols,
+                                     _vec(ctx, "w_post", w_post, cols, f32), _vec(ctx, "w_pre", w_pre, cols, f32), eps,
+                                     _vec(ctx, "gate", gate, cols if offsets is None else cols * n_seq, f32), scale, off,
+                                     n_seq, _stream_of(ctx, stream)))
 
 
 class AdapterBank:
@@ -291,8 +306,8 @@ class AdapterBank:
         self.n, self.rank, self.in_dim, self.out_dim = n, rank, in_dim, b.shape[1]
         h = ctypes.c_void_p()
         _lib.check(self.lib.sg_adapter_bank_create(
-            ctx.handle, _vec(ctx, "a", a, None, str(a.dtype)), _vec(ctx, "b", b, None, str(a.dtype)),
-            _vec(ctx, "scales", scales, n, "torch.float32"), _dtype(a), n, rank, in_dim, self.out_dim,
+            ctx.handle, _vec(ctx, "a", a, None, a.dtype), _vec(ctx, "b", b, None, a.dtype),
+            _vec(ctx, "scales", scales, n, _torch().float32), _dtype(a), n, rank, in_dim, self.out_dim,
             _stream_of(ctx, stream), ctypes.byref(h)))
         self.handle = h
 
@@ -316,18 +331,17 @@ def adapters_apply(ctx, dst, base, bank: AdapterBank, x, offsets, adapter_ids, *
     x [rows, in_dim], base and dst [rows, out_dim] (dst may be base); adapter_ids int32
     [n_seq], -1 for none.  work: a uint8 device tensor of bank.work_bytes(rows) at least,
     not shared by calls that may run at the same time; None: one from torch's allocator."""
+    torch = _torch()
     rows = x.shape[0]
+    xp, ldx = _rows_of(ctx, "x", x, rows, bank.in_dim, bank.dtype)
     d, ldd = _rows_of(ctx, "dst", dst, rows, bank.out_dim, bank.dtype)
     b, ldb = _rows_of(ctx, "base", base, rows, bank.out_dim, bank.dtype)
-    xp, ldx = _rows_of(ctx, "x", x, rows, bank.in_dim, bank.dtype)
-    n_seq = offsets.numel() - 1
+    off, n_seq = _offsets(ctx, offsets)
     if work is None:
-        import torch
         work = torch.empty(max(bank.work_bytes(rows), 16), dtype=torch.uint8, device=x.device)
         if stream is not None:  # not to be handed out again before the call's stream is done with it
             work.record_stream(torch.cuda.ExternalStream(stream, device=x.device))
-    _lib.check(ctx.lib.sg_adapters_apply(ctx.handle, d, ldd, b, ldb, bank.handle, xp, ldx, rows,
-                                         _vec(ctx, "offsets", offsets, None, "torch.int32"), n_seq,
-                                         _vec(ctx, "adapter_ids", adapter_ids, n_seq, "torch.int32"),
-                                         _vec(ctx, "work", work, None, "torch.uint8"), work.numel(),
+    _lib.check(ctx.lib.sg_adapters_apply(ctx.handle, d, ldd, b, ldb, bank.handle, xp, ldx, rows, off, n_seq,
+                                         _vec(ctx, "adapter_ids", adapter_ids, n_seq, torch.int32),
+                                         _vec(ctx, "work", work, None, torch.uint8), work.numel(),
                                          _stream_of(ctx, stream)))

@@ -35,9 +35,9 @@
 // visible keys only (careful_row).  That also covers float32 values past the
 // fp16 halves' reach (q and k above 2^113, values 2^53 times the first keys').
 //
-// Two forms (attention_masked has the rule): four waves of 32 rows each, or, for
-// batches with too few rows to fill the GPU, waves that share 32 (64) rows and
-// split each tile's keys between them, joined through LDS at the end.
+// Two forms (by_form has the rule): waves with 32 (16) rows of their own, 128 to a
+// workgroup, or, for batches with too few rows to fill the GPU, waves that share 32
+// rows and split each tile's keys between them, joined through LDS at the end.
 #include <algorithm>
 
 #include "semantica_gpu.h"
@@ -237,7 +237,7 @@ struct form {
   static constexpr int NW = RW * KW, NT = NW * SG_WAVE;
   static constexpr bool F32 = __is_same(T, float);
   static constexpr int PARTS = mul<T>::parts;
-  static constexpr int NSUB = KW > 1 || D == 256 || (F32 && D == 128) ? 1 : 2;  // 32-key blocks a wave takes of a tile
+  static constexpr int NSUB = KW > 1 || D == 256 || (F32 && D == 128 && QT == 32) ? 1 : 2;  // 32-key blocks a wave takes of a tile
   static constexpr int KB = kSub * NSUB;  // which are adjacent, and taken together
   static constexpr int BK = kSub * KW * NSUB, BM = QT * RW;
   static constexpr int HALF = BK * D * 2;             // bytes of one tile's K (or V), one part
@@ -334,8 +334,11 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rw = w % RW, kw = w / RW;
   const int n = lane % QT, g = lane / QT;
-  const int h = blockIdx.x % a.heads, tile_i = (int)(blockIdx.x / a.heads);
-  const int row0 = (a.causal ? row_tiles - 1 - tile_i : tile_i) * F::BM;  // causal: the long rows first
+  // Workgroups go round the 8 XCDs: heads are dealt so that one XCD's are neighbours, which
+  // share keys and values in its L2 (bf16, 4 x 4096, 32 heads over 8: 698 us against 705).
+  const int each = a.heads / 8;
+  const int h = a.heads % 8 == 0 ? (int)(blockIdx.x % 8) * each + (int)(blockIdx.x / 8) % each : (int)(blockIdx.x % a.heads);
+  const int row0 = (a.causal ? row_tiles - 1 - (int)(blockIdx.x / a.heads) : (int)(blockIdx.x / a.heads)) * F::BM;  // causal: the long rows first
   const int kvh = h / (a.heads / a.kv_heads);
   const int row = row0 + QT * rw + n, rc = min(row, a.rows - 1);
 
@@ -929,13 +932,30 @@ hipError_t launch(const sg_attn_masked_args& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Which form: waves that share 32 rows as long as a workgroup for each 32 rows and head
+// fits the GPU at once (one to a CU, two for 64 dims), else waves of their own rows.
+// Whole sequences of 512, 12 heads, microseconds of the shared and the own form:
+//                    512 rows          1024              2048
+//   bf16, 64 dims     8   13           10   13           16   13
+//   bf16, 128        11   19           21   17           32   19
+//   bf16, 256        18   33           36   33           57   35
+//   float32, 64      21   34           28   35           44   38
+//   float32, 128     29   36           56   37           86   40
+//   float32, 256     49   70           98   70          147   75
+// (512 rows are 192 such workgroups.)  float32 rows of their own are 16 to a wave above
+// 64 dims, so that they stay in registers (16384 rows: 150 us against 189 with 32 rows
+// at 128 dims, 230 against 263 at 256; 64 dims: 130 against 125).
 template <typename T, int D>
 hipError_t by_form(const sg_attn_masked_args& a, hipStream_t s) {
-  const int64_t wide = ((int64_t)a.rows + 127) / 128 * a.heads;
-  if constexpr (__is_same(T, float) && D == 256)
-    return wide >= 512 ? launch<T, D, 16, 8, 1>(a, s) : launch<T, D, 16, 2, 2>(a, s);
-  else
-    return wide >= 512 ? launch<T, D, 32, 4, 1>(a, s) : launch<T, D, 32, 1, 4>(a, s);
+  constexpr bool F32 = __is_same(T, float);
+  const bool share = ((int64_t)a.rows + 31) / 32 * a.heads <= (D == 64 ? 512 : 256);
+  if constexpr (F32 && D == 256) {
+    return share ? launch<T, D, 16, 2, 2>(a, s) : launch<T, D, 16, 8, 1>(a, s);
+  } else if constexpr (F32 && D == 128) {
+    return share ? launch<T, D, 32, 1, 4>(a, s) : launch<T, D, 16, 8, 1>(a, s);
+  } else {
+    return share ? launch<T, D, 32, 1, 4>(a, s) : launch<T, D, 32, 4, 1>(a, s);
+  }
 }
 
 template <typename T>

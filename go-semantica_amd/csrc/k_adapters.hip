@@ -633,6 +633,7 @@ template <typename T, int RT, int PAIRS>
 hipError_t up(const sg_adapters_args& a, int parts, hipStream_t s) {
   constexpr int CW = 128 * PAIRS;
   const int tiles = (a.rows + RT * kTile - 1) / (RT * kTile), slices = (a.out_dim + CW - 1) / CW;
+  if ((int64_t)tiles * slices > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tiles * slices);
   if (a.ready) {
     if (a.rank_pad == 16)

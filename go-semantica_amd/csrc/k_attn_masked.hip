@@ -122,7 +122,9 @@ constexpr int kTop = 13;  // rows are brought to 2^13 .. 2^14 before they are ha
 constexpr int kLim = 110;
 // V's exponents are kept within this of the workgroup's first keys': 2^-e then sums
 // without overflow, and a weight that underflows beside a row of larger values
-// is below 2^-26 of the softmax's sum as well.
+// is below 2^-26 of the softmax's sum as well.  A row of V below that span is held to
+// 2^-88 of the first keys' power, so an output above 2^-51 of it is as exact as any;
+// smaller ones (the large first keys were hidden from it) careful_row takes.
 constexpr int kSpan = 50;
 
 // 2^e for -126 <= e <= 127.
@@ -204,7 +206,9 @@ __device__ __forceinline__ float tanh_near32(float x) {
 }
 // bf16 has float32's exponents, so under a cap its weights need no running maximum:
 // 2^+-kMostCap2 and sums of them times values below 2^40 are in range (a value that
-// overflows the sum makes an output that is not finite, and careful_row takes it).
+// overflows the sum makes an output that is not finite, and careful_row takes it; so it
+// does outputs below 2^-110 before the division by a sum of weights that is small, where
+// products of tiny values underflow).
 constexpr float kMostCap2 = 80.0f;
 // Lambert's continued fraction to seven levels below 1.5 (relative error 5e-8 at its
 // end), and 1 - 2 / (e^2x + 1) above, where the second term's rounding no longer shows.
@@ -328,7 +332,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   __shared__ int range[kWaves][4];
   __shared__ uint32_t scan[kScanWords];
-  __shared__ int first_e;
+  __shared__ int first_e, raised;  // float32: the largest exponent of the first 32 keys' V; rows of V lie far below it
   __shared__ float ml[kWaves][2][QT];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -392,7 +396,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
     if (lane == 0)
 #pragma unroll
       for (int i = 0; i < 4; i++) range[w][i] = v[i];
-    if (tid == 0) first_e = INT32_MIN;
+    if (tid == 0) first_e = INT32_MIN, raised = 0;
   }
   __syncthreads();
   int all[4];
@@ -434,10 +438,13 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   const float cs = capped ? qf / a.softcap : qf * kLog2e;
   const float cap2 = a.softcap * kLog2e;
   const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
-  // 16-bit types: cap2 tanh(s cs) = s (t0 + s^2 (t1 + s^2 t2)) where |s| <= near.
-  const float t0 = cap2 * cs * kTanh16[0], t1 = cap2 * cs * cs * cs * kTanh16[1];
-  const float t2 = cap2 * cs * cs * (cs * cs) * cs * kTanh16[2];
-  const float near = F::F32 ? kNear32 : cs > 1e-6f && cs < 1e6f ? kNear16 / cs : -1.0f;
+  // 16-bit types: cap2 tanh(s ce) = s (t0 + s^2 (t1 + s^2 t2)) where |s| <= near; ce is
+  // cs, or 1 where its powers might leave float32's range and s is multiplied first.
+  const bool apart = F::F32 || !(cs > 1e-5f && cs < 1e5f);
+  const float ce = apart ? 1.0f : cs;
+  const float t0 = cap2 * ce * kTanh16[0], t1 = cap2 * ce * ce * ce * kTanh16[1];
+  const float t2 = cap2 * ce * ce * (ce * ce) * ce * kTanh16[2];
+  const float near = F::F32 ? kNear32 : kNear16 / ce;
   const bool fixed = __is_same(T, bf16_t) && capped && cap2 <= kMostCap2;
 
   // ---- tiles ----
@@ -497,7 +504,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   // pieces past head_dim the last piece: they meet zeros of Q, or make outputs
   // that are not stored.
   float* const key_muls = reinterpret_cast<float*>(lds + F::STAGES * F::TILE);  // [stage][3][BK]: K's power, V's exponent, V's power
-  int e_ref = INT32_MIN;  // float32: the largest exponent of the first 32 keys' V
+  int e_ref = INT32_MIN;  // first_e
   // 16-bit types: a copy is 64 pieces, RPC rows of the tile.  Row r of a tile is row
   // (w COPIES + i) RPC + lane / C; its piece index is xor-ed by swz(r), which is the
   // xor of the two terms' (their bits are apart), so all but an xor of a copy's
@@ -572,6 +579,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
             e_ref = __builtin_amdgcn_readfirstlane(first_e);
             if (e_ref == INT32_MIN) e_ref = 0;
           }
+          if (top > 0.0f && e < e_ref - kSpan) raised = 1;
           e = min(max(e, max(e_ref - kSpan, -kLim)), min(e_ref + kSpan, kLim));
         }
 #pragma unroll
@@ -661,11 +669,11 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
     }
     if (capped) {
       float most = 0.0f;
+      if (apart)
 #pragma unroll
-      for (int r = 0; r < SR; r++) {
-        if constexpr (F::F32) s[r] *= cs;
-        most = fmaxf(most, fabsf(s[r]));
-      }
+        for (int r = 0; r < SR; r++) s[r] *= cs;
+#pragma unroll
+      for (int r = 0; r < SR; r++) most = fmaxf(most, fabsf(s[r]));
       if (__ballot(most > near)) {
         // (Through an empty asm: the compiler would compute this side for both.)
 #pragma unroll
@@ -674,7 +682,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
         for (int r = 0; r < SR; r++)
           s[r] = F::F32 ? tanh_f32(s[r]) * cap2
                         : __builtin_fmaf(-2.0f * cap2,
-                                         __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * cs * (2.0f * kLog2e)) + 1.0f), cap2);
+                                         __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * ce * (2.0f * kLog2e)) + 1.0f), cap2);
       } else {
 #pragma unroll
         for (int r = 0; r < SR; r++) {
@@ -909,6 +917,14 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       }
       if (me.live) *reinterpret_cast<decltype(piece)*>(out + at) = piece;
     }
+  }
+  // Outputs that may have lost bits that their type holds.
+  if (F::F32 ? raised != 0 : fixed && __ballot(l < 0x1p-20f)) {
+    const float least = F::F32 ? pow2(max(e_ref - kSpan, -126)) : l < 0x1p-20f ? 0x1p-110f * inv : 0.0f;
+#pragma unroll
+    for (int d = 0; d < KEEP; d++)
+#pragma unroll
+      for (int r = 0; r < R; r++) bad |= sees && db0 + d < db1 && fabsf(o[d][r] * inv * back) < least;
   }
   uint64_t again = __ballot(bad && me.live);
 #pragma unroll

@@ -58,8 +58,9 @@ struct Span {
   bool same(const Span& o) const { return p == o.p && ld == o.ld; }
 };
 
-// A stride that holds a row and whose tensor stays within the address space.
+// Whole elements, and a stride that holds a row and whose tensor stays within the address space.
 int check_span(const char* name, const Span& t) {
+  if (t.lo() % elem_bytes(t.dtype)) return fail(SG_ERR_INVALID, "%s is not aligned to its elements", name);
   if (t.ld < t.cols || t.ld > (int64_t(1) << 28))
     return fail(SG_ERR_INVALID, "%s: row stride %lld for rows of %d", name, (long long)t.ld, t.cols);
   return SG_OK;
@@ -85,7 +86,7 @@ int sg_attention_masked(sg_ctx* ctx, void* out, int64_t ldo, const void* q, int6
                         const void* v, int64_t ldv, int32_t dtype, int32_t n_heads, int32_t n_kv_heads,
                         int32_t head_dim, int32_t rows, const int32_t* d_off, int32_t n_seq, const sg_attn_mask* mask,
                         void* stream) {
-  if (!ctx || !out || !q || !k || !v) return fail(SG_ERR_INVALID, "NULL argument");
+  if (!ctx || (rows > 0 && (!out || !q || !k || !v))) return fail(SG_ERR_INVALID, "NULL argument");
   SG_TRY(check_dtype(dtype));
   if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads > 65535)
     return fail(SG_ERR_INVALID, "%d query heads over %d key heads", n_heads, n_kv_heads);
@@ -142,10 +143,10 @@ int sg_block_norm(sg_ctx* ctx, void* xn, int64_t ldxn, void* sum, int64_t lds, c
                   const void* h, int64_t ldh, int32_t dtype, int32_t rows, int32_t cols, const float* w_post,
                   const float* w_pre, float eps, const float* gate, float scale, const int32_t* d_off, int32_t n_seq,
                   void* stream) {
-  if (!ctx || !sum || !x || !h) return fail(SG_ERR_INVALID, "NULL argument");
+  if (!ctx || (rows > 0 && (!sum || !x || !h))) return fail(SG_ERR_INVALID, "NULL argument");
   SG_TRY(check_dtype(dtype));
   if (xn && !w_pre) return fail(SG_ERR_INVALID, "xn needs w_pre");
-  if (!xn && w_pre) return fail(SG_ERR_INVALID, "w_pre needs xn");
+  if (!xn && w_pre && rows > 0) return fail(SG_ERR_INVALID, "w_pre needs xn");
   if (cols <= 0 || cols > sgk::kBlockNormCols)
     return fail(SG_ERR_INVALID, "cols %d out of range (1..%d)", cols, sgk::kBlockNormCols);
   if (!(eps >= 0.0f) || !std::isfinite(eps) || !std::isfinite(scale))
@@ -252,7 +253,7 @@ int sg_adapters_work_bytes(const sg_adapter_bank* bank, int32_t rows, size_t* by
 int sg_adapters_apply(sg_ctx* ctx, void* dst, int64_t ldd, const void* base, int64_t ldb, const sg_adapter_bank* bank,
                       const void* x, int64_t ldx, int32_t rows, const int32_t* d_off, int32_t n_seq,
                       const int32_t* d_adapter_ids, void* work, size_t work_bytes, void* stream) {
-  if (!ctx || !dst || !base || !bank || !x || !d_adapter_ids) return fail(SG_ERR_INVALID, "NULL argument");
+  if (!ctx || !bank || !d_adapter_ids || (rows > 0 && (!dst || !base || !x))) return fail(SG_ERR_INVALID, "NULL argument");
   SG_TRY(check_batch(d_off, rows, n_seq));
   if (bank->device != sgi::ctx_device(ctx)) return fail(SG_ERR_INVALID, "the adapters lie on another device");
   if (rows == 0) return SG_OK;
@@ -265,6 +266,9 @@ int sg_adapters_apply(sg_ctx* ctx, void* dst, int64_t ldd, const void* base, int
   const size_t need = sgk::adapters_work_bytes(bank->dtype, rows, bank->in_dim, bank->rank_pad);
   if (!work || work_bytes < need || reinterpret_cast<uintptr_t>(work) % 16)
     return fail(SG_ERR_INVALID, "work: %zu bytes, 16-byte aligned, are needed (%zu given)", need, work ? work_bytes : 0);
+  const uintptr_t w0 = reinterpret_cast<uintptr_t>(work), w1 = w0 + need;
+  for (const Span* t : {&sd, &sb, &sx})
+    if (w0 < t->hi() && t->lo() < w1) return fail(SG_ERR_INVALID, "work overlaps dst, base or x");
   OnDevice on;
   SG_TRY(on.enter(sgi::ctx_device(ctx)));
   sg_adapters_args a{};

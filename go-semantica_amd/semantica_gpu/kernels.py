@@ -220,9 +220,9 @@ def _rows_of(ctx, name, t, rows, cols, dtype):
     ld, inner = t.stride()
     if inner != 1 and cols > 1:
         raise ValueError(f"{name}: its rows must be contiguous")
-    if rows <= 1:  # torch leaves a single row's stride open: whole 16 bytes
+    if rows <= 1:  # a single row's stride means nothing: whole 16 bytes
         size = t.element_size()
-        ld = max(ld, -(-cols * size // 16) * 16 // size)
+        ld = -(-cols * size // 16) * 16 // size
     return t.data_ptr(), ld
 
 
@@ -269,7 +269,7 @@ def attention_masked(ctx, out, q, k, v, n_heads, n_kv_heads, offsets, *, scale=0
     off, n_seq = _offsets(ctx, offsets)
     mask = _lib.AttnMask(scale, softcap, _vec(ctx, "slopes", slopes, n_heads, torch.float32),
                          _vec(ctx, "doc_ids", doc_ids, rows, torch.int32),
-                         _vec(ctx, "prefix", prefix, n_seq, torch.int32), causal, window)
+                         _vec(ctx, "prefix", prefix, n_seq, torch.int32), causal, min(window, 2**31 - 1))
     _lib.check(ctx.lib.sg_attention_masked(ctx.handle, o, ldo, qp, ldq, kp, ldk, vp, ldv, _dtype(q), n_heads, n_kv_heads,
                                            hd, rows, off, n_seq, mask, _stream_of(ctx, stream)))
 

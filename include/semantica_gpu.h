@@ -341,7 +341,8 @@ int sg_pool_l2(sg_ctx *ctx, float *out, const float *x, int32_t ldx, int32_t out
  * threads or on several streams at once.  Rows of no sequence (before the first
  * or behind the last) are left as they were.  The contents of device arrays are
  * not checked; offsets outside 0 .. rows and ids that name nothing are never
- * followed out of the tensors.  Element types: */
+ * followed out of the tensors.  With no rows nothing is done, and the rows' tensors
+ * may be NULL.  Element types: */
 #define SG_F32 0
 #define SG_F16 1
 #define SG_BF16 2
@@ -383,8 +384,9 @@ int sg_attention_masked(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int6
  * x, h, sum, xn: [rows][cols] of type dtype with row strides in elements; w_post,
  * w_pre [cols] and gate float32.  d_seq_offsets NULL (n_seq 0): every row, one
  * gate [cols] for all.  Otherwise gate is [n_seq][cols], one for each sequence.
- * cols 1 .. 8192, rows and strides of any alignment (whole 16 bytes are
- * faster).  sum and xn may each be x or h (same pointer and stride); otherwise no
+ * cols 1 .. 8192, rows and strides of any whole elements (whole 16 bytes are
+ * faster).  The squares are summed in float32, as sg_rmsnorm's are: values past
+ * 2^63 overflow them.  sum and xn may each be x or h (same pointer and stride); otherwise no
  * output overlaps another tensor. */
 int sg_block_norm(sg_ctx *ctx, void *xn, int64_t ldxn, void *sum, int64_t lds, const void *x, int64_t ldx,
                   const void *h, int64_t ldh, int32_t dtype, int32_t rows, int32_t cols, const float *w_post,
@@ -413,8 +415,9 @@ int sg_adapters_work_bytes(const sg_adapter_bank *bank, int32_t rows, size_t *by
  * strides in elements, pointers 16-byte aligned, strides whole 16 bytes.  work:
  * sg_adapters_work_bytes of device memory, 16-byte aligned, in use until the
  * call's work on `stream` is done (one for each stream or graph that runs at the
- * same time).  dst does not overlap x, or base unless it is base.  The sums are
- * float32 and in the same order every time. */
+ * same time; a graph keeps its address, and the bank's).  dst does not overlap x,
+ * or base unless it is base; work overlaps none of them.  The sums are float32 and
+ * in the same order every time. */
 int sg_adapters_apply(sg_ctx *ctx, void *dst, int64_t ldd, const void *base, int64_t ldb, const sg_adapter_bank *bank,
                       const void *x, int64_t ldx, int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq,
                       const int32_t *d_adapter_ids, void *work, size_t work_bytes, void *stream);

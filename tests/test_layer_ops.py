@@ -490,6 +490,362 @@ def test_adapters_large_values_in_fp16(gpu_ctx):
     close(got, want, U["f16"] * want.abs() + (600 * F + 2.0 ** -16) * size + TINY["f16"], "adapters")
 
 
+# ---- what else may be in the tensors, and how else they may be called --------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("big", [1e4, 1e30])
+def test_attention_ignores_large_hidden_contents(gpu_ctx, dtype, hd, big):
+    """Finite values far above a query's own in what it does not see: padding first in its
+    sequence, and later keys that grow."""
+    if dtype == "f16" and big > 6e4:
+        pytest.skip("past the type's range")
+    for rows in (90, 2000):
+        g, off = gen(21), offsets([rows])
+        q, k, v = (rand(g, rows, c * hd, dtype=dtype) for c in (6, 2, 2))
+        ids = torch.zeros(rows, dtype=torch.int32)
+        ids[:33] = -1
+        k[:33], v[:33] = big, -big
+        k[70], v[70, ::2] = big, big
+        v[80] = 0
+        kw = {"doc_ids": ids, "causal": True}
+        say("large hidden", dtype, hd, big, rows)
+        got = run_attention(gpu_ctx, q, k, v, off, 6, 2, **kw)
+        want, mean, size = attention_ref(q[:70], k[:70], v[:70], offsets([70]), 6, 2, doc_ids=ids[:70], causal=True)
+        close(got[:70], want, attention_tol(dtype, hd, want, mean, size), "attention")
+        assert bool((got[:33] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 256])
+def test_attention_values_that_grow_and_fade(gpu_ctx, hd):
+    """Causal float32 rows whose values rise, then fall, by tens of powers of ten."""
+    g, off = gen(22), offsets([300, 300])
+    q, k, v = rand(g, 600, hd), rand(g, 600, hd), rand(g, 600, hd)
+    v[:300] *= (10.0 ** torch.linspace(-30, 30, 300))[:, None]
+    v[300:] *= (10.0 ** torch.linspace(30, -30, 300))[:, None]
+    for kw in ({"causal": True}, {"window": 3}):
+        got = run_attention(gpu_ctx, q, k, v, off, 1, 1, **kw)
+        want, mean, size = attention_ref(q, k, v, off, 1, 1, **kw)
+        close(got, want, attention_tol("f32", hd, want, mean, size), "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cap", [1e-3, 0.3, 50.0, 55.0, 60.0, 3e4, 1e6, 1e30])
+def test_attention_caps_of_any_size(gpu_ctx, dtype, cap):
+    """tanh from saturation to the identity, and queries whose scores all lie at the cap's
+    lower end over values of any size."""
+    g, off = gen(23), offsets([70, 40])
+    q, k, v = rand(g, 110, 128, by=6.0, dtype=dtype), rand(g, 110, 128, dtype=dtype), rand(g, 110, 128, dtype=dtype)
+    q[5], k[:70, :64] = -200.0, k[:70, :64].abs() + 1  # a row of the lowest scores
+    for by in (1.0,) if dtype == "f16" else (1.0, 1e-20):
+        vs = (v.float() * by).to(v.dtype)
+        got = run_attention(gpu_ctx, q, k, vs, off, 2, 2, softcap=cap)
+        want, mean, size = attention_ref(q, k, vs, off, 2, 2, softcap=cap)
+        # (A score off by d ahead of the cap is off by d at most behind it.)
+        close(got, want, attention_tol(dtype, 64, want, mean, size, min(cap, float(size.max()))), "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads", [(8, 8), (16, 2), (24, 8)])
+def test_attention_heads_dealt_over_the_xcds(gpu_ctx, dtype, heads, kv_heads):
+    check_attention(gpu_ctx, 24, dtype, heads, kv_heads, 64, [3, 200, 131], causal=True)
+    check_attention(gpu_ctx, 25, dtype, heads, kv_heads, 64, [1] * 40 + [700])
+
+
+@pytest.mark.gpu
+def test_attention_long_documents_scan(gpu_ctx):
+    """More tiles than one look at the document ids covers, a document in two halves far apart."""
+    rows, hd = 140001, 8
+    g = gen(26)
+    q, k, v = (rand(g, rows, hd, dtype="f16") for _ in range(3))
+    ids = (torch.arange(rows) // 37 + 1).to(torch.int32)
+    ids[:20] = 0
+    ids[-21:] = 0
+    got = run_attention(gpu_ctx, q, k, v, offsets([rows]), 1, 1, doc_ids=ids)
+    for doc in (0, 1, 500, 1891, 3782, int(ids.max())):
+        at = (ids == doc).nonzero()[:, 0]
+        want, mean, size = attention_ref(q[at], k[at], v[at], offsets([len(at)]), 1, 1)
+        close(got[at], want, attention_tol("f16", hd, want, mean, size), f"document {doc}")
+
+
+def layer_calls(ctx, dtype="bf16", seed=0):
+    """Each operator once, over buffers of its own: [(name, call(stream), inputs, outputs)]."""
+    from semantica_gpu import kernels
+    g, off = gen(seed), offsets([40, 0, 1, 90, 300], first=3)
+    rows, offd = 440, offsets([40, 0, 1, 90, 300], first=3).cuda()
+    assert int(off[-1]) <= rows
+    t = lambda cols, by=1.0: rand(g, rows, cols, by=by, dtype=dtype).cuda()
+    q, k, v, o = t(512), t(128), t(128), t(512)
+    ids = torch.tensor([0, 1, -1, 2, 1], dtype=torch.int32).cuda()
+    a, b = rand(g, 3, 16, 512, by=0.05, dtype=dtype).cuda(), rand(g, 3, 768, 16, dtype=dtype).cuda()
+    bank = kernels.AdapterBank(ctx, a, b, torch.tensor([0.5, 1.0, 2.0]).cuda())
+    base, dst = t(768), t(768)
+    work = torch.empty(bank.work_bytes(rows), dtype=torch.uint8, device="cuda")
+    x, h, s, n = t(768, 3.0), t(768), t(768), t(768)
+    wp, wn, gate = (torch.randn(*z, generator=g).cuda() for z in ((768,), (768,), (5, 768)))
+    slopes = torch.rand(4, generator=g).cuda()
+    torch.cuda.synchronize()
+    return [
+        ("attention", lambda stream=None: kernels.attention_masked(ctx, o, q, k, v, 4, 1, offd, softcap=8.0, slopes=slopes,
+                                                                   causal=True, stream=stream), [q, k, v], [o]),
+        ("adapters", lambda stream=None: kernels.adapters_apply(ctx, dst, base, bank, q, offd, ids, work=work, stream=stream),
+         [q, base], [dst]),
+        ("norm", lambda stream=None: kernels.block_norm(ctx, n, s, x, h, wp, wn, 1e-6, gate=gate, offsets=offd, stream=stream),
+         [x, h], [s, n])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_replayed_graphs_equal_eager_calls(gpu_ctx, dtype):
+    """One graph of all three operators, replayed with new inputs, eager calls and
+    synchronizations between; a second graph with its own workspace beside it."""
+    sets = [layer_calls(gpu_ctx, dtype, seed) for seed in (1, 2)]
+    graphs = []
+    for calls in sets:
+        for _, call, _, _ in calls:
+            call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        say("capturing", dtype)
+        with torch.cuda.graph(graph):
+            for _, call, _, _ in calls:
+                call()
+        graphs.append(graph)
+    for rep in range(4):
+        for calls, graph in zip(sets, graphs):
+            say("replay", rep)
+            for _, _, ins, outs in calls:
+                for t in ins:
+                    t.copy_(torch.randn(t.shape, generator=gen(rep)).to(t.dtype))
+                for t in outs:
+                    t.fill_(7.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for _, _, _, outs in calls for t in outs]
+            for _, call, _, outs in calls:
+                for t in outs:
+                    t.fill_(7.0)
+                call()
+            torch.cuda.synchronize()
+            want = [t for _, _, _, outs in calls for t in outs]
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_calls_from_two_threads_on_two_streams(gpu_ctx):
+    """Two threads, each on a stream of its own with outputs and workspace of its own."""
+    import threading
+    sets = [layer_calls(gpu_ctx, "f32", 5), layer_calls(gpu_ctx, "bf16", 6)]
+    alone = []
+    for calls in sets:
+        for _, call, _, _ in calls:
+            call()
+        torch.cuda.synchronize()
+        alone.append([t.clone() for _, _, _, outs in calls for t in outs])
+    streams = [torch.cuda.Stream() for _ in sets]
+    wrong = []
+
+    def work(i):
+        try:
+            for _ in range(20):
+                for _, call, _, _ in sets[i]:
+                    call(streams[i].cuda_stream)
+            streams[i].synchronize()
+        except Exception as e:  # pragma: no cover
+            wrong.append(e)
+
+    for calls in sets:
+        for _, _, _, outs in calls:
+            for t in outs:
+                t[3:434] = 0
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    for calls, want in zip(sets, alone):
+        for a, b in zip([t for _, _, _, outs in calls for t in outs], want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_no_rows_and_empty_sequences(gpu_ctx, dtype):
+    """No rows, no sequence with a row, and rows before and behind the only one."""
+    from semantica_gpu import kernels
+    check_attention(gpu_ctx, 31, dtype, 2, 1, 64, [0, 0, 0], first=2, behind=5)
+    check_attention(gpu_ctx, 32, dtype, 2, 1, 64, [1], causal=True)
+    check_attention(gpu_ctx, 33, dtype, 2, 1, 64, [0, 1, 0], first=1, behind=1, window=1)
+    check_norm(gpu_ctx, dtype, 4, 768, lens=[0, 0], first=2, gate=True)
+    check_adapters(gpu_ctx, dtype, 64, 64, 8, 2, [0, 0, 0], first=2, behind=5)
+    none = torch.empty(0, 64, dtype=dt(dtype), device="cuda")
+    off, ids = offsets([0, 0]).cuda(), torch.zeros(2, dtype=torch.int32, device="cuda")
+    kernels.attention_masked(gpu_ctx, none, none, none, none, 1, 1, off)
+    kernels.block_norm(gpu_ctx, none, none, none, none, None, torch.ones(64, device="cuda"), 1e-6, offsets=off)
+    bank = kernels.AdapterBank(gpu_ctx, torch.zeros(1, 8, 64, dtype=dt(dtype), device="cuda"),
+                               torch.zeros(1, 64, 8, dtype=dt(dtype), device="cuda"), torch.ones(1, device="cuda"))
+    kernels.adapters_apply(gpu_ctx, none, none, bank, none, off, ids)
+    bank.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_single_row_of_a_wider_tensor(gpu_ctx, dtype):
+    """A single row's stride does not matter, whatever the tensor that it is cut from."""
+    from semantica_gpu import kernels
+    wide = torch.randn(2, 203, device="cuda").to(dt(dtype))
+    q = wide[:1, 8:136]
+    out = torch.empty(1, 128, dtype=dt(dtype), device="cuda")
+    kernels.attention_masked(gpu_ctx, out, q, q, q, 2, 2, offsets([1]).cuda())
+    # One key, weight 1: its value.  float32 values are held as two halves of 11 bits, off by
+    # 2^-11 of 2^-11 at most (2^-37 of the row's largest where the second is subnormal), and
+    # the division and the scaling back are four roundings; 16-bit values pass unchanged.
+    tol = 2.0 ** -21 * q.abs() + 2.0 ** -37 * q.abs().max() if dtype == "f32" else 0.0 * q.abs()
+    close(out, q.double().cpu(), tol.double().cpu(), "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("off", [[5, 2, 9, 1], [-7, 400, 3, 1 << 30], [-(1 << 31), (1 << 31) - 1, 0, 64], [64, 64, 64, 64]])
+def test_offsets_and_ids_that_make_no_sense(gpu_ctx, off):
+    """Whatever device arrays hold, nothing outside the tensors is touched (every index
+    that is formed from them is clamped)."""
+    from semantica_gpu import kernels
+    rows = 64
+    wide = [torch.full((rows + 2, 144), 7.0, device="cuda") for _ in range(3)]
+    o, s, n = (w[1:-1, 8:136] for w in wide)
+    q = torch.randn(rows, 128, device="cuda")
+    offd = torch.tensor(off, dtype=torch.int64).to(torch.int32).cuda()
+    ids = torch.tensor([-9, 1 << 30, 3], dtype=torch.int32).cuda()
+    docs = torch.randint(-(1 << 31), (1 << 31) - 1, (rows,), generator=gen(1)).to(torch.int32).cuda()
+    say("offsets", off)
+    kernels.attention_masked(gpu_ctx, o, q, q, q, 2, 2, offd, causal=True, prefix=ids, doc_ids=docs)
+    torch.cuda.synchronize()
+    kernels.block_norm(gpu_ctx, n, s, q, q, None, torch.ones(128, device="cuda"), 1e-6,
+                       gate=torch.ones(3, 128, device="cuda"), offsets=offd)
+    torch.cuda.synchronize()
+    bank = kernels.AdapterBank(gpu_ctx, torch.ones(2, 8, 128, device="cuda"), torch.ones(2, 128, 8, device="cuda"),
+                               torch.ones(2, device="cuda"))
+    kernels.adapters_apply(gpu_ctx, o, q, bank, q, offd, ids)
+    torch.cuda.synchronize()
+    bank.close()
+    for w in wide:
+        assert bool((w[0] == 7).all()) and bool((w[-1] == 7).all())
+        assert bool((w[:, :8] == 7).all()) and bool((w[:, 136:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits(gpu_ctx):
+    """Rows that lie more than 2^32 bytes and 2^31 elements into their tensors."""
+    from semantica_gpu import kernels
+    rows, ld = 600, 1 << 22
+    g, off = gen(41), offsets([rows])
+    wide = torch.empty(rows, ld, dtype=torch.float16, device="cuda")
+    cols = {n: rand(g, rows, 64, dtype="f16") for n in ("q", "k", "v", "h")}
+    at = {n: wide[:, 64 * i:64 * i + 64] for i, n in enumerate(cols)}
+    for n, t in cols.items():
+        at[n].copy_(t.cuda())
+    far = torch.empty(rows, ld, dtype=torch.float16, device="cuda")[:, 8:72]
+    say("attention, strides of 2^22")
+    kernels.attention_masked(gpu_ctx, far, at["q"], at["k"], at["v"], 1, 1, off.cuda())
+    want, mean, size = attention_ref(cols["q"], cols["k"], cols["v"], off, 1, 1)
+    close(far, want, attention_tol("f16", 64, want, mean, size), "attention")
+    say("norm")
+    w = torch.randn(64, generator=g)
+    xn = torch.empty(rows, 64, dtype=torch.float16, device="cuda")
+    kernels.block_norm(gpu_ctx, xn, far, at["q"], at["h"], w.cuda(), w.cuda(), 1e-6)
+    s, n, ssize, nsize = norm_ref(cols["q"], cols["h"], w, w, 1e-6, None, 1.0, None)
+    close(far, s, U["f16"] * s.abs() + 42 * F * ssize + TINY["f16"], "sum")
+    close(xn, n, U["f16"] * n.abs() + 84 * F * nsize + TINY["f16"], "xn")
+    say("adapters")
+    a, b = rand(g, 2, 8, 64, by=0.1, dtype="f16"), rand(g, 2, 64, 8, dtype="f16")
+    scales, ids = torch.tensor([0.5, 2.0]), torch.tensor([1], dtype=torch.int32)
+    bank = kernels.AdapterBank(gpu_ctx, a.cuda(), b.cuda(), scales.cuda())
+    kernels.adapters_apply(gpu_ctx, far, at["h"], bank, at["q"], off.cuda(), ids.cuda())
+    want, size = adapters_ref(cols["q"], cols["h"], a, b, scales, off, ids)
+    close(far, want, U["f16"] * want.abs() + (104 * F + 2.0 ** -16) * size + TINY["f16"], "adapters")
+    bank.close()
+
+
+@pytest.mark.gpu
+def test_a_layer_with_adapters(gpu_ctx):
+    """The operators as one layer uses them, around the Q8_0 products: queries and keys from
+    shared weights with a low-rank change for each request, normed and rotated, masked attention,
+    the output product with its own adapters, the residual step.  Each result is checked
+    against its definition on what came before it."""
+    from semantica_gpu import kernels, synth
+    lens, hidden, heads, kv_heads, hd = [1, 37, 300, 2, 90], 768, 3, 1, 256
+    g, rng = gen(51), np.random.default_rng(51)
+    off, host_off = offsets(lens), np.concatenate([[0], np.cumsum(lens)])
+    rows, offd = int(off[-1]), offsets(lens).cuda()
+    x, h = rand(g, rows, hidden).cuda(), rand(g, rows, hidden).cuda()
+    ids = torch.tensor([0, -1, 2, 1, 0], dtype=torch.int32)
+    scales = torch.tensor([0.5, 1.0, 2.0])
+
+    def product(t, n):
+        """t @ w of Q8_0 weights, the shared part of a projection; and adapters for it."""
+        k = t.shape[1]
+        w = kernels.Q8Weight(gpu_ctx, synth.q8_0_random(rng, n, k), n, k)
+        q = torch.empty(t.shape, dtype=torch.int8, device="cuda")
+        scale, y = torch.empty(len(lens), device="cuda"), torch.empty(rows, n, device="cuda")
+        kernels.quantize_symmetric_int8(gpu_ctx, t, host_off, q, scale)
+        kernels.matmul_q8_0(gpu_ctx, y, w, q, scale.repeat_interleave(torch.tensor(lens, device="cuda")))
+        shared = y.cpu()
+        a, b = rand(g, 3, 16, k, by=k ** -0.5), rand(g, 3, n, 16)
+        bank = kernels.AdapterBank(gpu_ctx, a.cuda(), b.cuda(), scales.cuda())
+        kernels.adapters_apply(gpu_ctx, y, y, bank, t, offd, ids.cuda())
+        want, size = adapters_ref(t.cpu(), shared, a, b, scales, off, ids)
+        close(y, want, U["f32"] * want.abs() + (k + 48) * F * size + TINY["f32"], "adapters")
+        bank.close()
+        w.close()
+        return y
+
+    q, k, v = product(x, heads * hd), product(x, kv_heads * hd), product(x, kv_heads * hd)
+    one = torch.ones(hd, device="cuda")
+    kernels.qknorm_rope(gpu_ctx, q, k, one, one, heads, kv_heads, hd, 1e-6, 10000.0, 2048, host_off)
+    o = torch.empty(rows, heads * hd, device="cuda")
+    kw = {"softcap": 20.0, "causal": True, "window": 128}
+    kernels.attention_masked(gpu_ctx, o, q, k, v, heads, kv_heads, offd, **kw)
+    want, mean, size = attention_ref(q.cpu(), k.cpu(), v.cpu(), off, heads, kv_heads, **kw)
+    close(o, want, attention_tol("f32", hd, want, mean, size, 20.0), "attention")
+    y = product(o, hidden)
+    wp, wn, gate = (torch.randn(*z, generator=g) for z in ((hidden,), (hidden,), (len(lens), hidden)))
+    before, xn = h.cpu(), torch.empty_like(h)
+    kernels.block_norm(gpu_ctx, xn, h, y, h, wp.cuda(), wn.cuda(), 1e-6, gate=gate.cuda(), offsets=offd)
+    seq = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens))
+    s, n, ssize, nsize = norm_ref(y.cpu(), before, wp, wn, 1e-6, gate, 1.0, seq)
+    rel = (hidden / 2 + 10) * F
+    close(h, s, U["f32"] * s.abs() + rel * ssize, "sum")
+    close(xn, n, U["f32"] * n.abs() + 2 * rel * nsize, "xn")
+
+
+@pytest.mark.gpu
+def test_adapters_work_refusals(gpu_ctx):
+    from semantica_gpu import SemanticaError, kernels
+    bank = kernels.AdapterBank(gpu_ctx, torch.zeros(1, 8, 64, device="cuda"), torch.zeros(1, 64, 8, device="cuda"),
+                               torch.ones(1, device="cuda"))
+    x, off, ids = torch.zeros(32, 64, device="cuda"), offsets([32]).cuda(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    need = bank.work_bytes(32)
+    dst, big = torch.zeros(32, 64, device="cuda"), torch.zeros(need + 64, dtype=torch.uint8, device="cuda")
+    kernels.adapters_apply(gpu_ctx, dst, x, bank, x, off, ids, work=big[:need])
+    inside = torch.zeros(32 * 64 + need, device="cuda")
+    for work, to, word in ((big[:need - 1], dst, "bytes"), (big[8:], dst, "aligned"), (big[:0], dst, "bytes"),
+                           (inside.view(torch.uint8), inside[:2048].view(32, 64), "work overlaps"), (big, x, "overlaps x")):
+        with pytest.raises(SemanticaError, match=word):
+            kernels.adapters_apply(gpu_ctx, to, dst if to is x else x, bank, x, off, ids, work=work)
+    bank.close()
+    with pytest.raises(SemanticaError, match="NULL"):
+        kernels.adapters_apply(gpu_ctx, dst, x, bank, x, off, ids, work=big)
+
+
 # ---- refusals (no device is touched) -----------------------------------------------
 
 
@@ -538,7 +894,8 @@ NORM = dict(xn=1 << 40, ldxn=64, sum=2 << 40, lds=64, x=3 << 40, ldx=64, h=4 << 
     ({"dtype": -1}, "element type"), ({"cols": 0}, "cols"), ({"cols": 8193}, "cols"), ({"rows": -1}, "rows"),
     ({"eps": -1.0}, "eps"), ({"eps": math.nan}, "eps"), ({"scale": math.inf}, "scale"), ({"n_seq": 1}, "n_seq"),
     ({"off": 7 << 40}, "seq_offsets"), ({"ldx": 63}, "stride"), ({"sum": 1 << 40}, "overlaps"),
-    ({"sum": (4 << 40) + 4}, "overlaps"), ({"xn": 3 << 40, "ldxn": 65}, "overlaps")])
+    ({"sum": (4 << 40) + 4}, "overlaps"), ({"xn": 3 << 40, "ldxn": 65}, "overlaps"), ({"x": (3 << 40) + 2}, "aligned"),
+    ({"dtype": 2, "h": (4 << 40) + 1}, "aligned")])
 def test_norm_refusals(change, word):
     from semantica_gpu import _lib
     c = {**NORM, **change}
@@ -570,3 +927,67 @@ def test_adapters_null_arguments():
     _refused(lib.sg_adapters_work_bytes(None, 1, ctypes.byref(size)), "NULL")
     _refused(lib.sg_adapters_apply(_addr(), 1, 8, 1, 8, None, 1, 8, 1, 1, 1, 1, 1, 1, None), "NULL")
     lib.sg_adapter_bank_free(None)
+
+
+def test_no_rows_need_no_tensors():
+    from semantica_gpu import _lib
+    lib = _lib.load()
+    assert lib.sg_attention_masked(_addr(), None, 64, None, 64, None, 64, None, 64, 0, 1, 1, 64, 0, 1, 1, None, None) == 0
+    assert lib.sg_block_norm(_addr(), None, 0, None, 64, None, 64, None, 64, 0, 0, 64, None, None, 1e-6, None, 1.0, None, 0,
+                             None) == 0
+
+
+class _Ctx:  # tensors in host memory count as this one's device, so that only the later checks refuse them
+    device = -1
+
+    def __init__(self):
+        from semantica_gpu import _lib
+        self.lib, self.handle = _lib.load(), _addr()
+
+
+@pytest.mark.parametrize("change,word", [
+    ({"q": (10, 130)}, "columns for 4 heads"), ({"k": (10, 16)}, "k: shape"), ({"v": (9, 32)}, "v: shape"),
+    ({"out": (10, 136)}, "out: shape"), ({"k": "half"}, "k: torch.float16 beside"), ({"v": "turned"}, "contiguous"),
+    ({"q": "long"}, "float32, float16 or bfloat16"), ({"slopes": (3,)}, "slopes: 4"), ({"doc_ids": (9,)}, "doc_ids"),
+    ({"prefix": (2,)}, "prefix"), ({"offsets": "long"}, "offsets")])
+def test_attention_wrapper_refusals(change, word):
+    from semantica_gpu import kernels
+    shapes = {"out": (10, 128), "q": (10, 128), "k": (10, 32), "v": (10, 32), "offsets": (2,)}
+    kw = {}
+    for n, to in {**shapes, **change}.items():
+        t = torch.zeros(shapes.get(n, to) if isinstance(to, str) else to)
+        if n in ("offsets", "doc_ids", "prefix"):
+            t = t.to(torch.int32)
+        if to == "half":
+            t = t.half()
+        if to == "long":
+            t = t.long()
+        if to == "turned":
+            t = torch.zeros(t.shape[::-1]).t()
+        kw[n] = t
+    if change.get("q") == "long":
+        for n in ("out", "k", "v"):
+            kw[n] = kw[n].long()
+    args = [kw.pop(n) for n in ("out", "q", "k", "v")]
+    with pytest.raises(ValueError, match=word):
+        kernels.attention_masked(_Ctx(), *args, 4, 1, kw.pop("offsets"), **kw)
+
+
+def test_wrappers_refuse_other_devices_and_shapes():
+    from semantica_gpu import kernels
+    ctx, t, w = _Ctx(), torch.zeros(4, 64), torch.zeros(64)
+    with pytest.raises(ValueError, match="w_post"):
+        kernels.block_norm(ctx, None, t, t, t, torch.zeros(63), None, 1e-6)
+    with pytest.raises(ValueError, match="gate"):
+        kernels.block_norm(ctx, None, t, t, t, w, None, 1e-6, gate=w, offsets=torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="h: shape"):
+        kernels.block_norm(ctx, None, t, t, t[:3], w, None, 1e-6)
+    with pytest.raises(ValueError, match="b: shape"):
+        kernels.AdapterBank(ctx, torch.zeros(2, 8, 64), torch.zeros(2, 64, 4), torch.zeros(2))
+    with pytest.raises(ValueError, match="scales"):
+        kernels.AdapterBank(ctx, torch.zeros(2, 8, 64), torch.zeros(2, 64, 8), torch.zeros(3))
+    ctx.device = 0
+    with pytest.raises(ValueError, match="device"):
+        kernels.block_norm(ctx, None, t, t, t, w, None, 1e-6)
+    with pytest.raises(ValueError, match="device"):
+        kernels.attention_masked(ctx, t, t, t, t, 1, 1, torch.zeros(2, dtype=torch.int32))

@@ -949,26 +949,28 @@ hipError_t launch(const sg_attn_masked_args& a, hipStream_t s) {
 }
 
 // Which form: waves that share 32 rows as long as a workgroup for each 32 rows and head
-// fits the GPU at once (one to a CU, two for 64 dims), else waves of their own rows.
-// Whole sequences of 512, 12 heads, microseconds of the shared and the own form:
+// fits the GPU at once (one to a CU; two of the 16-bit types' four waves of 64 dims),
+// else waves of their own rows.  Whole sequences of 512, 12 heads, microseconds of the
+// shared and the own form:
 //                    512 rows          1024              2048
 //   bf16, 64 dims     8   13           10   13           16   13
 //   bf16, 128        11   19           21   17           32   19
 //   bf16, 256        18   33           36   33           57   35
-//   float32, 64      21   34           28   35           44   38
-//   float32, 128     29   36           56   37           86   40
+//   float32, 64      18   35           33   36           48   38
+//   float32, 128     24   36           47   37           71   40
 //   float32, 256     49   70           98   70          147   75
-// (512 rows are 192 such workgroups.)  float32 rows of their own are 16 to a wave above
-// 64 dims, so that they stay in registers (16384 rows: 150 us against 189 with 32 rows
-// at 128 dims, 230 against 263 at 256; 64 dims: 130 against 125).
+// (512 rows are 192 such workgroups.)  float32 rows are 16 to a wave above 64 dims, so
+// that they stay in registers (own form, 16384 rows: 150 us against 189 with 32 rows at
+// 128 dims, 230 against 263 at 256; 64 dims: 130 against 125).  Its shared form has
+// eight waves to split a tile's halving between, where LDS holds tiles that wide: 32
+// rows of 128 dims 11.2 us, 12.9 with four; 256 dims take four.
 template <typename T, int D>
 hipError_t by_form(const sg_attn_masked_args& a, hipStream_t s) {
   constexpr bool F32 = __is_same(T, float);
-  const bool share = ((int64_t)a.rows + 31) / 32 * a.heads <= (D == 64 ? 512 : 256);
-  if constexpr (F32 && D == 256) {
-    return share ? launch<T, D, 16, 2, 2>(a, s) : launch<T, D, 16, 8, 1>(a, s);
-  } else if constexpr (F32 && D == 128) {
-    return share ? launch<T, D, 32, 1, 4>(a, s) : launch<T, D, 16, 8, 1>(a, s);
+  const bool share = ((int64_t)a.rows + 31) / 32 * a.heads <= (D == 64 && !F32 ? 512 : 256);
+  if constexpr (F32) {
+    constexpr int OWN = D == 64 ? 32 : 16;
+    return share ? launch<T, D, 16, 2, D == 256 ? 2 : 4>(a, s) : launch<T, D, OWN, 128 / OWN, 1>(a, s);
   } else {
     return share ? launch<T, D, 32, 1, 4>(a, s) : launch<T, D, 32, 4, 1>(a, s);
   }

@@ -85,7 +85,7 @@ __device__ __forceinline__ void list_ids(int id, tile_ids<ROWS>& t, int lane) {
   int n = 0;
   uint64_t left = __ballot(lane < ROWS && id >= 0);
   while (left) {
-    const int pick = __builtin_amdgcn_readfirstlane(__shfl(id, __builtin_ctzll(left)));
+    const int pick = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
     const uint64_t its = __ballot(lane < ROWS && id == pick);
     int bits = 0;
 #pragma unroll
@@ -303,7 +303,14 @@ __global__ __launch_bounds__(kNT) void k_adapter_up(sg_adapters_args a, int part
       const int c = (tid % TPR + k * TPR) * 4;
       s[k] = f32x4_t{0, 0, 0, 0};
       if (c < a.rank_pad)
-        for (int p = 0; p < parts; p++) s[k] += *reinterpret_cast<const f32x4_t*>(u + (int64_t)p * a.rows * a.rank_pad + c);
+        for (int p = 0; p < parts; p += 8) {  // eight loads in flight; their sum in order
+          f32x4_t t[8] = {};
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (p + i < parts) t[i] = *reinterpret_cast<const f32x4_t*>(u + (int64_t)(p + i) * a.rows * a.rank_pad + c);
+#pragma unroll
+          for (int i = 0; i < 8; i++) s[k] += t[i];
+        }
     }
     rid = tid < ROWS && row0 + tid < a.rows ? a.row_ids[row0 + tid] : kNoRow;
   };

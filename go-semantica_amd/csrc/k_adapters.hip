@@ -176,8 +176,11 @@ __global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int pa
     x[r] = static_cast<const T*>(a.x) + (int64_t)min(row0 + r * kTile + n, a.rows - 1) * a.ldx + g * V;
   // U steps' loads go out before their products (the compiler does not unroll loops
   // with matrix instructions); a step past the wave's last is zeros.  The first of
-  // x go out before the rows' adapters are known.
-  constexpr int U = RT * NRB <= 2 ? 8 : RT * NRB <= 4 ? 4 : 2;
+  // x go out before the rows' adapters are known.  Eight steps for one tile of one
+  // block, whose waves are few; four else, so that four waves fit a SIMD and all of a
+  // batch's workgroups are resident (30725 float32 rows of 768: 34 us, 44 with eight,
+  // 35 with two; the next steps' x ahead of the products instead: 37 to 45).
+  constexpr int U = RT * NRB == 1 ? 8 : 4;
   chunk<T> xf[U][RT];
   auto load_x = [&](int k, int tiles) {
 #pragma unroll

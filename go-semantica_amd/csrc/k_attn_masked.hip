@@ -35,8 +35,8 @@
 // visible keys only (careful_row).  That also covers float32 values past the
 // fp16 halves' reach (q and k above 2^113, values 2^53 times the first keys').
 //
-// Two forms (by_form has the rule): waves with 32 (16) rows of their own, 128 to a
-// workgroup, or, for batches with too few rows to fill the GPU, waves that share 32
+// Two forms (by_form has the rule): waves with 32 (16) rows of their own, 128 (64) to
+// a workgroup, or, for batches with too few rows to fill the GPU, waves that share 32
 // rows and split each tile's keys between them, joined through LDS at the end.
 #include <algorithm>
 
@@ -246,7 +246,8 @@ struct form {
   static constexpr int BK = kSub * KW * NSUB, BM = QT * RW;
   static constexpr int HALF = BK * D * 2;             // bytes of one tile's K (or V), one part
   static constexpr int TILE = 2 * PARTS * HALF;       // K and V
-  static constexpr int STAGES = (!F32 || KW == 1) && 2 * TILE <= (128 << 10) ? 2 : 1;
+  // float32 rows of 64 dims hold no tile ahead: its registers are a third workgroup's.
+  static constexpr int STAGES = (!F32 || (KW == 1 && D != 64)) && 2 * TILE <= (128 << 10) ? 2 : 1;
   static constexpr int KEYS = F32 ? STAGES * 3 * BK * 4 : 0;  // per-key powers of a float32 tile
   static constexpr int JOIN = KW > 1 ? NW * QT * D * 4 : 0;
   static constexpr int LDS = (STAGES * TILE + KEYS) > JOIN ? (STAGES * TILE + KEYS) : JOIN;
@@ -959,18 +960,19 @@ hipError_t launch(const sg_attn_masked_args& a, hipStream_t s) {
 //   float32, 64      18   35           33   36           48   38
 //   float32, 128     24   36           47   37           71   40
 //   float32, 256     49   70           98   70          147   75
-// (512 rows are 192 such workgroups.)  float32 rows are 16 to a wave above 64 dims, so
-// that they stay in registers (own form, 16384 rows: 150 us against 189 with 32 rows at
-// 128 dims, 230 against 263 at 256; 64 dims: 130 against 125).  Its shared form has
-// eight waves to split a tile's halving between, where LDS holds tiles that wide: 32
-// rows of 128 dims 11.2 us, 12.9 with four; 256 dims take four.
+// (512 rows are 192 such workgroups.)  float32 rows are 16 to a wave, so that they stay
+// in registers (own form, 16384 rows: 150 us against 189 with 32 rows at 128 dims, 230
+// against 263 at 256), eight waves to a workgroup that halves a tile once for them all,
+// or four at 64 dims, where three workgroups of one tile stage fit a CU (116 us; two
+// stages 139; eight waves 130; four of 32 rows 125).  The shared form has eight waves
+// to split a tile's halving between, where LDS holds tiles that wide: 32 rows of 128
+// dims 11.2 us, 12.9 with four; 256 dims take four.
 template <typename T, int D>
 hipError_t by_form(const sg_attn_masked_args& a, hipStream_t s) {
   constexpr bool F32 = __is_same(T, float);
   const bool share = ((int64_t)a.rows + 31) / 32 * a.heads <= (D == 64 && !F32 ? 512 : 256);
   if constexpr (F32) {
-    constexpr int OWN = D == 64 ? 32 : 16;
-    return share ? launch<T, D, 16, 2, D == 256 ? 2 : 4>(a, s) : launch<T, D, OWN, 128 / OWN, 1>(a, s);
+    return share ? launch<T, D, 16, 2, D == 256 ? 2 : 4>(a, s) : launch<T, D, 16, D == 64 ? 4 : 8, 1>(a, s);
   } else {
     return share ? launch<T, D, 32, 1, 4>(a, s) : launch<T, D, 32, 4, 1>(a, s);
   }

@@ -35,6 +35,26 @@
 // visible keys only (careful_row).  That also covers float32 values past the
 // fp16 halves' reach (q and k above 2^113, values 2^53 times the first keys').
 //
+// What bounds it.  A SIMD's matrix and vector instructions do not overlap here (their
+// busy cycles add up to 94 % of 4 x 4096 bf16 tokens' time: 35 + 59), and a score costs
+// an exponential (16 cycles of a wave; a multiplication 2.6) and five to eight other
+// vector instructions beside 4 head_dim flops.  So few of them per score is what the code
+// goes for: the range check once a tile and wave, bf16 under a cap without a maximum,
+// tanh as a polynomial, the sum of weights as a dot product of the packed ones.  Measured
+// (us, and the rate of the visible pairs' 4 head_dim flops):
+//   4 x 4096, bf16, causal, cap, 32 heads over 8 of 128            691   796 TFLOP/s
+//   8 of 1024 .. 2048, fp16, causal, prefix, 16 over 8 of 128      152   640
+//   16391 rows, documents of 900, bf16, distance bias, 12 of 64    161   312
+//   64 x 512, float32, window of 256, 3 over 1 of 256              217   178
+// float32 (three products each; 372 TFLOP/s is the matrix cores' limit) waits about
+// half its time: a workgroup's eight waves load, halve, multiply in step, and no second
+// one fits beside two stages of its tiles (two workgroups of 64 rows and one stage each:
+// 265 us).  Its LDS reads of V meet two-way conflicts with 16 queries; a xor of three
+// bits that avoids them costs more in addresses (241 us against 236).  Tried as well:
+// eight 32-row waves a workgroup (4 x 4096 683 us for 697, but documents 213 for 162),
+// causal tiles sorted by length (193 for 171 at the prefix case: L2 locality lost), the
+// bias as the products' start value (175 for 163), s_setprio round the products (equal).
+//
 // Two forms (by_form has the rule): waves with 32 (16) rows of their own, 128 (64) to
 // a workgroup, or, for batches with too few rows to fill the GPU, waves that share 32
 // rows and split each tile's keys between them, joined through LDS at the end.
@@ -957,7 +977,7 @@ hipError_t launch(const sg_attn_masked_args& a, hipStream_t s) {
 //   bf16, 64 dims     8   13           10   13           16   13
 //   bf16, 128        11   19           21   17           32   19
 //   bf16, 256        18   33           36   33           57   35
-//   float32, 64      18   35           33   36           48   38
+//   float32, 64      18   25           33   26           50   35
 //   float32, 128     24   36           47   37           71   40
 //   float32, 256     49   70           98   70          147   75
 // (512 rows are 192 such workgroups.)  float32 rows are 16 to a wave, so that they stay

@@ -400,7 +400,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
     if (a.window > 0) {
       const int wd = min(a.window, a.rows);
       me.lo = max(me.lo, rc - wd + 1);
-      me.hi = min(me.hi, rc + wd);
+      me.hi = min(me.hi, rc + min(wd, a.rows - rc));
     }
     me.doc = a.docs ? a.docs[rc] : 0;
     if (!me.live || me.doc < 0) {

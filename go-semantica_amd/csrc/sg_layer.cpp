@@ -75,6 +75,7 @@ int check_pieces(const char* name, const Span& t) {
 int check_batch(const int32_t* d_off, int rows, int n_seq) {
   if (rows < 0 || rows > kMostRows) return fail(SG_ERR_INVALID, "rows %d out of range (0..%d)", rows, kMostRows);
   if (!d_off || n_seq <= 0) return fail(SG_ERR_INVALID, "seq_offsets must describe at least one sequence");
+  if (n_seq > (1 << 30)) return fail(SG_ERR_INVALID, "n_seq %d above 2^30", n_seq);
   return SG_OK;
 }
 
@@ -199,6 +200,9 @@ int sg_adapter_bank_create(sg_ctx* ctx, const void* d_a, const void* d_b, const 
     return fail(SG_ERR_INVALID, "rank %d out of range (1..%d)", rank, sgk::kAdapterMaxRank);
   if (in_dim <= 0 || in_dim % 8 || out_dim <= 0 || out_dim % 8 || in_dim > (1 << 24) || out_dim > (1 << 24))
     return fail(SG_ERR_INVALID, "in_dim and out_dim must be positive multiples of 8 (up to 2^24)");
+  // (Ahead of the sizes, which would leave 64 bits.)
+  if ((double)n_adapters * sgk::adapters_rank_pad(rank) * std::max(in_dim, out_dim) > 0x1p48)
+    return fail(SG_ERR_INVALID, "%d adapters: too many for one bank", n_adapters);
   const size_t na = sgk::adapters_a_bytes(dtype, n_adapters, rank, in_dim);
   const size_t nb = sgk::adapters_b_bytes(dtype, n_adapters, rank, out_dim);
   if (std::max(na, nb) / 4096 > UINT32_MAX / 2) return fail(SG_ERR_INVALID, "%d adapters: too many for one bank", n_adapters);

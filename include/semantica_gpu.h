@@ -368,9 +368,10 @@ typedef struct sg_attn_mask {
  * [rows][ldk] and v [rows][ldv] n_kv_heads (a divisor of n_heads) of them, all of
  * type dtype; strides in elements.  Sums and softmax statistics are float32.
  * float32 products keep 22 bits of each operand (2^-37 of its row's largest value
- * at worst), 16-bit types round the weights to their type.  head_dim: a multiple of 8 up to 256;
- * pointers 16-byte aligned, strides whole 16 bytes (k's and v's up to 2^22
- * elements); out apart from q, k and v.
+ * at worst); 16-bit types round the weights to their type, and tanh is off by
+ * 2^-19 at most.  head_dim: a multiple of 8 up to 256; pointers 16-byte aligned,
+ * strides whole 16 bytes (k's and v's up to 2^22 elements); out apart from q, k
+ * and v.
  * mask NULL: scale 1/sqrt(head_dim), nothing hidden. */
 int sg_attention_masked(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int64_t ldq, const void *k, int64_t ldk,
                         const void *v, int64_t ldv, int32_t dtype, int32_t n_heads, int32_t n_kv_heads,
@@ -386,8 +387,8 @@ int sg_attention_masked(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int6
  * gate [cols] for all.  Otherwise gate is [n_seq][cols], one for each sequence.
  * cols 1 .. 8192, rows and strides of any whole elements (whole 16 bytes are
  * faster).  The squares are summed in float32, as sg_rmsnorm's are: values past
- * 2^63 overflow them.  sum and xn may each be x or h (same pointer and stride); otherwise no
- * output overlaps another tensor. */
+ * 2^63 overflow them.  sum and xn may each be x or h (same pointer and stride);
+ * otherwise no output overlaps another tensor. */
 int sg_block_norm(sg_ctx *ctx, void *xn, int64_t ldxn, void *sum, int64_t lds, const void *x, int64_t ldx,
                   const void *h, int64_t ldh, int32_t dtype, int32_t rows, int32_t cols, const float *w_post,
                   const float *w_pre, float eps, const float *gate, float scale, const int32_t *d_seq_offsets,
@@ -397,8 +398,8 @@ int sg_block_norm(sg_ctx *ctx, void *xn, int64_t ldxn, void *sum, int64_t lds, c
  * [n_adapters][rank][in_dim] and d_b [n_adapters][out_dim][rank] (device memory,
  * contiguous, type dtype; an adapter of a smaller rank is padded with zeros),
  * d_scales [n_adapters] float32.  rank 1 .. 256, in_dim and out_dim multiples of
- * 8.  The arrays are read on the context's stream after what `stream` holds, and
- * may be freed after return.  Freeing the bank waits for the device. */
+ * 8.  The arrays are read on `stream` and may be freed after return, which waits
+ * for that (not to be captured).  Freeing the bank waits for the device. */
 typedef struct sg_adapter_bank sg_adapter_bank;
 int sg_adapter_bank_create(sg_ctx *ctx, const void *d_a, const void *d_b, const float *d_scales, int32_t dtype,
                            int32_t n_adapters, int32_t rank, int32_t in_dim, int32_t out_dim, void *stream,

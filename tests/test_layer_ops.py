@@ -871,7 +871,7 @@ ATT = dict(out=1 << 40, ldo=256, q=2 << 40, ldq=256, k=3 << 40, ldk=128, v=4 << 
     ({"out": None}, {}, "NULL"), ({"q": None}, {}, "NULL"), ({"dtype": 3}, {}, "element type"),
     ({"heads": 3, "kv": 2}, {}, "heads"), ({"heads": 0}, {}, "heads"), ({"kv": 0}, {}, "heads"), ({"hd": 12}, {}, "head_dim"),
     ({"hd": 264}, {}, "head_dim"), ({"hd": 0}, {}, "head_dim"), ({"rows": -1}, {}, "rows"), ({"off": None}, {}, "seq_offsets"),
-    ({"n_seq": 0}, {}, "seq_offsets"), ({"ldq": 255}, {}, "stride"), ({"ldk": 129}, {}, "aligned"), ({"v": (4 << 40) + 8}, {}, "aligned"),
+    ({"n_seq": 0}, {}, "seq_offsets"), ({"n_seq": (1 << 30) + 1}, {}, "2^30"), ({"ldq": 255}, {}, "stride"), ({"ldk": 129}, {}, "aligned"), ({"v": (4 << 40) + 8}, {}, "aligned"),
     ({"ldo": 260}, {}, "aligned"), ({"out": 2 << 40}, {}, "overlaps"), ({"out": (3 << 40) - 16}, {}, "overlaps"),
     ({"ldk": (1 << 22) + 8}, {}, "2^22"), ({"ldq": 1 << 40}, {}, "stride"),
     ({}, {"scale": math.nan}, "scale"), ({}, {"softcap": -1.0}, "softcap"), ({}, {"softcap": math.inf}, "softcap"),
@@ -910,7 +910,8 @@ BANK = dict(a=1 << 40, b=2 << 40, scales=3 << 40, dtype=0, n=4, rank=8, k=64, ou
 @pytest.mark.parametrize("change,word", [
     ({"a": None}, "NULL"), ({"scales": None}, "NULL"), ({"dtype": 7}, "element type"), ({"n": 0}, "n_adapters"),
     ({"rank": 0}, "rank"), ({"rank": 257}, "rank"), ({"k": 60}, "multiples of 8"), ({"out": 4}, "multiples of 8"),
-    ({"out": 0}, "multiples of 8"), ({"n": 1 << 30, "rank": 256, "k": 1 << 16}, "too many")])
+    ({"out": 0}, "multiples of 8"), ({"n": 1 << 30, "rank": 256, "k": 1 << 16}, "too many"),
+    ({"n": (1 << 31) - 1, "rank": 256, "k": 1 << 24, "out": 1 << 24}, "too many")])
 def test_bank_refusals(change, word):
     from semantica_gpu import _lib
     c = {**BANK, **change}

@@ -35,7 +35,7 @@
 // Bound by memory where rows are many, by the chain of dependent loads (offsets, ids,
 // weights, then the second launch) where they are few.  Measured, us of down + up and
 // the TB/s of x, base, dst and the weights (a copy of 1 GB moves 5.0):
-//   30725 float32 rows, 768 to 1280, rank 16, 8 adapters      35 + 64   4.1
+//   30,725 float32 rows, 768 to 1280, rank 16, 8 adapters      35 + 64   4.1
 //   16384 bf16 rows, 2048 to 8192, rank 64, 12 adapters       28 + 132  3.9
 //   64 single bf16 tokens, 4096 to 4096, rank 16, 48          6.5 + 9   0.7
 #include <algorithm>
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int pa
   // with matrix instructions); a step past the wave's last is zeros.  The first of
   // x go out before the rows' adapters are known.  Eight steps for one tile of one
   // block, whose waves are few; four else, so that four waves fit a SIMD and all of a
-  // batch's workgroups are resident (30725 float32 rows of 768: 34 us, 44 with eight,
+  // batch's workgroups are resident (30,725 float32 rows of 768: 34 us, 44 with eight,
   // 35 with two; the next steps' x ahead of the products instead: 37 to 45).
   constexpr int U = RT * NRB == 1 ? 8 : 4;
   chunk<T> xf[U][RT];
@@ -612,7 +612,7 @@ int row_tiles(int rows, int rank_pad, int least) {
     if (rt * rank_pad <= 256 && (rows + rt * kTile - 1) / (rt * kTile) >= least) return rt;
   return 1;
 }
-// Two workgroups a CU at least.  Both sides, us for 30725 float32 rows of 768 (rank
+// Two workgroups a CU at least.  Both sides, us for 30,725 float32 rows of 768 (rank
 // 16, 1280 columns) / 16384 bf16 rows of 2048 (rank 64, 8192 columns): up with one
 // tile 107 / 198, two 111 / 162, four (an earlier form) 126 / 192 for two's 115 / 190.
 int down_tiles(int rows, int rank_pad) { return row_tiles(rows, rank_pad, 2 * kCus); }

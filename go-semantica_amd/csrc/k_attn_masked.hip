@@ -458,7 +458,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   const bool capped = a.softcap > 0.0f;
   const float cs = capped ? qf / a.softcap : qf * kLog2e;
   const float cap2 = a.softcap * kLog2e;
-  const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.0f;
+  const float steep = a.slopes ? a.slopes[h] * kLog2e / (capped ? 1.0f : cs) : 0.0f;  // in scores before that factor
   // 16-bit types: cap2 tanh(s ce) = s (t0 + s^2 (t1 + s^2 t2)) where |s| <= near; ce is
   // cs, or 1 where its powers might leave float32's range and s is multiplied first.
   const bool apart = F::F32 || !(cs > 1e-5f && cs < 1e5f);
@@ -717,8 +717,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       const float far = (float)(row - k - 4 * g);
 #pragma unroll
       for (int r = 0; r < SR; r++)
-        s[r] = __builtin_fmaf(-slope, fabsf(far - (float)(F::KSTR * (r >> 2) + (r & 3))), s[r] * ca);
-      ca = 1.0f;
+        s[r] = __builtin_fmaf(-steep, fabsf(far - (float)(F::KSTR * (r >> 2) + (r & 3))), s[r]);
     }
     if constexpr (F::F32) {
 #pragma unroll

@@ -11,7 +11,7 @@
 // adds the parts in order, so a call gives the same bits every time.
 //
 // Rows of different adapters share a tile of 16: a workgroup takes its tile's
-// distinct adapters one by one, multiplies the whole tile and keeps the rows
+// distinct adapters one by one (down a few together where there are many), multiplies the whole tile and keeps the rows
 // that are that adapter's.  A tile of one sequence, the common case, takes one
 // turn; sixteen single tokens take sixteen, each with the 16-row product that a
 // single row needs as well (the matrix core's rows are free, the adapters'
@@ -161,9 +161,9 @@ __device__ __forceinline__ float to_range(const f32x4_t& s, float& back, float t
 
 // ---- down: u[part][row][rank], times the adapter's scale, and the rows' ids ----------
 // A workgroup: RT tiles of 16 rows, one part of in_dim, NRB blocks of 16 ranks, and
-// every gridDim.z-th of the rows' adapters.  Its four waves take a quarter of the
-// part's steps each and add up through LDS.
-template <typename T, int RT, int NRB>
+// every gridDim.z-th of the rows' adapters, G of them at a time.  Its four waves take a
+// quarter of the part's steps each and add up through LDS.
+template <typename T, int RT, int NRB, int G>
 __global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int parts, int steps_each) {
   constexpr int V = elem<T>::vec, STEP = step_of<T>(), ROWS = RT * kTile;
   __shared__ tile_ids<ROWS> ids;
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int pa
   // block, whose waves are few; four else, so that four waves fit a SIMD and all of a
   // batch's workgroups are resident (30,725 float32 rows of 768: 34 us, 44 with eight,
   // 35 with two; the next steps' x ahead of the products instead: 37 to 45).
-  constexpr int U = RT * NRB == 1 ? 8 : 4;
+  constexpr int U = RT * NRB * G == 1 ? 8 : RT * NRB * G <= 4 ? 4 : 2;
   chunk<T> xf[U][RT];
   auto load_x = [&](int k, int tiles) {
 #pragma unroll
@@ -202,33 +202,47 @@ __global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int pa
   find_ids<ROWS>(a, row0, ids, tid);
   if (tid < ROWS) scale[tid] = ids.own[tid] >= 0 ? a.scales[ids.own[tid]] : 0.0f;  // read behind the loop's barrier
 
-  for (int i = blockIdx.z; i < ids.count; i += gridDim.z) {
-    const int id = __builtin_amdgcn_readfirstlane(ids.list[i]), tiles = __builtin_amdgcn_readfirstlane(ids.tiles[i]);
-    const chunk<T>* wa = static_cast<const chunk<T>*>(a.wa) + ((int64_t)id * rbs + rb0) * steps * 64 + lane;
-    f32x4_t acc[RT][NRB] = {};
+  for (int i = blockIdx.z; i < ids.count; i += G * gridDim.z) {
+    int id[G], in[G], tiles = 0;  // in: the tiles that hold it
+    const chunk<T>* wa[G];
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+      const int at = min(i + j * (int)gridDim.z, ids.count - 1);
+      id[j] = __builtin_amdgcn_readfirstlane(ids.list[at]);
+      in[j] = i + j * (int)gridDim.z < ids.count ? __builtin_amdgcn_readfirstlane(ids.tiles[at]) : 0;
+      wa[j] = static_cast<const chunk<T>*>(a.wa) + ((int64_t)id[j] * rbs + rb0) * steps * 64 + lane;
+      tiles |= in[j];
+    }
+    f32x4_t acc[G][RT][NRB] = {};
     for (int k = k0; k < k1; k += U) {
-      chunk<T> af[U][NRB];
+      chunk<T> af[G][U][NRB];
 #pragma unroll
-      for (int u = 0; u < U; u++)
+      for (int j = 0; j < G; j++)
 #pragma unroll
-        for (int b = 0; b < NRB; b++)
-          af[u][b] = k + u < k1 && rb0 + b < rbs ? wa[((int64_t)b * steps + k + u) * 64] : chunk<T>{};
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int b = 0; b < NRB; b++)
+            af[j][u][b] = (G == 1 || in[j]) && k + u < k1 && rb0 + b < rbs ? wa[j][((int64_t)b * steps + k + u) * 64] : chunk<T>{};
       if (k > k0 || i != (int)blockIdx.z) load_x(k, tiles);
 #pragma unroll
-      for (int u = 0; u < U; u++)
+      for (int j = 0; j < G; j++)
 #pragma unroll
-        for (int b = 0; b < NRB; b++)
+        for (int u = 0; u < U; u++)
 #pragma unroll
-          for (int r = 0; r < RT; r++)
-            if (RT == 1 || (tiles >> r & 1)) acc[r][b] = mfma<T>(af[u][b], xf[u][r], acc[r][b]);
+          for (int b = 0; b < NRB; b++)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+              if (RT * G == 1 || (in[j] >> r & 1)) acc[j][r][b] = mfma<T>(af[j][u][b], xf[u][r], acc[j][r][b]);
     }
 #pragma unroll
-    for (int r = 0; r < RT; r++)
-      if (ids.own[r * kTile + n] == id) {
+    for (int j = 0; j < G; j++)
 #pragma unroll
-        for (int b = 0; b < NRB; b++)
-          *reinterpret_cast<f32x4_t*>(&sums[w][r * kTile + n][16 * b + 4 * g]) = acc[r][b];
-      }
+      for (int r = 0; r < RT; r++)
+        if ((G == 1 || in[j]) && ids.own[r * kTile + n] == id[j]) {
+#pragma unroll
+          for (int b = 0; b < NRB; b++)
+            *reinterpret_cast<f32x4_t*>(&sums[w][r * kTile + n][16 * b + 4 * g]) = acc[j][r][b];
+        }
   }
   __syncthreads();
   constexpr int WIDTH = NRB * 4;  // float4 a row
@@ -627,23 +641,33 @@ int parts_of(int rows, int in_dim, int rank_pad) {
   return std::max(1, std::min(most, kCus / std::max(1, wgs)));
 }
 
+template <typename T, int RT, bool MANY>
+hipError_t down(const sg_adapters_args& a, int parts, dim3 grid, hipStream_t s) {
+  constexpr int G = MANY ? 4 : 1, G4 = MANY ? 2 : 1;  // (of four rank blocks two adapters: 53 us, four 57)
+  const int rbs = a.rank_pad / 16, steps = (a.in_dim + step_of<T>() - 1) / step_of<T>(), each = (steps + parts - 1) / parts;
+  if (rbs == 1)
+    hipLaunchKernelGGL((k_adapter_down<T, RT, 1, G>), grid, dim3(kNT), 0, s, a, parts, each);
+  else if (rbs == 2)
+    hipLaunchKernelGGL((k_adapter_down<T, RT, 2, G>), grid, dim3(kNT), 0, s, a, parts, each);
+  else
+    hipLaunchKernelGGL((k_adapter_down<T, RT, 4, G4>), grid, dim3(kNT), 0, s, a, parts, each);
+  return hipGetLastError();
+}
+
 template <typename T, int RT>
 hipError_t down(const sg_adapters_args& a, int parts, hipStream_t s) {
   const int tiles = (a.rows + RT * kTile - 1) / (RT * kTile), rbs = a.rank_pad / 16;
-  const int steps = (a.in_dim + step_of<T>() - 1) / step_of<T>(), each = (steps + parts - 1) / parts;
   // Adapters that a workgroup's rows are likely to have, over as many workgroups
   // while those are few (64 single tokens with 48 adapters: 6.8 us, 16.4 one after
   // another).
   const int64_t likely = std::min<int64_t>(std::min(a.n_adapters, a.n_seq), ((int64_t)RT * kTile * a.n_seq + a.rows - 1) / a.rows);
   const int z = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(likely, RT * kTile), 4 * kCus / ((int64_t)tiles * parts)));
   const dim3 grid((unsigned)(tiles * parts), rbs <= 2 ? 1 : (rbs + 3) / 4, z);
-  if (rbs == 1)
-    hipLaunchKernelGGL((k_adapter_down<T, RT, 1>), grid, dim3(kNT), 0, s, a, parts, each);
-  else if (rbs == 2)
-    hipLaunchKernelGGL((k_adapter_down<T, RT, 2>), grid, dim3(kNT), 0, s, a, parts, each);
-  else
-    hipLaunchKernelGGL((k_adapter_down<T, RT, 4>), grid, dim3(kNT), 0, s, a, parts, each);
-  return hipGetLastError();
+  // Where a workgroup still has several, it takes them together: their weights' loads are
+  // in flight at once, and x is read once for them (4907 sequences of three bf16 tokens
+  // with 18 adapters, 2944 dims, rank 7: 47 us, 89 one after another; from two on: 2716 of
+  // two fp16 tokens, rank 24, a call 22 us for 18).
+  return likely >= 3 * z ? down<T, RT, true>(a, parts, grid, s) : down<T, RT, false>(a, parts, grid, s);
 }
 
 template <typename T, int RT, int PAIRS>

@@ -44,7 +44,7 @@
 // (us, and the rate of the visible pairs' 4 head_dim flops):
 //   4 x 4096, bf16, causal, cap, 32 heads over 8 of 128            691   796 TFLOP/s
 //   8 of 1024 .. 2048, fp16, causal, prefix, 16 over 8 of 128      152   640
-//   16391 rows, documents of 900, bf16, distance bias, 12 of 64    161   312
+//   16391 rows, documents of 900, bf16, distance bias, 12 of 64    156   323
 //   64 x 512, float32, window of 256, 3 over 1 of 256              217   178
 // float32 (three products each; 372 TFLOP/s is the matrix cores' limit) waits about
 // half its time: a workgroup's eight waves load, halve, multiply in step, and no second

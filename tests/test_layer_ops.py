@@ -464,6 +464,14 @@ def test_adapters_many_rows(gpu_ctx, dtype, rank):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rank", [7, 20, 48])
+def test_adapters_many_short_sequences(gpu_ctx, dtype, rank):
+    """Several adapters in every 16 rows, more than a workgroup takes at a time."""
+    check_adapters(gpu_ctx, dtype, 1000, 72, rank, 9, [3] * 4000 + [0, 1, 2] * 20, first=1, behind=2)
+
+
+@pytest.mark.gpu
 def test_adapters_keep_to_their_rows(gpu_ctx):
     """One request's NaN, in its input or in its adapter, stays with it."""
     for dtype in ("f32", "f16"):
@@ -475,6 +483,23 @@ def test_adapters_keep_to_their_rows(gpu_ctx):
         rest = [i for i in range(16) if i % 4 not in (1, 2) and i != 4]
         assert torch.equal(got[rest], clean[rest])
         assert bool(torch.isnan(got[4]).all()) and bool(torch.isnan(got[1::4]).all())
+
+
+@pytest.mark.gpu
+def test_adapters_keep_to_their_rows_in_large_batches(gpu_ctx):
+    """The same where a workgroup multiplies several adapters together."""
+    for dtype in ("f32", "bf16"):
+        c = adapter_case(dtype, 96, 80, 8, 6, [2] * 8000)
+        c["ids"] = torch.arange(8000, dtype=torch.int32) % 6
+        clean = run_adapters(gpu_ctx, c)
+        c["a"][1, 0, 3], c["b"][2, 5, 1], c["x"][8, 9] = math.nan, math.inf, math.nan
+        got = run_adapters(gpu_ctx, c)
+        rest = torch.ones(16000, dtype=torch.bool)
+        for i in (1, 2):
+            rest[2 * i::12] = rest[2 * i + 1::12] = False
+        rest[8] = False
+        assert torch.equal(got[rest], clean[rest])
+        assert bool(torch.isnan(got[8]).all()) and bool(torch.isnan(got[2::12]).all())
 
 
 @pytest.mark.gpu

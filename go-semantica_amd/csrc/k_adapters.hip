@@ -11,11 +11,12 @@
 // adds the parts in order, so a call gives the same bits every time.
 //
 // Rows of different adapters share a tile of 16: a workgroup takes its tile's
-// distinct adapters one by one (down a few together where there are many), multiplies the whole tile and keeps the rows
-// that are that adapter's.  A tile of one sequence, the common case, takes one
-// turn; sixteen single tokens take sixteen, each with the 16-row product that a
-// single row needs as well (the matrix core's rows are free, the adapters'
-// weights are what such a batch has to read).
+// distinct adapters one by one (down a few together where there are many),
+// multiplies the whole tile and keeps the rows that are that adapter's.  A tile of
+// one sequence, the common case, takes one turn; sixteen single tokens take
+// sixteen, each with the 16-row product that a single row needs as well (the
+// matrix core's rows are free, the adapters' weights are what such a batch has to
+// read).
 //
 // Operands.  Weights are laid out once in fragment order, a wave's load being one
 // contiguous kilobyte:
@@ -184,10 +185,10 @@ __global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int pa
   // U steps' loads go out before their products (the compiler does not unroll loops
   // with matrix instructions); a step past the wave's last is zeros.  The first of
   // x go out before the rows' adapters are known.  Eight steps for one tile of one
-  // block, whose waves are few; four else, so that four waves fit a SIMD and all of a
+  // block, whose waves are few; four else (two for several adapters), so that four waves fit a SIMD and all of a
   // batch's workgroups are resident (30,725 float32 rows of 768: 34 us, 44 with eight,
   // 35 with two; the next steps' x ahead of the products instead: 37 to 45).
-  constexpr int U = RT * NRB * G == 1 ? 8 : RT * NRB * G <= 4 ? 4 : 2;
+  constexpr int U = RT * NRB * G == 1 ? 8 : G == 1 || RT * NRB * G <= 4 ? 4 : 2;
   chunk<T> xf[U][RT];
   auto load_x = [&](int k, int tiles) {
 #pragma unroll

@@ -185,9 +185,10 @@ __global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int pa
   // U steps' loads go out before their products (the compiler does not unroll loops
   // with matrix instructions); a step past the wave's last is zeros.  The first of
   // x go out before the rows' adapters are known.  Eight steps for one tile of one
-  // block, whose waves are few; four else (two for several adapters), so that four waves fit a SIMD and all of a
-  // batch's workgroups are resident (30,725 float32 rows of 768: 34 us, 44 with eight,
-  // 35 with two; the next steps' x ahead of the products instead: 37 to 45).
+  // block, whose waves are few; four else (two for several adapters), so that four
+  // waves fit a SIMD and all of a batch's workgroups are resident (30,725 float32
+  // rows of 768: 34 us, 44 with eight, 35 with two; the next steps' x ahead of the
+  // products instead: 37 to 45).
   constexpr int U = RT * NRB * G == 1 ? 8 : G == 1 || RT * NRB * G <= 4 ? 4 : 2;
   chunk<T> xf[U][RT];
   auto load_x = [&](int k, int tiles) {

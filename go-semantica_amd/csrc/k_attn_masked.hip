@@ -458,10 +458,13 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   const bool capped = a.softcap > 0.0f;
   const float cs = capped ? qf / a.softcap : qf * kLog2e;
   const float cap2 = a.softcap * kLog2e;
-  const float steep = a.slopes ? a.slopes[h] * kLog2e / (capped ? 1.0f : cs) : 0.0f;  // in scores before that factor
   // 16-bit types: cap2 tanh(s ce) = s (t0 + s^2 (t1 + s^2 t2)) where |s| <= near; ce is
   // cs, or 1 where its powers might leave float32's range and s is multiplied first.
   const bool apart = F::F32 || !(cs > 1e-5f && cs < 1e5f);
+  // What a key's distance takes off a score.  16-bit types take it off ahead of cs, which
+  // saves the multiplication; not float32, whose cs holds the row's own power of two (of a
+  // row of zeros 2^-110, and the quotient would leave float32's range), nor a far-off cs.
+  const float steep = a.slopes ? a.slopes[h] * kLog2e / (capped || apart ? 1.0f : cs) : 0.0f;
   const float ce = apart ? 1.0f : cs;
   const float t0 = cap2 * ce * kTanh16[0], t1 = cap2 * ce * ce * ce * kTanh16[1];
   const float t2 = cap2 * ce * ce * (ce * ce) * ce * kTanh16[2];
@@ -713,12 +716,6 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       }
       ca = 1.0f;
     }
-    if (a.slopes) {
-      const float far = (float)(row - k - 4 * g);
-#pragma unroll
-      for (int r = 0; r < SR; r++)
-        s[r] = __builtin_fmaf(-steep, fabsf(far - (float)(F::KSTR * (r >> 2) + (r & 3))), s[r]);
-    }
     if constexpr (F::F32) {
 #pragma unroll
       for (int b = 0; b < SR / 4; b++) {
@@ -727,6 +724,16 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
         for (int i = 0; i < 4; i++) s[4 * b + i] = __builtin_fmaf(s[4 * b + i], ca, ve[i]);
       }
       ca = 1.0f;
+    } else if (a.slopes && apart && !capped) {
+#pragma unroll
+      for (int r = 0; r < SR; r++) s[r] *= cs;
+      ca = 1.0f;
+    }
+    if (a.slopes) {
+      const float far = (float)(row - k - 4 * g);
+#pragma unroll
+      for (int r = 0; r < SR; r++)
+        s[r] = __builtin_fmaf(-steep, fabsf(far - (float)(F::KSTR * (r >> 2) + (r & 3))), s[r]);
     }
     if (masked) {
       const int c0 = lo - k - 4 * g, c1 = hi - k - 4 * g;

@@ -1017,3 +1017,46 @@ def test_wrappers_refuse_other_devices_and_shapes():
         kernels.block_norm(ctx, None, t, t, t, w, None, 1e-6)
     with pytest.raises(ValueError, match="device"):
         kernels.attention_masked(ctx, t, t, t, t, 1, 1, torch.zeros(2, dtype=torch.int32))
+
+
+# ---- queries near zero, biases of any sign and size --------------------------------------
+
+
+def check_bias(ctx, dtype, hd, lens, heads, kv_heads, slopes, by=None, v_by=1.0, **kw):
+    g, off = gen(61), offsets(lens)
+    rows = int(off[-1])
+    q, k, v = (rand(g, rows, c * hd, dtype=dtype) for c in (heads, kv_heads, kv_heads))
+    v = (v.float() * v_by).to(v.dtype)
+    for i, f in enumerate(by or ()):  # every seventh row each
+        q[i::7] = (q[i::7].float() * f).to(q.dtype)
+    slopes = torch.tensor([slopes[h % len(slopes)] for h in range(heads)], dtype=torch.float32)
+    say("bias", dtype, "hd", hd, "lens", lens, "heads", heads, kw)
+    got = run_attention(ctx, q, k, v, off, heads, kv_heads, slopes=slopes, **kw)
+    want, mean, _ = attention_ref(q, k, v, off, heads, kv_heads, slopes=slopes, **kw)
+    # A score's size, at most: the products' (the cap, if that is less) and the farthest key's bias.
+    scale = abs(kw.get("scale") or hd ** -0.5)
+    dots = scale * float(q.double().abs().max() * k.double().abs().max()) * hd
+    size = torch.full_like(mean, min(dots, kw.get("softcap") or dots) + float(slopes.abs().max()) * max(lens))
+    close(got, want, attention_tol(dtype, hd, want, mean, size), "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("lens,heads,kv_heads", [([90, 40], 4, 2), ([700, 300], 24, 8)])
+def test_attention_bias_of_queries_near_zero(gpu_ctx, dtype, hd, lens, heads, kv_heads):
+    """Queries of zeros and of tiny values: the bias alone makes their weights.  In the form
+    whose waves share rows and in the other; masked, and under a cap."""
+    by, slopes = (0.0, 1e-38, 1e-36, 1e-30, 1e-22), (0.5, 2.0 ** -4, 2.0 ** -8)
+    check_bias(gpu_ctx, dtype, hd, lens, heads, kv_heads, slopes, by)
+    check_bias(gpu_ctx, dtype, hd, lens, heads, kv_heads, slopes, by, causal=True, window=50, scale=-0.2)
+    check_bias(gpu_ctx, dtype, hd, lens, heads, kv_heads, slopes, by, softcap=5.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [1e-39, 1e-37, -1e-30, 1e-6, 3e5])
+def test_attention_bias_beside_scales_of_any_size(gpu_ctx, dtype, scale):
+    """A scale that leaves nothing of the scores but the bias, or makes one key take all."""
+    check_bias(gpu_ctx, dtype, 64, [90, 140], 4, 2, (0.5, 2.0 ** -6), scale=scale)
+    check_bias(gpu_ctx, dtype, 64, [90, 140], 4, 2, (0.5, 2.0 ** -6), (0.0,), scale=scale, causal=True)

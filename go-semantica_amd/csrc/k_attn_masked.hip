@@ -464,7 +464,9 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   // What a key's distance takes off a score.  16-bit types take it off ahead of cs, which
   // saves the multiplication; not float32, whose cs holds the row's own power of two (of a
   // row of zeros 2^-110, and the quotient would leave float32's range), nor a far-off cs.
-  const float steep = a.slopes ? a.slopes[h] * kLog2e / (capped || apart ? 1.0f : cs) : 0.0f;
+  const bool first = apart && (F::F32 ? capped : capped || a.slopes);  // scores are multiplied by cs ahead of all else
+  const float after = capped || first ? 1.0f : cs;                    // and by this behind it
+  const float steep = a.slopes ? a.slopes[h] * kLog2e / (F::F32 ? 1.0f : after) : 0.0f;
   const float ce = apart ? 1.0f : cs;
   const float t0 = cap2 * ce * kTanh16[0], t1 = cap2 * ce * ce * ce * kTanh16[1];
   const float t2 = cap2 * ce * ce * (ce * ce) * ce * kTanh16[2];
@@ -681,8 +683,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
     for (int sub = 0; sub < NS; sub++)
 #pragma unroll
       for (int r = 0; r < R; r++) s[sub * R + r] = F::F32 ? c[sub][0][r] + (c[sub][CH / 2][r] + c[sub][CH - 1][r]) : c[sub][0][r];
-    // Register r: key KSTR (r / 4) + 4 g + r % 4.  The score is s ca.
-    float ca = cs;
+    // Register r: key KSTR (r / 4) + 4 g + r % 4.  The score is s after.
     if constexpr (F::F32) {
 #pragma unroll
       for (int b = 0; b < SR / 4; b++) {
@@ -691,11 +692,12 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
         for (int i = 0; i < 4; i++) s[4 * b + i] *= km[i];
       }
     }
+    if (first) {
+#pragma unroll
+      for (int r = 0; r < SR; r++) s[r] *= cs;
+    }
     if (capped) {
       float most = 0.0f;
-      if (apart)
-#pragma unroll
-        for (int r = 0; r < SR; r++) s[r] *= cs;
 #pragma unroll
       for (int r = 0; r < SR; r++) most = fmaxf(most, fabsf(s[r]));
       if (__ballot(most > near)) {
@@ -714,20 +716,14 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
           s[r] = F::F32 ? tanh_near32(s[r]) * cap2 : s[r] * __builtin_fmaf(z, __builtin_fmaf(z, t2, t1), t0);
         }
       }
-      ca = 1.0f;
     }
     if constexpr (F::F32) {
 #pragma unroll
       for (int b = 0; b < SR / 4; b++) {
         const f32x4_t ve = *reinterpret_cast<const f32x4_t*>(key_mul + F::BK + F::KSTR * b + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[4 * b + i] = __builtin_fmaf(s[4 * b + i], ca, ve[i]);
+        for (int i = 0; i < 4; i++) s[4 * b + i] = __builtin_fmaf(s[4 * b + i], after, ve[i]);
       }
-      ca = 1.0f;
-    } else if (a.slopes && apart && !capped) {
-#pragma unroll
-      for (int r = 0; r < SR; r++) s[r] *= cs;
-      ca = 1.0f;
     }
     if (a.slopes) {
       const float far = (float)(row - k - 4 * g);
@@ -751,7 +747,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       float top = s[0];
 #pragma unroll
       for (int r = 1; r < SR; r++) top = fmaxf(top, s[r]);
-      top = query_max<QT>(top) * ca;
+      top = query_max<QT>(top) * (F::F32 ? 1.0f : after);
       if (__ballot(top > m + kSlack)) {  // (-inf + 8 is -inf: a row's first visible key raises it)
         const float to = fmaxf(m, top);
         const float by = to > m ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
@@ -771,7 +767,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
       float pv[8];
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        pv[i] = __builtin_amdgcn_exp2f(F::F32 ? s[8 * ps + i] + from : fixed ? s[8 * ps + i] : __builtin_fmaf(s[8 * ps + i], ca, from));
+        pv[i] = __builtin_amdgcn_exp2f(F::F32 ? s[8 * ps + i] + from : fixed ? s[8 * ps + i] : __builtin_fmaf(s[8 * ps + i], after, from));
       if constexpr (F::F32) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {

@@ -224,11 +224,12 @@ __device__ __forceinline__ float tanh_near32(float x) {
   p = __builtin_fmaf(z, p, 1.0f);
   return x * p;
 }
-// bf16 has float32's exponents, so under a cap its weights need no running maximum:
-// 2^+-kMostCap2 and sums of them times values below 2^40 are in range (a value that
-// overflows the sum makes an output that is not finite, and careful_row takes it; so it
-// does outputs below 2^-110 before the division by a sum of weights that is small, where
-// products of tiny values underflow).
+// bf16 has float32's exponents, so under a cap its weights need no running maximum, unless
+// a negative slope lets scores grow with the distance: 2^+-kMostCap2 (a bias only lowers
+// weights, and a query's own not at all) and sums of them times values below 2^40 are in range
+// (a value that overflows the sum makes an output that is not finite, and careful_row takes
+// it; so it does outputs below 2^-110 before the division by a sum of weights that is small,
+// where products of tiny values underflow).
 constexpr float kMostCap2 = 80.0f;
 // Lambert's continued fraction to seven levels below 1.5 (relative error 5e-8 at its
 // end), and 1 - 2 / (e^2x + 1) above, where the second term's rounding no longer shows.
@@ -471,7 +472,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   const float t0 = cap2 * ce * kTanh16[0], t1 = cap2 * ce * ce * ce * kTanh16[1];
   const float t2 = cap2 * ce * ce * (ce * ce) * ce * kTanh16[2];
   const float near = F::F32 ? kNear32 : kNear16 / ce;
-  const bool fixed = __is_same(T, bf16_t) && capped && cap2 <= kMostCap2;
+  const bool fixed = __is_same(T, bf16_t) && capped && cap2 <= kMostCap2 && (!a.slopes || a.slopes[h] >= 0.0f);
 
   // ---- tiles ----
   // The first tile from t on that may hold a key of a document of this

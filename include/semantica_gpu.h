@@ -352,7 +352,7 @@ int sg_pool_l2(sg_ctx *ctx, float *out, const float *x, int32_t ldx, int32_t out
 typedef struct sg_attn_mask {
   float scale;            /* of q . k; 0: 1/sqrt(head_dim) */
   float softcap;          /* > 0: scores become softcap * tanh(score / softcap); 0: they stay */
-  const float *slopes;    /* [n_heads]: slopes[h] * |i - j| is subtracted after the cap; NULL: nothing */
+  const float *slopes;    /* [n_heads]: slopes[h] * |i - j| is subtracted after the cap (slopes of any sign); NULL: nothing */
   const int32_t *doc_ids; /* [rows]: keys of the query's own document are visible, and none if its id is
                              negative (padding); NULL: the whole sequence is one document */
   const int32_t *prefix;  /* [n_seq]: with causal, a sequence's first prefix[i] keys are visible to all of

@@ -1060,3 +1060,15 @@ def test_attention_bias_beside_scales_of_any_size(gpu_ctx, dtype, scale):
     """A scale that leaves nothing of the scores but the bias, or makes one key take all."""
     check_bias(gpu_ctx, dtype, 64, [90, 140], 4, 2, (0.5, 2.0 ** -6), scale=scale)
     check_bias(gpu_ctx, dtype, 64, [90, 140], 4, 2, (0.5, 2.0 ** -6), (0.0,), scale=scale, causal=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cap", [0.0, 20.0, 50.0])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 1), (24, 8)])
+def test_attention_bias_that_grows_with_distance(gpu_ctx, dtype, cap, heads, kv_heads):
+    """Negative slopes: far keys weigh most, and scores leave float32's exponents in powers of
+    two (90 at slope 0.1, 225 at 0.25) ahead of the softmax."""
+    for v_by in (0.05, 1e-3):
+        check_bias(gpu_ctx, dtype, 64, [900], heads, kv_heads, (-0.1, -0.25), v_by=v_by, softcap=cap)
+    check_bias(gpu_ctx, dtype, 128, [330, 900], heads, kv_heads, (-0.1, 0.1), softcap=cap, causal=True)

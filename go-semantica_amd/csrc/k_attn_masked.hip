@@ -314,13 +314,19 @@ __device__ __forceinline__ void careful_row(const sg_attn_masked_args& a, int ro
       if (lane + 64 * i < a.hd) s = __builtin_fmaf(qv[i], elem<T>::to(kp[(int64_t)j * a.ldk + lane + 64 * i]), s);
     return score_of<T>(a, sgp::wave_sum(s), slope, row - j);
   };
+  // The weights' sum comes first, so that what is added up is a mean: values near the type's
+  // end leave no range.
   float m = -INFINITY, l = 0.0f;
-  for (int j = lo; j < hi; j++)
-    if (!a.docs || a.docs[j] == doc) m = fmaxf(m, score(j));
   for (int j = lo; j < hi; j++) {
     if (a.docs && a.docs[j] != doc) continue;
-    const float p = __builtin_amdgcn_exp2f(score(j) - m);
-    l += p;
+    const float s = score(j), to = fmaxf(m, s), from = to == -INFINITY ? 0.0f : to;
+    l = l * __builtin_amdgcn_exp2f(m - from) + __builtin_amdgcn_exp2f(s - from);
+    m = to;
+  }
+  const float inv = 1.0f / l;
+  for (int j = lo; j < hi; j++) {
+    if (a.docs && a.docs[j] != doc) continue;
+    const float p = __builtin_amdgcn_exp2f(score(j) - m) * inv;
 #pragma unroll
     for (int i = 0; i < N; i++)
       if (lane + 64 * i < a.hd) o[i] = __builtin_fmaf(p, elem<T>::to(vp[(int64_t)j * a.ldv + lane + 64 * i]), o[i]);
@@ -329,7 +335,7 @@ __device__ __forceinline__ void careful_row(const sg_attn_masked_args& a, int ro
 #pragma unroll
   for (int i = 0; i < N; i++) {
     const int d = lane + 64 * i;
-    if (d >= d0 && d < d1) out[d] = elem<T>::from(o[i] / l);
+    if (d >= d0 && d < d1) out[d] = elem<T>::from(o[i]);
   }
 }
 

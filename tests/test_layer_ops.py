@@ -1072,3 +1072,19 @@ def test_attention_bias_that_grows_with_distance(gpu_ctx, dtype, cap, heads, kv_
     for v_by in (0.05, 1e-3):
         check_bias(gpu_ctx, dtype, 64, [900], heads, kv_heads, (-0.1, -0.25), v_by=v_by, softcap=cap)
     check_bias(gpu_ctx, dtype, 128, [330, 900], heads, kv_heads, (-0.1, 0.1), softcap=cap, causal=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_attention_values_at_the_types_end(gpu_ctx, dtype, hd):
+    """Values whose sum over the keys leaves float32's range, though no mean of them does."""
+    g, off = gen(62), offsets([50, 70])
+    q, k, v = (rand(g, 120, hd, dtype=dtype) for _ in range(3))
+    v = torch.sign(v) * 3.2e38
+    v[:, ::3] = 3.2e38
+    assert bool(torch.isfinite(v).all())
+    got = run_attention(gpu_ctx, q, k, v, off, 1, 1)
+    want, mean, size = attention_ref(q, k, v, off, 1, 1)
+    # (careful_row's weights are float32 whatever the type: a division more each.)
+    close(got, want, attention_tol(dtype, hd, want, mean, size) + 4 * F * mean, "attention")

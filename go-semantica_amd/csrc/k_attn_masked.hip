@@ -324,7 +324,7 @@ __device__ __forceinline__ void careful_row(const sg_attn_masked_args& a, int ro
     m = to;
   }
   const float inv = 1.0f / l;
-  for (int j = lo; j < hi; j++) {
+  for (int j = l != 0.0f ? lo : hi; j < hi; j++) {  // (scores of -inf alone: zeros, as where all is hidden)
     if (a.docs && a.docs[j] != doc) continue;
     const float p = __builtin_amdgcn_exp2f(score(j) - m) * inv;
 #pragma unroll

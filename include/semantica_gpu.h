@@ -362,8 +362,9 @@ typedef struct sg_attn_mask {
 } sg_attn_mask;
 
 /* Attention of every sequence with itself: out_i = sum_j softmax_j(score_ij) v_j
- * over the visible keys; zeros for a query that sees none.  Hidden keys do not
- * touch the result, whatever they hold (infinities and NaN included).  q
+ * over the visible keys; zeros for a query that sees none, or none whose score
+ * is above -infinity.  Hidden keys do not touch the result, whatever they hold
+ * (infinities and NaN included).  q
  * [rows][ldq] and out [rows][ldo] hold n_heads heads of head_dim side by side, k
  * [rows][ldk] and v [rows][ldv] n_kv_heads (a divisor of n_heads) of them, all of
  * type dtype; strides in elements.  Sums and softmax statistics are float32.

@@ -1088,3 +1088,20 @@ def test_attention_values_at_the_types_end(gpu_ctx, dtype, hd):
     want, mean, size = attention_ref(q, k, v, off, 1, 1)
     # (careful_row's weights are float32 whatever the type: a division more each.)
     close(got, want, attention_tol(dtype, hd, want, mean, size) + 4 * F * mean, "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("odd", [1.0, math.inf, math.nan])
+def test_attention_scores_of_minus_infinity(gpu_ctx, dtype, odd):
+    """Visible keys whose scores are all -inf weigh nothing, as hidden ones do: zeros, whatever
+    their values are."""
+    g, off = gen(63), offsets([40])
+    q, k, v = (rand(g, 40, 64, dtype=dtype) for _ in range(3))
+    q[:, 0] = q[:, 0].abs() + 0.5
+    k[:3, 0], v[:3, 5] = -math.inf, odd
+    got = run_attention(gpu_ctx, q, k, v, off, 1, 1, causal=True)
+    assert bool((got[:3] == 0).all())
+    if odd == 1.0:
+        want, mean, size = attention_ref(q[3:], k[3:], v[3:], offsets([37]), 1, 1, causal=True)
+        close(got[3:], want, attention_tol(dtype, 64, want, mean, size), "attention")

@@ -732,10 +732,20 @@ hipError_t adapters_pack(int dtype, const void* a, const void* b, int n, int ran
   if (dtype == SG_F16) return pack<_Float16>(a, b, n, rank, in_dim, out_dim, wa, wb, s);
   return pack<bf16_t>(a, b, n, rank, in_dim, out_dim, wa, wb, s);
 }
+// Enough for every batch of up to `rows` rows, so that a workspace for the largest one
+// serves them all: fewer rows may be split into more parts, whose sums take more than
+// one part's of the larger batch.
 size_t adapters_work_bytes(int dtype, int rows, int in_dim, int rank_pad) {
-  const int parts = dtype == SG_F32 ? parts_of<float>(rows, in_dim, rank_pad) : parts_of<_Float16>(rows, in_dim, rank_pad);
-  const size_t tiled = (size_t)(rows + kTile - 1) / kTile * kTile;
-  return sizeof(float) * ((parts > 1 ? parts * (size_t)rows : tiled) * rank_pad + 2 * (size_t)rows);
+  auto parts_at = [&](int r) { return dtype == SG_F32 ? parts_of<float>(r, in_dim, rank_pad) : parts_of<_Float16>(r, in_dim, rank_pad); };
+  auto bytes = [&](size_t held, size_t r) { return sizeof(float) * (held * rank_pad + 2 * r); };
+  size_t most = 0;
+  if (parts_at(rows) == 1) most = bytes((size_t)(rows + kTile - 1) / kTile * kTile, rows);
+  // The most rows that p parts are taken for (they are tiles of 16 there).
+  for (int p = 2; p <= kMostSplit; p++) {
+    const int r = std::min(rows, kCus / p * kTile);
+    if (parts_at(r) >= p) most = std::max(most, bytes((size_t)p * r, r));
+  }
+  return most;
 }
 hipError_t adapters_apply(const sg_adapters_args& a, int dtype, hipStream_t s) {
   if (dtype == SG_F32) return apply<float>(a, s);

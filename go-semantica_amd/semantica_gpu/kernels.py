@@ -312,6 +312,7 @@ class AdapterBank:
         self.handle = h
 
     def work_bytes(self, rows):
+        """Bytes of `work` that adapters_apply needs for `rows` rows or fewer."""
         size = ctypes.c_size_t()
         _lib.check(self.lib.sg_adapters_work_bytes(self.handle, rows, ctypes.byref(size)))
         return size.value

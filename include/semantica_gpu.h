@@ -407,7 +407,8 @@ int sg_adapter_bank_create(sg_ctx *ctx, const void *d_a, const void *d_b, const 
                            sg_adapter_bank **out);
 void sg_adapter_bank_free(sg_adapter_bank *bank);
 
-/* Bytes of workspace that sg_adapters_apply needs for `rows` rows. */
+/* Bytes of workspace that sg_adapters_apply needs for `rows` rows or fewer (so a program
+ * that allocates once asks for its largest batch). */
 int sg_adapters_work_bytes(const sg_adapter_bank *bank, int32_t rows, size_t *bytes);
 
 /* dst_t = base_t + scale_a * B_a (A_a x_t) for every row t, a = d_adapter_ids[i] of

@@ -1105,3 +1105,31 @@ def test_attention_scores_of_minus_infinity(gpu_ctx, dtype, odd):
     if odd == 1.0:
         want, mean, size = attention_ref(q[3:], k[3:], v[3:], offsets([37]), 1, 1, causal=True)
         close(got[3:], want, attention_tol(dtype, 64, want, mean, size), "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,k,rank", [("bf16", 4096, 16), ("bf16", 2048, 64), ("f32", 4096, 16), ("f16", 776, 100),
+                                          ("f32", 64, 8)])
+def test_adapters_workspace_of_the_largest_batch_serves_all(gpu_ctx, dtype, k, rank):
+    """Smaller batches may be split into more parts: a workspace for more rows is enough
+    for them, and what they get does not depend on its size."""
+    from semantica_gpu import kernels
+    c = adapter_case(dtype, k, 72, rank, 3, [2064], seed=3)
+    bank = kernels.AdapterBank(gpu_ctx, c["a"].cuda(), c["b"].cuda(), c["scales"].cuda())
+    x, base = c["x"].cuda(), c["base"].cuda()
+    counts = sorted({0, 1, 2, 15, 16, 17, 33000, 40000} | {16 * t + d for t in range(1, 140) for d in (-1, 0, 1)})
+    needs = [bank.work_bytes(rows) for rows in counts]
+    assert needs == sorted(needs)
+    largest = torch.empty(bank.work_bytes(2064), dtype=torch.uint8, device="cuda")
+    ids = torch.tensor([1], dtype=torch.int32, device="cuda")
+    for rows in (1, 16, 17, 200, 512, 1000, 1024, 1365, 2048, 2064):
+        say("workspace", dtype, k, rank, "rows", rows)
+        got, want = (torch.full_like(base[:rows], 7.0) for _ in range(2))
+        off = offsets([rows]).cuda()
+        kernels.adapters_apply(gpu_ctx, got, base[:rows], bank, x[:rows], off, ids, work=largest)
+        kernels.adapters_apply(gpu_ctx, want, base[:rows], bank, x[:rows], off, ids)
+        assert torch.equal(got, want)
+        true, size = adapters_ref(c["x"][:rows], c["base"][:rows], c["a"], c["b"], c["scales"], offsets([rows]), ids.cpu())
+        rel = (k + rank + 32) * F + (0 if dtype == "f32" else 2.0 ** -16)
+        close(got, true, U[dtype] * true.abs() + rel * size + TINY[dtype], "adapters")
+    bank.close()

@@ -613,11 +613,11 @@ template <typename T>
 hipError_t pack(const void* a, const void* b, int n, int rank, int in_dim, int out_dim, void* wa, void* wb, hipStream_t s) {
   const int rbs = sgk::adapters_rank_pad(rank) / 16;
   const int64_t na = a_chunks<T>(n, rank, in_dim), nb = b_chunks<T>(n, rank, out_dim);
-  hipLaunchKernelGGL((k_pack_a<T>), dim3((unsigned)((na + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(a), rank, in_dim,
-                     rbs, (in_dim + step_of<T>() - 1) / step_of<T>(), na, static_cast<chunk<T>*>(wa));
-  hipLaunchKernelGGL((k_pack_b<T>), dim3((unsigned)((nb + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(b), rank, out_dim,
-                     rbs, (out_dim + 31) / 32, nb, static_cast<chunk<T>*>(wb));
-  return hipGetLastError();
+  const hipError_t e = sgp::run_kernel(k_pack_a<T>, dim3((unsigned)((na + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(a),
+                                       rank, in_dim, rbs, (in_dim + step_of<T>() - 1) / step_of<T>(), na, static_cast<chunk<T>*>(wa));
+  if (e != hipSuccess) return e;
+  return sgp::run_kernel(k_pack_b<T>, dim3((unsigned)((nb + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(b), rank, out_dim,
+                         rbs, (out_dim + 31) / 32, nb, static_cast<chunk<T>*>(wb));
 }
 
 // ---- launches ----------------------------------------------------------------------
@@ -647,13 +647,9 @@ template <typename T, int RT, bool MANY>
 hipError_t down(const sg_adapters_args& a, int parts, dim3 grid, hipStream_t s) {
   constexpr int G = MANY ? 4 : 1, G4 = MANY ? 2 : 1;  // (of four rank blocks two adapters: 53 us, four 57)
   const int rbs = a.rank_pad / 16, steps = (a.in_dim + step_of<T>() - 1) / step_of<T>(), each = (steps + parts - 1) / parts;
-  if (rbs == 1)
-    hipLaunchKernelGGL((k_adapter_down<T, RT, 1, G>), grid, dim3(kNT), 0, s, a, parts, each);
-  else if (rbs == 2)
-    hipLaunchKernelGGL((k_adapter_down<T, RT, 2, G>), grid, dim3(kNT), 0, s, a, parts, each);
-  else
-    hipLaunchKernelGGL((k_adapter_down<T, RT, 4, G4>), grid, dim3(kNT), 0, s, a, parts, each);
-  return hipGetLastError();
+  if (rbs == 1) return sgp::run_kernel(k_adapter_down<T, RT, 1, G>, grid, dim3(kNT), 0, s, a, parts, each);
+  if (rbs == 2) return sgp::run_kernel(k_adapter_down<T, RT, 2, G>, grid, dim3(kNT), 0, s, a, parts, each);
+  return sgp::run_kernel(k_adapter_down<T, RT, 4, G4>, grid, dim3(kNT), 0, s, a, parts, each);
 }
 
 template <typename T, int RT>
@@ -679,17 +675,12 @@ hipError_t up(const sg_adapters_args& a, int parts, hipStream_t s) {
   if ((int64_t)tiles * slices > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tiles * slices);
   if (a.ready) {
-    if (a.rank_pad == 16)
-      hipLaunchKernelGGL((k_adapter_up_ready<T, RT, PAIRS, 1>), grid, dim3(kNT), 0, s, a, slices);
-    else if (a.rank_pad == 32)
-      hipLaunchKernelGGL((k_adapter_up_ready<T, RT, PAIRS, 2>), grid, dim3(kNT), 0, s, a, slices);
-    else
-      hipLaunchKernelGGL((k_adapter_up_ready<T, RT, PAIRS, 4>), grid, dim3(kNT), 0, s, a, slices);
-    return hipGetLastError();
+    if (a.rank_pad == 16) return sgp::run_kernel(k_adapter_up_ready<T, RT, PAIRS, 1>, grid, dim3(kNT), 0, s, a, slices);
+    if (a.rank_pad == 32) return sgp::run_kernel(k_adapter_up_ready<T, RT, PAIRS, 2>, grid, dim3(kNT), 0, s, a, slices);
+    return sgp::run_kernel(k_adapter_up_ready<T, RT, PAIRS, 4>, grid, dim3(kNT), 0, s, a, slices);
   }
   const size_t lds = (size_t)RT * a.rank_pad / 16 * 64 * 16 + sizeof(float) * RT * kTile * (CW + 4);
-  hipLaunchKernelGGL((k_adapter_up<T, RT, PAIRS>), grid, dim3(kNT), lds, s, a, parts, slices);
-  return hipGetLastError();
+  return sgp::run_kernel(k_adapter_up<T, RT, PAIRS>, grid, dim3(kNT), lds, s, a, parts, slices);
 }
 
 template <typename T, int RT>

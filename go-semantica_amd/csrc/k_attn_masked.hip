@@ -973,9 +973,8 @@ hipError_t launch(const sg_attn_masked_args& a, hipStream_t s) {
   typedef form<T, D, QT, RW, KW> F;
   const int64_t tiles = ((int64_t)a.rows + F::BM - 1) / F::BM;
   if (tiles * a.heads > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_attn_masked<T, D, QT, RW, KW>), dim3((unsigned)(tiles * a.heads)), dim3(F::NT), F::LDS, s, a,
-                     (int)tiles);
-  return hipGetLastError();
+  return sgp::run_kernel(k_attn_masked<T, D, QT, RW, KW>, dim3((unsigned)(tiles * a.heads)), dim3(F::NT), F::LDS, s, a,
+                         (int)tiles);
 }
 
 // Which form: waves that share 32 rows as long as a workgroup for each 32 rows and head

@@ -193,8 +193,7 @@ hipError_t launch(const sg_block_norm_args& a, hipStream_t s) {
   const int64_t groups = 256 * (2048 / NT) * RPB;
   const int each = (int)((a.rows + groups - 1) / groups);
   const int64_t blocks = ((int64_t)a.rows + (int64_t)RPB * each - 1) / ((int64_t)RPB * each);
-  hipLaunchKernelGGL((k_block_norm<T, TPR, NCH, FULL>), dim3((unsigned)blocks), dim3(NT), 0, s, a, each);
-  return hipGetLastError();
+  return sgp::run_kernel(k_block_norm<T, TPR, NCH, FULL>, dim3((unsigned)blocks), dim3(NT), 0, s, a, each);
 }
 
 template <typename T, int TPR, bool FULL>

@@ -230,6 +230,7 @@ int sg_adapter_bank_create(sg_ctx* ctx, const void* d_a, const void* d_b, const 
   }
   if (r != SG_OK) {
     sg_adapter_bank_free(b);
+    (void)hipGetLastError();  // reported here, and to no later call's check
     return r;
   }
   *out = b;

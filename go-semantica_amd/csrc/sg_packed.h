@@ -38,6 +38,20 @@ struct alignas(16) chunk {
   T v[elem<T>::vec];
 };
 
+// A launch that answers for itself: hipGetLastError would report what an earlier call of the
+// thread left behind, and a launch that fails leaves nothing for the next caller's check.
+template <typename T>
+struct as_is {
+  typedef T type;
+};
+template <typename... P>
+hipError_t run_kernel(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t s, typename as_is<P>::type... p) {
+  void* at[] = {&p...};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, at, lds, s);
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
+}
+
 // Offsets come from device memory, so no host check has seen them: whatever
 // they hold, an index formed from one is clamped to the tensors' rows.
 __device__ __forceinline__ int clamp_row(int v, int rows) { return min(max(v, 0), rows); }

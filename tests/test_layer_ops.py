@@ -1133,3 +1133,41 @@ def test_adapters_workspace_of_the_largest_batch_serves_all(gpu_ctx, dtype, k, r
         rel = (k + rank + 32) * F + (0 if dtype == "f32" else 2.0 ** -16)
         close(got, true, U[dtype] * true.abs() + rel * size + TINY[dtype], "adapters")
     bank.close()
+
+
+@pytest.mark.gpu
+def test_a_refused_bank_leaves_no_error_behind(gpu_ctx):
+    """More adapters than the device's memory holds, then calls that succeed: this library's
+    and torch's."""
+    from semantica_gpu import _lib
+    lib = _lib.load()
+    c = adapter_case("f32", 96, 80, 8, 4, [1] * 16)
+    clean = run_adapters(gpu_ctx, c)
+    some, h = torch.zeros(64, device="cuda"), ctypes.c_void_p()
+    for _ in range(2):
+        # A: 2^24 adapters x 16 ranks x 1024 float32, 2^40 bytes.  The allocation is the first step.
+        rc = lib.sg_adapter_bank_create(gpu_ctx.handle, some.data_ptr(), some.data_ptr(), some.data_ptr(), 0, 1 << 24, 16,
+                                        1024, 64, None, ctypes.byref(h))
+        assert rc == _lib.SG_ERR_NOMEM and not h.value
+        for name, call, _, outs in layer_calls(gpu_ctx):
+            say(name, "after a refused allocation")
+            call()
+        assert float((some + 1).sum()) == 64
+    assert torch.equal(run_adapters(gpu_ctx, c), clean)
+
+
+@pytest.mark.gpu
+def test_a_call_does_not_report_an_earlier_error(gpu_ctx):
+    """An error that another call of the thread left behind (a device that is not there) stays
+    that call's."""
+    from semantica_gpu import _lib
+    calls = layer_calls(gpu_ctx)
+    hip = _lib.load()  # (its symbols reach the HIP runtime that it is linked to)
+    try:
+        for name, call, _, _ in calls:
+            assert hip.hipSetDevice(1 << 20) != 0
+            say(name, "after another call's error")
+            call()
+    finally:
+        hip.hipGetLastError()
+    torch.cuda.synchronize()

@@ -185,10 +185,10 @@ __global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int pa
   // U steps' loads go out before their products (the compiler does not unroll loops
   // with matrix instructions); a step past the wave's last is zeros.  The first of
   // x go out before the rows' adapters are known.  Eight steps for one tile of one
-  // block, whose waves are few; four else (two for several adapters), so that four
-  // waves fit a SIMD and all of a batch's workgroups are resident (30,725 float32
-  // rows of 768: 34 us, 44 with eight, 35 with two; the next steps' x ahead of the
-  // products instead: 37 to 45).
+  // block, whose waves are few; four else (two for several adapters), which keeps three
+  // or four waves on a SIMD, two where two tiles meet four rank blocks or several adapters'
+  // two (30,725 float32 rows of 768, rank 16, four waves: 34 us, 44 with eight steps, 35 with
+  // two; the next steps' x ahead of the products instead: 37 to 45).
   constexpr int U = RT * NRB * G == 1 ? 8 : G == 1 || RT * NRB * G <= 4 ? 4 : 2;
   chunk<T> xf[U][RT];
   auto load_x = [&](int k, int tiles) {
@@ -621,23 +621,22 @@ hipError_t pack(const void* a, const void* b, int n, int rank, int in_dim, int o
 }
 
 // ---- launches ----------------------------------------------------------------------
-// Tiles a workgroup takes: more rows share its weight loads, as long as that leaves
-// `least` workgroups.
-int row_tiles(int rows, int rank_pad, int least) {
-  for (int rt = 4; rt > 1; rt /= 2)
-    if (rt * rank_pad <= 256 && (rows + rt * kTile - 1) / (rt * kTile) >= least) return rt;
-  return 1;
+// Tiles of 16 rows a workgroup takes: two, which share its weight loads, from ranks of
+// 128 down (up's u lies in LDS) and where that leaves two workgroups a CU at least.  Both sides,
+// us for 30,725 float32 rows of 768 (rank 16, 1280 columns) / 16384 bf16 rows of 2048
+// (rank 64, 8192 columns): up with one tile 107 / 198, two 111 / 162.  Four lose, down's for
+// want of registers: 32,768 float32 rows of 768, rank 16, 36 us for two's 32; 65,536
+// bf16 rows of 2048, rank 64, 106 for 100; 33,000 rows of eleven thousand sequences, bf16,
+// 2944 dims, rank 64, 534 for 339 (rank 32 of the first is the other way, 40 for 46);
+// up (an earlier form) 126 / 192 for 115 / 190.
+int row_tiles(int rows, int rank_pad) {
+  return 2 * rank_pad <= 256 && (rows + 2 * kTile - 1) / (2 * kTile) >= 2 * kCus ? 2 : 1;
 }
-// Two workgroups a CU at least.  Both sides, us for 30,725 float32 rows of 768 (rank
-// 16, 1280 columns) / 16384 bf16 rows of 2048 (rank 64, 8192 columns): up with one
-// tile 107 / 198, two 111 / 162, four (an earlier form) 126 / 192 for two's 115 / 190.
-int down_tiles(int rows, int rank_pad) { return row_tiles(rows, rank_pad, 2 * kCus); }
-int up_tiles(int rows, int rank_pad) { return std::min(2, row_tiles(rows, rank_pad, 2 * kCus)); }
 
 // Parts of down's sum: enough workgroups for the CUs, four steps of each wave at least.
 template <typename T>
 int parts_of(int rows, int in_dim, int rank_pad) {
-  const int rt = down_tiles(rows, rank_pad);
+  const int rt = row_tiles(rows, rank_pad);
   const int wgs = (rows + rt * kTile - 1) / (rt * kTile), steps = (in_dim + step_of<T>() - 1) / step_of<T>();
   const int most = std::min(kMostSplit, std::max(1, steps / (4 * kWaves)));
   return std::max(1, std::min(most, kCus / std::max(1, wgs)));
@@ -701,10 +700,12 @@ hipError_t apply(sg_adapters_args a, hipStream_t s) {
   a.row_ids = reinterpret_cast<int32_t*>(a.u + (parts > 1 ? parts * (size_t)a.rows : tiled) * a.rank_pad);
   a.back = reinterpret_cast<float*>(a.row_ids + a.rows);
   a.ready = parts == 1 && a.rank_pad <= 64 ? a.u : nullptr;
-  const int d = down_tiles(a.rows, a.rank_pad), u = up_tiles(a.rows, a.rank_pad);
-  const hipError_t e = d == 4 ? down<T, 4>(a, parts, s) : d == 2 ? down<T, 2>(a, parts, s) : down<T, 1>(a, parts, s);
-  if (e != hipSuccess) return e;
-  return u == 2 ? up<T, 2>(a, parts, s) : up<T, 1>(a, parts, s);
+  if (row_tiles(a.rows, a.rank_pad) == 2) {
+    const hipError_t e = down<T, 2>(a, parts, s);
+    return e == hipSuccess ? up<T, 2>(a, parts, s) : e;
+  }
+  const hipError_t e = down<T, 1>(a, parts, s);
+  return e == hipSuccess ? up<T, 1>(a, parts, s) : e;
 }
 
 }  // namespace

@@ -1171,3 +1171,77 @@ def test_a_call_does_not_report_an_earlier_error(gpu_ctx):
     finally:
         hip.hipGetLastError()
     torch.cuda.synchronize()
+
+
+# ---- the forms that only large batches take ------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rank", [16, 32, 48, 64])
+def test_adapters_of_33000_rows(gpu_ctx, dtype, rank):
+    """A thousand workgroups of two row tiles and more: tiles of one adapter, and several in
+    every tile."""
+    check_adapters(gpu_ctx, dtype, 136, 72, rank, 9, [33000], first=5, behind=3)
+    check_adapters(gpu_ctx, dtype, 136, 72, rank, 9, [3] * 10000 + [1, 0, 2999, 33], first=1, behind=9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rank,rows", [(16, 33000), (32, 33000), (64, 33000), (100, 33000), (256, 17000)])
+def test_adapters_over_wide_slices(gpu_ctx, dtype, rank, rows):
+    """2048 slices of 256 columns and more in the second product, the last one narrow, with
+    ranks that the first product leaves ready and with larger ones."""
+    check_adapters(gpu_ctx, dtype, 64, 520, rank, 7, [rows - 1003, 3, 500, 500], behind=1)
+    check_adapters(gpu_ctx, dtype, 64, 520, rank, 7, [5] * (rows // 5), in_place=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rank", [16, 32, 48, 100])
+def test_adapters_over_wide_slices_of_one_tile(gpu_ctx, dtype, rank):
+    """The same with rows too few for two tiles to a workgroup."""
+    check_adapters(gpu_ctx, dtype, 64, 2056, rank, 5, [4000, 1, 99], first=1)
+    check_adapters(gpu_ctx, dtype, 64, 2056, rank, 5, [2] * 2100, behind=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cols,rows", [("f32", 1100, 5000), ("bf16", 2100, 5000), ("f16", 4104, 4300),
+                                             ("f32", 5000, 2300), ("f32", 4097, 2300)])
+def test_norm_rows_one_after_another(gpu_ctx, dtype, cols, rows):
+    """Workgroups that share a row's sums and take several rows in turn, some of no sequence."""
+    check_norm(gpu_ctx, dtype, rows, cols, lens=[1, 0, 0, 7, rows - 15, 3], first=2, gate=True)
+    check_norm(gpu_ctx, dtype, rows, cols, lens=[1] * 700 + [rows - 2000], first=650, gate=True, post=False)
+    check_norm(gpu_ctx, dtype, rows, cols, in_place=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [8, 40, 72, 136, 200, 248])
+def test_attention_odd_head_dims_many_rows(gpu_ctx, dtype, hd):
+    """Head dims that fill no layout, with rows enough for waves of their own rows."""
+    lens = [300, 1, 0, 400, 63]
+    check_attention(gpu_ctx, hd, dtype, 24, 8, hd, lens, first=1, behind=2, **mask_of("all", 24, lens, 1, 2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [1, 2, 3])
+def test_attention_document_ids_at_any_alignment(gpu_ctx, at):
+    """Ids that start inside a 16-byte piece, one look over many tiles and a ragged end."""
+    rows, hd = 5003, 8
+    g = gen(64)
+    q, k, v = (rand(g, rows, hd, dtype="bf16") for _ in range(3))
+    ids = (torch.arange(rows) // 61).to(torch.int32)
+    ids[100:120] = -1
+    wide = torch.zeros(rows + at, dtype=torch.int32)
+    wide[at:] = ids
+    from semantica_gpu import kernels
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+    kernels.attention_masked(gpu_ctx, out, q.cuda(), k.cuda(), v.cuda(), 1, 1, offsets([rows]).cuda(),
+                             doc_ids=wide.cuda()[at:], causal=True)
+    out = out.cpu()
+    assert bool((out[100:120] == 0).all())
+    for doc in (0, 1, 40, int(ids.max())):
+        to = (ids == doc).nonzero()[:, 0]
+        want, mean, size = attention_ref(q[to], k[to], v[to], offsets([len(to)]), 1, 1, causal=True)
+        close(out[to], want, attention_tol("bf16", hd, want, mean, size), f"document {doc}")

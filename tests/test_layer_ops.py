@@ -1245,3 +1245,68 @@ def test_attention_document_ids_at_any_alignment(gpu_ctx, at):
         to = (ids == doc).nonzero()[:, 0]
         want, mean, size = attention_ref(q[to], k[to], v[to], offsets([len(to)]), 1, 1, causal=True)
         close(out[to], want, attention_tol("bf16", hd, want, mean, size), f"document {doc}")
+
+
+# ---- float32's bits -----------------------------------------------------------------------
+# float32 attention holds q, k, the weights and the values as two fp16 halves each and drops
+# the products of two low halves.  A half is off by 2^-12 of it at most, so an operand of two
+# by 2^-22 (2^-12 2^-11 and the low half's own 11 bits: 2^-23), and what is dropped is 2^-22 of a
+# product at most.  Over the terms of a sum these are of either sign: with normal q and k a
+# score (of deviation 1) is off by some 2^-22 for each of q, k and the dropped part, a weight by
+# as much, and an output of many keys, relative to the outputs' size, by those of the scores,
+# the weights, the values and the dropped part again: sqrt(6) 2^-22, and float32's sums of
+# hd products and of the keys, a few 2^-24.  Together below 2^-20.  The limit is twice that; any
+# one low half left out is off by 2^-12 / sqrt(3) / 2 and more (2^-14).
+FLOAT32_L2 = 2.0 ** -19
+
+
+def halves(x, low=True):
+    """x as two fp16 halves, its rows brought to 2^13 .. 2^14 first."""
+    e = torch.floor(torch.log2(x.abs().amax(-1, keepdim=True)))
+    y = x * 2.0 ** (13 - e)
+    hi = y.half().double()
+    lo = (y - hi).half().double() if low else torch.zeros_like(hi)
+    return hi, lo, 2.0 ** (e - 13)
+
+
+def attention_in_halves(q, k, v, without=""):
+    """One sequence and head as the float32 kernel multiplies it, `without` a low half."""
+    qh, ql, qe = halves(q.double(), "q" not in without)
+    kh, kl, ke = halves(k.double(), "k" not in without)
+    vh, vl, ve = halves(v.double(), "v" not in without)
+    s = (qh @ kh.T + qh @ kl.T + ql @ kh.T) * qe * ke.T / math.sqrt(q.shape[1])
+    p = torch.exp(s - s.amax(-1, keepdim=True))
+    w = p * ve.T
+    by = 2.0 ** (5 - torch.floor(torch.log2(w.amax(-1, keepdim=True))))
+    wh = (w * by).half().double()
+    wl = (w * by - wh).half().double() if "p" not in without else torch.zeros_like(wh)
+    return (wh @ vh + wh @ vl + wl @ vh) / by / p.sum(-1, keepdim=True)
+
+
+def l2(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_float32_limit_tells_a_lost_half(hd):
+    g = gen(hd)
+    q, k, v = (rand(g, 300, hd) for _ in range(3))
+    want, _, _ = attention_ref(q, k, v, offsets([300]), 1, 1)
+    assert l2(attention_in_halves(q, k, v), want) < FLOAT32_L2 / 2
+    for half in "qkpv":
+        assert l2(attention_in_halves(q, k, v, half), want) > 4 * FLOAT32_L2, half
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("lens,heads,kv_heads", [([300, 90], 3, 1), ([1501], 2, 1), ([700, 333], 24, 8)])
+def test_attention_keeps_float32s_bits(gpu_ctx, hd, lens, heads, kv_heads):
+    g, off = gen(65), offsets(lens)
+    rows = int(off[-1])
+    q, k, v = (rand(g, rows, c * hd) for c in (heads, kv_heads, kv_heads))
+    slopes = torch.tensor([2.0 ** -(4 + h % 4) for h in range(heads)])
+    for kw in ({}, {"causal": True, "softcap": 20.0}, {"softcap": 2.0}, {"slopes": slopes, "window": 200}):
+        got = run_attention(gpu_ctx, q, k, v, off, heads, kv_heads, **kw)
+        want, _, _ = attention_ref(q, k, v, off, heads, kv_heads, **kw)
+        say("float32 bits", hd, lens, sorted(kw), l2(got, want))
+        assert l2(got, want) < FLOAT32_L2

@@ -54,7 +54,14 @@ struct Span {
   int rows, cols, dtype;
   uintptr_t lo() const { return reinterpret_cast<uintptr_t>(p); }
   uintptr_t hi() const { return lo() + ((uintptr_t)(rows - 1) * ld + cols) * elem_bytes(dtype); }
-  bool overlaps(const Span& o) const { return lo() < o.hi() && o.lo() < hi(); }
+  bool overlaps(const Span& o) const {
+    if (lo() >= o.hi() || o.lo() >= hi()) return false;
+    const uintptr_t step = (uintptr_t)ld * elem_bytes(dtype);
+    if (ld != o.ld || dtype != o.dtype || step == 0) return true;
+    // Columns of one wide tensor: where o's rows begin within (or before) this one's.
+    const uintptr_t at = o.lo() >= lo() ? (o.lo() - lo()) % step : (step - (lo() - o.lo()) % step) % step;
+    return at < (uintptr_t)cols * elem_bytes(dtype) || at + (uintptr_t)o.cols * elem_bytes(dtype) > step;
+  }
   bool same(const Span& o) const { return p == o.p && ld == o.ld; }
 };
 

@@ -372,7 +372,7 @@ typedef struct sg_attn_mask {
  * at worst); 16-bit types round the weights to their type, and tanh is off by
  * 2^-19 at most.  head_dim: a multiple of 8 up to 256; pointers 16-byte aligned,
  * strides whole 16 bytes (k's and v's up to 2^22 elements); out apart from q, k
- * and v.
+ * and v (other columns of one tensor, with the same stride, are).
  * mask NULL: scale 1/sqrt(head_dim), nothing hidden. */
 int sg_attention_masked(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int64_t ldq, const void *k, int64_t ldk,
                         const void *v, int64_t ldv, int32_t dtype, int32_t n_heads, int32_t n_kv_heads,
@@ -389,7 +389,8 @@ int sg_attention_masked(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int6
  * cols 1 .. 8192, rows and strides of any whole elements (whole 16 bytes are
  * faster).  The squares are summed in float32, as sg_rmsnorm's are: values past
  * 2^63 overflow them.  sum and xn may each be x or h (same pointer and stride);
- * otherwise no output overlaps another tensor. */
+ * otherwise no output overlaps another tensor (other columns of the same one, with
+ * the same stride, do not). */
 int sg_block_norm(sg_ctx *ctx, void *xn, int64_t ldxn, void *sum, int64_t lds, const void *x, int64_t ldx,
                   const void *h, int64_t ldh, int32_t dtype, int32_t rows, int32_t cols, const float *w_post,
                   const float *w_pre, float eps, const float *gate, float scale, const int32_t *d_seq_offsets,
@@ -419,7 +420,8 @@ int sg_adapters_work_bytes(const sg_adapter_bank *bank, int32_t rows, size_t *by
  * sg_adapters_work_bytes of device memory, 16-byte aligned, in use until the
  * call's work on `stream` is done (one for each stream or graph that runs at the
  * same time; a graph keeps its address, and the bank's).  dst does not overlap x,
- * or base unless it is base; work overlaps none of them.  The sums are float32 and
+ * or base unless it is base (other columns of one tensor, with the same stride, do not
+ * overlap); work lies outside them all.  The sums are float32 and
  * in the same order every time. */
 int sg_adapters_apply(sg_ctx *ctx, void *dst, int64_t ldd, const void *base, int64_t ldb, const sg_adapter_bank *bank,
                       const void *x, int64_t ldx, int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq,

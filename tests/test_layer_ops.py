@@ -1310,3 +1310,67 @@ def test_attention_keeps_float32s_bits(gpu_ctx, hd, lens, heads, kv_heads):
         want, _, _ = attention_ref(q, k, v, off, heads, kv_heads, **kw)
         say("float32 bits", hd, lens, sorted(kw), l2(got, want))
         assert l2(got, want) < FLOAT32_L2
+
+
+# ---- tensors that are columns of one -------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_outputs_beside_their_inputs_in_one_tensor(gpu_ctx, dtype):
+    """Inputs and outputs as columns of one wide tensor, in any order; what lies between stays."""
+    from semantica_gpu import kernels
+    g, rows, off = gen(71), 70, offsets([50, 20])
+    t = dt(dtype)
+
+    def wide(*cols):
+        """One tensor of these widths side by side, eight columns of sevens behind each."""
+        w = torch.full((rows, sum(cols) + 8 * len(cols)), 7.0, dtype=t, device="cuda")
+        at = np.concatenate([[0], np.cumsum([c + 8 for c in cols])])
+        parts = [w[:, a:a + c] for a, c in zip(at, cols)]
+        for p in parts:
+            p.copy_(rand(g, *p.shape).to(t).cuda())
+        return parts, [w[:, a + c:a + c + 8] for a, c in zip(at, cols)]
+
+    (out, k, q, v), gaps = wide(128, 64, 128, 64)
+    kernels.attention_masked(gpu_ctx, out, q, k, v, 2, 1, off.cuda(), causal=True)
+    want, mean, size = attention_ref(q.cpu(), k.cpu(), v.cpu(), off, 2, 1, causal=True)
+    close(out, want, attention_tol(dtype, 64, want, mean, size), "attention")
+    assert all(bool((p == 7).all()) for p in gaps)
+
+    (xn, x, s, h), gaps = wide(96, 96, 96, 96)
+    w = torch.randn(96, generator=g)
+    kernels.block_norm(gpu_ctx, xn, s, x, h, w.cuda(), w.cuda(), 1e-6)
+    ws, wn, ssize, nsize = norm_ref(x.cpu(), h.cpu(), w, w, 1e-6, None, 1.0, None)
+    close(s, ws, U[dtype] * ws.abs() + 58 * F * ssize + TINY[dtype], "sum")
+    close(xn, wn, U[dtype] * wn.abs() + 116 * F * nsize + TINY[dtype], "xn")
+    assert all(bool((p == 7).all()) for p in gaps)
+
+    (x, dst, base), gaps = wide(64, 72, 72)
+    a, b = rand(g, 2, 8, 64, by=0.1, dtype=dtype), rand(g, 2, 72, 8, dtype=dtype)
+    scales, ids = torch.tensor([0.5, 2.0]), torch.tensor([1, 0], dtype=torch.int32)
+    bank = kernels.AdapterBank(gpu_ctx, a.cuda(), b.cuda(), scales.cuda())
+    kernels.adapters_apply(gpu_ctx, dst, base, bank, x, off.cuda(), ids.cuda())
+    want, size = adapters_ref(x.cpu(), base.cpu(), a, b, scales, off, ids)
+    close(dst, want, U[dtype] * want.abs() + (104 * F + 2.0 ** -16) * size + TINY[dtype], "adapters")
+    assert all(bool((p == 7).all()) for p in gaps)
+    bank.close()
+
+
+# heads of 128 in float16: 256 columns of out and q, 128 of k and v; all of them columns of one
+# tensor of 1024, q's first.
+BESIDE = {**ATT, **{n: 1024 for n in ("ldo", "ldq", "ldk", "ldv")}, "q": 2 << 40, "out": (2 << 40) + 2 * 256,
+          "k": (2 << 40) + 2 * 512, "v": (2 << 40) + 2 * 640}
+
+
+@pytest.mark.parametrize("change", [
+    {"out": (2 << 40) + 2 * 248}, {"out": (2 << 40) + 2 * 264}, {"out": (2 << 40) + 2 * 760},
+    {"out": (2 << 40) + 2 * (1024 + 248)}, {"out": (2 << 40) - 2 * 248}, {"out": (2 << 40) + 2 * (8 * 1024 + 776)},
+    {"ldo": 512}])
+def test_attention_refuses_columns_that_meet(change):
+    """A piece of 16 bytes too far to either side, in the same row or another; another stride."""
+    from semantica_gpu import _lib
+    c = {**BESIDE, **change}
+    _refused(_lib.load().sg_attention_masked(_addr(), c["out"], c["ldo"], c["q"], c["ldq"], c["k"], c["ldk"], c["v"], c["ldv"],
+                                             c["dtype"], c["heads"], c["kv"], c["hd"], c["rows"], c["off"], c["n_seq"], None,
+                                             None), "overlaps")

@@ -339,9 +339,12 @@ def adapters_apply(ctx, dst, base, bank: AdapterBank, x, offsets, adapter_ids, *
     b, ldb = _rows_of(ctx, "base", base, rows, bank.out_dim, bank.dtype)
     off, n_seq = _offsets(ctx, offsets)
     if work is None:
-        work = torch.empty(max(bank.work_bytes(rows), 16), dtype=torch.uint8, device=x.device)
-        if stream is not None:  # not to be handed out again before the call's stream is done with it
-            work.record_stream(torch.cuda.ExternalStream(stream, device=x.device))
+        size = max(bank.work_bytes(rows), 16)
+        if stream is None:
+            work = torch.empty(size, dtype=torch.uint8, device=x.device)
+        else:  # of that stream: what the current one gave back, its work may still write
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=x.device)):
+                work = torch.empty(size, dtype=torch.uint8, device=x.device)
     _lib.check(ctx.lib.sg_adapters_apply(ctx.handle, d, ldd, b, ldb, bank.handle, xp, ldx, rows, off, n_seq,
                                          _vec(ctx, "adapter_ids", adapter_ids, n_seq, torch.int32),
                                          _vec(ctx, "work", work, None, torch.uint8), work.numel(),

@@ -1374,3 +1374,46 @@ def test_attention_refuses_columns_that_meet(change):
     _refused(_lib.load().sg_attention_masked(_addr(), c["out"], c["ldo"], c["q"], c["ldq"], c["k"], c["ldk"], c["v"], c["ldv"],
                                              c["dtype"], c["heads"], c["kv"], c["hd"], c["rows"], c["off"], c["n_seq"], None,
                                              None), "overlaps")
+
+
+@pytest.mark.gpu
+def test_default_workspace_is_the_streams_own(gpu_ctx):
+    """A workspace for another stream is not memory that the current one gave back and may
+    still be writing."""
+    from semantica_gpu import kernels
+    c = adapter_case("f32", 64, 72, 32, 3, [20000], seed=5)
+    bank = kernels.AdapterBank(gpu_ctx, c["a"].cuda(), c["b"].cuda(), c["scales"].cuda())
+    x, base, off, ids = c["x"].cuda(), c["base"].cuda(), c["off"].cuda(), torch.tensor([1], dtype=torch.int32, device="cuda")
+    need, dst, side = bank.work_bytes(20000), torch.full_like(base, 7.0), torch.cuda.Stream()
+
+    class Spy:  # takes the call's workspace and runs nothing
+        handle, device = gpu_ctx.handle, gpu_ctx.device
+
+        def __init__(self):
+            self.lib = self
+
+        def sg_adapters_apply(self, *args):
+            self.work, self.bytes = args[12], args[13]
+            return 0
+
+    spy = Spy()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    back = torch.empty(need, dtype=torch.uint8, device="cuda")
+    at = back.data_ptr()
+    del back
+    seen = []
+    for _ in range(2):
+        kernels.adapters_apply(spy, dst, base, bank, x, off, ids, stream=side.cuda_stream)
+        assert spy.bytes >= need and abs(spy.work - at) >= need
+        seen.append(spy.work)
+    assert seen[0] == seen[1]  # in order on its own stream
+    kernels.adapters_apply(spy, dst, base, bank, x, off, ids)
+    assert spy.work == at
+    side.wait_stream(torch.cuda.current_stream())
+    kernels.adapters_apply(gpu_ctx, dst, base, bank, x, off, ids, stream=side.cuda_stream)
+    side.synchronize()
+    c["ids"] = ids.cpu()
+    want, size = adapters_ref(c["x"], c["base"], c["a"], c["b"], c["scales"], c["off"], c["ids"])
+    close(dst, want, U["f32"] * want.abs() + 128 * F * size + TINY["f32"], "adapters")
+    bank.close()

@@ -21,6 +21,7 @@ workspace.
 """
 from __future__ import annotations
 
+import collections
 import ctypes
 
 import numpy as np
@@ -293,9 +294,25 @@ def block_norm(ctx, xn, sum, x, h, w_post, w_pre, eps, *, gate=None, scale=1.0, 
                                      n_seq, _stream_of(ctx, stream)))
 
 
+_COLLECTED = collections.deque()  # banks' handles
+
+
+def _free_collected():
+    while _COLLECTED:
+        try:
+            lib, handle = _COLLECTED.popleft()
+        except IndexError:  # another thread's
+            return
+        lib.sg_adapter_bank_free(handle)
+
+
 class AdapterBank:
     """Low-rank adapters of one projection (sg_adapter_bank_create): a [n, rank, in_dim]
-    and b [n, out_dim, rank] device tensors, scales float32 [n]."""
+    and b [n, out_dim, rank] device tensors, scales float32 [n].
+
+    Making and closing a bank wait for the device and are not for a time when any thread
+    captures a graph.  A bank that is dropped may be collected at such a time, so its memory
+    is kept until the next one is made or closed; close() frees it at once."""
 
     def __init__(self, ctx, a, b, scales, stream=None):
         self.handle = None
@@ -304,6 +321,7 @@ class AdapterBank:
             raise ValueError(f"b: shape {tuple(b.shape)} beside a's {tuple(a.shape)}")
         self.ctx, self.lib, self.dtype = ctx, ctx.lib, a.dtype
         self.n, self.rank, self.in_dim, self.out_dim = n, rank, in_dim, b.shape[1]
+        _free_collected()
         h = ctypes.c_void_p()
         _lib.check(self.lib.sg_adapter_bank_create(
             ctx.handle, _vec(ctx, "a", a, None, a.dtype), _vec(ctx, "b", b, None, a.dtype),
@@ -318,12 +336,14 @@ class AdapterBank:
         return size.value
 
     def close(self):
+        _free_collected()
         if self.handle:
             self.lib.sg_adapter_bank_free(self.handle)
             self.handle = None
 
     def __del__(self):
-        self.close()
+        if self.handle and _COLLECTED is not None:  # (None: the interpreter ends)
+            _COLLECTED.append((self.lib, self.handle))
 
 
 def adapters_apply(ctx, dst, base, bank: AdapterBank, x, offsets, adapter_ids, *, work=None, stream=None):

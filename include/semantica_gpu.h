@@ -401,7 +401,8 @@ int sg_block_norm(sg_ctx *ctx, void *xn, int64_t ldxn, void *sum, int64_t lds, c
  * contiguous, type dtype; an adapter of a smaller rank is padded with zeros),
  * d_scales [n_adapters] float32.  rank 1 .. 256, in_dim and out_dim multiples of
  * 8.  The arrays are read on `stream` and may be freed after return, which waits
- * for that (not to be captured).  Freeing the bank waits for the device. */
+ * for that.  Freeing the bank waits for the device.  Neither is for a time when a thread
+ * captures a graph. */
 typedef struct sg_adapter_bank sg_adapter_bank;
 int sg_adapter_bank_create(sg_ctx *ctx, const void *d_a, const void *d_b, const float *d_scales, int32_t dtype,
                            int32_t n_adapters, int32_t rank, int32_t in_dim, int32_t out_dim, void *stream,

@@ -1417,3 +1417,42 @@ def test_default_workspace_is_the_streams_own(gpu_ctx):
     want, size = adapters_ref(c["x"], c["base"], c["a"], c["b"], c["scales"], c["off"], c["ids"])
     close(dst, want, U["f32"] * want.abs() + 128 * F * size + TINY["f32"], "adapters")
     bank.close()
+
+
+@pytest.mark.gpu
+def test_banks_collected_during_a_capture(gpu_ctx):
+    """By the capturing thread and by another: the graph is whole, and the memory comes back
+    with the next bank that is made or closed."""
+    import threading
+    from semantica_gpu import kernels
+    calls = layer_calls(gpu_ctx, "bf16", 7)
+    for _, call, _, _ in calls:
+        call()
+    torch.cuda.synchronize()
+    want = [t.clone() for _, _, _, outs in calls for t in outs]
+    a, b, scales = (torch.zeros(s, device="cuda") for s in ((2048, 16, 1024), (2048, 1024, 16), (2048,)))
+    banks = [kernels.AdapterBank(gpu_ctx, a, b, scales) for _ in range(2)]
+    last = kernels.AdapterBank(gpu_ctx, a[:1], b[:1], scales[:1])
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    graph = torch.cuda.CUDAGraph()
+    say("capturing")
+    with torch.cuda.graph(graph):
+        calls[0][1]()
+        banks.pop()
+        calls[1][1]()
+        other = threading.Thread(target=banks.clear)
+        other.start()
+        other.join()
+        calls[2][1]()
+    last.close()
+    assert torch.cuda.mem_get_info()[0] >= free + 4 * (a.numel() + b.numel())
+    for _ in range(3):
+        for _, _, _, outs in calls:
+            for t in outs:
+                t.fill_(7.0)
+        say("replay")
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip([t for _, _, _, outs in calls for t in outs], want):
+            assert torch.equal(x[3:434], y[3:434])

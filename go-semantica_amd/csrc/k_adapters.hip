@@ -564,40 +564,43 @@ __global__ __launch_bounds__(kNT) void k_adapter_up_ready(sg_adapters_args a, in
 }
 
 // ---- packing ---------------------------------------------------------------------
+// (In a loop: a bank may have more chunks than a launch has threads, 2^32.)
+constexpr int kPackBlocks = 1 << 16;
+
 template <typename T>
 __global__ void k_pack_a(const T* __restrict__ a, int rank, int in_dim, int rbs, int steps, int64_t total,
                          chunk<T>* __restrict__ out) {
   constexpr int V = elem<T>::vec;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= total) return;
-  const int lane = (int)(i & 63);
-  const int64_t f = i >> 6;
-  const int k = (int)(f % steps), rb = (int)(f / steps % rbs);
-  const int64_t id = f / steps / rbs;
-  const int r = 16 * rb + (lane & 15), c = k * 4 * V + (lane >> 4) * V;
-  chunk<T> o{};
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int lane = (int)(i & 63);
+    const int64_t f = i >> 6;
+    const int k = (int)(f % steps), rb = (int)(f / steps % rbs);
+    const int64_t id = f / steps / rbs;
+    const int r = 16 * rb + (lane & 15), c = k * 4 * V + (lane >> 4) * V;
+    chunk<T> o{};
 #pragma unroll
-  for (int e = 0; e < V; e++)
-    if (r < rank && c + e < in_dim) o.v[e] = a[(id * rank + r) * in_dim + c + e];
-  out[i] = o;
+    for (int e = 0; e < V; e++)
+      if (r < rank && c + e < in_dim) o.v[e] = a[(id * rank + r) * in_dim + c + e];
+    out[i] = o;
+  }
 }
 
 template <typename T>
 __global__ void k_pack_b(const T* __restrict__ b, int rank, int out_dim, int rbs, int pairs, int64_t total,
                          chunk<T>* __restrict__ out) {
   constexpr int V = elem<T>::vec, BL = V == 4 ? 64 : 32;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= total) return;
-  const int lane = (int)(i % BL);
-  const int64_t f = i / BL;
-  const int rb = (int)(f % rbs), j = (int)(f / rbs % 2), p = (int)(f / rbs / 2 % pairs);
-  const int64_t id = f / rbs / 2 / pairs;
-  const int m = lane & 15, col = 32 * p + 8 * (m >> 2) + 4 * j + (m & 3), r = 16 * rb + (lane >> 4) * V;
-  chunk<T> o{};
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int lane = (int)(i % BL);
+    const int64_t f = i / BL;
+    const int rb = (int)(f % rbs), j = (int)(f / rbs % 2), p = (int)(f / rbs / 2 % pairs);
+    const int64_t id = f / rbs / 2 / pairs;
+    const int m = lane & 15, col = 32 * p + 8 * (m >> 2) + 4 * j + (m & 3), r = 16 * rb + (lane >> 4) * V;
+    chunk<T> o{};
 #pragma unroll
-  for (int e = 0; e < V; e++)
-    if (col < out_dim && r + e < rank) o.v[e] = b[(id * out_dim + col) * rank + r + e];
-  out[i] = o;
+    for (int e = 0; e < V; e++)
+      if (col < out_dim && r + e < rank) o.v[e] = b[(id * out_dim + col) * rank + r + e];
+    out[i] = o;
+  }
 }
 
 template <typename T>
@@ -613,11 +616,12 @@ template <typename T>
 hipError_t pack(const void* a, const void* b, int n, int rank, int in_dim, int out_dim, void* wa, void* wb, hipStream_t s) {
   const int rbs = sgk::adapters_rank_pad(rank) / 16;
   const int64_t na = a_chunks<T>(n, rank, in_dim), nb = b_chunks<T>(n, rank, out_dim);
-  const hipError_t e = sgp::run_kernel(k_pack_a<T>, dim3((unsigned)((na + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(a),
-                                       rank, in_dim, rbs, (in_dim + step_of<T>() - 1) / step_of<T>(), na, static_cast<chunk<T>*>(wa));
+  auto blocks = [](int64_t chunks) { return dim3((unsigned)std::min<int64_t>((chunks + 255) / 256, kPackBlocks)); };
+  const hipError_t e = sgp::run_kernel(k_pack_a<T>, blocks(na), dim3(256), 0, s, static_cast<const T*>(a), rank, in_dim, rbs,
+                                       (in_dim + step_of<T>() - 1) / step_of<T>(), na, static_cast<chunk<T>*>(wa));
   if (e != hipSuccess) return e;
-  return sgp::run_kernel(k_pack_b<T>, dim3((unsigned)((nb + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(b), rank, out_dim,
-                         rbs, (out_dim + 31) / 32, nb, static_cast<chunk<T>*>(wb));
+  return sgp::run_kernel(k_pack_b<T>, blocks(nb), dim3(256), 0, s, static_cast<const T*>(b), rank, out_dim, rbs,
+                         (out_dim + 31) / 32, nb, static_cast<chunk<T>*>(wb));
 }
 
 // ---- launches ----------------------------------------------------------------------

@@ -212,7 +212,6 @@ int sg_adapter_bank_create(sg_ctx* ctx, const void* d_a, const void* d_b, const 
     return fail(SG_ERR_INVALID, "%d adapters: too many for one bank", n_adapters);
   const size_t na = sgk::adapters_a_bytes(dtype, n_adapters, rank, in_dim);
   const size_t nb = sgk::adapters_b_bytes(dtype, n_adapters, rank, out_dim);
-  if (std::max(na, nb) / 4096 > UINT32_MAX / 2) return fail(SG_ERR_INVALID, "%d adapters: too many for one bank", n_adapters);
   OnDevice on;
   SG_TRY(on.enter(sgi::ctx_device(ctx)));
   sg_adapter_bank* b = new (std::nothrow) sg_adapter_bank;

@@ -1456,3 +1456,30 @@ def test_banks_collected_during_a_capture(gpu_ctx):
         torch.cuda.synchronize()
         for x, y in zip([t for _, _, _, outs in calls for t in outs], want):
             assert torch.equal(x[3:434], y[3:434])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_bank_of_more_pieces_than_packing_threads(gpu_ctx, dtype):
+    """Over 2^24 pieces of 16 bytes in both arrays, which the packing threads take in turn."""
+    from semantica_gpu import kernels
+    n, rank, wide = (1100, 16, 16384) if dtype == "bf16" else (550, 16, 16384)
+    g = gen(81)
+    by = torch.randn(n, generator=g)
+    a0, b0 = rand(g, rank, wide, by=wide ** -0.5, dtype=dtype), rand(g, wide, rank, dtype=dtype)
+    a = (a0.cuda() * by.to(a0.dtype).cuda()[:, None, None]).contiguous()
+    b = (b0.cuda() * by.flip(0).to(b0.dtype).cuda()[:, None, None]).contiguous()
+    assert a.numel() * a.element_size() > 16 << 24
+    say("bank", dtype, a.numel() * a.element_size() * 2 >> 20, "MiB")
+    scales = torch.rand(n, generator=g) + 0.5
+    bank = kernels.AdapterBank(gpu_ctx, a, b, scales.cuda())
+    ids = torch.tensor([0, 1, n // 2, n - 2, n - 1], dtype=torch.int32)
+    off, rows = offsets([2, 1, 3, 1, 2]), 9
+    x, base = rand(g, rows, wide, dtype=dtype), rand(g, rows, wide, dtype=dtype)
+    dst = torch.empty(rows, wide, dtype=dt(dtype), device="cuda")
+    kernels.adapters_apply(gpu_ctx, dst, base.cuda(), bank, x.cuda(), off.cuda(), ids.cuda())
+    bank.close()
+    used = ids.long()
+    want, size = adapters_ref(x, base, a[used].cpu(), b[used].cpu(), scales[used], off, torch.arange(5))
+    rel = (wide + rank + 32) * F + (0 if dtype == "f32" else 2.0 ** -16)
+    close(dst, want, U[dtype] * want.abs() + rel * size + TINY[dtype], "adapters")

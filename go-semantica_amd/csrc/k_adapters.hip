@@ -675,7 +675,6 @@ template <typename T, int RT, int PAIRS>
 hipError_t up(const sg_adapters_args& a, int parts, hipStream_t s) {
   constexpr int CW = 128 * PAIRS;
   const int tiles = (a.rows + RT * kTile - 1) / (RT * kTile), slices = (a.out_dim + CW - 1) / CW;
-  if ((int64_t)tiles * slices > INT32_MAX) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tiles * slices);
   if (a.ready) {
     if (a.rank_pad == 16) return sgp::run_kernel(k_adapter_up_ready<T, RT, PAIRS, 1>, grid, dim3(kNT), 0, s, a, slices);
@@ -742,6 +741,11 @@ size_t adapters_work_bytes(int dtype, int rows, int in_dim, int rank_pad) {
     if (parts_at(r) >= p) most = std::max(most, bytes((size_t)p * r, r));
   }
   return most;
+}
+// Up's, with slices of 256 columns (those of 128 are for small batches, as down's parts are).
+int64_t adapters_threads(int rows, int out_dim, int rank_pad) {
+  const int rt = row_tiles(rows, rank_pad);
+  return ((int64_t)rows + rt * kTile - 1) / (rt * kTile) * ((out_dim + 255) / 256) * kNT;
 }
 hipError_t adapters_apply(const sg_adapters_args& a, int dtype, hipStream_t s) {
   if (dtype == SG_F32) return apply<float>(a, s);

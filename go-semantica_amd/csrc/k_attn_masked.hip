@@ -972,7 +972,6 @@ template <typename T, int D, int QT, int RW, int KW>
 hipError_t launch(const sg_attn_masked_args& a, hipStream_t s) {
   typedef form<T, D, QT, RW, KW> F;
   const int64_t tiles = ((int64_t)a.rows + F::BM - 1) / F::BM;
-  if (tiles * a.heads > INT32_MAX) return hipErrorInvalidValue;
   return sgp::run_kernel(k_attn_masked<T, D, QT, RW, KW>, dim3((unsigned)(tiles * a.heads)), dim3(F::NT), F::LDS, s, a,
                          (int)tiles);
 }
@@ -1015,6 +1014,10 @@ hipError_t by_dim(const sg_attn_masked_args& a, hipStream_t s) {
 
 namespace sgk {
 
+// (64 rows to 256 threads are no more than 128 to 512; rows are shared in small batches only.)
+int64_t attention_masked_threads(int dtype, int rows, int heads) {
+  return ((int64_t)rows + 127) / 128 * heads * (dtype == SG_F32 ? 512 : 256);
+}
 hipError_t attention_masked(const sg_attn_masked_args& a, int dtype, hipStream_t s) {
   if (dtype == SG_F32) return by_dim<float>(a, s);
   if (dtype == SG_F16) return by_dim<_Float16>(a, s);

@@ -313,6 +313,10 @@ hipError_t attention_exact(const float* q, int ldq, const float* k, const float*
 constexpr int kBlockNormCols = 8192;  // longest row
 hipError_t block_norm(const sg_block_norm_args& a, int dtype, hipStream_t s);
 hipError_t attention_masked(const sg_attn_masked_args& a, int dtype, hipStream_t s);
+// Threads of the call's largest launch, at most: one dimension of a launch takes kMostThreads.
+constexpr int64_t kMostThreads = UINT32_MAX;
+int64_t attention_masked_threads(int dtype, int rows, int heads);
+int64_t adapters_threads(int rows, int out_dim, int rank_pad);
 // Adapter weights, one after another: a [n][rank][in], b [n][out][rank] (contiguous)
 // into the fragment order of k_adapters.hip, rank and in_dim padded with zeros.
 constexpr int kAdapterMaxRank = 256;

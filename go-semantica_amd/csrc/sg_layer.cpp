@@ -109,6 +109,8 @@ int sg_attention_masked(sg_ctx* ctx, void* out, int64_t ldo, const void* q, int6
   if (m.prefix && !m.causal) return fail(SG_ERR_INVALID, "a prefix needs causal");
   if (rows == 0) return SG_OK;
   if ((int64_t)n_heads * head_dim > INT32_MAX) return fail(SG_ERR_INVALID, "rows of more than 2^31 elements");
+  if (sgk::attention_masked_threads(dtype, rows, n_heads) > sgk::kMostThreads)
+    return fail(SG_ERR_INVALID, "%d rows of %d heads are more than one launch takes", rows, n_heads);
   const int qd = n_heads * head_dim, kd = n_kv_heads * head_dim;
   const Span so{out, ldo, rows, qd, dtype}, sq{q, ldq, rows, qd, dtype}, sk{k, ldk, rows, kd, dtype},
       sv{v, ldv, rows, kd, dtype};
@@ -268,6 +270,8 @@ int sg_adapters_apply(sg_ctx* ctx, void* dst, int64_t ldd, const void* base, int
   SG_TRY(check_batch(d_off, rows, n_seq));
   if (bank->device != sgi::ctx_device(ctx)) return fail(SG_ERR_INVALID, "the adapters lie on another device");
   if (rows == 0) return SG_OK;
+  if (sgk::adapters_threads(rows, bank->out_dim, bank->rank_pad) > sgk::kMostThreads)
+    return fail(SG_ERR_INVALID, "%d rows of %d columns are more than one launch takes", rows, bank->out_dim);
   const Span sd{dst, ldd, rows, bank->out_dim, bank->dtype}, sb{base, ldb, rows, bank->out_dim, bank->dtype},
       sx{x, ldx, rows, bank->in_dim, bank->dtype};
   SG_TRY(check_pieces("dst", sd));

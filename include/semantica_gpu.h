@@ -373,6 +373,7 @@ typedef struct sg_attn_mask {
  * 2^-19 at most.  head_dim: a multiple of 8 up to 256; pointers 16-byte aligned,
  * strides whole 16 bytes (k's and v's up to 2^22 elements); out apart from q, k
  * and v (other columns of one tensor, with the same stride, are).
+ * rows * n_heads: up to 2^30 or a little less.
  * mask NULL: scale 1/sqrt(head_dim), nothing hidden. */
 int sg_attention_masked(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int64_t ldq, const void *k, int64_t ldk,
                         const void *v, int64_t ldv, int32_t dtype, int32_t n_heads, int32_t n_kv_heads,
@@ -422,8 +423,8 @@ int sg_adapters_work_bytes(const sg_adapter_bank *bank, int32_t rows, size_t *by
  * call's work on `stream` is done (one for each stream or graph that runs at the
  * same time; a graph keeps its address, and the bank's).  dst does not overlap x,
  * or base unless it is base (other columns of one tensor, with the same stride, do not
- * overlap); work lies outside them all.  The sums are float32 and
- * in the same order every time. */
+ * overlap); work lies outside them all.  rows * out_dim: up to 2^36 or a little less.
+ * The sums are float32 and in the same order every time. */
 int sg_adapters_apply(sg_ctx *ctx, void *dst, int64_t ldd, const void *base, int64_t ldb, const sg_adapter_bank *bank,
                       const void *x, int64_t ldx, int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq,
                       const int32_t *d_adapter_ids, void *work, size_t work_bytes, void *stream);

@@ -1483,3 +1483,15 @@ def test_bank_of_more_pieces_than_packing_threads(gpu_ctx, dtype):
     want, size = adapters_ref(x, base, a[used].cpu(), b[used].cpu(), scales[used], off, torch.arange(5))
     rel = (wide + rank + 32) * F + (0 if dtype == "f32" else 2.0 ** -16)
     close(dst, want, U[dtype] * want.abs() + rel * size + TINY[dtype], "adapters")
+
+
+@pytest.mark.parametrize("change", [
+    {"heads": 64, "kv": 1, "hd": 8, "rows": 1 << 26}, {"heads": 65535, "kv": 1, "hd": 8, "rows": 1 << 21},
+    {"heads": 1, "kv": 1, "hd": 8, "rows": (1 << 31) - (1 << 17), "dtype": 0}])
+def test_attention_refuses_more_than_a_launch(change):
+    """2^32 threads and more."""
+    from semantica_gpu import _lib
+    c = {**ATT, **change, "ldo": 8 * 65536, "ldq": 8 * 65536}
+    _refused(_lib.load().sg_attention_masked(_addr(), c["out"], c["ldo"], c["q"], c["ldq"], c["k"], c["ldk"], c["v"], c["ldv"],
+                                             c["dtype"], c["heads"], c["kv"], c["hd"], c["rows"], c["off"], c["n_seq"], None,
+                                             None), "one launch")

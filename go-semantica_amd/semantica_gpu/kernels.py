@@ -238,8 +238,17 @@ def _vec(ctx, name, t, n, dtype):
     return t.data_ptr()
 
 
+_MOST = 2**31 - 1  # what the C ABI's counts hold; ctypes would drop the bits above
+
+
+def _too_many(what, n):
+    raise ValueError(f"{what}: {n} are more than a call takes")
+
+
 def _offsets(ctx, t):
     """The pointer of the CSR offsets and the number of sequences."""
+    if t.numel() > _MOST:
+        _too_many("offsets", t.numel())
     return _vec(ctx, "offsets", t, None, _torch().int32), t.numel() - 1
 
 
@@ -259,6 +268,8 @@ def attention_masked(ctx, out, q, k, v, n_heads, n_kv_heads, offsets, *, scale=0
     slopes float32 [n_heads]; doc_ids int32 [rows]; prefix int32 [n_seq]."""
     torch = _torch()
     rows, qd = q.shape
+    if rows > _MOST or qd > _MOST:
+        _too_many("rows or columns of q", max(rows, qd))
     hd = qd // max(n_heads, 1)
     if hd * n_heads != qd:
         raise ValueError(f"q: {qd} columns for {n_heads} heads")
@@ -270,7 +281,7 @@ def attention_masked(ctx, out, q, k, v, n_heads, n_kv_heads, offsets, *, scale=0
     off, n_seq = _offsets(ctx, offsets)
     mask = _lib.AttnMask(scale, softcap, _vec(ctx, "slopes", slopes, n_heads, torch.float32),
                          _vec(ctx, "doc_ids", doc_ids, rows, torch.int32),
-                         _vec(ctx, "prefix", prefix, n_seq, torch.int32), causal, min(window, 2**31 - 1))
+                         _vec(ctx, "prefix", prefix, n_seq, torch.int32), causal, max(-1, min(window, _MOST)))
     _lib.check(ctx.lib.sg_attention_masked(ctx.handle, o, ldo, qp, ldq, kp, ldk, vp, ldv, _dtype(q), n_heads, n_kv_heads,
                                            hd, rows, off, n_seq, mask, _stream_of(ctx, stream)))
 
@@ -282,6 +293,8 @@ def block_norm(ctx, xn, sum, x, h, w_post, w_pre, eps, *, gate=None, scale=1.0, 
     gate float32 [cols], or [n_seq, cols] with offsets."""
     f32 = _torch().float32
     rows, cols = x.shape
+    if rows > _MOST or cols > _MOST:
+        _too_many("rows or columns of x", max(rows, cols))
     dtype = x.dtype
     xp, ldx = _rows_of(ctx, "x", x, rows, cols, dtype)
     hp, ldh = _rows_of(ctx, "h", h, rows, cols, dtype)
@@ -319,6 +332,8 @@ class AdapterBank:
         n, rank, in_dim = a.shape
         if b.dim() != 3 or b.shape[0] != n or b.shape[2] != rank:
             raise ValueError(f"b: shape {tuple(b.shape)} beside a's {tuple(a.shape)}")
+        if max(*a.shape, *b.shape) > _MOST:
+            _too_many("a or b", max(*a.shape, *b.shape))
         self.ctx, self.lib, self.dtype = ctx, ctx.lib, a.dtype
         self.n, self.rank, self.in_dim, self.out_dim = n, rank, in_dim, b.shape[1]
         _free_collected()
@@ -331,6 +346,8 @@ class AdapterBank:
 
     def work_bytes(self, rows):
         """Bytes of `work` that adapters_apply needs for `rows` rows or fewer."""
+        if rows > _MOST:
+            _too_many("rows", rows)
         size = ctypes.c_size_t()
         _lib.check(self.lib.sg_adapters_work_bytes(self.handle, rows, ctypes.byref(size)))
         return size.value
@@ -354,6 +371,8 @@ def adapters_apply(ctx, dst, base, bank: AdapterBank, x, offsets, adapter_ids, *
     not shared by calls that may run at the same time; None: one from torch's allocator."""
     torch = _torch()
     rows = x.shape[0]
+    if rows > _MOST:
+        _too_many("rows of x", rows)
     xp, ldx = _rows_of(ctx, "x", x, rows, bank.in_dim, bank.dtype)
     d, ldd = _rows_of(ctx, "dst", dst, rows, bank.out_dim, bank.dtype)
     b, ldb = _rows_of(ctx, "base", base, rows, bank.out_dim, bank.dtype)

@@ -1495,3 +1495,37 @@ def test_attention_refuses_more_than_a_launch(change):
     _refused(_lib.load().sg_attention_masked(_addr(), c["out"], c["ldo"], c["q"], c["ldq"], c["k"], c["ldk"], c["v"], c["ldv"],
                                              c["dtype"], c["heads"], c["kv"], c["hd"], c["rows"], c["off"], c["n_seq"], None,
                                              None), "one launch")
+
+
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 8])
+def test_wrappers_refuse_counts_past_32_bits(n):
+    """Counts that would lose their upper bits on the way to the C ABI."""
+    from semantica_gpu import kernels
+    ctx, off = _Ctx(), torch.zeros(2, dtype=torch.int32)
+    rows, cols = torch.zeros(1, 64).expand(n, 64), torch.zeros(1, 1).expand(1, n)
+    one, w = torch.zeros(1, 64), torch.zeros(64)
+
+    class Bank:
+        in_dim, out_dim, dtype, handle = 64, 64, torch.float32, None
+
+        def work_bytes(self, rows):
+            return 16
+
+    for call in (lambda: kernels.attention_masked(ctx, rows, rows, rows, rows, 1, 1, off),
+                 lambda: kernels.attention_masked(ctx, cols, cols, cols, cols, 1, 1, off),
+                 lambda: kernels.attention_masked(ctx, one, one, one, one, 1, 1, torch.zeros(1, dtype=torch.int32).expand(n)),
+                 lambda: kernels.block_norm(ctx, None, rows, rows, rows, w, None, 1e-6),
+                 lambda: kernels.block_norm(ctx, None, cols, cols, cols, None, None, 1e-6),
+                 lambda: kernels.adapters_apply(ctx, rows, rows, Bank(), rows, off, off[:1]),
+                 lambda: kernels.AdapterBank(ctx, torch.zeros(1, 1, 8).expand(n, 1, 8), torch.zeros(1, 8, 1).expand(n, 8, 1), w),
+                 lambda: kernels.AdapterBank.work_bytes(Bank(), n)):
+        with pytest.raises(ValueError, match="more than a call takes"):
+            call()
+
+
+@pytest.mark.parametrize("window", [-1, -(1 << 32), -(1 << 32) + 5])
+def test_attention_wrapper_refuses_any_negative_window(window):
+    from semantica_gpu import SemanticaError, kernels
+    t = torch.zeros(0, 64)
+    with pytest.raises(SemanticaError, match="window"):
+        kernels.attention_masked(_Ctx(), t, t, t, t, 1, 1, torch.zeros(2, dtype=torch.int32), window=window, stream=0)

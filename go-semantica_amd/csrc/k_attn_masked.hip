@@ -438,6 +438,9 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   const int kend = -all[1];
   const int kbeg = all[0] < kend ? all[0] & ~(kSub - 1) : 0;
   const int nt = all[0] < kend ? (kend - kbeg + F::BK - 1) / F::BK : 0;
+  // The rows that tiles are read from: the sequences', whatever lies before and behind them
+  // (as far as the offsets can be believed: never less than the keys that are seen).
+  const int from_row = min(max(a.off[0], 0), all[0]), last_row = max(min(a.off[a.n_seq], a.rows), kend) - 1;
 
   // ---- Q as the B operand, its sign turned where the scale is negative ----
   s16x8_t q[F::PARTS][KS];
@@ -471,8 +474,8 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   // What a key's distance takes off a score.  16-bit types take it off ahead of cs, which
   // saves the multiplication; not float32, whose cs holds the row's own power of two (of a
   // row of zeros 2^-110, and the quotient would leave float32's range), nor a far-off cs.
-  const bool first = apart && (F::F32 ? capped : capped || a.slopes);  // scores are multiplied by cs ahead of all else
-  const float after = capped || first ? 1.0f : cs;                    // and by this behind it
+  const bool early = apart && (F::F32 ? capped : capped || a.slopes);  // scores are multiplied by cs ahead of all else
+  const float after = capped || early ? 1.0f : cs;                    // and by this behind it
   const float steep = a.slopes ? a.slopes[h] * kLog2e / (F::F32 ? 1.0f : after) : 0.0f;
   const float ce = apart ? 1.0f : cs;
   const float t0 = cap2 * ce * kTanh16[0], t1 = cap2 * ce * ce * ce * kTanh16[1];
@@ -533,9 +536,10 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
     return nt;
   };
 
-  // Tile t's K and V into LDS.  Keys past the tensors' end repeat the last row,
-  // pieces past head_dim the last piece: they meet zeros of Q, or make outputs
-  // that are not stored.
+  // Tile t's K and V into LDS.  Keys before the first sequence or behind the last repeat
+  // the row next to them (padding there may hold NaN, which would send every row of the
+  // tile to careful_row), pieces past head_dim the last piece: they meet zeros of Q, or
+  // make outputs that are not stored.
   float* const key_muls = reinterpret_cast<float*>(lds + F::STAGES * F::TILE);  // [stage][3][BK]: K's power, V's exponent, V's power
   int e_ref = INT32_MIN;  // first_e
   // 16-bit types: a copy is 64 pieces, RPC rows of the tile.  Row r of a tile is row
@@ -551,7 +555,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
     const uint32_t base = (uint32_t)(uintptr_t)(lds_ptr)(lds + st * F::TILE) + (uint32_t)(w * COPIES) * 1024u;
     const i32x4_t rk = sg_raw_rsrc(static_cast<const T*>(a.k) + (int64_t)k0 * a.ldk + kvh * a.hd);
     const i32x4_t rv = sg_raw_rsrc(static_cast<const T*>(a.v) + (int64_t)k0 * a.ldv + kvh * a.hd);
-    if (a.hd == D && k0 + F::BK <= a.rows) {
+    if (a.hd == D && k0 >= from_row && k0 + F::BK - 1 <= last_row) {
 #pragma unroll
       for (int i = 0; i < COPIES; i++) {
         const int r = (w * COPIES + i) * RPC;
@@ -563,7 +567,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
 #pragma unroll 1
       for (int i = 0; i < COPIES; i++) {
         const int r = (w * COPIES + i) * RPC + lane / C;
-        const uint32_t from = (uint32_t)min(r, a.rows - 1 - k0);
+        const uint32_t from = (uint32_t)(min(max(k0 + r, from_row), last_row) - k0);
         const int ck = min((lane % C) ^ swz_k<D>(r), a.hd / 8 - 1), cv = min((lane % C) ^ swz_v<D>(r), a.hd / 8 - 1);
         sg_lds_copy16(base + 1024u * i, (from * (uint32_t)a.ldk + ck * 8) * 2u, rk, 0);
         sg_lds_copy16(base + F::HALF + 1024u * i, (from * (uint32_t)a.ldv + cv * 8) * 2u, rv, 0);
@@ -581,7 +585,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
     const int k0 = kbeg + t * F::BK;
 #pragma unroll
     for (int p = 0; p < ROUNDS; p++) {
-      const int64_t from = min(k0 + p * (kNT / TPR) + tid / TPR, a.rows - 1);
+      const int64_t from = min(max(k0 + p * (kNT / TPR) + tid / TPR, from_row), last_row);
 #pragma unroll
       for (int v = 0; v < 2; v++) {
         const T* src = v ? static_cast<const T*>(a.v) + from * a.ldv : static_cast<const T*>(a.k) + from * a.ldk;
@@ -699,7 +703,7 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
         for (int i = 0; i < 4; i++) s[4 * b + i] *= km[i];
       }
     }
-    if (first) {
+    if (early) {
 #pragma unroll
       for (int r = 0; r < SR; r++) s[r] *= cs;
     }

@@ -364,16 +364,20 @@ typedef struct sg_attn_mask {
 /* Attention of every sequence with itself: out_i = sum_j softmax_j(score_ij) v_j
  * over the visible keys; zeros for a query that sees none, or none whose score
  * is above -infinity.  Hidden keys do not touch the result, whatever they hold
- * (infinities and NaN included).  q
- * [rows][ldq] and out [rows][ldo] hold n_heads heads of head_dim side by side, k
+ * (infinities and NaN included).  What lies before the first sequence or behind the
+ * last is not read as a key.  Inside a sequence a hidden key or value that is not finite
+ * costs time: queries that see others of the same 32 to 64 keys are computed
+ * again one key at a time (400 times as long at 1000 tokens).
+ * q [rows][ldq] and out [rows][ldo] hold n_heads heads of head_dim side by side, k
  * [rows][ldk] and v [rows][ldv] n_kv_heads (a divisor of n_heads) of them, all of
  * type dtype; strides in elements.  Sums and softmax statistics are float32.
  * float32 products keep 22 bits of each operand (2^-37 of its row's largest value
- * at worst); 16-bit types round the weights to their type, and tanh is off by
- * 2^-19 at most.  head_dim: a multiple of 8 up to 256; pointers 16-byte aligned,
- * strides whole 16 bytes (k's and v's up to 2^22 elements); out apart from q, k
- * and v (other columns of one tensor, with the same stride, are).
- * rows * n_heads: up to 2^30 or a little less.
+ * at worst); 16-bit types round the weights to their type (float32 tensors keep
+ * them), and tanh is off by 2^-19 at most.
+ * head_dim: a multiple of 8 up to 256; pointers 16-byte aligned, strides whole 16
+ * bytes (k's and v's up to 2^22 elements); rows * n_heads up to 2^30 or a little
+ * less; out apart from q, k and v (other columns of one tensor, with the same
+ * stride, are).
  * mask NULL: scale 1/sqrt(head_dim), nothing hidden. */
 int sg_attention_masked(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int64_t ldq, const void *k, int64_t ldk,
                         const void *v, int64_t ldv, int32_t dtype, int32_t n_heads, int32_t n_kv_heads,

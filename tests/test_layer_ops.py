@@ -1529,3 +1529,29 @@ def test_attention_wrapper_refuses_any_negative_window(window):
     t = torch.zeros(0, 64)
     with pytest.raises(SemanticaError, match="window"):
         kernels.attention_masked(_Ctx(), t, t, t, t, 1, 1, torch.zeros(2, dtype=torch.int32), window=window, stream=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 72, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 1), (24, 8)])
+def test_attention_does_not_read_padding_rows(gpu_ctx, dtype, hd, heads, kv_heads):
+    """What lies before the first sequence and behind the last: keys and values of NaN there give
+    the very bits that zeros give, so no row is computed again for them."""
+    lens = [50, 1, 300, 97]
+    g, off = gen(91), offsets(lens, first=5)
+    rows = int(off[-1]) + 90
+    q, k, v = (rand(g, rows, c * hd, dtype=dtype) for c in (heads, kv_heads, kv_heads))
+    slopes = torch.tensor([2.0 ** -(2 + h % 5) for h in range(heads)])
+    for kw in ({}, {"causal": True, "window": 70, "softcap": 9.0, "slopes": slopes}):
+        outs = []
+        q[:5] = q[int(off[-1]):] = math.nan
+        for fill in (0.0, math.nan):
+            for t in (k, v):
+                t[:5] = t[int(off[-1]):] = fill
+            outs.append(run_attention(gpu_ctx, q, k, v, off, heads, kv_heads, **kw))
+        assert torch.equal(*outs)
+        inside = slice(5, int(off[-1]))
+        want, mean, size = attention_ref(q, k, v, off, heads, kv_heads, **kw)
+        close(outs[0][inside], want[inside], attention_tol(dtype, hd, want, mean, size, kw.get("softcap", 0.0))[inside],
+              "attention")

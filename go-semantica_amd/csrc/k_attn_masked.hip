@@ -272,7 +272,7 @@ struct form {
   static constexpr int KEYS = F32 ? STAGES * 3 * BK * 4 : 0;  // per-key powers of a float32 tile
   static constexpr int JOIN = KW > 1 ? NW * QT * D * 4 : 0;
   static constexpr int LDS = (STAGES * TILE + KEYS) > JOIN ? (STAGES * TILE + KEYS) : JOIN;
-  static constexpr int WAVES = (QT == 32 && D == 256) || (NW == 4 && KW > 1) ? 1 : D == 64 && !F32 ? 3 : 2;  // a SIMD has registers for
+  static constexpr int WAVES = (QT == 32 && D == 256) || (NW == 4 && KW > 1) ? 1 : D == 64 && (!F32 || KW == 1) ? 3 : 2;  // a SIMD has registers for
   // Lane (n, g): query n; of a 32-key block, register r is key KSTR (r / 4) + 4 g + r % 4.
   static constexpr int G = SG_WAVE / QT, KSTR = 4 * G;
   static constexpr int SR = KB / G;            // a lane's scores of its keys of a tile
@@ -474,9 +474,9 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
   // What a key's distance takes off a score.  16-bit types take it off ahead of cs, which
   // saves the multiplication; not float32, whose cs holds the row's own power of two (of a
   // row of zeros 2^-110, and the quotient would leave float32's range), nor a far-off cs.
-  const bool early = apart && (F::F32 ? capped : capped || a.slopes);  // scores are multiplied by cs ahead of all else
-  const float after = capped || early ? 1.0f : cs;                    // and by this behind it
-  const float steep = a.slopes ? a.slopes[h] * kLog2e / (F::F32 ? 1.0f : after) : 0.0f;
+  const bool early = !F::F32 && apart && (capped || a.slopes);  // scores are multiplied by cs ahead of all else
+  const float after = F::F32 || capped || early ? 1.0f : cs;    // and by this behind it
+  const float steep = a.slopes ? a.slopes[h] * kLog2e / after : 0.0f;
   const float ce = apart ? 1.0f : cs;
   const float t0 = cap2 * ce * kTanh16[0], t1 = cap2 * ce * ce * ce * kTanh16[1];
   const float t2 = cap2 * ce * ce * (ce * ce) * ce * kTanh16[2];
@@ -695,12 +695,16 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
 #pragma unroll
       for (int r = 0; r < R; r++) s[sub * R + r] = F::F32 ? c[sub][0][r] + (c[sub][CH / 2][r] + c[sub][CH - 1][r]) : c[sub][0][r];
     // Register r: key KSTR (r / 4) + 4 g + r % 4.  The score is s after.
+    // float32: the key's power of two times cs first, since either alone may take a score
+    // out of range that both bring back.
     if constexpr (F::F32) {
+      if (capped) {
 #pragma unroll
-      for (int b = 0; b < SR / 4; b++) {
-        const f32x4_t km = *reinterpret_cast<const f32x4_t*>(key_mul + F::KSTR * b + 4 * g);
+        for (int b = 0; b < SR / 4; b++) {
+          const f32x4_t km = *reinterpret_cast<const f32x4_t*>(key_mul + F::KSTR * b + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[4 * b + i] *= km[i];
+          for (int i = 0; i < 4; i++) s[4 * b + i] *= km[i] * cs;
+        }
       }
     }
     if (early) {
@@ -731,9 +735,10 @@ __global__ __launch_bounds__(RW * KW * SG_WAVE, (form<T, D, QT, RW, KW>::WAVES))
     if constexpr (F::F32) {
 #pragma unroll
       for (int b = 0; b < SR / 4; b++) {
+        const f32x4_t km = *reinterpret_cast<const f32x4_t*>(key_mul + F::KSTR * b + 4 * g);
         const f32x4_t ve = *reinterpret_cast<const f32x4_t*>(key_mul + F::BK + F::KSTR * b + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[4 * b + i] = __builtin_fmaf(s[4 * b + i], after, ve[i]);
+        for (int i = 0; i < 4; i++) s[4 * b + i] = capped ? s[4 * b + i] + ve[i] : __builtin_fmaf(s[4 * b + i], km[i] * cs, ve[i]);
       }
     }
     if (a.slopes) {

@@ -1555,3 +1555,21 @@ def test_attention_does_not_read_padding_rows(gpu_ctx, dtype, hd, heads, kv_head
         want, mean, size = attention_ref(q, k, v, off, heads, kv_heads, **kw)
         close(outs[0][inside], want[inside], attention_tol(dtype, hd, want, mean, size, kw.get("softcap", 0.0))[inside],
               "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 1), (24, 8)])
+@pytest.mark.parametrize("qs,ks", [(1e-34, 1e33), (1e33, 1e-34), (1e-30, 3e33), (3e33, 1e-30)])
+def test_attention_of_opposite_powers(gpu_ctx, hd, heads, kv_heads, qs, ks):
+    """float32 queries and keys of far-apart powers of two, all in one direction or against it:
+    the scores are small, what they are made of is not."""
+    g, off = gen(92), offsets([300, 90])
+    rows = 390
+    q = (1 + torch.rand(rows, heads * hd, generator=g)) * torch.where(torch.rand(rows, 1, generator=g) < 0.5, -qs, qs)
+    k = (1 + torch.rand(rows, kv_heads * hd, generator=g)) * torch.where(torch.rand(rows, 1, generator=g) < 0.5, -ks, ks)
+    v = rand(g, rows, kv_heads * hd)
+    for kw in ({}, {"softcap": 3.0, "causal": True}, {"scale": 1e-5 if qs * ks > 1 else 0.0}):
+        got = run_attention(gpu_ctx, q, k, v, off, heads, kv_heads, **kw)
+        want, mean, size = attention_ref(q, k, v, off, heads, kv_heads, **kw)
+        close(got, want, attention_tol("f32", hd, want, mean, size, kw.get("softcap", 0.0)), "attention")

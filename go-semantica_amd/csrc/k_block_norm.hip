@@ -116,14 +116,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_block_norm(sg_block_n
   load(row0);
 
   // The sequence of the current row: rows [s0, s1).
-  int seq = 0, s0 = 0, s1 = a.rows;
+  int seq = a.off ? -1 : 0, s0 = a.off ? INT32_MIN : 0, s1 = a.off ? INT32_MIN : a.rows;
   bool fresh = true;  // gate not loaded for this sequence yet
   int half = 0;
-  if (a.off) {
-    seq = sgp::find_seq(a.off, a.n_seq, row0, lane);
-    s0 = seq < 0 ? a.off[0] : a.off[seq];
-    s1 = seq < 0 ? s0 : a.off[seq + 1];
-  }
   for (int row = row0; row < row1; row++) {
     float xv[NCH][V], hv[NCH][V];
 #pragma unroll
@@ -135,11 +130,17 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_block_norm(sg_block_n
       }
     if (row + 1 < row1) load(row + 1);
     if (a.off) {
-      while (row >= s1 && seq + 1 < a.n_seq) {
+      // The next one, as a rule; else (the first row's, or past empty ones) it is looked up.
+      if (row >= s1 && seq + 1 < a.n_seq) {
+        fresh = true;
         seq++;
         s0 = a.off[seq];
         s1 = a.off[seq + 1];
-        fresh = true;
+        if (row >= s1) {
+          seq = max(sgp::find_seq(a.off, a.n_seq, row, lane), 0);
+          s0 = a.off[seq];
+          s1 = a.off[seq + 1];
+        }
       }
       if (row < s0 || row >= s1) continue;  // of no sequence: left as it was
     }

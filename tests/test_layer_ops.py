@@ -1573,3 +1573,14 @@ def test_attention_of_opposite_powers(gpu_ctx, hd, heads, kv_heads, qs, ks):
         got = run_attention(gpu_ctx, q, k, v, off, heads, kv_heads, **kw)
         want, mean, size = attention_ref(q, k, v, off, heads, kv_heads, **kw)
         close(got, want, attention_tol("f32", hd, want, mean, size, kw.get("softcap", 0.0)), "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,cols", [("f32", 20000, 40), ("bf16", 20000, 72), ("f32", 5000, 1100), ("f32", 2300, 4200)])
+def test_norm_passes_over_runs_of_empty_sequences(gpu_ctx, dtype, rows, cols):
+    """Runs of empty sequences between rows that one workgroup takes in turn: a few, hundreds,
+    and more than a lookup's first step covers; rows of no sequence at both ends."""
+    lens = [1] * 5 + [0] * 3 + [2] + [0] * 70 + [1, 1] + [0] * 5000 + [rows // 2] + [0] * 64 + [1] + [0] * 700 + [3] + [0] * 9
+    lens = [0] * 90 + lens + [rows - 3 - sum(lens) - 4] + [0] * 300
+    check_norm(gpu_ctx, dtype, rows, cols, lens=lens, first=3, gate=True)
+    check_norm(gpu_ctx, dtype, rows, cols, lens=lens[:-301], first=3)

@@ -20,11 +20,16 @@
 // the lane's dim each).  Rows of 16-byte pieces are stored in LDS with the piece
 // index xor-ed by the row (swz_k, swz_v), so neither read meets bank conflicts.
 //
-// 16-bit types go to LDS by buffer_load ... lds, a tile ahead.  float32 operands
-// are split into two fp16 halves each, hi + lo, and products run as hi.hi + hi.lo
-// + lo.hi (22 bits of each operand; the dropped lo.lo is 2^-22 of the product).
+// 16-bit types go to LDS by buffer_load ... lds, a tile ahead.  Their weights are rounded to
+// the type for the second product and summed as they are multiplied: against 64 bits
+// bf16 outputs are off by 2.1e-3 (1.6e-3 with float32 weights, which is the outputs' own
+// rounding), fp16 by 2.6e-4 (2.1e-4); weights of two halves would be half as much matrix work
+// again.
+//
+// float32 operands are split into two fp16 halves each, hi + lo, and products run as hi.hi +
+// hi.lo + lo.hi (22 bits of each operand; the dropped lo.lo is 2^-22 of the product).
 // Every row of Q, K and V is first brought to the same power of two, so fp16's
-// range does not matter: K's power multiplies the score, V's is added to the
+// range does not matter: Q's and K's powers multiply the score, V's is added to the
 // score that the weight is formed from (p' = 2^(s + e_j - m'), |v'| alike for all
 // keys), and the softmax's sum takes it out again (sum p' 2^-e_j).  A value keeps
 // 22 bits down to 2^-15 of its row's largest and 2^-37 of the largest below that.
@@ -32,20 +37,26 @@
 // A hidden key has weight zero, and zero times an infinity or a NaN in its value
 // is a NaN.  Instead of looking at every value, a wave looks at its outputs: rows
 // that did not come out finite are computed again one key at a time from the
-// visible keys only (careful_row).  That also covers float32 values past the
-// fp16 halves' reach (q and k above 2^113, values 2^53 times the first keys').
+// visible keys only (careful_row; some 400 times slower at 1000 tokens, so tiles leave
+// out what lies around the batch, where padding may hold anything).  That also covers
+// float32 values past the fp16 halves' reach (q and k above 2^113, values 2^53 times
+// the first keys').
 //
-// What bounds it.  A SIMD's matrix and vector instructions do not overlap here (their
-// busy cycles add up to 94 % of 4 x 4096 bf16 tokens' time: 35 + 59), and a score costs
-// an exponential (16 cycles of a wave; a multiplication 2.6) and five to eight other
-// vector instructions beside 4 head_dim flops.  So few of them per score is what the code
-// goes for: the range check once a tile and wave, bf16 under a cap without a maximum,
+// What bounds it.  A wave's products and exponentials come one after the other, and two
+// or three waves a SIMD fill each other's gaps only in part: at 4 x 4096 bf16 tokens the
+// matrix core is busy 36 % of the time and the vector unit 60 %.  A score costs an
+// exponential (16 cycles of a wave; a multiplication 2.6) and about ten other vector
+// instructions under a cap beside 4 head_dim flops, so few of them per score is what the
+// code goes for: the range check once a tile and wave, bf16 under a cap without a maximum,
 // tanh as a polynomial, the sum of weights as a dot product of the packed ones.  Measured
 // (us, and the rate of the visible pairs' 4 head_dim flops):
-//   4 x 4096, bf16, causal, cap, 32 heads over 8 of 128            691   796 TFLOP/s
-//   8 of 1024 .. 2048, fp16, causal, prefix, 16 over 8 of 128      152   640
-//   16391 rows, documents of 900, bf16, distance bias, 12 of 64    156   323
-//   64 x 512, float32, window of 256, 3 over 1 of 256              217   178
+//   4 x 4096, bf16, causal, cap, 32 heads over 8 of 128            708   776 TFLOP/s
+//   8 of 1024 .. 2048, fp16, causal, prefix, 16 over 8 of 128      155   625
+//   16391 rows, documents of 900, bf16, distance bias, 12 of 64    159   317
+//   64 x 512, float32, window of 256, 3 over 1 of 256              218   178
+// (700 to 720 for the first over several cards.  Its scores stay below 0.35 of the cap of 50,
+// so tanh is the polynomial throughout: with a cap of 20, where half of the blocks take the
+// exact form, 766 for 743 on one card, with a cap of 8 789, without one 616.)
 // float32 (three products each; 372 TFLOP/s is the matrix cores' limit) waits about
 // half its time: a workgroup's eight waves load, halve, multiply in step, and no second
 // one fits beside two stages of its tiles (two workgroups of 64 rows and one stage each:

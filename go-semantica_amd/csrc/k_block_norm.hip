@@ -13,7 +13,7 @@
 // in registers from row to row (read again for every row they would be 12 bytes
 // of L2 traffic beside a float32 column's 16), and the next row's loads are
 // issued before the current row's two reductions.  Measured: 32768 x 768 float32 82
-// us, 20001 x 5120 bf16 180 us, 4.9 and 4.5 TB/s of the four tensors (a copy of 1 GB
+// us, 20001 x 5120 bf16 182 us, 4.9 and 4.5 TB/s of the four tensors (a copy of 1 GB
 // moves 5.0); 32 rows 5.7 us, three dependent round trips to memory.
 #include <algorithm>
 

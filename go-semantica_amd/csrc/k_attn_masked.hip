@@ -32,7 +32,8 @@
 // range does not matter: Q's and K's powers multiply the score, V's is added to the
 // score that the weight is formed from (p' = 2^(s + e_j - m'), |v'| alike for all
 // keys), and the softmax's sum takes it out again (sum p' 2^-e_j).  A value keeps
-// 22 bits down to 2^-15 of its row's largest and 2^-37 of the largest below that.
+// 22 bits down to 2^-15 of its row's largest and 2^-37 of the largest below that; p', which
+// has the maximum at 2^5 or above, 22 bits down to 2^-9 and 2^-25 below.
 //
 // A hidden key has weight zero, and zero times an infinity or a NaN in its value
 // is a NaN.  Instead of looking at every value, a wave looks at its outputs: rows

@@ -372,8 +372,9 @@ typedef struct sg_attn_mask {
  * [rows][ldk] and v [rows][ldv] n_kv_heads (a divisor of n_heads) of them, all of
  * type dtype; strides in elements.  Sums and softmax statistics are float32.
  * float32 products keep 22 bits of each operand (2^-37 of its row's largest value
- * at worst); 16-bit types round the weights to their type (float32 tensors keep
- * them), and tanh is off by 2^-19 at most.
+ * at worst, of a weight times its value's size 2^-30 of the largest); 16-bit types round
+ * the weights to their type (float32 tensors keep them; fp16's to 2^-31 of the
+ * largest), and tanh is off by 2^-19 at most.
  * head_dim: a multiple of 8 up to 256; pointers 16-byte aligned, strides whole 16
  * bytes (k's and v's up to 2^22 elements); rows * n_heads up to 2^30 or a little
  * less; out apart from q, k and v (other columns of one tensor, with the same

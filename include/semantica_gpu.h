@@ -394,9 +394,9 @@ int sg_attention_masked(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int6
  * gate [cols] for all.  Otherwise gate is [n_seq][cols], one for each sequence.
  * cols 1 .. 8192, rows and strides of any whole elements (whole 16 bytes are
  * faster).  The squares are summed in float32, as sg_rmsnorm's are: values past
- * 2^63 overflow them, and with eps 0 a row below 2^-63 is taken for zeros.  sum and xn may each be x or h (same pointer and stride);
- * otherwise no output overlaps another tensor (other columns of the same one, with
- * the same stride, do not). */
+ * 2^63 overflow them, and those of a row below 2^-75 are zeros, which eps 0 divides by.
+ * sum and xn may each be x or h (same pointer and stride); otherwise no output overlaps
+ * another tensor (other columns of the same one, with the same stride, do not). */
 int sg_block_norm(sg_ctx *ctx, void *xn, int64_t ldxn, void *sum, int64_t lds, const void *x, int64_t ldx,
                   const void *h, int64_t ldh, int32_t dtype, int32_t rows, int32_t cols, const float *w_post,
                   const float *w_pre, float eps, const float *gate, float scale, const int32_t *d_seq_offsets,

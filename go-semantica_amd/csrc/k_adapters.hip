@@ -144,12 +144,15 @@ __device__ __forceinline__ void put_u<float>(chunk<float>* at, int n, int r4, co
   *reinterpret_cast<f32x4_t*>(&at[16 * (r4 >> 2) + n]) = u;
 }
 
-// A row's u, four values in each of TPR lanes side by side, is multiplied by the
+// fp16: a row's u, four values in each of TPR lanes side by side, is multiplied by the
 // power of two that brings its largest value to 2^10 .. 2^11 (exact, and undone by
 // `back`): fp16 then holds every u that float32 holds, and its second half stays
-// clear of the subnormals.
-template <int TPR>
+// clear of the subnormals.  The other types have float32's range: u as it is, since with
+// their weights (above 2^109) the product of a u brought up could leave it.
+template <typename T, int TPR>
 __device__ __forceinline__ float to_range(const f32x4_t& s, float& back, float top = 0.0f) {
+  back = 1.0f;
+  if constexpr (!__is_same(T, _Float16)) return 1.0f;
 #pragma unroll
   for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(s[i]));
 #pragma unroll
@@ -259,7 +262,7 @@ __global__ __launch_bounds__(kNT) void k_adapter_down(sg_adapters_args a, int pa
         s *= scale[r];
       }
       float by;
-      const float up = to_range<WIDTH>(s, by);
+      const float up = to_range<T, WIDTH>(s, by);
       bool mine = ids.own[r] < 0 && blockIdx.z == 0;  // (zeros) or of an adapter that this workgroup took
       for (int j = blockIdx.z; j < ids.count; j += gridDim.z) mine |= ids.own[r] == ids.list[j];
       if (row0 + r >= a.rows || !mine) continue;
@@ -355,7 +358,7 @@ __global__ __launch_bounds__(kNT) void k_adapter_up(sg_adapters_args a, int part
 #pragma unroll
       for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(s[k][i]));
     }
-    const float up = to_range<TPR>(s[0], by, top);
+    const float up = to_range<T, TPR>(s[0], by, top);
     if (tid % TPR == 0) back[r] = by;
 #pragma unroll
     for (int k = 0; k < kHeld; k++) {

@@ -1584,3 +1584,19 @@ def test_norm_passes_over_runs_of_empty_sequences(gpu_ctx, dtype, rows, cols):
     lens = [0] * 90 + lens + [rows - 3 - sum(lens) - 4] + [0] * 300
     check_norm(gpu_ctx, dtype, rows, cols, lens=lens, first=3, gate=True)
     check_norm(gpu_ctx, dtype, rows, cols, lens=lens[:-301], first=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,rank", [([9, 20, 3], 16), ([1] * 40, 100), ([9000, 8000], 32)])
+@pytest.mark.parametrize("by_x,by_b", [(1e-34, 1e35), (1e-20, 1e25), (1e25, 1e-30), (1e-34, 1.0)])
+def test_adapters_of_far_apart_powers(gpu_ctx, dtype, lens, rank, by_x, by_b):
+    """Small low-rank values against large weights and the other way round."""
+    c = adapter_case(dtype, 64, 72, rank, 2, lens, seed=7, by=by_x)
+    c["b"] = (c["b"].float() * by_b).to(c["b"].dtype)
+    c["ids"] = torch.arange(len(lens), dtype=torch.int32) % 2
+    say("adapters", dtype, lens[:4], rank, by_x, by_b)
+    got = run_adapters(gpu_ctx, c)
+    want, size = adapters_ref(c["x"], c["base"], c["a"], c["b"], c["scales"], c["off"], c["ids"])
+    rel = (64 + rank + 32) * F + (0 if dtype == "f32" else 2.0 ** -16)
+    close(got, want, U[dtype] * want.abs() + rel * size + TINY[dtype], "adapters")

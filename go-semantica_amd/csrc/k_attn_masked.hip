@@ -55,7 +55,7 @@
 //   8 of 1024 .. 2048, fp16, causal, prefix, 16 over 8 of 128      155   625
 //   16391 rows, documents of 900, bf16, distance bias, 12 of 64    159   317
 //   64 x 512, float32, window of 256, 3 over 1 of 256              218   178
-// (700 to 720 for the first over several cards.  Its scores stay below 0.35 of the cap of 50,
+// (690 to 730 for the first over several cards.  Its scores stay below 0.35 of the cap of 50,
 // so tanh is the polynomial throughout: with a cap of 20, where half of the blocks take the
 // exact form, 766 for 743 on one card, with a cap of 8 789, without one 616.)
 // float32 (three products each; 372 TFLOP/s is the matrix cores' limit) waits about

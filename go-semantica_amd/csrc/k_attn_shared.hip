@@ -1,0 +1,358 @@
+// k_attn_shared.hip -- attention over kept keys and values (sg_attention_shared): the plan of a
+// call, the join of its pieces, and what is launched.  sg_attn_shared.h has the kernels between.
+//
+// The plan is one workgroup's work: for every row which places it sees, for every job its tiles,
+// and the running total of those, from which workers find their shares.  Offsets, ranges and
+// lengths come from device memory, so everything that is addressed later is cut here to the
+// tensors and the cache.
+#include <algorithm>
+
+#include "semantica_gpu.h"
+#include "sg_kernels.h"
+#include "sg_kv_cache.h"
+
+namespace {
+
+using sgc::kTile;
+using sgp::clamp_row;
+using sgp::elem;
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanSeqs = 8192;  // offsets kept in LDS up to so many sequences
+
+// The largest i in [0, n) with at(i) <= x for ascending at, 0 if there is none.
+template <typename F>
+__device__ __forceinline__ int last_at_most(int n, int x, F at) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo + 1) / 2;
+    if (at(mid) <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Running totals over a workgroup: out[0] = base, out[i + 1] = out[i] + count(i), none above
+// `most`.  Returns the last.
+template <typename O, typename F>
+__device__ int64_t running(int n, int64_t base, int64_t most, O* out, F count) {
+  __shared__ int64_t wave_sum[kPlanThreads / 64];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  if (t == 0) out[0] = (O)base;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + t;
+    int64_t v = i < n ? count(i) : 0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t u = __shfl_up(v, o);
+      if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) wave_sum[wave] = v;
+    __syncthreads();
+    int64_t total = base;
+    for (int w = 0; w < kPlanThreads / 64; w++) {
+      if (w == wave) v += total;
+      total += wave_sum[w];
+    }
+    if (i < n) out[i + 1] = (O)min(v, most);
+    base = min(total, most);
+  }
+  __syncthreads();
+  return base;
+}
+
+// A range of slots, empty unless it lies in the cache.
+__device__ __forceinline__ int kept_length(int start, int length, int64_t slots) {
+  return start >= 0 && length > 0 && (int64_t)start + length <= slots ? length : 0;
+}
+
+__device__ __forceinline__ int clamp32(int64_t v, int64_t most) { return (int)min(max(v, (int64_t)0), most); }
+
+__global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args a, sg_attn_batch b, sg_attn_list la,
+                                                            sg_attn_list lb, int one_list, int4* seen_out, int4* where_out) {
+  __shared__ int32_t off_lds[kPlanSeqs + 1];
+  const int t = threadIdx.x;
+  const bool small = b.n_seq <= kPlanSeqs;
+  if (small)
+    for (int i = t; i <= b.n_seq; i += kPlanThreads) off_lds[i] = clamp_row(b.off[i], a.rows);
+  __syncthreads();
+  auto off = [&](int i) { return small ? off_lds[i] : clamp_row(b.off[i], a.rows); };
+  auto rows_of = [&](int i) { return max(off(i + 1) - off(i), 0); };
+  auto group_at = [&](int p) { return min(max(b.shared[p], 0), b.n_seq); };
+
+  // Jobs of each prefix and sequence: those of prefixes first where both stand in one list.
+  const int prefix_jobs =
+      b.n_prefix > 0 ? (int)running(b.n_prefix, 0, la.cap, b.prefix_jobs,
+                                    [&](int p) {
+                                      const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
+                                      return (rows * a.group + la.m - 1) / la.m;
+                                    })
+                     : 0;
+  const int own0 = one_list ? prefix_jobs : 0;
+  const int own_end = (int)running(b.n_seq, own0, lb.cap, b.seq_jobs,
+                                   [&](int i) { return ((int64_t)rows_of(i) * a.group + lb.m - 1) / lb.m; });
+
+  // What each row sees.
+  for (int row = t; row < a.rows; row += kPlanThreads) {
+    const int i = last_at_most(b.n_seq, row, off);
+    const int r0 = off(i), r1 = off(i + 1);
+    int4 seen = make_int4(0, 0, 0, 0), where = make_int4(-2, 0, -2, 0);
+    if (row >= r0 && row < r1) {
+      const int64_t len = kept_length(b.starts[i], b.lengths[i], b.slots);
+      int64_t plen = 0;
+      where = make_int4(-1, 0, b.seq_jobs[i], r0);
+      if (b.n_prefix > 0) {
+        const int p = last_at_most(b.n_prefix, i, group_at);
+        if (i >= group_at(p) && i < group_at(p + 1)) {
+          plen = kept_length(b.prefix_starts[p], b.prefix_lengths[p], b.slots);
+          where.x = b.prefix_jobs[p];
+          where.y = off(group_at(p));
+        }
+      }
+      const int64_t pos = plen + len - (r1 - r0) + (row - r0);
+      int64_t lo = 0, hi = plen + len;
+      if (b.causal) hi = min(hi, pos + 1);
+      if (b.window > 0) {
+        lo = max(lo, pos - b.window + 1);
+        hi = min(hi, pos + b.window);
+      }
+      seen = make_int4(clamp32(lo, plen), clamp32(hi, plen), clamp32(lo - plen, len), clamp32(hi - plen, len));
+    }
+    seen_out[row] = seen;
+    where_out[row] = where;
+  }
+  __syncthreads();
+
+  // The jobs, and the running total of their tiles.
+  auto fill = [&](const sg_attn_list& list, int j0, int n, int own, int64_t base) {
+    const int32_t* jobs = own ? b.seq_jobs : b.prefix_jobs;
+    const int64_t units = running(n, base, INT64_MAX, list.cum + j0, [&](int j) {
+      const int i = last_at_most(own ? b.n_seq : b.n_prefix, j + j0, [&](int k) { return jobs[k]; });
+      const int first = own ? i : group_at(i), r0 = off(first), r1 = off(own ? i + 1 : group_at(i + 1));
+      const int start = own ? b.starts[i] : b.prefix_starts[i];
+      sg_attn_job job{r0, max(r1 - r0, 0), j + j0 - jobs[i], max(start, 0), 0, own};
+      const int from = r0 + (int)((int64_t)job.tile * list.m / a.group);
+      const int to = (int)min((int64_t)r1 - 1, r0 + ((int64_t)(job.tile + 1) * list.m - 1) / a.group);
+      const int len = kept_length(start, own ? b.lengths[i] : b.prefix_lengths[i], b.slots);
+      int lo = INT32_MAX, hi = 0;
+      for (int r = from; r <= to; r++) {
+        const int4 s = seen_out[r];
+        // (Cut once more: where offsets do not ascend, a row's range is another sequence's.)
+        const int l = own ? s.z : s.x, h = min(own ? s.w : s.y, len);
+        if (l < h) {
+          lo = min(lo, l);
+          hi = max(hi, h);
+        }
+      }
+      int64_t count = 0;
+      if (lo < hi) {
+        job.slot_tile = (int)(((int64_t)start + lo) / kTile);
+        count = ((int64_t)start + hi - 1) / kTile - job.slot_tile + 1;
+      }
+      list.jobs[j + j0] = job;
+      return count;
+    });
+    if (t == 0) {
+      list.plan->units = units;
+      list.plan->jobs = j0 + n;
+      list.plan->per = max((units * a.kv_heads + list.workers - 1) / list.workers, (int64_t)list.min_units);
+    }
+    return units;
+  };
+  int64_t base = 0;
+  if (b.n_prefix > 0) base = fill(la, 0, prefix_jobs, 0, 0);
+  if (!one_list) base = 0;
+  fill(lb, own0, own_end - own0, 1, base);
+}
+
+// One (row, head) for NW waves: the pieces of its prefix's job and of its own keys', put
+// together under their largest maximum.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_attn_join(sg_attn_shared_args a, sg_attn_list la, sg_attn_list lb) {
+  constexpr int V = D / 64;
+  typedef float vec __attribute__((ext_vector_type(V)));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t i = NW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  if (i >= (int64_t)a.rows * a.heads) return;
+  const int row = (int)(i / a.heads), head = (int)(i - (int64_t)row * a.heads);
+  const int4 where = a.where[row];
+  if (where.z == -2) return;  // a row of no sequence
+  const int kv = head / a.group, hg = head - kv * a.group;
+  float m = -INFINITY, l = 0.0f;
+  vec o = 0.0f;
+#pragma unroll
+  for (int own = 0; own < 2; own++) {
+    const sg_attn_list& list = own ? lb : la;
+    const int job0 = own ? where.z : where.x;
+    if (job0 < 0) continue;
+    const int64_t pair = (int64_t)(row - (own ? where.w : where.y)) * a.group + hg;
+    const int64_t job = job0 + pair / list.m;
+    if (pair < 0 || job >= list.plan->jobs) continue;  // (offsets that do not ascend)
+    const int64_t c0 = list.cum[job], c1 = list.cum[job + 1];
+    if (c0 == c1) continue;
+    const int64_t first = kv * list.plan->units, per = list.plan->per;
+    const int64_t w0 = (first + c0) / per, w1 = (first + c1 - 1) / per;
+    const int in_job = (int)(pair % list.m);
+    for (int64_t w = w0 + (NW == 1 ? 0 : wave); w <= w1; w += NW) {
+      const int64_t at = w0 == w1 ? (int64_t)(own ? a.rows : 0) * a.heads + i
+                                  : list.piece0 + (w * 2 + (w == w0 ? 1 : 0)) * list.piece_pairs + in_job;
+      const float2 ml = a.part_ml[at];
+      const vec x = *reinterpret_cast<const vec*>(a.part_o + at * D + lane * V);
+      const float top = fmaxf(m, ml.x);  // (maxima are no NaN)
+      if (top == -INFINITY && ml.y == 0.0f) continue;
+      const float base = top == -INFINITY ? 0.0f : top;
+      const float by = __builtin_amdgcn_exp2f(m - base), now = __builtin_amdgcn_exp2f(ml.x - base);
+      l = l * by + ml.y * now;
+      o = o * by + x * now;
+      m = top;
+    }
+  }
+  if constexpr (NW > 1) {
+    __shared__ float ms[NW], ls[NW];
+    __shared__ vec os[NW][64];
+    os[wave][lane] = o;
+    if (lane == 0) {
+      ms[wave] = m;
+      ls[wave] = l;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    for (int w = 0; w < NW; w++) m = fmaxf(m, ms[w]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+    o = 0.0f;
+    for (int w = 0; w < NW; w++) {
+      const float by = __builtin_amdgcn_exp2f(ms[w] - base);
+      l += ls[w] * by;
+      o += os[w][lane] * by;
+    }
+  }
+  // A query that sees nothing, or nothing but scores of -infinity, has zeros.
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* out = static_cast<T*>(a.out) + row * a.ldo + (int64_t)head * a.hd;
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const int dim = lane * V + v;
+    if (dim < a.hd) out[dim] = elem<T>::from(l == 0.0f ? 0.0f : o[v] * inv);
+  }
+}
+
+// The form of each kind of job.  Up to so many pairs of a group on average, waves work for
+// themselves.
+constexpr int kNarrowPairs = 32;
+constexpr int kJoinWaves = 16;
+constexpr int64_t kJoinFew = 2048;  // (row, head) up to here: so many waves each
+
+struct layout {
+  size_t plan, cum[2], jobs[2], seq_jobs, prefix_jobs, seen, where, ml, o, total;
+  int64_t full, pieces[2];
+  int cap, workers[2], m[2], piece_pairs[2];
+};
+
+// Lists: 0 narrow, 1 wide.  All sizes grow with each of the arguments.
+layout lay_out(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix) {
+  layout y{};
+  const int64_t pairs = (int64_t)rows * (heads / kv_heads);
+  y.cap = (int)std::min<int64_t>(2 * (pairs / 16) + n_seq + n_prefix + 2, INT32_MAX);
+  const int cus = 256;
+  y.workers[0] = cus * 4 * (dtype == SG_F32 ? 1 : 2);
+  y.workers[1] = cus * (dtype == SG_F32 && D == 256 ? 1 : 2);
+  y.m[0] = 16;
+  y.m[1] = sgk::attn_wide_pairs(D);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  y.plan = take(2 * sizeof(sg_attn_plan));
+  for (int i = 0; i < 2; i++) {
+    y.cum[i] = take(sizeof(int64_t) * ((size_t)y.cap + 1));
+    y.jobs[i] = take(sizeof(sg_attn_job) * (size_t)y.cap);
+  }
+  y.seq_jobs = take(sizeof(int32_t) * ((size_t)n_seq + 1));
+  y.prefix_jobs = take(sizeof(int32_t) * ((size_t)n_prefix + 1));
+  y.seen = take(sizeof(int4) * (size_t)rows);
+  y.where = take(sizeof(int4) * (size_t)rows);
+  int64_t rows_of_o = 2 * (int64_t)rows * heads;
+  for (int i = 0; i < 2; i++) {
+    y.pieces[i] = rows_of_o;
+    y.piece_pairs[i] = (int)std::min<int64_t>(y.m[i], pairs);
+    rows_of_o += (int64_t)y.workers[i] * 2 * y.piece_pairs[i];
+  }
+  y.ml = take(sizeof(float2) * (size_t)rows_of_o);
+  y.o = take(sizeof(float) * (size_t)rows_of_o * D);
+  y.total = at;
+  return y;
+}
+
+template <typename T, int D>
+hipError_t join(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, hipStream_t s) {
+  const int64_t n = (int64_t)a.rows * a.heads;
+  if (n <= kJoinFew) return sgp::run_kernel(k_attn_join<T, D, kJoinWaves>, dim3(n), dim3(64 * kJoinWaves), 0, s, a, la, lb);
+  return sgp::run_kernel(k_attn_join<T, D, 1>, dim3((n + 3) / 4), dim3(256), 0, s, a, la, lb);
+}
+template <typename T>
+hipError_t join_dims(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, int D, hipStream_t s) {
+  if (D == 64) return join<T, 64>(a, la, lb, s);
+  if (D == 128) return join<T, 128>(a, la, lb, s);
+  return join<T, 256>(a, la, lb, s);
+}
+
+}  // namespace
+
+namespace sgk {
+
+size_t attn_shared_work_bytes(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix) {
+  return lay_out(dtype, rows, heads, kv_heads, D, n_seq, n_prefix).total;
+}
+
+hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q8, int D, void* work, hipStream_t s) {
+  const layout y = lay_out(dtype, a.rows, a.heads, a.kv_heads, D, b.n_seq, b.n_prefix);
+  char* w = static_cast<char*>(work);
+  int4* seen = reinterpret_cast<int4*>(w + y.seen);
+  int4* where = reinterpret_cast<int4*>(w + y.where);
+  a.seen = seen;
+  a.where = where;
+  a.part_o = reinterpret_cast<float*>(w + y.o);
+  a.part_ml = reinterpret_cast<float2*>(w + y.ml);
+  b.seq_jobs = reinterpret_cast<int32_t*>(w + y.seq_jobs);
+  b.prefix_jobs = reinterpret_cast<int32_t*>(w + y.prefix_jobs);
+  sg_attn_list lists[2];
+  for (int i = 0; i < 2; i++) {
+    sg_attn_list& l = lists[i];
+    l.plan = reinterpret_cast<sg_attn_plan*>(w + y.plan) + i;
+    l.cum = reinterpret_cast<int64_t*>(w + y.cum[i]);
+    l.jobs = reinterpret_cast<sg_attn_job*>(w + y.jobs[i]);
+    l.piece0 = y.pieces[i];
+    l.piece_pairs = y.piece_pairs[i];
+    l.m = y.m[i];
+    l.workers = y.workers[i];
+    l.blocks = i ? l.workers : l.workers / 4;
+    l.wide = i;
+    l.cap = y.cap;
+    l.min_units = i ? 4 : 2;
+  }
+  const int64_t pairs = (int64_t)a.rows * a.group;
+  const int wide_prefix = b.n_prefix > 0 && pairs > (int64_t)kNarrowPairs * b.n_prefix;
+  const int wide_own = pairs > (int64_t)kNarrowPairs * b.n_seq;
+  const sg_attn_list& lb = lists[wide_own];
+  const sg_attn_list& la = b.n_prefix > 0 ? lists[wide_prefix] : lb;
+  const int one_list = &la == &lb;
+  hipError_t e = sgp::run_kernel(k_attn_plan, dim3(1), dim3(kPlanThreads), 0, s, a, b, la, lb, one_list, seen, where);
+  auto run = [&](const sg_attn_list& l) {
+    if (e != hipSuccess) return;
+    e = dtype == SG_F32   ? attn_shared_f32(a, l, q8, D, s)
+        : dtype == SG_F16 ? attn_shared_f16(a, l, q8, D, s)
+                          : attn_shared_bf16(a, l, q8, D, s);
+  };
+  run(la);
+  if (!one_list) run(lb);
+  if (e != hipSuccess) return e;
+  if (dtype == SG_F32) return join_dims<float>(a, la, lb, D, s);
+  if (dtype == SG_F16) return join_dims<_Float16>(a, la, lb, D, s);
+  return join_dims<sgp::bf16_t>(a, la, lb, D, s);
+}
+
+}  // namespace sgk

@@ -1,0 +1,665 @@
+// sg_attn_shared.h -- attention of a batch's queries over kept keys and values
+// (sg_attention_shared): the kernels, shared by the files that instantiate them.
+// k_attn_shared.hip has the plan, the join and what was measured.
+//
+// A query's keys are places 0 .. plen - 1, its prefix, and plen .. plen + len - 1, its
+// sequence's own.  Query rows times the query heads of a key head are pairs; a job is M
+// consecutive pairs of one group -- all sequences behind one prefix, over that prefix, or one
+// sequence, over its own keys -- and a list of jobs is laid end to end in units (a tile of 32
+// slots) and dealt to workers in equal shares, whatever the lengths: a worker ends in the
+// middle of a job and the next one goes on there.  So a long prefix is split over the GPU
+// when there are few queries and read once for all of them when there are many, and nothing
+// about the lengths is needed on the host.  What a worker has of a job -- running maximum m,
+// sum l and output O, unnormalised -- goes to the workspace, and k_attn_join adds up.
+//
+// Scores are formed transposed, S^T = K Q^T on 16x16 tiles: a lane has one pair's scores of
+// four keys in a row, twice for 32 keys, and these eight are, as they stand, its part of the
+// B operand of O^T += V^T P^T, for values are kept in that order (sg_kv_cache.h).
+//
+// Codes of 8 bits are whole numbers, exact in the type: the keys' scale multiplies the
+// score, the values' the weight.  With fp16 queries that product would leave fp16's range,
+// so weights are split into two bf16 halves (2^-17 of each, exponents of float32) and the
+// codes taken as bf16; with bf16 queries one rounding to bf16 is what the plain form of the
+// type has as well.  float32 goes through float32 matrix products.
+#pragma once
+#include <atomic>
+
+#include "semantica_gpu.h"
+#include "sg_kernels.h"
+#include "sg_kv_cache.h"
+
+namespace sga {
+
+using sgc::kTail;
+using sgc::kTile;
+using sgp::bf16_t;
+using sgp::elem;
+
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+constexpr float kLog2e = 1.44269504088896340736f;
+// A pair's maximum is raised (its sums rescaled) when a score passes it by so many powers of
+// two, so most tiles rescale nothing; weights stay below 2^8.
+constexpr float kSlack = 8.0f;
+
+// Eight elements in a row of a matrix core operand.
+template <typename T>
+struct frag {
+  typedef s16x8_t type;
+};
+struct f32x8_t {
+  f32x4_t v[2];
+};
+template <>
+struct frag<float> {
+  typedef f32x8_t type;
+};
+
+__device__ __forceinline__ f32x4_t mma(_Float16, s16x8_t a, s16x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mma(bf16_t, s16x8_t a, s16x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(sgp::bf16x8_t, a), __builtin_bit_cast(sgp::bf16x8_t, b), c,
+                                                 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mma(float, const f32x8_t& a, const f32x8_t& b, f32x4_t c) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j >> 2][j & 3], b.v[j >> 2][j & 3], c, 0, 0, 0);
+  return c;
+}
+
+// Eight codes (two words) as M.
+template <typename M>
+__device__ __forceinline__ typename frag<M>::type decode(uint32_t lo, uint32_t hi) {
+  const uint32_t w[2] = {lo, hi};
+  if constexpr (__is_same(M, float)) {
+    f32x8_t x;
+#pragma unroll
+    for (int j = 0; j < 8; j++) x.v[j >> 2][j & 3] = (float)(int8_t)(w[j >> 2] >> ((j & 3) * 8));
+    return x;
+  } else if constexpr (__is_same(M, _Float16)) {
+    // 0x6400 + u is fp16's 1024 + u: bytes c + 128 behind 0x64, less 1152.
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    u32x4_t x;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const uint32_t u = w[i] ^ 0x80808080u;
+      const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+      x[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off);
+      x[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off);
+    }
+    return __builtin_bit_cast(s16x8_t, x);
+  } else {
+    // A float's upper half is the bf16: whole numbers below 2^8 have nothing in the lower.
+    u32x4_t x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t v = w[i >> 1] >> ((i & 1) * 16);
+      const float a = (float)(int8_t)v, b = (float)(int8_t)(v >> 8);
+      x[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    }
+    return __builtin_bit_cast(s16x8_t, x);
+  }
+}
+
+template <typename M>
+__device__ __forceinline__ typename frag<M>::type load_frag(const char* base, int f, int lane) {
+  if constexpr (__is_same(M, float)) {
+    f32x8_t x;
+    x.v[0] = *reinterpret_cast<const f32x4_t*>(base + f * 2048 + lane * 16);
+    x.v[1] = *reinterpret_cast<const f32x4_t*>(base + f * 2048 + 1024 + lane * 16);
+    return x;
+  } else {
+    return *reinterpret_cast<const s16x8_t*>(base + f * 1024 + lane * 16);
+  }
+}
+
+template <typename M>
+__device__ __forceinline__ void store_frag(char* base, int f, int lane, const typename frag<M>::type& x) {
+  if constexpr (__is_same(M, float)) {
+    *reinterpret_cast<f32x4_t*>(base + f * 2048 + lane * 16) = x.v[0];
+    *reinterpret_cast<f32x4_t*>(base + f * 2048 + 1024 + lane * 16) = x.v[1];
+  } else {
+    *reinterpret_cast<s16x8_t*>(base + f * 1024 + lane * 16) = x;
+  }
+}
+
+// 2^x, -infinity to 0.
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// tanh: x P(x^2) below 1/2 (9e-8 relative), 1 - 2 / (1 + e^2x) above.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float z = x * x, ax = fabsf(x);
+  float p = __builtin_fmaf(z, -0.00661201408f, 0.021273822f);
+  p = __builtin_fmaf(z, p, -0.0538932246f);
+  p = __builtin_fmaf(z, p, 0.133329003f);
+  p = __builtin_fmaf(z, p, -0.333333241f);
+  p = __builtin_fmaf(z, p, 1.0f) * x;
+  const float e = exp2_of(2.0f * kLog2e * ax);
+  const float far = __builtin_copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), x);
+  return ax < 0.5f ? p : far;  // (a NaN is far's)
+}
+
+// The largest over the four lanes that share a pair: lane, lane ^ 16, ^ 32, ^ 48.
+__device__ __forceinline__ float pair_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// The type that a kernel's values and weights are multiplied in, and the weights' halves.
+template <typename T, bool Q8>
+struct weight {
+  typedef T type;
+  static constexpr int parts = 1;
+};
+template <>
+struct weight<_Float16, true> {
+  typedef bf16_t type;
+  static constexpr int parts = 2;
+};
+template <>
+struct weight<bf16_t, true> {
+  typedef bf16_t type;
+  static constexpr int parts = 1;
+};
+// fp16 weights are multiplied by 2^6, so that they keep their bits down to 2^-20 (and with
+// the slack stay below 2^14); sums and outputs alike, so it leaves by itself.
+template <typename T, bool Q8>
+constexpr float kShift = __is_same(T, _Float16) && !Q8 ? 6.0f : 0.0f;
+
+// What a wave has of its QT * 16 pairs: queries, running maxima and sums, outputs.
+template <typename T, bool Q8, int D, int QT>
+struct state {
+  typename frag<T>::type q[QT][D / 32];
+  f32x4_t o[QT][D / 16];
+  float m[QT], l[QT];
+  int lo[QT], hi[QT];  // visible keys of the lane's pairs, counted from the job's first
+  int all_lo, all_hi;  // keys that every pair of the wave sees
+};
+
+// Eight weights as operands of the second product.
+template <typename T, bool Q8>
+__device__ __forceinline__ void pack_weights(const float* p, typename frag<typename weight<T, Q8>::type>::type* w) {
+  typedef typename weight<T, Q8>::type M;
+  if constexpr (__is_same(M, float)) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[0].v[j >> 2][j & 3] = p[j];
+  } else if constexpr (__is_same(M, _Float16)) {
+    half8_t x;
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = (_Float16)p[j];
+    w[0] = __builtin_bit_cast(s16x8_t, x);
+  } else {
+    sgp::bf16x8_t x;
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = (__bf16)p[j];
+    w[0] = __builtin_bit_cast(s16x8_t, x);
+    if constexpr (weight<T, Q8>::parts == 2) {
+      sgp::bf16x8_t y;
+#pragma unroll
+      for (int j = 0; j < 8; j++) y[j] = (__bf16)(p[j] - (float)x[j]);
+      w[1] = __builtin_bit_cast(s16x8_t, y);
+    }
+  }
+}
+
+// A tile's scores become weights: first: the place of the tile's first slot among the job's
+// keys (negative where the tile begins before them).  s: products; tail: the tile's, in LDS or
+// memory.
+template <typename T, bool Q8, int D, int QT>
+__device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8, D, QT>& st, f32x4_t (&s)[2][QT], int first,
+                                      const float* tail, int lane, float (&p)[QT][8]) {
+  const int g = lane >> 4;
+  float vs[8];
+  if constexpr (Q8) {
+    f32x4_t ks[2], v[2];
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      ks[half] = *reinterpret_cast<const f32x4_t*>(tail + half * 16 + g * 4);
+      v[half] = *reinterpret_cast<const f32x4_t*>(tail + kTile + half * 16 + g * 4);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float c = ks[j >> 2][j & 3] * a.scale;
+      vs[j] = v[j >> 2][j & 3];
+#pragma unroll
+      for (int t = 0; t < QT; t++) p[t][j] = s[j >> 2][t][j & 3] * c;
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) p[t][j] = s[j >> 2][t][j & 3] * a.scale;
+  }
+  if (a.cap != 0.0f) {
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) p[t][j] = a.cap * tanh_of(p[t][j]);
+  }
+  const bool part = first < st.all_lo || first + kTile > st.all_hi;
+  if (part) {
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int key = first + (j >> 2) * 16 + g * 4 + (j & 3);
+        p[t][j] = key >= st.lo[t] && key < st.hi[t] ? p[t][j] : -INFINITY;
+      }
+  }
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    float top = fmaxf(fmaxf(fmaxf(p[t][0], p[t][1]), fmaxf(p[t][2], p[t][3])),
+                      fmaxf(fmaxf(p[t][4], p[t][5]), fmaxf(p[t][6], p[t][7])));
+    if (__ballot(top > st.m[t] + kSlack)) {
+      top = fmaxf(pair_max(top), st.m[t]);
+      const float by = top > st.m[t] ? exp2_of(st.m[t] - top) : 1.0f;  // (m may be -infinity: 0)
+      st.m[t] = top;
+      st.l[t] *= by;
+#pragma unroll
+      for (int f = 0; f < D / 16; f++) st.o[t][f] *= by;
+    }
+    const float m = (st.m[t] == -INFINITY ? 0.0f : st.m[t]) - kShift<T, Q8>;
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      p[t][j] = exp2_of(p[t][j] - m);
+      sum += p[t][j];
+    }
+    st.l[t] += sum;
+    if constexpr (Q8) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) p[t][j] *= vs[j];
+      if (part) {  // a hidden key's scale may be NaN
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const int key = first + (j >> 2) * 16 + g * 4 + (j & 3);
+          p[t][j] = key >= st.lo[t] && key < st.hi[t] ? p[t][j] : 0.0f;
+        }
+      }
+    }
+  }
+}
+
+// A fragment of values without those of the keys in `bad`.
+template <typename T>
+__device__ __forceinline__ void drop_bad(typename frag<T>::type& x, uint32_t bad, int lane) {
+  const int g = lane >> 4;
+#pragma unroll
+  for (int j = 0; j < 8; j++)
+    if (bad >> ((j >> 2) * 16 + g * 4 + (j & 3)) & 1) {
+      if constexpr (__is_same(T, float)) x.v[j >> 2][j & 3] = 0.0f;
+      else x[j] = 0;
+    }
+}
+
+// Values that are not finite: a hidden key's zero weight times one is a NaN.  The products leave
+// such keys out (drop_bad), and the pairs that see them have them added here, one key at a time.
+// vals: the tile's values in memory.
+template <typename T, bool Q8, int D, int QT>
+__device__ __forceinline__ void add_bad(state<T, Q8, D, QT>& st, const float (&p)[QT][8], int first, uint32_t bad,
+                                        const char* vals, int lane) {
+  const int g = lane >> 4;
+  for (; bad; bad &= bad - 1) {
+    const int key = __builtin_ctz(bad), j = (key >> 4) * 4 + (key & 3), from = ((key >> 2) & 3) * 16;
+    float wt[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      float mine = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) mine = i == j ? p[t][i] : mine;
+      wt[t] = __shfl(mine, from + (lane & 15));
+    }
+#pragma unroll
+    for (int f = 0; f < D / 16; f++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float v = elem<T>::to(*reinterpret_cast<const T*>(vals + sgc::place<(int)sizeof(T)>(f, from + g * 4 + i, j)));
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+          st.o[t][f][i] = first + key >= st.lo[t] && first + key < st.hi[t] ? st.o[t][f][i] + wt[t] * v : st.o[t][f][i];
+      }
+      asm volatile("" ::: "memory");  // (one fragment's loads at a time: registers)
+    }
+  }
+}
+
+// Worker index of a workgroup: workgroups go round the eight XCDs, and neighbouring workers, which
+// read the same head's tiles, stay on one.
+__device__ __forceinline__ int spread(int block, int blocks) { return (block & 7) * (blocks >> 3) + (block >> 3); }
+
+// Which (job, units) a worker has: the list laid out head by head, `per` units a worker.
+struct share {
+  int head, job;
+  int64_t at, left;  // unit within the head's, units to do
+};
+
+template <int D, int QT>
+__device__ __forceinline__ share first_share(const sg_attn_list& list, int64_t worker, int heads, int lane) {
+  share s{0, 0, 0, 0};
+  const int64_t units = list.plan->units, per = list.plan->per, total = units * heads;
+  const int64_t begin = worker * per;
+  if (begin >= total) return s;
+  s.left = min(per, total - begin);
+  s.head = (int)(begin / units);
+  s.at = begin - s.head * units;
+  // The last job that begins at or before the unit and is not empty: 64 candidates a step.
+  int lo = 0, len = list.plan->jobs;
+  while (len > 1) {
+    const int step = (len + 63) >> 6, j = lane * step;
+    const int c = __popcll(__ballot(j < len && list.cum[lo + j] <= s.at));
+    lo += (c - 1) * step;
+    len = min(step, len - (c - 1) * step);
+  }
+  s.job = __builtin_amdgcn_readfirstlane(lo);
+  return s;
+}
+
+// Loads the wave's pairs of a job: queries and the keys each sees.
+template <typename T, bool Q8, int D, int QT>
+__device__ __forceinline__ void begin_job(const sg_attn_shared_args& a, state<T, Q8, D, QT>& st, const sg_attn_job& job, int head,
+                                          int pair0, int lane) {
+  const int g = lane >> 4;
+  int all_lo = 0, all_hi = INT32_MAX;
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const int64_t pair = (int64_t)pair0 + t * 16 + (lane & 15);
+    const bool in = pair < (int64_t)job.rows * a.group;
+    const int r = in ? (int)(pair / a.group) : 0, row = job.row0 + r;
+    const int h = head * a.group + (in ? (int)(pair - (int64_t)r * a.group) : 0);
+    const T* q = static_cast<const T*>(a.q) + row * a.ldq + (int64_t)h * a.hd;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++) {
+      const int dim = d * 32 + g * 8;
+      typename frag<T>::type x{};
+      if (in && dim < a.hd) {
+        if constexpr (__is_same(T, float)) {
+          x.v[0] = *reinterpret_cast<const f32x4_t*>(q + dim);
+          x.v[1] = *reinterpret_cast<const f32x4_t*>(q + dim + 4);
+        } else {
+          x = *reinterpret_cast<const s16x8_t*>(q + dim);
+        }
+      }
+      st.q[t][d] = x;
+    }
+    const int4 seen = a.seen[row];
+    st.lo[t] = in ? (job.own ? seen.z : seen.x) : 0;
+    st.hi[t] = in ? (job.own ? seen.w : seen.y) : 0;
+    if (in) {
+      all_lo = max(all_lo, st.lo[t]);
+      all_hi = min(all_hi, st.hi[t]);
+    }
+    st.m[t] = -INFINITY;
+    st.l[t] = 0.0f;
+#pragma unroll
+    for (int f = 0; f < D / 16; f++) st.o[t][f] = f32x4_t{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) {  // (lanes 16 apart have the same pairs)
+    all_lo = max(all_lo, __shfl_xor(all_lo, o));
+    all_hi = min(all_hi, __shfl_xor(all_hi, o));
+  }
+  st.all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  st.all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+}
+
+// What a wave has of a job to the workspace: the pairs' own place when the worker did the whole
+// job, the worker's first or last piece otherwise.
+template <typename T, bool Q8, int D, int QT>
+__device__ __forceinline__ void end_job(const sg_attn_shared_args& a, const sg_attn_list& list, state<T, Q8, D, QT>& st,
+                                        const sg_attn_job& job, int head, int pair0, int in_job, int64_t worker, bool whole,
+                                        bool later, int lane) {
+  const int g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const float l = pair_sum(st.l[t]);
+    const int64_t pair = (int64_t)pair0 + t * 16 + (lane & 15);
+    if (pair >= (int64_t)job.rows * a.group) continue;
+    int64_t at;
+    if (whole) {
+      const int r = (int)(pair / a.group);
+      at = ((int64_t)(job.own ? a.rows : 0) + job.row0 + r) * a.heads + head * a.group + (pair - (int64_t)r * a.group);
+    } else {
+      at = list.piece0 + (worker * 2 + (later ? 0 : 1)) * list.piece_pairs + in_job + t * 16 + (lane & 15);
+    }
+    float* o = a.part_o + at * D;
+#pragma unroll
+    for (int f = 0; f < D / 16; f++) *reinterpret_cast<f32x4_t*>(o + f * 16 + g * 4) = st.o[t][f];
+    if (g == 0) a.part_ml[at] = make_float2(st.m[t], l);
+  }
+}
+
+// Few pairs: every wave is a worker and takes fragments from memory, no barrier anywhere.
+template <typename T, bool Q8, int D>
+__global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narrow(sg_attn_shared_args a, sg_attn_list list) {
+  typedef typename weight<T, Q8>::type M;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t worker = (int64_t)spread(blockIdx.x, gridDim.x) * 4 + wave;
+  share sh = first_share<D, 1>(list, worker, a.kv_heads, lane);
+  state<T, Q8, D, 1> st;
+  while (sh.left > 0) {
+    const sg_attn_job job = list.jobs[sh.job];
+    const int64_t c0 = list.cum[sh.job], c1 = list.cum[sh.job + 1];
+    const int64_t skip = sh.at - c0, n = min(c1 - sh.at, sh.left);
+    if (n > 0) {
+      const int pair0 = job.tile * 16;
+      begin_job(a, st, job, sh.head, pair0, lane);
+      int64_t tile = job.slot_tile + skip;
+      int first = (int)(tile * kTile - job.key0);
+      const char* at = a.cache + (int64_t)sh.head * a.head_bytes + tile * a.tile_bytes;
+      for (int64_t u = 0; u < n; u++, first += kTile, at += a.tile_bytes) {
+        const char* vals = at + (int64_t)kTile * D * sizeof(typename sgc::kept<T, Q8>::type);
+        const char* tail = at + a.tile_bytes - kTail;
+        f32x4_t s[2][1] = {};
+        float p[1][8];
+        typename frag<M>::type w[weight<T, Q8>::parts];
+        if constexpr (Q8) {
+          constexpr int NU = D / 32;  // kilobytes of the keys, and of the values
+          u32x4_t kc[NU], vc[NU];
+#pragma unroll
+          for (int i = 0; i < NU; i++) kc[i] = *reinterpret_cast<const u32x4_t*>(at + i * 1024 + lane * 16);
+#pragma unroll
+          for (int i = 0; i < NU; i++) vc[i] = *reinterpret_cast<const u32x4_t*>(vals + i * 1024 + lane * 16);
+#pragma unroll
+          for (int i = 0; i < NU; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const int f = i * 2 + e, half = f / (D / 32), d = f % (D / 32);
+              s[half][0] = mma(T{}, decode<T>(kc[i][e * 2], kc[i][e * 2 + 1]), st.q[0][d], s[half][0]);
+            }
+          weigh<T, Q8, D, 1>(a, st, s, first, reinterpret_cast<const float*>(tail), lane, p);
+          pack_weights<T, Q8>(p[0], w);
+#pragma unroll
+          for (int i = 0; i < NU; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const typename frag<M>::type x = decode<M>(vc[i][e * 2], vc[i][e * 2 + 1]);
+#pragma unroll
+              for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[0][i * 2 + e] = mma(M{}, x, w[h], st.o[0][i * 2 + e]);
+            }
+        } else {
+          const uint32_t bad = *reinterpret_cast<const uint32_t*>(tail);
+#pragma unroll
+          for (int half = 0; half < 2; half++)
+#pragma unroll
+            for (int d = 0; d < D / 32; d++)
+              s[half][0] = mma(T{}, load_frag<T>(at, half * (D / 32) + d, lane), st.q[0][d], s[half][0]);
+          weigh<T, Q8, D, 1>(a, st, s, first, nullptr, lane, p);
+          pack_weights<T, Q8>(p[0], w);
+#pragma unroll
+          for (int f = 0; f < D / 16; f++) {
+            typename frag<T>::type x = load_frag<T>(vals, f, lane);
+            if (bad) drop_bad<T>(x, bad, lane);
+            st.o[0][f] = mma(M{}, x, w[0], st.o[0][f]);
+          }
+          if (bad) add_bad(st, p, first, bad, vals, lane);
+        }
+      }
+      end_job(a, list, st, job, sh.head, pair0, 0, worker, n == c1 - c0, skip > 0, lane);
+      sh.left -= n;
+      sh.at += n;
+    }
+    if (++sh.job >= list.plan->jobs) {  // the next head's first job
+      sh.job = 0;
+      sh.at = 0;
+      sh.head++;
+    }
+  }
+}
+
+// Many pairs: a workgroup is a worker, its four waves have QT * 16 pairs each and share the tiles
+// in LDS, two stages.  Types go there by direct copies; codes through registers, and lie there
+// as the type that multiplies them.
+template <typename T, bool Q8, int D, int QT>
+__global__ __launch_bounds__(256, __is_same(T, float) && D == 256 ? 1 : 2) void k_attn_wide(sg_attn_shared_args a,
+                                                                                          sg_attn_list list) {
+  typedef typename weight<T, Q8>::type M;
+  constexpr int ES = sizeof(T), KB = kTile * D * ES, STAGE = 2 * KB + (Q8 ? kTail : 0);
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t worker = spread(blockIdx.x, gridDim.x);
+  share sh = first_share<D, QT>(list, worker, a.kv_heads, lane);
+  state<T, Q8, D, QT> st;
+  while (sh.left > 0) {
+    const sg_attn_job job = list.jobs[sh.job];
+    const int64_t c0 = list.cum[sh.job], c1 = list.cum[sh.job + 1];
+    const int64_t skip = sh.at - c0, n = min(c1 - sh.at, sh.left);
+    if (n > 0) {
+      const int in_job = wave * QT * 16, pair0 = job.tile * (64 * QT) + in_job;
+      const int64_t tile = job.slot_tile + skip;
+      int first = (int)(tile * kTile - job.key0);
+      const char* at = a.cache + (int64_t)sh.head * a.head_bytes + tile * a.tile_bytes;
+      constexpr int NU = Q8 ? D / 16 / 4 : 2 * KB / 1024 / 4;  // kilobytes of a tile for each wave
+      u32x4_t codes[Q8 ? NU : 1];
+      float tail_of = 0.0f;
+      auto fetch = [&](const char* from, int stage) {
+        if constexpr (Q8) {
+#pragma unroll
+          for (int i = 0; i < NU; i++) codes[i] = *reinterpret_cast<const u32x4_t*>(from + (wave * NU + i) * 1024 + lane * 16);
+          if (wave == 0) tail_of = *reinterpret_cast<const float*>(from + a.tile_bytes - kTail + lane * 4);
+        } else {
+          const i32x4_t rsrc = sg_raw_rsrc(from);
+#pragma unroll
+          for (int i = 0; i < NU; i++) {
+            const uint32_t u = wave * NU + i;
+            sg_lds_copy16((uint32_t)(stage * STAGE + u * 1024), lane * 16, rsrc, u * 1024);
+          }
+        }
+      };
+      auto put = [&](int stage) {
+        if constexpr (Q8) {
+          char* to = lds + stage * STAGE;
+#pragma unroll
+          for (int i = 0; i < NU; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const int u = wave * NU + i, f = u * 2 + e;  // fragment of keys, then of values
+              if (u < D / 32) store_frag<T>(to, f, lane, decode<T>(codes[i][e * 2], codes[i][e * 2 + 1]));
+              else store_frag<M>(to + KB, f - D / 16, lane, decode<M>(codes[i][e * 2], codes[i][e * 2 + 1]));
+            }
+          if (wave == 0) *reinterpret_cast<float*>(to + 2 * KB + lane * 4) = tail_of;
+        }
+      };
+      __syncthreads();  // the last job's stages have been read
+      fetch(at, 0);
+      begin_job(a, st, job, sh.head, pair0, lane);
+      put(0);
+      for (int64_t u = 0; u < n; u++, first += kTile) {
+        const int stage = (int)(u & 1);
+        if constexpr (!Q8) sg_wait_vmcnt<0>();
+        __syncthreads();
+        const char* here = at;
+        at += a.tile_bytes;
+        if (u + 1 < n) fetch(at, stage ^ 1);
+        const char* keys = lds + stage * STAGE;
+        const char* vals = keys + KB;
+        f32x4_t s[2][QT] = {};
+        float p[QT][8];
+#pragma unroll
+        for (int half = 0; half < 2; half++)
+#pragma unroll
+          for (int d = 0; d < D / 32; d++) {
+            const typename frag<T>::type x = load_frag<T>(keys, half * (D / 32) + d, lane);
+#pragma unroll
+            for (int t = 0; t < QT; t++) s[half][t] = mma(T{}, x, st.q[t][d], s[half][t]);
+          }
+        weigh<T, Q8, D, QT>(a, st, s, first, Q8 ? reinterpret_cast<const float*>(keys + 2 * KB) : nullptr, lane, p);
+        typename frag<M>::type w[QT][weight<T, Q8>::parts];
+#pragma unroll
+        for (int t = 0; t < QT; t++) pack_weights<T, Q8>(p[t], w[t]);
+        uint32_t bad = 0;
+        if constexpr (!Q8) {
+          bad = *reinterpret_cast<const uint32_t*>(here + a.tile_bytes - kTail);
+          if (bad) {  // (alike for the workgroup)
+            char* own = lds + stage * STAGE + KB;
+            for (int f = wave; f < D / 16; f += 4) {
+              typename frag<T>::type x = load_frag<T>(own, f, lane);
+              drop_bad<T>(x, bad, lane);
+              store_frag<T>(own, f, lane, x);
+            }
+            __syncthreads();
+          }
+        }
+#pragma unroll
+        for (int f = 0; f < D / 16; f++) {
+          const typename frag<M>::type x = load_frag<M>(vals, f, lane);
+#pragma unroll
+          for (int t = 0; t < QT; t++)
+#pragma unroll
+            for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[t][f] = mma(M{}, x, w[t][h], st.o[t][f]);
+        }
+        if constexpr (!Q8)
+          if (bad) add_bad(st, p, first, bad, here + KB, lane);
+        if (u + 1 < n) put(stage ^ 1);
+      }
+      end_job(a, list, st, job, sh.head, pair0, in_job, worker, n == c1 - c0, skip > 0, lane);
+      sh.left -= n;
+      sh.at += n;
+    }
+    if (++sh.job >= list.plan->jobs) {
+      sh.job = 0;
+      sh.at = 0;
+      sh.head++;
+    }
+  }
+}
+
+template <typename T, bool Q8, int D>
+hipError_t launch_list(const sg_attn_shared_args& a, const sg_attn_list& list, hipStream_t s) {
+  if (!list.wide) return sgp::run_kernel(k_attn_narrow<T, Q8, D>, dim3(list.blocks), dim3(256), 0, s, a, list);
+  constexpr int QT = sgk::attn_wide_pairs(D) / 64;
+  constexpr size_t lds = 2 * (2 * kTile * D * sizeof(T) + (Q8 ? kTail : 0));
+  auto kernel = k_attn_wide<T, Q8, D, QT>;
+  // More than 64 KB has to be asked for, on every device.
+  static std::atomic<uint64_t> asked{0};
+  int device = 0;
+  hipError_t e = hipGetDevice(&device);
+  if (e != hipSuccess) return e;
+  if (device >= 64 || !(asked.load(std::memory_order_relaxed) >> device & 1)) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return e;
+    }
+    if (device < 64) asked.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+  }
+  return sgp::run_kernel(kernel, dim3(list.blocks), dim3(256), lds, s, a, list);
+}
+
+template <typename T>
+hipError_t launch_type(const sg_attn_shared_args& a, const sg_attn_list& list, bool q8, int D, hipStream_t s) {
+  if (q8) {
+    if (D == 64) return launch_list<T, true, 64>(a, list, s);
+    if (D == 128) return launch_list<T, true, 128>(a, list, s);
+    return launch_list<T, true, 256>(a, list, s);
+  }
+  if (D == 64) return launch_list<T, false, 64>(a, list, s);
+  if (D == 128) return launch_list<T, false, 128>(a, list, s);
+  return launch_list<T, false, 256>(a, list, s);
+}
+
+}  // namespace sga

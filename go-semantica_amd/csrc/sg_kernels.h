@@ -92,6 +92,64 @@ struct sg_adapters_args {
   int rows, n_seq, n_adapters, in_dim, out_dim, rank_pad;
 };
 
+// One sg_kv_cache_write or _read call (k_kv_cache.hip); strides in elements.  k and v are
+// written by a read only.
+struct sg_kv_rows_args {
+  char* cache;
+  int64_t head_bytes, tile_bytes, slots;
+  void* k;
+  void* v;
+  int64_t ldk, ldv;
+  const int32_t* off;
+  const int32_t* starts;
+  int rows, n_seq, heads, hd, D;
+};
+
+// One sg_attention_shared call (k_attn_shared.hip); strides in elements.
+struct sg_attn_shared_args {
+  void* out;
+  const void* q;
+  const char* cache;
+  int64_t ldo, ldq, head_bytes, tile_bytes;
+  const int4* seen;   // [rows]: visible places of the prefix, of the own keys (begin, end)
+  const int4* where;  // [rows]: first job and first row of its prefix's group, of its sequence's
+  float* part_o;      // [2 rows * heads, then pieces][D]
+  float2* part_ml;
+  float scale, cap;   // in powers of two
+  int rows, heads, kv_heads, group, hd;
+};
+// Consecutive pairs of a group over a range of tiles.
+struct sg_attn_job {
+  int row0, rows, tile;  // the group's rows; which M pairs of them
+  int key0, slot_tile;   // the slot of the first key; the first tile with a visible one
+  int own;               // 0: a prefix, 1: a sequence's own keys
+};
+struct sg_attn_plan {
+  int64_t units, per;  // units of a head, of a worker
+  int32_t jobs;
+};
+struct sg_attn_list {
+  sg_attn_plan* plan;
+  int64_t* cum;  // [jobs + 1]: units before a job
+  sg_attn_job* jobs;
+  int64_t piece0;  // first row of the list's pieces in part_o
+  int m, piece_pairs;  // pairs of a job, of a piece of one
+  int blocks, workers, wide, cap, min_units;  // cap: jobs that fit
+};
+// What the plan is made from (device arrays as sg_shared_keys names them).
+struct sg_attn_batch {
+  const int32_t* off;
+  const int32_t* starts;
+  const int32_t* lengths;
+  const int32_t* shared;
+  const int32_t* prefix_starts;
+  const int32_t* prefix_lengths;
+  int32_t* seq_jobs;     // [n_seq + 1]
+  int32_t* prefix_jobs;  // [n_prefix + 1]
+  int64_t slots;
+  int n_seq, n_prefix, causal, window;
+};
+
 namespace sgk {
 
 // GEMM operands are block-major int8 [K/32][rows][32]; activation buffers hold
@@ -327,6 +385,18 @@ hipError_t adapters_pack(int dtype, const void* a, const void* b, int n, int ran
                          void* wb, hipStream_t s);
 size_t adapters_work_bytes(int dtype, int rows, int in_dim, int rank_pad);
 hipError_t adapters_apply(const sg_adapters_args& a, int dtype, hipStream_t s);
+
+// ---- kept keys and values (k_kv_cache.hip, k_attn_shared*.hip) ----
+int64_t kv_rows_threads(int rows);
+hipError_t kv_write(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
+hipError_t kv_read(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
+constexpr int attn_wide_pairs(int D) { return D == 256 ? 64 : 128; }  // of a job of the wide form
+size_t attn_shared_work_bytes(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix);
+// a's workspace pointers, seen and where, and the batch's arrays, are placed in work.
+hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q8, int D, void* work, hipStream_t s);
+hipError_t attn_shared_f32(const sg_attn_shared_args& a, const sg_attn_list& list, bool q8, int D, hipStream_t s);
+hipError_t attn_shared_f16(const sg_attn_shared_args& a, const sg_attn_list& list, bool q8, int D, hipStream_t s);
+hipError_t attn_shared_bf16(const sg_attn_shared_args& a, const sg_attn_list& list, bool q8, int D, hipStream_t s);
 
 // ---- brute-force search (k_search.hip) ----
 // Storage modes, the values of brute.QuantizationMode (search/brute/quant.go:8-15).

@@ -95,6 +95,12 @@ class AttnMask(ctypes.Structure):
                 ("prefix", _vp), ("causal", ctypes.c_int32), ("window", ctypes.c_int32)]
 
 
+class SharedKeys(ctypes.Structure):
+    _fields_ = [("starts", _vp), ("lengths", _vp), ("shared", _vp), ("prefix_starts", _vp), ("prefix_lengths", _vp),
+                ("n_prefix", ctypes.c_int32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+                ("causal", ctypes.c_int32), ("window", ctypes.c_int32)]
+
+
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
@@ -148,6 +154,14 @@ _PROTOS = {
     "sg_adapters_work_bytes": (ctypes.c_int, [_vp, _i32, ctypes.POINTER(ctypes.c_size_t)]),
     "sg_adapters_apply": (ctypes.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _vp,
                                          ctypes.c_size_t, _vp]),
+    "sg_kv_cache_create": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i32, _i32, _vp, _pp]),
+    "sg_kv_cache_free": (None, [_vp]),
+    "sg_kv_cache_bytes": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_size_t)]),
+    "sg_kv_cache_write": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp]),
+    "sg_kv_cache_read": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp]),
+    "sg_attention_shared_work_bytes": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i32, ctypes.POINTER(ctypes.c_size_t)]),
+    "sg_attention_shared": (ctypes.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _i32,
+                                           ctypes.POINTER(SharedKeys), _vp, ctypes.c_size_t, _vp]),
     "sg_index_build": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _i32, _pp]),
     "sg_index_build_device": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, ctypes.c_int64, _i32, _vp, _pp]),
     "sg_index_deserialize": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _pp]),

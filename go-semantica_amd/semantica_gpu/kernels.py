@@ -13,11 +13,12 @@ device tensors (torch is used only to hold HIP device memory and streams).
 and the layer operators of sibling models, which have no counterpart there:
 
   attention_masked, block_norm, AdapterBank + adapters_apply
+  KVCache + kv_cache_write, kv_cache_read, attention_shared
 
 They take row-strided 2-D tensors of float32, float16 or bfloat16 and the CSR
 offsets as an int32 device tensor, run asynchronously on the current stream of the
-tensors' device (or `stream`), and allocate nothing but adapters_apply's default
-workspace.
+tensors' device (or `stream`), and allocate nothing but the default workspaces of
+adapters_apply and attention_shared.
 """
 from __future__ import annotations
 
@@ -307,16 +308,16 @@ def block_norm(ctx, xn, sum, x, h, w_post, w_pre, eps, *, gate=None, scale=1.0, 
                                      n_seq, _stream_of(ctx, stream)))
 
 
-_COLLECTED = collections.deque()  # banks' handles
+_COLLECTED = collections.deque()  # handles of banks, caches, and how they are freed
 
 
 def _free_collected():
     while _COLLECTED:
         try:
-            lib, handle = _COLLECTED.popleft()
+            free, handle = _COLLECTED.popleft()
         except IndexError:  # another thread's
             return
-        lib.sg_adapter_bank_free(handle)
+        free(handle)
 
 
 class AdapterBank:
@@ -360,7 +361,17 @@ class AdapterBank:
 
     def __del__(self):
         if self.handle and _COLLECTED is not None:  # (None: the interpreter ends)
-            _COLLECTED.append((self.lib, self.handle))
+            _COLLECTED.append((self.lib.sg_adapter_bank_free, self.handle))
+
+
+def _workspace(size, like, stream):
+    """`size` bytes from torch's allocator, of the stream that will use them."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(size, dtype=torch.uint8, device=like.device)
+    # Of that stream: what the current one gave back, its work may still write.
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=like.device)):
+        return torch.empty(size, dtype=torch.uint8, device=like.device)
 
 
 def adapters_apply(ctx, dst, base, bank: AdapterBank, x, offsets, adapter_ids, *, work=None, stream=None):
@@ -378,13 +389,116 @@ def adapters_apply(ctx, dst, base, bank: AdapterBank, x, offsets, adapter_ids, *
     b, ldb = _rows_of(ctx, "base", base, rows, bank.out_dim, bank.dtype)
     off, n_seq = _offsets(ctx, offsets)
     if work is None:
-        size = max(bank.work_bytes(rows), 16)
-        if stream is None:
-            work = torch.empty(size, dtype=torch.uint8, device=x.device)
-        else:  # of that stream: what the current one gave back, its work may still write
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=x.device)):
-                work = torch.empty(size, dtype=torch.uint8, device=x.device)
+        work = _workspace(max(bank.work_bytes(rows), 16), x, stream)
     _lib.check(ctx.lib.sg_adapters_apply(ctx.handle, d, ldd, b, ldb, bank.handle, xp, ldx, rows, off, n_seq,
                                          _vec(ctx, "adapter_ids", adapter_ids, n_seq, torch.int32),
                                          _vec(ctx, "work", work, None, torch.uint8), work.numel(),
                                          _stream_of(ctx, stream)))
+
+
+class KVCache:
+    """Keys and values of `slots` tokens kept on the GPU (sg_kv_cache_create), n_kv_heads heads
+    of head_dim; dtype: of rows in and out and of queries.  bits 8: codes and a scale for each
+    token and head; bits 0: the values themselves.
+
+    Made and closed as an AdapterBank is: neither is for a time when any thread captures a graph."""
+
+    def __init__(self, ctx, slots, n_kv_heads, head_dim, dtype, bits=8, stream=None):
+        self.handle = None
+        _torch()
+        if dtype not in _DTYPES:
+            raise ValueError(f"{dtype}: float32, float16 or bfloat16 is needed")
+        if max(slots, n_kv_heads, head_dim) > _MOST:
+            _too_many("slots, heads or dims", max(slots, n_kv_heads, head_dim))
+        self.ctx, self.lib, self.dtype, self.bits = ctx, ctx.lib, dtype, bits
+        self.slots, self.n_kv_heads, self.head_dim = slots, n_kv_heads, head_dim
+        _free_collected()
+        h = ctypes.c_void_p()
+        _lib.check(self.lib.sg_kv_cache_create(ctx.handle, slots, n_kv_heads, head_dim, _DTYPES[dtype], bits,
+                                               _stream_of(ctx, stream), ctypes.byref(h)))
+        self.handle = h
+
+    @property
+    def nbytes(self):
+        """Bytes of device memory that it holds."""
+        size = ctypes.c_size_t()
+        _lib.check(self.lib.sg_kv_cache_bytes(self.handle, ctypes.byref(size)))
+        return size.value
+
+    def work_bytes(self, n_heads, rows, n_seq, n_prefix):
+        """Bytes of `work` that attention_shared needs for so many rows, sequences and prefixes or fewer."""
+        if max(n_heads, rows, n_seq, n_prefix) > _MOST:
+            _too_many("heads, rows, sequences or prefixes", max(n_heads, rows, n_seq, n_prefix))
+        size = ctypes.c_size_t()
+        _lib.check(self.lib.sg_attention_shared_work_bytes(self.handle, n_heads, rows, n_seq, n_prefix,
+                                                           ctypes.byref(size)))
+        return size.value
+
+    def close(self):
+        _free_collected()
+        if self.handle:
+            self.lib.sg_kv_cache_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        if self.handle and _COLLECTED is not None:  # (None: the interpreter ends)
+            _COLLECTED.append((self.lib.sg_kv_cache_free, self.handle))
+
+
+def _kv_rows(call, ctx, cache, k, v, offsets, starts, stream):
+    rows, cols = k.shape[0], cache.n_kv_heads * cache.head_dim
+    if rows > _MOST:
+        _too_many("rows of k", rows)
+    kp, ldk = _rows_of(ctx, "k", k, rows, cols, cache.dtype)
+    vp, ldv = _rows_of(ctx, "v", v, rows, cols, cache.dtype)
+    off, n_seq = _offsets(ctx, offsets)
+    st = _vec(ctx, "starts", starts, n_seq, _torch().int32)
+    _lib.check(call(ctx.handle, cache.handle, kp, ldk, vp, ldv, rows, off, n_seq, st, _stream_of(ctx, stream)))
+
+
+def kv_cache_write(ctx, cache: KVCache, k, v, offsets, starts, *, stream=None):
+    """Rows of k and v [rows, n_kv_heads * head_dim] into the cache (sg_kv_cache_write): those of
+    sequence i, offsets[i] .. offsets[i + 1], go to the slots from starts[i] (int32 [n_seq]) on."""
+    _kv_rows(ctx.lib.sg_kv_cache_write, ctx, cache, k, v, offsets, starts, stream)
+
+
+def kv_cache_read(ctx, k, v, cache: KVCache, offsets, starts, *, stream=None):
+    """The cache's rows back into k and v (sg_kv_cache_read), as kv_cache_write places them."""
+    _kv_rows(ctx.lib.sg_kv_cache_read, ctx, cache, k, v, offsets, starts, stream)
+
+
+def attention_shared(ctx, out, q, cache: KVCache, n_heads, offsets, starts, lengths, shared=None, prefix_starts=None,
+                     prefix_lengths=None, *, scale=0.0, softcap=0.0, causal=True, window=0, work=None, stream=None):
+    """Attention of a batch's queries over kept keys, long prefixes read once for all the
+    sequences that share them (sg_attention_shared).
+
+    q, out [rows, n_heads * head_dim]; offsets int32 [n_seq + 1].  Sequence i's own keys, its
+    queries' tokens last, are slots starts[i] .. starts[i] + lengths[i]; sequences shared[p] ..
+    shared[p + 1] stand behind prefix p, slots prefix_starts[p] .. prefix_starts[p] +
+    prefix_lengths[p] (all int32 device tensors; shared None: no prefixes).  work: a uint8
+    device tensor of cache.work_bytes(...) at least, not shared by calls that may run at the
+    same time; None: one from torch's allocator."""
+    torch = _torch()
+    i32 = torch.int32
+    rows, cols = q.shape[0], n_heads * cache.head_dim
+    if rows > _MOST or n_heads > _MOST:
+        _too_many("rows or heads of q", max(rows, n_heads))
+    qp, ldq = _rows_of(ctx, "q", q, rows, cols, cache.dtype)
+    o, ldo = _rows_of(ctx, "out", out, rows, cols, cache.dtype)
+    off, n_seq = _offsets(ctx, offsets)
+    n_prefix = 0
+    if shared is not None:
+        if shared.numel() > _MOST:
+            _too_many("shared", shared.numel())
+        n_prefix = shared.numel() - 1
+        if n_prefix < 0 or prefix_starts is None or prefix_lengths is None:
+            raise ValueError("shared: [n_prefix + 1] offsets, with prefix_starts and prefix_lengths")
+    keys = _lib.SharedKeys(_vec(ctx, "starts", starts, n_seq, i32), _vec(ctx, "lengths", lengths, n_seq, i32),
+                           _vec(ctx, "shared", shared, None, i32), _vec(ctx, "prefix_starts", prefix_starts, n_prefix, i32),
+                           _vec(ctx, "prefix_lengths", prefix_lengths, n_prefix, i32), n_prefix, scale, softcap, causal,
+                           max(-1, min(window, _MOST)))
+    if work is None:
+        work = _workspace(max(cache.work_bytes(n_heads, rows, max(n_seq, 0), n_prefix), 16), q, stream)
+    _lib.check(ctx.lib.sg_attention_shared(ctx.handle, o, ldo, qp, ldq, cache.handle, n_heads, rows, off, n_seq, keys,
+                                           _vec(ctx, "work", work, None, torch.uint8), work.numel(),
+                                           _stream_of(ctx, stream)))

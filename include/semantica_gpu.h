@@ -434,6 +434,83 @@ int sg_adapters_apply(sg_ctx *ctx, void *dst, int64_t ldd, const void *base, int
                       const void *x, int64_t ldx, int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq,
                       const int32_t *d_adapter_ids, void *work, size_t work_bytes, void *stream);
 
+/* ---- kept keys and values ------------------------------------------------
+ * For a causal sibling of the built-in model that answers requests behind text it
+ * has run before: a document or an instruction is run once, its keys and values are
+ * kept, and every request runs only its own tokens.  No counterpart in the reference.
+ * The calls are asynchronous on `stream` (NULL: the context's), allocate nothing and may
+ * be captured; the order of calls that write slots and calls that read them is the
+ * caller's, by streams, as with any memory. */
+
+/* A cache of `slots` tokens' keys and values, n_kv_heads heads of head_dim (a multiple of
+ * 8 up to 256; kept as 64, 128 or 256).  dtype: the type of rows in and out, and of
+ * queries.  bits 0: kept as they are; bits 8: for each slot and head
+ *   scale = max(max|x| / 127, 2^-126) as float32, code = the whole number nearest to
+ *   x / scale (halves to even),
+ * one scale for its key, one for its value.  A key or value that holds an infinity or a NaN
+ * has a NaN for its scale: it reads as NaNs.  Slots that were never written are zeros.
+ * Making a cache waits for its clearing, freeing it for the device; neither is for a time when
+ * a thread captures a graph. */
+typedef struct sg_kv_cache sg_kv_cache;
+int sg_kv_cache_create(sg_ctx *ctx, int32_t slots, int32_t n_kv_heads, int32_t head_dim, int32_t dtype, int32_t bits,
+                       void *stream, sg_kv_cache **out);
+void sg_kv_cache_free(sg_kv_cache *cache);
+/* Bytes of device memory that it holds. */
+int sg_kv_cache_bytes(const sg_kv_cache *cache, size_t *bytes);
+
+/* Rows of a packed batch into the cache and out of it: row t of sequence i (offsets
+ * d_seq_offsets [n_seq+1] in device memory, ascending) is slot d_starts[i] + t -
+ * d_seq_offsets[i].  k, v [rows][n_kv_heads * head_dim] of the cache's type with row strides
+ * in elements, pointers 16-byte aligned, strides whole 16 bytes; a read's k and v do not
+ * overlap (columns of one tensor, with the same stride, do not).  Rows of no sequence are
+ * neither written nor read.  A slot outside the cache (every slot of a negative start)
+ * is not written, and reads as zeros.  Where two sequences of a write name the same slot, the
+ * later one's row is kept.  rows: up to 2^29 or a little less. */
+int sg_kv_cache_write(sg_ctx *ctx, sg_kv_cache *cache, const void *k, int64_t ldk, const void *v, int64_t ldv,
+                      int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq, const int32_t *d_starts, void *stream);
+int sg_kv_cache_read(sg_ctx *ctx, const sg_kv_cache *cache, void *k, int64_t ldk, void *v, int64_t ldv, int32_t rows,
+                     const int32_t *d_seq_offsets, int32_t n_seq, const int32_t *d_starts, void *stream);
+
+/* Which keys a batch's queries see, all arrays in device memory.  Sequence i's own keys are
+ * slots starts[i] .. starts[i] + lengths[i] - 1, behind those of its prefix: sequences
+ * shared[p] .. shared[p+1] - 1 (shared [n_prefix+1], ascending) share prefix p, slots
+ * prefix_starts[p] .. + prefix_lengths[p] - 1; a sequence outside them all has none.
+ * A range that does not lie in the cache is empty. */
+typedef struct {
+  const int32_t *starts;         /* [n_seq]                                             */
+  const int32_t *lengths;        /* [n_seq]: own keys, the queries' tokens among them    */
+  const int32_t *shared;         /* [n_prefix+1]                                         */
+  const int32_t *prefix_starts;  /* [n_prefix]                                           */
+  const int32_t *prefix_lengths; /* [n_prefix]                                           */
+  int32_t n_prefix;              /* 0: no prefixes, the three above may be NULL           */
+  float scale;                   /* of q.k; 0: 1/sqrt(head_dim)                          */
+  float softcap;                 /* s = cap * tanh(s / cap); 0: none                     */
+  int32_t causal;                /* a query sees no key behind its own place             */
+  int32_t window;                /* ... none window places away or farther; 0: any       */
+} sg_shared_keys;
+
+/* Bytes of workspace that sg_attention_shared needs for so many rows, sequences and prefixes
+ * or fewer of each. */
+int sg_attention_shared_work_bytes(const sg_kv_cache *cache, int32_t n_heads, int32_t rows, int32_t n_seq,
+                                   int32_t n_prefix, size_t *bytes);
+
+/* Softmax attention of a packed batch's queries over kept keys, a prefix read once for all
+ * that share it.  The n queries of a sequence are the last n places of its prefix and
+ * own keys together (a query before the first place has none, and sees under causal nothing);
+ * a row that sees no key, or only scores of -infinity, is zeros, rows of no sequence stay as
+ * they were.  What hidden slots hold does not matter.  q, out [rows][n_heads * head_dim] of
+ * the cache's type with row strides in elements, pointers 16-byte aligned, strides whole 16
+ * bytes, apart from each other (other columns of one tensor are); n_heads is a multiple of the
+ * cache's heads, head h reads key head h * n_kv_heads / n_heads.  rows * n_heads up to 2^25.
+ * scale and softcap are 0 or lie within 1e-15 .. 1e15 (a scale of either sign).  work:
+ * sg_attention_shared_work_bytes of device memory, 16-byte aligned, in use until the call's
+ * work on `stream` is done (one for each stream or graph that runs at the same time; a graph
+ * keeps its address, and the cache's), apart from q and out.  The same call on the same values
+ * gives the same bits. */
+int sg_attention_shared(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int64_t ldq, const sg_kv_cache *cache,
+                        int32_t n_heads, int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq,
+                        const sg_shared_keys *keys, void *work, size_t work_bytes, void *stream);
+
 /* ---- tokenizer (internal/tokenizer) -------------------------------------
  * The reference's SentencePiece-style BPE tokenizer on the host: text ->
  * the token IDs sg_forward takes.  Same normalization (NFKC / accents /

@@ -1,0 +1,555 @@
+"""Kept keys and values against their definitions in 64 bits, and what they refuse:
+sg_kv_cache_write, sg_kv_cache_read, sg_attention_shared.
+
+Tolerances, element by element, count roundings.  u(T) is half a step of the
+output's type; f = 2^-24 half a step of float32, in which every sum is formed.
+"""
+import ctypes
+import math
+import sys
+
+import numpy as np
+import pytest
+
+try:
+    import torch
+except ImportError:  # pragma: no cover
+    torch = None
+
+U = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TINY = {"f32": 2.0 ** -126, "f16": 2.0 ** -24, "bf16": 2.0 ** -126}  # the types' own floor
+F = 2.0 ** -24
+
+
+def say(*a):
+    print(*a, flush=True)
+    sys.stdout.flush()
+
+
+def dt(name):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rand(g, *shape, by=1.0, dtype="f32"):
+    return (torch.randn(*shape, generator=g) * by).to(dt(dtype))
+
+
+def ints(a):
+    return torch.tensor(np.asarray(a, np.int64).astype(np.int32))
+
+
+def offsets(lens, first=0):
+    return ints(np.concatenate([[first], first + np.cumsum(lens)]))
+
+
+def same(got, want, what):
+    """Equal, NaN for NaN."""
+    got, want = got.cpu(), want.cpu()
+    ok = (got == want) | (torch.isnan(got) & torch.isnan(want))
+    assert bool(ok.all()), f"{what}: {int((~ok).sum())} of {ok.numel()} differ"
+
+
+def close(got, want, tol, what):
+    got = got.double().cpu()
+    err = (got - want).abs()
+    ok = (err <= tol) | (got == want) | (torch.isnan(got) & torch.isnan(want))
+    worst = (err / tol.clamp_min(1e-300)).nan_to_num(math.inf)[~ok]
+    assert bool(ok.all()), f"{what}: {int((~ok).sum())} of {ok.numel()} off, up to {float(worst.max()):.3g} tolerances"
+
+
+# ---- the cache --------------------------------------------------------------------
+
+
+def kept_ref(x, kv_heads, bits):
+    """What a cache stands for, in 64 bits and as it is read: [rows, kv_heads * hd] each."""
+    if bits == 0:
+        return x.double(), x
+    y = x.double().reshape(x.shape[0], kv_heads, -1)
+    top = y.abs().amax(-1, keepdim=True)  # (NaN where a NaN is)
+    scale = (top / 127).float().double().clamp_min(2.0 ** -126)  # 53 bits round to 24 as the quotient does
+    scale = torch.where(torch.isfinite(top), scale, math.nan)
+    y = torch.round(y / scale).clamp(-127, 127) * scale
+    return y.reshape(x.shape), y.float().to(x.dtype).reshape(x.shape)
+
+
+def make_cache(ctx, slots, kv_heads, hd, dtype, bits):
+    from semantica_gpu import kernels
+    return kernels.KVCache(ctx, slots, kv_heads, hd, dt(dtype), bits=bits)
+
+
+def fill_cache(ctx, cache, k, v):
+    from semantica_gpu import kernels
+    kernels.kv_cache_write(ctx, cache, k.cuda(), v.cuda(), ints([0, k.shape[0]]).cuda(), ints([0]).cuda())
+
+
+def read_cache(ctx, cache):
+    from semantica_gpu import kernels
+    k = torch.empty(cache.slots, cache.n_kv_heads * cache.head_dim, dtype=cache.dtype, device="cuda")
+    v = torch.empty_like(k)
+    kernels.kv_cache_read(ctx, k, v, cache, ints([0, cache.slots]).cuda(), ints([0]).cuda())
+    return k.cpu(), v.cpu()
+
+
+def check_rows(ctx, seed, dtype, bits, kv_heads, hd, lens, starts, slots, first=0, behind=0):
+    """Rows in over what was there, everything out; the later of two sequences keeps a slot."""
+    from semantica_gpu import kernels
+    say("rows", dtype, bits, "heads", kv_heads, "hd", hd, "lens", list(lens)[:8], "starts", list(starts)[:8], "slots", slots)
+    g = gen(seed)
+    off = offsets(lens, first)
+    rows = int(off[-1]) + behind
+    k, v = rand(g, rows, kv_heads * hd, by=3.0, dtype=dtype), rand(g, rows, kv_heads * hd, dtype=dtype)
+    k0, v0 = rand(g, slots, kv_heads * hd, dtype=dtype), rand(g, slots, kv_heads * hd, by=2.0, dtype=dtype)
+    cache = make_cache(ctx, slots, kv_heads, hd, dtype, bits)
+    try:
+        fill_cache(ctx, cache, k0, v0)
+        kernels.kv_cache_write(ctx, cache, k.cuda(), v.cuda(), off.cuda(), ints(starts).cuda())
+        want_k, want_v = kept_ref(k0, kv_heads, bits)[1].clone(), kept_ref(v0, kv_heads, bits)[1].clone()
+        rk, rv = kept_ref(k, kv_heads, bits)[1], kept_ref(v, kv_heads, bits)[1]
+        back_k, back_v = torch.full_like(k, 7.0), torch.full_like(v, 7.0)
+        for i, s in enumerate(starts):
+            for r in range(int(off[i]), int(off[i + 1])):
+                at = s + r - int(off[i])
+                if s >= 0 and at < slots:
+                    want_k[at], want_v[at] = rk[r], rv[r]
+        for i, s in enumerate(starts):
+            for r in range(int(off[i]), int(off[i + 1])):
+                at = s + r - int(off[i])
+                there = s >= 0 and at < slots
+                back_k[r] = want_k[at] if there else 0
+                back_v[r] = want_v[at] if there else 0
+        got_k, got_v = read_cache(ctx, cache)
+        same(got_k, want_k, "keys")
+        same(got_v, want_v, "values")
+        out_k, out_v = torch.full_like(k, 7.0).cuda(), torch.full_like(v, 7.0).cuda()
+        kernels.kv_cache_read(ctx, out_k, out_v, cache, off.cuda(), ints(starts).cuda())
+        same(out_k, back_k, "keys read")
+        same(out_v, back_v, "values read")
+    finally:
+        cache.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("hd", [8, 64, 72, 128, 200, 256])
+def test_rows(gpu_ctx, dtype, bits, hd):
+    """Ranges that begin and end anywhere in a tile, empty sequences, rows of none, one slot at a time."""
+    check_rows(gpu_ctx, hd, dtype, bits, 2, hd, [1, 0, 5, 33, 70, 1, 3], [9, 4, 100, 131, 30, 0, 65], 171, first=3, behind=4)
+    check_rows(gpu_ctx, hd, dtype, bits, 3, hd, [1], [0], 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+def test_rows_many(gpu_ctx, dtype, bits):
+    """Rows enough for workgroups of 32 of them."""
+    check_rows(gpu_ctx, 3, dtype, bits, 8, 128, [1900, 31, 0, 33, 400], [7, 2000, 0, 2100, 2133], 2600, first=2, behind=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [0, 8])
+def test_rows_outside_and_twice(gpu_ctx, bits):
+    """Starts below zero and ends past the cache; slots that several sequences name."""
+    check_rows(gpu_ctx, 5, "bf16", bits, 2, 64, [10, 40, 3, 9], [-1, 30, 64, 2**31 - 5], 64)
+    check_rows(gpu_ctx, 6, "f32", bits, 2, 64, [20, 20, 1, 7], [5, 10, 12, 3], 64)
+    lens = [1] * 300 + [40]
+    check_rows(gpu_ctx, 7, "f16", bits, 8, 64, lens, [i % 17 for i in range(300)] + [9], 64)
+    r = np.random.RandomState(1)
+    lens = [30] * 80
+    check_rows(gpu_ctx, 8, "f16", bits, 8, 64, lens, r.randint(-5, 600, 80).tolist(), 610)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_codes_at_borders(gpu_ctx, dtype):
+    """Values halfway between codes, next to halfway, tiny, huge, zero."""
+    g = gen(2)
+    hd, rows = 64, 600
+    top = (127 * 2.0 ** torch.randint(-8, 8, (rows, 1), generator=g).double()) * torch.where(
+        torch.rand(rows, 1, generator=g) < 0.5, 1.0, 1.0 + torch.rand(rows, 1, generator=g))
+    half = torch.randint(-127, 127, (rows, hd), generator=g).double() + 0.5
+    k = (half * top / 127).to(dt(dtype))
+    k[:, :1] = top.to(dt(dtype))
+    bits = {torch.float32: torch.int32}.get(dt(dtype), torch.int16)
+    v = (k.view(bits) + torch.randint(-1, 2, (rows, hd), generator=g).to(bits)).view(dt(dtype))  # one step aside
+    if dtype != "f16":
+        k[0], k[1], k[2] = 1e-44, 3e38, 0.0
+        k[3] = torch.linspace(-1e-37, 1e-37, hd).to(dt(dtype))
+    cache = make_cache(gpu_ctx, rows, 1, hd, dtype, 8)
+    fill_cache(gpu_ctx, cache, k, v)
+    got_k, got_v = read_cache(gpu_ctx, cache)
+    cache.close()
+    same(got_k, kept_ref(k, 1, 8)[1], "keys")
+    same(got_v, kept_ref(v, 1, 8)[1], "values")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+def test_rows_not_finite(gpu_ctx, dtype, bits):
+    """An infinity or a NaN is that slot's and head's alone, and goes when it is written over."""
+    g = gen(8)
+    k, v = rand(g, 40, 128, dtype=dtype), rand(g, 40, 128, dtype=dtype)
+    clean_k, clean_v = k.clone(), v.clone()
+    k[3, 7], v[5, 64 + 3], v[33, 0], k[33, 70] = math.nan, math.inf, -math.inf, math.inf
+    cache = make_cache(gpu_ctx, 40, 2, 64, dtype, bits)
+    fill_cache(gpu_ctx, cache, k, v)
+    got_k, got_v = read_cache(gpu_ctx, cache)
+    same(got_k, kept_ref(k, 2, bits)[1], "keys")
+    same(got_v, kept_ref(v, 2, bits)[1], "values")
+    fill_cache(gpu_ctx, cache, clean_k, clean_v)
+    got_k, got_v = read_cache(gpu_ctx, cache)
+    cache.close()
+    same(got_k, kept_ref(clean_k, 2, bits)[1], "keys")
+    same(got_v, kept_ref(clean_v, 2, bits)[1], "values")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_of_one_projection(gpu_ctx, dtype):
+    """k and v as columns of one tensor, in and out."""
+    from semantica_gpu import kernels
+    g = gen(4)
+    qkv = rand(g, 50, 64 + 2 * 128 + 8, dtype=dtype).cuda()
+    cache = make_cache(gpu_ctx, 70, 2, 64, dtype, 8)
+    off, starts = offsets([20, 30]).cuda(), ints([33, 1]).cuda()
+    kernels.kv_cache_write(gpu_ctx, cache, qkv[:, 64:192], qkv[:, 192:320], off, starts)
+    wide = torch.full((50, 320), 7.0, dtype=dt(dtype), device="cuda")
+    kernels.kv_cache_read(gpu_ctx, wide[:, 16:144], wide[:, 144:272], cache, off, starts)
+    cache.close()
+    same(wide[:, 16:144], kept_ref(qkv[:, 64:192].cpu(), 2, 8)[1], "keys")
+    same(wide[:, 144:272], kept_ref(qkv[:, 192:320].cpu(), 2, 8)[1], "values")
+    assert bool((wide[:, :16] == 7).all()) and bool((wide[:, 272:] == 7).all())
+
+
+# ---- attention ----------------------------------------------------------------------
+
+
+def shared_ref(q, k, v, off, heads, kv_heads, starts, lengths, shared=None, prefix_starts=None, prefix_lengths=None,
+               scale=0.0, softcap=0.0, causal=True, window=0):
+    """The definition in 64 bits over what the cache stands for, and the mean of |v| and the
+    scores' size that the tolerance needs.  Rows of no sequence are NaN."""
+    rows, hd, slots = q.shape[0], q.shape[1] // heads, k.shape[0]
+    q, k, v = q.double().reshape(rows, heads, hd), k.reshape(slots, kv_heads, hd), v.reshape(slots, kv_heads, hd)
+    scale = scale or 1.0 / math.sqrt(hd)
+    out = torch.full((rows, heads, hd), math.nan, dtype=torch.float64)
+    mean, size = torch.zeros(rows, heads, hd, dtype=torch.float64), torch.zeros(rows, heads, 1, dtype=torch.float64)
+
+    def slots_of(start, length):
+        start, length = int(start), int(length)
+        return list(range(start, start + length)) if start >= 0 and length > 0 and start + length <= slots else []
+
+    for i in range(off.shape[0] - 1):
+        a, b = int(off[i]), int(off[i + 1])
+        if a == b:
+            continue
+        at = []
+        for p in range(shared.shape[0] - 1 if shared is not None else 0):
+            if int(shared[p]) <= i < int(shared[p + 1]):
+                at = slots_of(prefix_starts[p], prefix_lengths[p])
+        at = torch.tensor(at + slots_of(starts[i], lengths[i]), dtype=torch.long)
+        pos = at.shape[0] - (b - a) + torch.arange(b - a)
+        gap = pos[:, None] - torch.arange(at.shape[0])[None, :]
+        seen = torch.ones_like(gap, dtype=torch.bool)
+        if causal:
+            seen &= gap >= 0
+        if window:
+            seen &= gap.abs() < window
+        some = seen.any(0)  # hidden slots' contents do not count
+        for h in range(heads):
+            kh, vh = k[at, h * kv_heads // heads], v[at, h * kv_heads // heads]
+            kh, vh = torch.where(some[:, None], kh, 0.0), torch.where(some[:, None], vh, 0.0)
+            s = q[a:b, h] @ kh.t() * scale
+            big = q[a:b, h].abs() @ kh.abs().t() * abs(scale)
+            if softcap:
+                s = softcap * torch.tanh(s / softcap)
+            s = s.masked_fill(~seen, -math.inf)
+            p = torch.softmax(s, -1).nan_to_num(0.0) if bool(torch.isfinite(kh).all()) else softmax_seen(s, seen)
+            vz = vh.nan_to_num(0, 0, 0)
+            o = p @ vz
+            for j in torch.nonzero(~torch.isfinite(vh).all(-1)).flatten().tolist():  # by themselves, where seen
+                o = o + torch.where(seen[:, j, None], p[:, j, None] * vh[j] - p[:, j, None] * vz[j], 0.0)
+            out[a:b, h] = o
+            mean[a:b, h] = p.nan_to_num(0.0) @ vz.abs()
+            size[a:b, h, 0] = (big.nan_to_num(0, 0, 0) * (p > 2.0 ** -40)).amax(-1) if at.shape[0] else 0.0
+    return out.reshape(rows, -1), mean.reshape(rows, -1), size.expand(rows, heads, hd).reshape(rows, -1)
+
+
+def softmax_seen(s, seen):
+    """softmax where a row that sees a score of NaN is NaN, and one that sees nothing zeros."""
+    p = torch.softmax(s, -1)
+    none = ~(seen & ~(s == -math.inf)).any(-1, keepdim=True)
+    return torch.where(none, 0.0, p)
+
+
+def shared_tol(dtype, bits, hd, keys, out, mean, size, softcap=0.0):
+    # A score: hd products and sums of float32 and some ten roundings behind it (codes are exact,
+    # their scales are float32); an error of d in a score is one of 2 d in a weight relative to
+    # the sum.
+    score = (hd + 16) * F * size + 16 * F * (size + 1) + softcap * 2.0 ** -22
+    # The weights' rounding for the second product (float32: none; fp16 over codes: two bf16
+    # halves), a weight's own roundings, the sums over the keys (half of the keys' number is
+    # far more additions than any one sum has in a row), as many joins.
+    own = {"f32": 0.0, "f16": U["f16"] if bits == 0 else 2.0 ** -16, "bf16": U["bf16"]}[dtype]
+    weights = own + (keys / 2 + 64) * F
+    return 1.01 * U[dtype] * out.abs() + (2 * score + weights) * mean * (1 + 2 * own) + weights * F * out.abs() + \
+        (keys / 2 + 64) * F * out.abs() + TINY[dtype]
+
+
+def run_shared(ctx, q, cache, heads, off, fill=7.0, **kw):
+    from semantica_gpu import kernels
+    dev = {n: (t.cuda() if isinstance(t, torch.Tensor) else t) for n, t in kw.items()}
+    out = torch.full(q.shape, fill, dtype=q.dtype, device="cuda")
+    kernels.attention_shared(ctx, out, q.cuda(), cache, heads, off.cuda(), **dev)
+    return out.cpu()
+
+
+def ranges(lens, gap=3, first=5):
+    """Starts of ranges one after another, and the slots in all."""
+    starts = first + np.cumsum(np.concatenate([[0], np.asarray(lens[:-1], np.int64) + gap])) if len(lens) else np.zeros(0)
+    return starts.astype(np.int64), int(starts[-1] + lens[-1] + 2) if len(lens) else 1
+
+
+def check_shared(ctx, seed, dtype, bits, heads, kv_heads, hd, queries, lengths, plens=(), shared=None, first=0, behind=0,
+                 by=1.0, poison=None, **kw):
+    say("shared", dtype, bits, "heads", heads, kv_heads, "hd", hd, "queries", list(queries)[:6], "lengths",
+        list(lengths)[:6], "prefixes", list(plens), kw)
+    g = gen(seed)
+    off = offsets(queries, first)
+    rows = int(off[-1]) + behind
+    places, slots = ranges(list(plens) + list(lengths))
+    q = rand(g, rows, heads * hd, by=by, dtype=dtype)
+    k, v = rand(g, slots, kv_heads * hd, dtype=dtype), rand(g, slots, kv_heads * hd, by=2.0, dtype=dtype)
+    if poison is not None:  # what lies around the ranges
+        out_of = torch.ones(slots, dtype=torch.bool)
+        for s, m in zip(places, list(plens) + list(lengths)):
+            out_of[int(s):int(s) + m] = False
+        k[out_of], v[out_of] = poison, poison
+    cache = make_cache(ctx, slots, kv_heads, hd, dtype, bits)
+    keys = dict(starts=ints(places[len(plens):]), lengths=ints(lengths))
+    if len(plens):
+        if shared is None:
+            shared = [0] + [len(queries) * (p + 1) // len(plens) for p in range(len(plens))]
+        keys.update(shared=ints(shared), prefix_starts=ints(places[:len(plens)]), prefix_lengths=ints(plens))
+    try:
+        fill_cache(ctx, cache, k, v)
+        got = run_shared(ctx, q, cache, heads, off, **keys, **kw)
+    finally:
+        cache.close()
+    kr, vr = kept_ref(k, kv_heads, bits)[0], kept_ref(v, kv_heads, bits)[0]
+    want, mean, size = shared_ref(q, kr, vr, off, heads, kv_heads, **keys, **kw)
+    there = torch.zeros(rows, dtype=torch.bool)
+    there[first:int(off[-1])] = True
+    assert bool((got[~there] == 7.0).all()), "rows of no sequence were written"
+    most = max([0] + [int(p) for p in plens]) + max([0] + [int(m) for m in lengths])
+    close(got[there], want[there], shared_tol(dtype, bits, hd, most, want, mean, size, kw.get("softcap", 0.0))[there],
+          "attention")
+
+
+MASKS = {
+    "causal": {},
+    "whole": {"causal": False},
+    "scale": {"scale": -0.31},
+    "cap": {"softcap": 5.0},
+    "window": {"window": 9},
+    "window-whole": {"window": 40, "causal": False, "softcap": 30.0},
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("mask", list(MASKS))
+def test_shared_masks(gpu_ctx, dtype, bits, mask):
+    """Every mask in each form: few pairs of both kinds, many of both, many behind the prefix and few own."""
+    for hd, heads, kv_heads in ((64, 4, 2), (128, 3, 1), (256, 3, 1)):
+        check_shared(gpu_ctx, hd, dtype, bits, heads, kv_heads, hd, [1, 0, 2, 3], [7, 0, 70, 40], [83], first=3, behind=4,
+                     **MASKS[mask])
+        check_shared(gpu_ctx, hd + 1, dtype, bits, heads, kv_heads, hd, [33, 40, 64, 70], [33, 45, 64, 170], [150, 31],
+                     first=2, behind=1, **MASKS[mask])
+        check_shared(gpu_ctx, hd + 2, dtype, bits, heads, kv_heads, hd, [1] * 90, [1 + i % 50 for i in range(90)],
+                     [200, 65], **MASKS[mask])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+def test_shared_few_behind_many_prefixes(gpu_ctx, dtype, bits):
+    """Few pairs behind each prefix (more prefixes than sequences), many of each sequence."""
+    check_shared(gpu_ctx, 1, dtype, bits, 2, 1, 64, [50, 40], [50, 60], [5, 40, 33, 70, 12, 9], shared=[0, 0, 1, 1, 2, 2, 2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+def test_shared_long(gpu_ctx, dtype, bits):
+    """A prefix split over the GPU for one query, and for a few; running maxima that rise late."""
+    check_shared(gpu_ctx, 2, dtype, bits, 8, 2, 128, [1], [3], [20011], by=3.0)
+    check_shared(gpu_ctx, 3, dtype, bits, 3, 1, 256, [1, 1, 2], [30, 5, 7], [5000], by=3.0)
+    check_shared(gpu_ctx, 4, dtype, bits, 4, 1, 64, [1] * 40, [9] * 40, [6001], by=4.0)
+    check_shared(gpu_ctx, 5, dtype, bits, 2, 1, 64, [300], [4001], by=4.0)  # no prefix
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("hd", [8, 40, 72, 136, 200, 248])
+def test_shared_odd_head_dims(gpu_ctx, dtype, bits, hd):
+    check_shared(gpu_ctx, hd, dtype, bits, 2, 1, hd, [3, 1], [17, 40], [61])
+    check_shared(gpu_ctx, hd, dtype, bits, 6, 2, hd, [40, 21], [41, 40], [61])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [0, 8])
+def test_shared_edges(gpu_ctx, bits):
+    """No own keys, empty prefixes, more queries than keys, sequences behind no prefix, ranges outside the cache."""
+    for dtype in ("f32", "bf16"):
+        check_shared(gpu_ctx, 1, dtype, bits, 2, 1, 64, [3, 2, 4], [0, 0, 9], [40, 0], shared=[0, 1, 3])
+        check_shared(gpu_ctx, 2, dtype, bits, 2, 1, 64, [60, 5], [20, 1], [10], shared=[0, 1])
+        check_shared(gpu_ctx, 3, dtype, bits, 2, 1, 64, [60, 5], [20, 1], [10], shared=[0, 1], causal=False, window=4)
+        check_shared(gpu_ctx, 4, dtype, bits, 2, 1, 64, [1, 2, 3, 4], [5, 6, 7, 8], [33, 70], shared=[1, 2, 3])
+    from semantica_gpu import kernels  # noqa: F401
+    g = gen(9)
+    k, v, q = rand(g, 64, 64, dtype="f32"), rand(g, 64, 64, dtype="f32"), rand(g, 4, 128, dtype="f32")
+    cache = make_cache(gpu_ctx, 64, 1, 64, "f32", bits)
+    fill_cache(gpu_ctx, cache, k, v)
+    kr, vr = kept_ref(k, 1, bits)[0], kept_ref(v, 1, bits)[0]
+    off = offsets([1, 1, 2])
+    keys = dict(starts=ints([-1, 60, 10]), lengths=ints([5, 5, 2**31 - 1]), shared=ints([0, 2, 3]),
+                prefix_starts=ints([3, 2**31 - 1]), prefix_lengths=ints([20, 20]))
+    got = run_shared(gpu_ctx, q, cache, 2, off, **keys)
+    want, mean, size = shared_ref(q, kr, vr, off, 2, 1, **keys)
+    cache.close()
+    assert bool((got[2:] == 0).all())
+    close(got, want, shared_tol("f32", bits, 64, 64, want, mean, size), "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_shared_hidden_slots(gpu_ctx, dtype, bits, bad):
+    """Infinities and NaN around the ranges, and in later tokens of the same sequence."""
+    for queries, lengths in (([1, 2], [7, 40]), ([40, 64], [50, 64])):
+        check_shared(gpu_ctx, 3, dtype, bits, 2, 1, 64, queries, lengths, [45], poison=bad)
+    # A bad token in the middle of a sequence: earlier queries do not see it, later ones do.
+    for n, hd in ((6, 64), (90, 128)):
+        g = gen(n)
+        q = rand(g, n, 2 * hd, dtype=dtype)
+        k, v = rand(g, n + 40, hd, dtype=dtype), rand(g, n + 40, hd, dtype=dtype)
+        v[40 + n // 2, 3] = bad
+        cache = make_cache(gpu_ctx, n + 40, 1, hd, dtype, bits)
+        fill_cache(gpu_ctx, cache, k, v)
+        keys = dict(starts=ints([40]), lengths=ints([n]), shared=ints([0, 1]), prefix_starts=ints([1]),
+                    prefix_lengths=ints([35]))
+        got = run_shared(gpu_ctx, q, cache, 2, offsets([n]), **keys)
+        cache.close()
+        kr, vr = kept_ref(k, 1, bits)[0], kept_ref(v, 1, bits)[0]
+        want, mean, size = shared_ref(q, kr, vr, offsets([n]), 2, 1, **keys)
+        assert bool(torch.isfinite(got[:n // 2]).all()) and not bool(torch.isfinite(got[n // 2:]).all(-1).any())
+        fin = torch.isfinite(want)
+        same(torch.isfinite(got.float()), fin, "which are finite")
+        if bits == 0:
+            same(got[~fin].double(), want[~fin], "infinities")
+        tol = shared_tol(dtype, bits, hd, n + 35, want.nan_to_num(0, 0, 0), mean, size)
+        close(got[fin], want[fin], tol[fin], "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+def test_shared_visible_not_finite(gpu_ctx, dtype, bits):
+    """A NaN in a key reaches the queries that see it and no others; scores of -infinity alone give zeros."""
+    n, hd = 40, 64
+    for pick in ("key", "lowest"):
+        g = gen(7)
+        q, k, v = rand(g, n, hd, dtype=dtype), rand(g, n, hd, dtype=dtype), rand(g, n, hd, dtype=dtype)
+        if pick == "key":
+            k[11] = math.nan
+        elif bits == 0:
+            k[:] = -math.inf
+            q = q.abs() + dt(dtype).itemsize
+        else:
+            continue
+        cache = make_cache(gpu_ctx, n, 1, hd, dtype, bits)
+        fill_cache(gpu_ctx, cache, k, v)
+        got = run_shared(gpu_ctx, q, cache, 1, offsets([n]), starts=ints([0]), lengths=ints([n]))
+        cache.close()
+        if pick == "key":
+            assert bool(torch.isfinite(got[:11]).all()) and bool(torch.isnan(got[11:]).all())
+        else:
+            assert bool((got == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,limit", [("f32", 3e-6), ("f16", 6e-4), ("bf16", 5e-3)])
+@pytest.mark.parametrize("bits", [0, 8])
+def test_shared_error_norm(gpu_ctx, dtype, limit, bits):
+    """The error's norm: a lost half of a weight, or a key counted twice, would show.
+
+    float32: 320 products and scales of a score of size 20 at most, off by about the root of
+    their number times f each, 2e-7 absolutely, so 4e-7 in a weight; 16-bit types: their
+    output's and their weights' rounding, u / sqrt(3) each."""
+    g = gen(11)
+    n, hd, plen = 50, 128, 3001
+    q = rand(g, n, 4 * hd, dtype=dtype)
+    k, v = rand(g, plen + n, hd, dtype=dtype), rand(g, plen + n, hd, dtype=dtype)
+    cache = make_cache(gpu_ctx, plen + n, 1, hd, dtype, bits)
+    fill_cache(gpu_ctx, cache, k, v)
+    kr, vr = kept_ref(k, 1, bits)[0], kept_ref(v, 1, bits)[0]
+    for queries, own in (([n], [n]), ([1] * 5, [3] * 5)):
+        off = offsets(queries)
+        starts = plen + np.concatenate([[0], np.cumsum(own)[:-1]])
+        keys = dict(starts=ints(starts), lengths=ints(own), shared=ints([0, len(own)]), prefix_starts=ints([0]),
+                    prefix_lengths=ints([plen]))
+        rows = int(off[-1])
+        got = run_shared(gpu_ctx, q[:rows], cache, 4, off, **keys)
+        want, _, _ = shared_ref(q[:rows], kr, vr, off, 4, 1, **keys)
+        err = float((got.double() - want).norm() / want.norm())
+        say("error", dtype, bits, rows, err)
+        assert err < limit
+    cache.close()
+
+
+@pytest.mark.gpu
+def test_shared_far_apart_scales(gpu_ctx):
+    """Values of far-apart powers of two: a query that sees small ones alone keeps their bits."""
+    hd, n = 64, 64
+    for dtype in ("f32", "f16", "bf16"):
+        for bits in (0, 8):
+            g = gen(3)
+            q, k, v = rand(g, n, hd, dtype=dtype), rand(g, n, hd, dtype=dtype), rand(g, n, hd, dtype=dtype)
+            v[:32] *= 2.0 ** -12 if dtype == "f16" else 2.0 ** -60
+            v[32:] *= 2.0 ** 12 if dtype == "f16" else 2.0 ** 60
+            cache = make_cache(gpu_ctx, n, 1, hd, dtype, bits)
+            fill_cache(gpu_ctx, cache, k, v)
+            kr, vr = kept_ref(k, 1, bits)[0], kept_ref(v, 1, bits)[0]
+            off = offsets([n])
+            got = run_shared(gpu_ctx, q, cache, 1, off, starts=ints([0]), lengths=ints([n]))
+            cache.close()
+            want, mean, size = shared_ref(q, kr, vr, off, 1, 1, ints([0]), ints([n]))
+            close(got, want, shared_tol(dtype, bits, hd, n, want, mean, size), "attention")
+
+
+# ---- refusals ---------------------------------------------------------------------------
+
+
+def test_refusals_without_a_gpu():
+    """Argument checks come before any device call."""
+    from semantica_gpu import _lib
+    lib = _lib.load()
+    out, size = ctypes.c_void_p(), ctypes.c_size_t()
+    bad = _lib.SG_ERR_INVALID
+    assert lib.sg_kv_cache_create(None, 10, 1, 64, 0, 8, None, ctypes.byref(out)) == bad
+    assert lib.sg_kv_cache_write(None, None, None, 0, None, 0, 1, None, 1, None, None) == bad
+    assert lib.sg_kv_cache_read(None, None, None, 0, None, 0, 1, None, 1, None, None) == bad
+    assert lib.sg_kv_cache_bytes(None, ctypes.byref(size)) == bad
+    assert lib.sg_attention_shared_work_bytes(None, 1, 1, 1, 1, ctypes.byref(size)) == bad
+    keys = _lib.SharedKeys()
+    assert lib.sg_attention_shared(None, None, 0, None, 0, None, 1, 1, None, 1, keys, None, 0, None) == bad
+    assert b"NULL" in lib.sg_last_error()
+    lib.sg_kv_cache_free(None)

@@ -150,6 +150,17 @@ struct sg_attn_batch {
   int n_seq, n_prefix, causal, window;
 };
 
+// One sg_matmul_q4 call (k_q4.hip): packed weights, strides in elements.
+struct sg_q4_args {
+  void* dst;
+  const void* x;
+  int64_t ldd, ldx;
+  const uint32_t* w;
+  const void* scales;
+  const uint8_t* zeros;
+  int rows, out_dim, in_dim, group, scales_f32;
+};
+
 namespace sgk {
 
 // GEMM operands are block-major int8 [K/32][rows][32]; activation buffers hold
@@ -397,6 +408,14 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
 hipError_t attn_shared_f32(const sg_attn_shared_args& a, const sg_attn_list& list, bool q8, int D, hipStream_t s);
 hipError_t attn_shared_f16(const sg_attn_shared_args& a, const sg_attn_list& list, bool q8, int D, hipStream_t s);
 hipError_t attn_shared_bf16(const sg_attn_shared_args& a, const sg_attn_list& list, bool q8, int D, hipStream_t s);
+
+// ---- 4-bit weights (k_q4.hip) ----
+int64_t q4_blocks(int out_dim, int in_dim);  // of a kilobyte; 16 * 128 / group scales (and zeros) each
+int64_t q4_threads(int rows, int out_dim);
+hipError_t q4_pack(const uint8_t* codes, const void* scales, int scale_dtype, const uint8_t* zeros, int out_dim, int in_dim,
+                   int group, uint32_t* w, void* packed_scales, uint8_t* packed_zeros, hipStream_t s);
+hipError_t q4_pack_q4_0(const uint8_t* raw, int out_dim, int in_dim, uint32_t* w, void* packed_scales, hipStream_t s);
+hipError_t matmul_q4(const sg_q4_args& a, int dtype, hipStream_t s);
 
 // ---- brute-force search (k_search.hip) ----
 // Storage modes, the values of brute.QuantizationMode (search/brute/quant.go:8-15).

@@ -162,6 +162,10 @@ _PROTOS = {
     "sg_attention_shared_work_bytes": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i32, ctypes.POINTER(ctypes.c_size_t)]),
     "sg_attention_shared": (ctypes.c_int, [_vp, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _i32,
                                            ctypes.POINTER(SharedKeys), _vp, ctypes.c_size_t, _vp]),
+    "sg_q4_weight_create": (ctypes.c_int, [_vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _pp]),
+    "sg_q4_weight_create_q4_0": (ctypes.c_int, [_vp, _vp, _i32, _i32, _pp]),
+    "sg_q4_weight_free": (None, [_vp]),
+    "sg_matmul_q4": (ctypes.c_int, [_vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _vp]),
     "sg_index_build": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _i32, _pp]),
     "sg_index_build_device": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, ctypes.c_int64, _i32, _vp, _pp]),
     "sg_index_deserialize": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _pp]),

@@ -14,6 +14,7 @@ and the layer operators of sibling models, which have no counterpart there:
 
   attention_masked, block_norm, AdapterBank + adapters_apply
   KVCache + kv_cache_write, kv_cache_read, attention_shared
+  Q4Weight + matmul_q4
 
 They take row-strided 2-D tensors of float32, float16 or bfloat16 and the CSR
 offsets as an int32 device tensor, run asynchronously on the current stream of the
@@ -502,3 +503,67 @@ def attention_shared(ctx, out, q, cache: KVCache, n_heads, offsets, starts, leng
     _lib.check(ctx.lib.sg_attention_shared(ctx.handle, o, ldo, qp, ldq, cache.handle, n_heads, rows, off, n_seq, keys,
                                            _vec(ctx, "work", work, None, torch.uint8), work.numel(),
                                            _stream_of(ctx, stream)))
+
+
+class Q4Weight:
+    """A matrix of 4-bit weights with group scales (sg_q4_weight_create): w = scale * (code - zero).
+
+    codes uint8 [out_dim, in_dim / 2], the even input in a byte's lower four bits; scales
+    [out_dim, in_dim / group] float16 (kept so) or float32 or bfloat16 (kept as float32); zeros
+    uint8 [out_dim, in_dim / group] or None for 8; device tensors.  group: 32, 64 or 128.
+
+    Made and closed as an AdapterBank is: neither is for a time when any thread captures a graph."""
+
+    def __init__(self, ctx, codes, scales, zeros=None, stream=None):
+        self.handle = None
+        torch = _torch()
+        out_dim, half = codes.shape
+        groups = scales.shape[1] if scales.dim() == 2 else 0
+        if groups <= 0 or 2 * half % groups:
+            raise ValueError(f"scales: shape {tuple(scales.shape)} beside codes {tuple(codes.shape)}")
+        if max(out_dim, 2 * half) > _MOST:
+            _too_many("rows or columns of codes", max(out_dim, 2 * half))
+        h = ctypes.c_void_p()
+        args = (_vec(ctx, "codes", codes, None, torch.uint8), _vec(ctx, "scales", scales, out_dim * groups, scales.dtype),
+                _dtype(scales), _vec(ctx, "zeros", zeros, out_dim * groups, torch.uint8))
+        _free_collected()
+        _lib.check(ctx.lib.sg_q4_weight_create(ctx.handle, *args, out_dim, 2 * half, 2 * half // groups,
+                                               _stream_of(ctx, stream), ctypes.byref(h)))
+        self.ctx, self.lib, self.handle = ctx, ctx.lib, h
+        self.out_dim, self.in_dim, self.group = out_dim, 2 * half, 2 * half // groups
+
+    @classmethod
+    def from_q4_0(cls, ctx, raw_q4: np.ndarray, out_dim: int, in_dim: int):
+        """From GGUF's raw Q4_0 blocks [out_dim][in_dim/32][18 B] (sg_q4_weight_create_q4_0)."""
+        raw = np.ascontiguousarray(raw_q4, np.uint8)
+        if raw.size != out_dim * (in_dim // 32) * 18:
+            raise ValueError("raw Q4_0 size does not match out_dim x in_dim")
+        self = cls.__new__(cls)
+        self.handle = None
+        h = ctypes.c_void_p()
+        _free_collected()
+        _lib.check(ctx.lib.sg_q4_weight_create_q4_0(ctx.handle, ctypes.c_void_p(raw.ctypes.data), out_dim, in_dim,
+                                                    ctypes.byref(h)))
+        self.ctx, self.lib, self.handle = ctx, ctx.lib, h
+        self.out_dim, self.in_dim, self.group = out_dim, in_dim, 32
+        return self
+
+    def close(self):
+        _free_collected()
+        if self.handle:
+            self.lib.sg_q4_weight_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        if self.handle and _COLLECTED is not None:  # (None: the interpreter ends)
+            _COLLECTED.append((self.lib.sg_q4_weight_free, self.handle))
+
+
+def matmul_q4(ctx, dst, w: Q4Weight, x, *, stream=None):
+    """dst = x @ w^T for a few rows (sg_matmul_q4): x [rows, in_dim], dst [rows, out_dim]."""
+    rows = x.shape[0]
+    if rows > _MOST:
+        _too_many("rows of x", rows)
+    xp, ldx = _rows_of(ctx, "x", x, rows, w.in_dim, x.dtype)
+    d, ldd = _rows_of(ctx, "dst", dst, rows, w.out_dim, x.dtype)
+    _lib.check(ctx.lib.sg_matmul_q4(ctx.handle, d, ldd, w.handle, xp, ldx, _dtype(x), rows, _stream_of(ctx, stream)))

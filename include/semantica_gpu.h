@@ -511,6 +511,34 @@ int sg_attention_shared(sg_ctx *ctx, void *out, int64_t ldo, const void *q, int6
                         int32_t n_heads, int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq,
                         const sg_shared_keys *keys, void *work, size_t work_bytes, void *stream);
 
+/* ---- 4-bit weights --------------------------------------------------------
+ * A matrix [out_dim][in_dim] of 4-bit codes with a scale, and if need be a zero, for each
+ * group of 32, 64 or 128 inputs: w = scale * (code - zero).  d_codes [out_dim][in_dim/2]: byte b
+ * of a row holds input 2 b in its lower four bits and 2 b + 1 in its upper; d_scales
+ * [out_dim][in_dim/group] of type scale_dtype, d_zeros the same as bytes 0 .. 15 (NULL: 8).
+ * Laid out for the GPU once: the arrays (device memory, contiguous) are read on `stream` and
+ * may be freed after return, which waits for that.  Making and freeing are not for a time when a
+ * thread captures a graph.  No counterpart in the reference, which runs Q8_0 only. */
+typedef struct sg_q4_weight sg_q4_weight;
+int sg_q4_weight_create(sg_ctx *ctx, const uint8_t *d_codes, const void *d_scales, int32_t scale_dtype,
+                        const uint8_t *d_zeros, int32_t out_dim, int32_t in_dim, int32_t group, void *stream,
+                        sg_q4_weight **out);
+/* The same from GGUF's raw Q4_0 blocks in host memory, row-major [out_dim][in_dim/32][18 B]: an
+ * fp16 scale, then 16 bytes, the lower four bits of which are the block's inputs 0 .. 15 and the
+ * upper ones 16 .. 31; zero 8.  Synchronous. */
+int sg_q4_weight_create_q4_0(sg_ctx *ctx, const void *raw, int32_t out_dim, int32_t in_dim, sg_q4_weight **out);
+void sg_q4_weight_free(sg_q4_weight *weight);
+
+/* dst[m][n] = sum over k of w[n][k] x[m][k] for a few rows (64 or fewer share one pass over the
+ * weights, more take one for every 64).  x [rows][in_dim], dst [rows][out_dim] of type dtype with
+ * row strides in elements; x 16-byte aligned, its stride whole 16 bytes; dst does not overlap
+ * x (other columns of one tensor, with the same stride, do not).  Weights are not rounded, sums
+ * are float32 and in the same order every time; float32 rows keep their bits down to 2^-102 (what
+ * lies below 2^-126 is lost of smaller values).  Asynchronous on `stream`, allocates nothing,
+ * may be captured. */
+int sg_matmul_q4(sg_ctx *ctx, void *dst, int64_t ldd, const sg_q4_weight *weight, const void *x, int64_t ldx,
+                 int32_t dtype, int32_t rows, void *stream);
+
 /* ---- tokenizer (internal/tokenizer) -------------------------------------
  * The reference's SentencePiece-style BPE tokenizer on the host: text ->
  * the token IDs sg_forward takes.  Same normalization (NFKC / accents /

@@ -1,5 +1,5 @@
-"""Kept keys and values against their definitions in 64 bits, and what they refuse:
-sg_kv_cache_write, sg_kv_cache_read, sg_attention_shared.
+"""What answers requests behind kept text, against its definitions in 64 bits, and what it
+refuses: sg_kv_cache_write, sg_kv_cache_read, sg_attention_shared, sg_matmul_q4.
 
 Tolerances, element by element, count roundings.  u(T) is half a step of the
 output's type; f = 2^-24 half a step of float32, in which every sum is formed.
@@ -535,6 +535,138 @@ def test_shared_far_apart_scales(gpu_ctx):
             close(got, want, shared_tol(dtype, bits, hd, n, want, mean, size), "attention")
 
 
+# ---- 4-bit weights -------------------------------------------------------------------------
+
+
+def q4_make(g, out_dim, in_dim, group, scale="f16", zeros=False):
+    codes = torch.randint(0, 256, (out_dim, in_dim // 2), generator=g, dtype=torch.uint8)
+    scales = ((torch.rand(out_dim, in_dim // group, generator=g) + 0.2) * 0.1).to(dt(scale))
+    z = torch.randint(0, 16, (out_dim, in_dim // group), generator=g, dtype=torch.uint8) if zeros else None
+    return codes, scales, z
+
+
+def q4_dense(codes, scales, z):
+    w = torch.stack([codes % 16, codes // 16], -1).reshape(codes.shape[0], scales.shape[1], -1).double()
+    w = (w - (z.double()[..., None] if z is not None else 8.0)) * scales.double()[..., None]
+    return w.reshape(codes.shape[0], -1)
+
+
+def q4_tol(dtype, x, w, out):
+    # The result's rounding; an inner sum of up to 3 * 128 products, the groups' sum, the eight
+    # waves': fewer than in_dim / 8 + 400 additions of float32 in a row, and a scaling.
+    size = x.double().nan_to_num(0, 0, 0).abs() @ w.abs().t()
+    return 1.01 * U[dtype] * out.abs() + (x.shape[1] / 8 + 400) * F * size + TINY[dtype]
+
+
+def check_q4(ctx, seed, dtype, rows, out_dim, in_dim, group, scale="f16", zeros=False, x=None):
+    from semantica_gpu import kernels
+    say("q4", dtype, rows, out_dim, in_dim, group, scale, zeros)
+    g = gen(seed)
+    codes, scales, z = q4_make(g, out_dim, in_dim, group, scale, zeros)
+    x = rand(g, rows, in_dim, dtype=dtype) if x is None else x
+    wt = kernels.Q4Weight(ctx, codes.cuda(), scales.cuda(), z.cuda() if zeros else None)
+    wide = torch.full((rows, out_dim + 5), 7.0, dtype=dt(dtype), device="cuda")
+    try:
+        kernels.matmul_q4(ctx, wide[:, 3:3 + out_dim], wt, x.cuda())
+    finally:
+        wt.close()
+    w = q4_dense(codes, scales, z)
+    want = x.double() @ w.t()
+    close(wide[:, 3:3 + out_dim], want, q4_tol(dtype, x, w, want), "products")
+    assert bool((wide[:, :3] == 7).all()) and bool((wide[:, 3 + out_dim:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_q4(gpu_ctx, dtype, group, zeros):
+    """Rows of each form, outputs that end inside a tile, inputs that end inside a block."""
+    for rows, out_dim, groups in ((1, 1, 1), (1, 100, 3), (2, 33, 24), (16, 130, 5), (17, 64, 9), (33, 70, 40),
+                                  (64, 16, 2), (130, 49, 7), (5, 16401, 2)):
+        check_q4(gpu_ctx, rows, dtype, rows, out_dim, groups * group, group, ("f16", "f32", "bf16")[rows % 3], zeros)
+
+
+@pytest.mark.gpu
+def test_q4_exact_weights(gpu_ctx):
+    """Weights of zero take nothing, however large the input beside them; float32 rows keep their bits."""
+    from semantica_gpu import kernels
+    for dtype in ("f32", "f16", "bf16"):
+        for rows in (1, 40):
+            g = gen(rows)
+            codes, scales, _ = q4_make(g, 40, 256, 32)
+            codes = codes & 0xf0 | 8  # even inputs' weights are zero
+            x = rand(g, rows, 256, dtype=dtype)
+            x[:, ::2] = 6e4 if dtype == "f16" else 1e30
+            w = q4_dense(codes, scales, None)
+            wt = kernels.Q4Weight(gpu_ctx, codes.cuda(), scales.cuda())
+            dst = torch.empty(rows, 40, dtype=dt(dtype), device="cuda")
+            kernels.matmul_q4(gpu_ctx, dst, wt, x.cuda())
+            wt.close()
+            want = x.double() @ w.t()
+            close(dst, want, q4_tol(dtype, x[:, 1::2], w[:, 1::2], want), "products")
+    # One weight a row: the product's own rounding and no other.
+    g = gen(1)
+    codes = torch.full((32, 64), 0x88, dtype=torch.uint8)
+    codes[:, 0] = 0x89  # weight one for input 0
+    x = torch.zeros(16, 128)
+    x[:, 0] = torch.randn(16, generator=g) * 2.0 ** torch.arange(-120, 120, 15).float()
+    wt = kernels.Q4Weight(gpu_ctx, codes.cuda(), torch.ones(32, 4, device="cuda"))
+    dst = torch.empty(16, 32, device="cuda")
+    kernels.matmul_q4(gpu_ctx, dst, wt, x.cuda())
+    wt.close()
+    # Parts of eight bits: the third holds what lies 16 to 23 places below the first bit, the second
+    # 8 to 15, and a part is lost where it falls below bf16's smallest normal number (as part of
+    # a subnormal or for a matrix core that takes those as zeros).  So nothing is lost of an input of
+    # 2^-102 or more, and less than 2^-126 by each of two parts of a smaller one.
+    want = x[:, :1].expand(16, 32)
+    big = want.abs() >= 2.0 ** -102
+    same(dst.cpu()[big], want[big], "float32 rows")
+    assert bool(((dst.cpu().double() - want.double()).abs() <= 2.0 ** -125).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_q4_not_finite(gpu_ctx, dtype):
+    """An infinity or a NaN is its row's alone; an infinity times a weight that is not zero is one."""
+    from semantica_gpu import kernels
+    g = gen(5)
+    codes, scales, _ = q4_make(g, 48, 128, 64)
+    codes[:, 3] = 0x9f  # weights 7 and 1 for inputs 6 and 7
+    x = rand(g, 20, 128, dtype=dtype)
+    x[4, 6], x[9, 11] = math.inf, math.nan
+    wt = kernels.Q4Weight(gpu_ctx, codes.cuda(), scales.cuda())
+    dst = torch.empty(20, 48, dtype=dt(dtype), device="cuda")
+    kernels.matmul_q4(gpu_ctx, dst, wt, x.cuda())
+    wt.close()
+    got = dst.cpu().float()
+    assert bool((got[4] == math.inf).all()) and bool(torch.isnan(got[9]).all())
+    rest = torch.ones(20, dtype=torch.bool)
+    rest[4] = rest[9] = False
+    w = q4_dense(codes, scales, None)
+    want = x[rest].double() @ w.t()
+    close(got[rest], want, q4_tol(dtype, x[rest], w, want), "products")
+
+
+@pytest.mark.gpu
+def test_q4_from_gguf_blocks(gpu_ctx):
+    """Raw Q4_0 blocks: the same products as their codes and scales."""
+    from semantica_gpu import kernels
+    r = np.random.RandomState(3)
+    out_dim, in_dim = 50, 224
+    d = (r.uniform(0.001, 0.1, (out_dim, in_dim // 32)) * r.choice([-1, 1], (out_dim, in_dim // 32))).astype(np.float16)
+    q = r.randint(0, 16, (out_dim, in_dim // 32, 32)).astype(np.uint8)
+    raw = np.concatenate([d[..., None].view(np.uint8), q[..., :16] | q[..., 16:] << 4], -1)
+    w = torch.from_numpy(((q.astype(np.float64) - 8) * d.astype(np.float64)[..., None]).reshape(out_dim, in_dim))
+    x = rand(gen(2), 3, in_dim)
+    wt = kernels.Q4Weight.from_q4_0(gpu_ctx, raw, out_dim, in_dim)
+    dst = torch.empty(3, out_dim, device="cuda")
+    kernels.matmul_q4(gpu_ctx, dst, wt, x.cuda())
+    wt.close()
+    want = x.double() @ w.t()
+    close(dst, want, q4_tol("f32", x, w, want), "products")
+
+
 # ---- refusals ---------------------------------------------------------------------------
 
 
@@ -553,3 +685,7 @@ def test_refusals_without_a_gpu():
     assert lib.sg_attention_shared(None, None, 0, None, 0, None, 1, 1, None, 1, keys, None, 0, None) == bad
     assert b"NULL" in lib.sg_last_error()
     lib.sg_kv_cache_free(None)
+    assert lib.sg_q4_weight_create(None, None, None, 0, None, 1, 32, 32, None, ctypes.byref(out)) == bad
+    assert lib.sg_q4_weight_create_q4_0(None, None, 1, 32, ctypes.byref(out)) == bad
+    assert lib.sg_matmul_q4(None, None, 0, None, None, 0, 0, 1, None) == bad
+    lib.sg_q4_weight_free(None)

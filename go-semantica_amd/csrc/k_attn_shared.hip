@@ -81,17 +81,24 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
   auto rows_of = [&](int i) { return max(off(i + 1) - off(i), 0); };
   auto group_at = [&](int p) { return min(max(b.shared[p], 0), b.n_seq); };
 
-  // Jobs of each prefix and sequence: those of prefixes first where both stand in one list.
+  // Jobs of each prefix and sequence: those of prefixes first where both stand in one list; with
+  // all_keys there are only sequences'.
+  const bool prefixes = b.n_prefix > 0 && !b.all_keys;
   const int prefix_jobs =
-      b.n_prefix > 0 ? (int)running(b.n_prefix, 0, la.cap, b.prefix_jobs,
-                                    [&](int p) {
-                                      const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
-                                      return (rows * a.group + la.m - 1) / la.m;
-                                    })
-                     : 0;
+      prefixes ? (int)running(b.n_prefix, 0, la.cap, b.prefix_jobs,
+                              [&](int p) {
+                                const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
+                                return (rows * a.group + la.m - 1) / la.m;
+                              })
+               : 0;
   const int own0 = one_list ? prefix_jobs : 0;
   const int own_end = (int)running(b.n_seq, own0, lb.cap, b.seq_jobs,
                                    [&](int i) { return ((int64_t)rows_of(i) * a.group + lb.m - 1) / lb.m; });
+  auto prefix_of = [&](int i) {  // of a sequence; -1: none
+    if (b.n_prefix == 0) return -1;
+    const int p = last_at_most(b.n_prefix, i, group_at);
+    return i >= group_at(p) && i < group_at(p + 1) ? p : -1;
+  };
 
   // What each row sees.
   for (int row = t; row < a.rows; row += kPlanThreads) {
@@ -102,10 +109,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
       const int64_t len = kept_length(b.starts[i], b.lengths[i], b.slots);
       int64_t plen = 0;
       where = make_int4(-1, 0, b.seq_jobs[i], r0);
-      if (b.n_prefix > 0) {
-        const int p = last_at_most(b.n_prefix, i, group_at);
-        if (i >= group_at(p) && i < group_at(p + 1)) {
-          plen = kept_length(b.prefix_starts[p], b.prefix_lengths[p], b.slots);
+      const int p = prefix_of(i);
+      if (p >= 0) {
+        plen = kept_length(b.prefix_starts[p], b.prefix_lengths[p], b.slots);
+        if (prefixes) {
           where.x = b.prefix_jobs[p];
           where.y = off(group_at(p));
         }
@@ -124,34 +131,43 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
   }
   __syncthreads();
 
-  // The jobs, and the running total of their tiles.
-  auto fill = [&](const sg_attn_list& list, int j0, int n, int own, int64_t base) {
-    const int32_t* jobs = own ? b.seq_jobs : b.prefix_jobs;
+  // The jobs, and the running total of their costs.
+  auto fill = [&](const sg_attn_list& list, int j0, int n, int kind, int64_t base) {
+    const int32_t* jobs = kind == kPrefixKeys ? b.prefix_jobs : b.seq_jobs;
     const int64_t units = running(n, base, INT64_MAX, list.cum + j0, [&](int j) {
-      const int i = last_at_most(own ? b.n_seq : b.n_prefix, j + j0, [&](int k) { return jobs[k]; });
-      const int first = own ? i : group_at(i), r0 = off(first), r1 = off(own ? i + 1 : group_at(i + 1));
-      const int start = own ? b.starts[i] : b.prefix_starts[i];
-      sg_attn_job job{r0, max(r1 - r0, 0), j + j0 - jobs[i], max(start, 0), 0, own};
+      const int i = last_at_most(kind == kPrefixKeys ? b.n_prefix : b.n_seq, j + j0, [&](int k) { return jobs[k]; });
+      const int r0 = off(kind == kPrefixKeys ? group_at(i) : i), r1 = off(kind == kPrefixKeys ? group_at(i + 1) : i + 1);
+      sg_attn_job job{r0, max(r1 - r0, 0), j + j0 - jobs[i], kind, {0, 0}, {0, 0}, {0, 0}};
       const int from = r0 + (int)((int64_t)job.tile * list.m / a.group);
       const int to = (int)min((int64_t)r1 - 1, r0 + ((int64_t)(job.tile + 1) * list.m - 1) / a.group);
-      const int len = kept_length(start, own ? b.lengths[i] : b.prefix_lengths[i], b.slots);
-      int lo = INT32_MAX, hi = 0;
+      int lo[2] = {INT32_MAX, INT32_MAX}, hi[2] = {0, 0};
       for (int r = from; r <= to; r++) {
         const int4 s = seen_out[r];
-        // (Cut once more: where offsets do not ascend, a row's range is another sequence's.)
-        const int l = own ? s.z : s.x, h = min(own ? s.w : s.y, len);
-        if (l < h) {
-          lo = min(lo, l);
-          hi = max(hi, h);
+        if (s.x < s.y) {
+          lo[0] = min(lo[0], s.x);
+          hi[0] = max(hi[0], s.y);
+        }
+        if (s.z < s.w) {
+          lo[1] = min(lo[1], s.z);
+          hi[1] = max(hi[1], s.w);
         }
       }
       int64_t count = 0;
-      if (lo < hi) {
-        job.slot_tile = (int)(((int64_t)start + lo) / kTile);
-        count = ((int64_t)start + hi - 1) / kTile - job.slot_tile + 1;
+      for (int own = 0; own < 2; own++) {
+        const int p = kind == kPrefixKeys ? i : kind == kAllKeys ? prefix_of(i) : -1;
+        if (own ? kind == kPrefixKeys : p < 0) continue;
+        const int64_t start = own ? b.starts[i] : b.prefix_starts[p];
+        // (Cut once more: where offsets do not ascend, a row's range is another sequence's.)
+        const int end = min(hi[own], kept_length((int)start, own ? b.lengths[i] : b.prefix_lengths[p], b.slots));
+        if (lo[own] >= end) continue;
+        const int at = kind == kAllKeys ? own : 0;
+        job.key0[at] = (int)start;
+        job.slot_tile[at] = (int)((start + lo[own]) / kTile);
+        job.tiles[at] = (int)((start + end - 1) / kTile) - job.slot_tile[at] + 1;
+        count += job.tiles[at];
       }
       list.jobs[j + j0] = job;
-      return count;
+      return count + (count > 0 || kind == kAllKeys ? list.job_cost : 0);
     });
     if (t == 0) {
       list.plan->units = units;
@@ -161,17 +177,66 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
     return units;
   };
   int64_t base = 0;
-  if (b.n_prefix > 0) base = fill(la, 0, prefix_jobs, 0, 0);
+  if (prefixes) base = fill(la, 0, prefix_jobs, kPrefixKeys, 0);
   if (!one_list) base = 0;
-  fill(lb, own0, own_end - own0, 1, base);
+  fill(lb, own0, own_end - own0, b.all_keys ? kAllKeys : kOwnKeys, base);
 }
 
-// One (row, head) for NW waves: the pieces of its prefix's job and of its own keys', put
-// together under their largest maximum.
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_attn_join(sg_attn_shared_args a, sg_attn_list la, sg_attn_list lb) {
-  constexpr int V = D / 64;
+// The workers that have tiles of a job: [first, last], as of a whole list.
+struct holders {
+  int64_t first, last;
+  bool any;
+};
+__device__ __forceinline__ holders holders_of(const sg_attn_list& list, int kv, int64_t job) {
+  const int64_t c0 = list.cum[job], c1 = list.cum[job + 1], head = kv * list.plan->units, per = list.plan->per;
+  holders h{0, 0, c1 - c0 > list.job_cost};
+  if (h.any) {
+    h.first = (head + c0 + list.job_cost) / per;
+    h.last = (head + c1 - 1) / per;
+  }
+  return h;
+}
+
+// A pair's running maximum, sum and output, D / 64 dims a lane, and what it is joined with.
+template <int D>
+struct joined {
+  static constexpr int V = D / 64;
   typedef float vec __attribute__((ext_vector_type(V)));
+  float m = -INFINITY, l = 0.0f;
+  vec o = 0.0f;
+  __device__ __forceinline__ void add(float om, float ol, vec oo) {
+    const float top = fmaxf(m, om);  // (maxima are no NaN)
+    if (top == -INFINITY && ol == 0.0f) return;
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float by = __builtin_amdgcn_exp2f(m - base), now = __builtin_amdgcn_exp2f(om - base);
+    l = l * by + ol * now;
+    o = o * by + oo * now;
+    m = top;
+  }
+  __device__ __forceinline__ void add(const sg_attn_shared_args& a, int64_t at, int lane) {
+    const float2 ml = a.part_ml[at];
+    add(ml.x, ml.y, *reinterpret_cast<const vec*>(a.part_o + at * D + lane * V));
+  }
+  // A query that sees nothing, or nothing but scores of -infinity, has zeros.
+  template <typename T>
+  __device__ __forceinline__ void put(const sg_attn_shared_args& a, int row, int head, int lane) const {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(a.out) + row * a.ldo + (int64_t)head * a.hd;
+#pragma unroll
+    for (int v = 0; v < V; v++)
+      if (lane * V + v < a.hd) out[lane * V + v] = elem<T>::from(l == 0.0f ? 0.0f : o[v] * inv);
+  }
+};
+
+__device__ __forceinline__ int64_t piece_of(const sg_attn_list& list, int64_t worker, bool first, int in_job) {
+  return list.piece0 + (worker * 2 + (first ? 1 : 0)) * list.piece_pairs + in_job;
+}
+
+// One (row, head) for NW waves: what there is of its prefix's job and of its own keys', or of
+// the job that has both.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_attn_join(sg_attn_shared_args a, sg_attn_list la, sg_attn_list lb,
+                                                                       int all_keys) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t i = NW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   if (i >= (int64_t)a.rows * a.heads) return;
@@ -179,68 +244,63 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_attn_join(sg_attn_s
   const int4 where = a.where[row];
   if (where.z == -2) return;  // a row of no sequence
   const int kv = head / a.group, hg = head - kv * a.group;
-  float m = -INFINITY, l = 0.0f;
-  vec o = 0.0f;
+  joined<D> x;
 #pragma unroll
   for (int own = 0; own < 2; own++) {
     const sg_attn_list& list = own ? lb : la;
     const int job0 = own ? where.z : where.x;
     if (job0 < 0) continue;
-    const int64_t pair = (int64_t)(row - (own ? where.w : where.y)) * a.group + hg;
-    const int64_t job = job0 + pair / list.m;
+    const int64_t pair = (int64_t)(row - (own ? where.w : where.y)) * a.group + hg, job = job0 + pair / list.m;
     if (pair < 0 || job >= list.plan->jobs) continue;  // (offsets that do not ascend)
-    const int64_t c0 = list.cum[job], c1 = list.cum[job + 1];
-    if (c0 == c1) continue;
-    const int64_t first = kv * list.plan->units, per = list.plan->per;
-    const int64_t w0 = (first + c0) / per, w1 = (first + c1 - 1) / per;
+    const holders h = holders_of(list, kv, job);
+    if (all_keys && (!h.any || h.first == h.last)) return;  // written
+    if (!h.any) continue;
     const int in_job = (int)(pair % list.m);
-    for (int64_t w = w0 + (NW == 1 ? 0 : wave); w <= w1; w += NW) {
-      const int64_t at = w0 == w1 ? (int64_t)(own ? a.rows : 0) * a.heads + i
-                                  : list.piece0 + (w * 2 + (w == w0 ? 1 : 0)) * list.piece_pairs + in_job;
-      const float2 ml = a.part_ml[at];
-      const vec x = *reinterpret_cast<const vec*>(a.part_o + at * D + lane * V);
-      const float top = fmaxf(m, ml.x);  // (maxima are no NaN)
-      if (top == -INFINITY && ml.y == 0.0f) continue;
-      const float base = top == -INFINITY ? 0.0f : top;
-      const float by = __builtin_amdgcn_exp2f(m - base), now = __builtin_amdgcn_exp2f(ml.x - base);
-      l = l * by + ml.y * now;
-      o = o * by + x * now;
-      m = top;
-    }
+    for (int64_t w = h.first + (NW == 1 ? 0 : wave); w <= h.last; w += NW)
+      x.add(a, h.first == h.last ? (int64_t)(own ? a.rows : 0) * a.heads + i : piece_of(list, w, w == h.first, in_job), lane);
   }
   if constexpr (NW > 1) {
     __shared__ float ms[NW], ls[NW];
-    __shared__ vec os[NW][64];
-    os[wave][lane] = o;
+    __shared__ typename joined<D>::vec os[NW][64];
+    os[wave][lane] = x.o;
     if (lane == 0) {
-      ms[wave] = m;
-      ls[wave] = l;
+      ms[wave] = x.m;
+      ls[wave] = x.l;
     }
     __syncthreads();
     if (wave != 0) return;
-    for (int w = 0; w < NW; w++) m = fmaxf(m, ms[w]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    l = 0.0f;
-    o = 0.0f;
-    for (int w = 0; w < NW; w++) {
-      const float by = __builtin_amdgcn_exp2f(ms[w] - base);
-      l += ls[w] * by;
-      o += os[w][lane] * by;
-    }
+    for (int w = 1; w < NW; w++) x.add(ms[w], ls[w], os[w][lane]);
   }
-  // A query that sees nothing, or nothing but scores of -infinity, has zeros.
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T* out = static_cast<T*>(a.out) + row * a.ldo + (int64_t)head * a.hd;
-#pragma unroll
-  for (int v = 0; v < V; v++) {
-    const int dim = lane * V + v;
-    if (dim < a.hd) out[dim] = elem<T>::from(l == 0.0f ? 0.0f : o[v] * inv);
+  x.template put<T>(a, row, head, lane);
+}
+
+// The jobs with all keys that lie across workers, for many rows: a block column for each
+// worker that ends inside a job and began it.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attn_join_split(sg_attn_shared_args a, sg_attn_list list) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t units = list.plan->units, per = list.plan->per, worker = blockIdx.x, end = (worker + 1) * per;
+  if (end >= units * a.kv_heads) return;
+  const int kv = (int)(end / units);
+  const int64_t at = end - kv * units;
+  const int job = sgc::last_at_most(list.cum, list.plan->jobs, at, lane);
+  const holders h = holders_of(list, kv, job);
+  if (!h.any || h.first != worker || h.last == worker) return;
+  const sg_attn_job jb = list.jobs[job];
+  for (int in_job = blockIdx.y * 16 + wave; in_job < min((int)blockIdx.y * 16 + 16, list.m); in_job += 4) {
+    const int64_t pair = (int64_t)jb.tile * list.m + in_job;
+    if (pair >= (int64_t)jb.rows * a.group) return;
+    const int r = (int)(pair / a.group);
+    joined<D> x;
+    for (int64_t w = h.first; w <= h.last; w++) x.add(a, piece_of(list, w, w == h.first, in_job), lane);
+    x.template put<T>(a, jb.row0 + r, kv * a.group + (int)(pair - (int64_t)r * a.group), lane);
   }
 }
 
 // The form of each kind of job.  Up to so many pairs of a group on average, waves work for
 // themselves.
 constexpr int kNarrowPairs = 32;
+constexpr int kFullJobs = 4;
 constexpr int kJoinWaves = 16;
 constexpr int64_t kJoinFew = 2048;  // (row, head) up to here: so many waves each
 
@@ -257,7 +317,7 @@ layout lay_out(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, i
   y.cap = (int)std::min<int64_t>(2 * (pairs / 16) + n_seq + n_prefix + 2, INT32_MAX);
   const int cus = 256;
   y.workers[0] = cus * 4 * (dtype == SG_F32 ? 1 : 2);
-  y.workers[1] = cus * (dtype == SG_F32 && D == 256 ? 1 : 2);
+  y.workers[1] = cus * (dtype == SG_F32 && D >= 128 ? 1 : 2);
   y.m[0] = 16;
   y.m[1] = sgk::attn_wide_pairs(D);
   size_t at = 0;
@@ -288,16 +348,19 @@ layout lay_out(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, i
 }
 
 template <typename T, int D>
-hipError_t join(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, hipStream_t s) {
+hipError_t join(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, int all_keys, hipStream_t s) {
   const int64_t n = (int64_t)a.rows * a.heads;
-  if (n <= kJoinFew) return sgp::run_kernel(k_attn_join<T, D, kJoinWaves>, dim3(n), dim3(64 * kJoinWaves), 0, s, a, la, lb);
-  return sgp::run_kernel(k_attn_join<T, D, 1>, dim3((n + 3) / 4), dim3(256), 0, s, a, la, lb);
+  if (n <= kJoinFew)
+    return sgp::run_kernel(k_attn_join<T, D, kJoinWaves>, dim3(n), dim3(64 * kJoinWaves), 0, s, a, la, lb, all_keys);
+  if (all_keys) return sgp::run_kernel(k_attn_join_split<T, D>, dim3(lb.workers, lb.m / 16), dim3(256), 0, s, a, lb);
+  return sgp::run_kernel(k_attn_join<T, D, 1>, dim3((n + 3) / 4), dim3(256), 0, s, a, la, lb, 0);
 }
 template <typename T>
-hipError_t join_dims(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, int D, hipStream_t s) {
-  if (D == 64) return join<T, 64>(a, la, lb, s);
-  if (D == 128) return join<T, 128>(a, la, lb, s);
-  return join<T, 256>(a, la, lb, s);
+hipError_t join_dims(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, int all_keys, int D,
+                     hipStream_t s) {
+  if (D == 64) return join<T, 64>(a, la, lb, all_keys, s);
+  if (D == 128) return join<T, 128>(a, la, lb, all_keys, s);
+  return join<T, 256>(a, la, lb, all_keys, s);
 }
 
 }  // namespace
@@ -333,12 +396,16 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
     l.wide = i;
     l.cap = y.cap;
     l.min_units = i ? 4 : 2;
+    l.job_cost = i ? 4 : 2;
   }
   const int64_t pairs = (int64_t)a.rows * a.group;
-  const int wide_prefix = b.n_prefix > 0 && pairs > (int64_t)kNarrowPairs * b.n_prefix;
+  // A job for each M pairs of a sequence, over prefix and own keys in one go, where no prefix is
+  // shared or sequences fill several jobs themselves; otherwise prefixes and own keys by themselves.
+  b.all_keys = b.n_seq <= b.n_prefix || b.n_prefix == 0 || pairs >= (int64_t)kFullJobs * y.m[1] * b.n_seq;
   const int wide_own = pairs > (int64_t)kNarrowPairs * b.n_seq;
+  const int wide_prefix = b.all_keys ? wide_own : pairs > (int64_t)kNarrowPairs * b.n_prefix;
   const sg_attn_list& lb = lists[wide_own];
-  const sg_attn_list& la = b.n_prefix > 0 ? lists[wide_prefix] : lb;
+  const sg_attn_list& la = lists[wide_prefix];
   const int one_list = &la == &lb;
   hipError_t e = sgp::run_kernel(k_attn_plan, dim3(1), dim3(kPlanThreads), 0, s, a, b, la, lb, one_list, seen, where);
   auto run = [&](const sg_attn_list& l) {
@@ -350,9 +417,9 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
   run(la);
   if (!one_list) run(lb);
   if (e != hipSuccess) return e;
-  if (dtype == SG_F32) return join_dims<float>(a, la, lb, D, s);
-  if (dtype == SG_F16) return join_dims<_Float16>(a, la, lb, D, s);
-  return join_dims<sgp::bf16_t>(a, la, lb, D, s);
+  if (dtype == SG_F32) return join_dims<float>(a, la, lb, b.all_keys, D, s);
+  if (dtype == SG_F16) return join_dims<_Float16>(a, la, lb, b.all_keys, D, s);
+  return join_dims<sgp::bf16_t>(a, la, lb, b.all_keys, D, s);
 }
 
 }  // namespace sgk

@@ -171,12 +171,17 @@ struct weight<bf16_t, true> {
 template <typename T, bool Q8>
 constexpr float kShift = __is_same(T, _Float16) && !Q8 ? 6.0f : 0.0f;
 
+// Sums of weights by the matrix core: 16-bit types whose weights are multiplied as they are.
+template <typename T, bool Q8>
+constexpr bool kSumByProduct = !Q8 && sizeof(T) == 2;
+
 // What a wave has of its QT * 16 pairs: queries, running maxima and sums, outputs.
 template <typename T, bool Q8, int D, int QT>
 struct state {
   typename frag<T>::type q[QT][D / 32];
   f32x4_t o[QT][D / 16];
   float m[QT], l[QT];
+  f32x4_t sum[QT];  // in place of l where the matrix core adds up: each of the four is the sum
   int lo[QT], hi[QT];  // visible keys of the lane's pairs, counted from the job's first
   int all_lo, all_hi;  // keys that every pair of the wave sees
 };
@@ -207,9 +212,10 @@ __device__ __forceinline__ void pack_weights(const float* p, typename frag<typen
   }
 }
 
-// A tile's scores become weights: first: the place of the tile's first slot among the job's
-// keys (negative where the tile begins before them).  s: products; tail: the tile's, in LDS or
-// memory.
+// A tile's products become weights.  first: the place of the tile's first slot among the keys
+// that lo and hi count (negative where the tile begins before them); tail: the tile's, in LDS or
+// memory.  Weights are 2^(s c - m) of scores s as they come: c > 0 holds the scale (queries are
+// negated for a negative one), so a maximum is taken before it and one fma does the rest.
 template <typename T, bool Q8, int D, int QT>
 __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8, D, QT>& st, f32x4_t (&s)[2][QT], int first,
                                       const float* tail, int lane, float (&p)[QT][8]) {
@@ -224,22 +230,21 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      const float c = ks[j >> 2][j & 3] * a.scale;
       vs[j] = v[j >> 2][j & 3];
 #pragma unroll
-      for (int t = 0; t < QT; t++) p[t][j] = s[j >> 2][t][j & 3] * c;
+      for (int t = 0; t < QT; t++) p[t][j] = s[j >> 2][t][j & 3] * ks[j >> 2][j & 3];
     }
   } else {
 #pragma unroll
     for (int t = 0; t < QT; t++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) p[t][j] = s[j >> 2][t][j & 3] * a.scale;
+      for (int j = 0; j < 8; j++) p[t][j] = s[j >> 2][t][j & 3];
   }
   if (a.cap != 0.0f) {
 #pragma unroll
     for (int t = 0; t < QT; t++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) p[t][j] = a.cap * tanh_of(p[t][j]);
+      for (int j = 0; j < 8; j++) p[t][j] = a.cap * tanh_of(p[t][j] * a.to_cap);
   }
   const bool part = first < st.all_lo || first + kTile > st.all_hi;
   if (part) {
@@ -254,23 +259,25 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
 #pragma unroll
   for (int t = 0; t < QT; t++) {
     float top = fmaxf(fmaxf(fmaxf(p[t][0], p[t][1]), fmaxf(p[t][2], p[t][3])),
-                      fmaxf(fmaxf(p[t][4], p[t][5]), fmaxf(p[t][6], p[t][7])));
+                      fmaxf(fmaxf(p[t][4], p[t][5]), fmaxf(p[t][6], p[t][7]))) * a.scale;
     if (__ballot(top > st.m[t] + kSlack)) {
       top = fmaxf(pair_max(top), st.m[t]);
       const float by = top > st.m[t] ? exp2_of(st.m[t] - top) : 1.0f;  // (m may be -infinity: 0)
       st.m[t] = top;
-      st.l[t] *= by;
+      if constexpr (kSumByProduct<T, Q8>) st.sum[t] *= by;
+      else st.l[t] *= by;
 #pragma unroll
       for (int f = 0; f < D / 16; f++) st.o[t][f] *= by;
     }
     const float m = (st.m[t] == -INFINITY ? 0.0f : st.m[t]) - kShift<T, Q8>;
-    float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      p[t][j] = exp2_of(p[t][j] - m);
-      sum += p[t][j];
+    for (int j = 0; j < 8; j++) p[t][j] = exp2_of(__builtin_fmaf(p[t][j], a.scale, -m));
+    if constexpr (!kSumByProduct<T, Q8>) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum += p[t][j];
+      st.l[t] += sum;
     }
-    st.l[t] += sum;
     if constexpr (Q8) {
 #pragma unroll
       for (int j = 0; j < 8; j++) p[t][j] *= vs[j];
@@ -285,46 +292,70 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
   }
 }
 
-// A fragment of values without those of the keys in `bad`.
-template <typename T>
-__device__ __forceinline__ void drop_bad(typename frag<T>::type& x, uint32_t bad, int lane) {
-  const int g = lane >> 4;
+// The packed weights' sums, by a product with ones: a sixteenth of the second product's work in
+// place of eight additions a lane, and the sum of the weights as they are multiplied.
+template <typename T, bool Q8, int D, int QT>
+__device__ __forceinline__ void add_sums(state<T, Q8, D, QT>& st, const s16x8_t (&w)[QT][1]) {
+  const short one = __builtin_bit_cast(short, elem<T>::from(1.0f));
+  const s16x8_t ones = {one, one, one, one, one, one, one, one};
 #pragma unroll
-  for (int j = 0; j < 8; j++)
-    if (bad >> ((j >> 2) * 16 + g * 4 + (j & 3)) & 1) {
-      if constexpr (__is_same(T, float)) x.v[j >> 2][j & 3] = 0.0f;
-      else x[j] = 0;
-    }
+  for (int t = 0; t < QT; t++) st.sum[t] = mma(T{}, ones, w[t][0], st.sum[t]);
 }
 
-// Values that are not finite: a hidden key's zero weight times one is a NaN.  The products leave
-// such keys out (drop_bad), and the pairs that see them have them added here, one key at a time.
-// vals: the tile's values in memory.
-template <typename T, bool Q8, int D, int QT>
-__device__ __forceinline__ void add_bad(state<T, Q8, D, QT>& st, const float (&p)[QT][8], int first, uint32_t bad,
-                                        const char* vals, int lane) {
-  const int g = lane >> 4;
-  for (; bad; bad &= bad - 1) {
-    const int key = __builtin_ctz(bad), j = (key >> 4) * 4 + (key & 3), from = ((key >> 2) & 3) * 16;
-    float wt[QT];
+// Values that are not finite, in a tile that may be hidden in part: a zero weight times one is a
+// NaN.  So they are zeros in the product, and which pairs see an infinity or a NaN of a dim is
+// counted by products of ones: exact, and no business of the weights'.
+template <typename M>
+__device__ __forceinline__ void set_elem(typename frag<M>::type& x, int j, float v) {
+  if constexpr (__is_same(M, float)) x.v[j >> 2][j & 3] = v;
+  else x[j] = __builtin_bit_cast(short, elem<M>::from(v));
+}
+template <typename M>
+__device__ __forceinline__ float get_elem(const typename frag<M>::type& x, int j) {
+  if constexpr (__is_same(M, float)) return x.v[j >> 2][j & 3];
+  else return elem<M>::to(__builtin_bit_cast(M, (short)x[j]));
+}
+template <typename T, int D, int QT>
+__device__ __forceinline__ void values_bad(state<T, false, D, QT>& st, int first, const float (&p)[QT][8], const char* vals,
+                                           int lane) {
+  typedef typename frag<T>::type X;
+  X sees[QT], w[QT][1];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    pack_weights<T, false>(p[t], w[t]);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int key = first + (j >> 2) * 16 + (lane >> 4) * 4 + (j & 3);
+      set_elem<T>(sees[t], j, key >= st.lo[t] && key < st.hi[t] ? 1.0f : 0.0f);
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < D / 16; f++) {
+    const X x = load_frag<T>(vals, f, lane);
+    X one[3], clean;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float v = get_elem<T>(x, j);
+      set_elem<T>(clean, j, fabsf(v) < INFINITY ? v : 0.0f);
+      set_elem<T>(one[0], j, v == INFINITY ? 1.0f : 0.0f);
+      set_elem<T>(one[1], j, v == -INFINITY ? 1.0f : 0.0f);
+      set_elem<T>(one[2], j, v != v ? 1.0f : 0.0f);
+    }
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-      float mine = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; i++) mine = i == j ? p[t][i] : mine;
-      wt[t] = __shfl(mine, from + (lane & 15));
-    }
-#pragma unroll
-    for (int f = 0; f < D / 16; f++) {
+      const f32x4_t none = {0, 0, 0, 0};
+      const f32x4_t up = mma(T{}, one[0], sees[t], none), down = mma(T{}, one[1], sees[t], none),
+                    nan = mma(T{}, one[2], sees[t], none);
+      f32x4_t o = mma(T{}, clean, w[t][0], st.o[t][f]);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const float v = elem<T>::to(*reinterpret_cast<const T*>(vals + sgc::place<(int)sizeof(T)>(f, from + g * 4 + i, j)));
-#pragma unroll
-        for (int t = 0; t < QT; t++)
-          st.o[t][f][i] = first + key >= st.lo[t] && first + key < st.hi[t] ? st.o[t][f][i] + wt[t] * v : st.o[t][f][i];
+        o[i] = up[i] != 0.0f ? o[i] + INFINITY : o[i];
+        o[i] = down[i] != 0.0f ? o[i] - INFINITY : o[i];
+        o[i] = nan[i] != 0.0f ? __builtin_nanf("") : o[i];
       }
-      asm volatile("" ::: "memory");  // (one fragment's loads at a time: registers)
+      st.o[t][f] = o;
     }
+    asm volatile("" ::: "memory");  // (one fragment at a time: registers)
   }
 }
 
@@ -338,7 +369,6 @@ struct share {
   int64_t at, left;  // unit within the head's, units to do
 };
 
-template <int D, int QT>
 __device__ __forceinline__ share first_share(const sg_attn_list& list, int64_t worker, int heads, int lane) {
   share s{0, 0, 0, 0};
   const int64_t units = list.plan->units, per = list.plan->per, total = units * heads;
@@ -347,34 +377,24 @@ __device__ __forceinline__ share first_share(const sg_attn_list& list, int64_t w
   s.left = min(per, total - begin);
   s.head = (int)(begin / units);
   s.at = begin - s.head * units;
-  // The last job that begins at or before the unit and is not empty: 64 candidates a step.
-  int lo = 0, len = list.plan->jobs;
-  while (len > 1) {
-    const int step = (len + 63) >> 6, j = lane * step;
-    const int c = __popcll(__ballot(j < len && list.cum[lo + j] <= s.at));
-    lo += (c - 1) * step;
-    len = min(step, len - (c - 1) * step);
-  }
-  s.job = __builtin_amdgcn_readfirstlane(lo);
+  // The last job that begins at or before the unit: it is not empty.
+  s.job = sgc::last_at_most(list.cum, list.plan->jobs, s.at, lane);
   return s;
 }
 
-// Loads the wave's pairs of a job: queries and the keys each sees.
+// Loads the queries of the wave's pairs of a job.
 template <typename T, bool Q8, int D, int QT>
 __device__ __forceinline__ void begin_job(const sg_attn_shared_args& a, state<T, Q8, D, QT>& st, const sg_attn_job& job, int head,
                                           int pair0, int lane) {
-  const int g = lane >> 4;
-  int all_lo = 0, all_hi = INT32_MAX;
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    const int64_t pair = (int64_t)pair0 + t * 16 + (lane & 15);
-    const bool in = pair < (int64_t)job.rows * a.group;
-    const int r = in ? (int)(pair / a.group) : 0, row = job.row0 + r;
-    const int h = head * a.group + (in ? (int)(pair - (int64_t)r * a.group) : 0);
-    const T* q = static_cast<const T*>(a.q) + row * a.ldq + (int64_t)h * a.hd;
+    const int pair = pair0 + t * 16 + (lane & 15);
+    const bool in = pair < job.rows * a.group;
+    const int r = in ? pair / a.group : 0, h = head * a.group + (in ? pair - r * a.group : 0);
+    const T* q = static_cast<const T*>(a.q) + (int64_t)(job.row0 + r) * a.ldq + (int64_t)h * a.hd;
 #pragma unroll
     for (int d = 0; d < D / 32; d++) {
-      const int dim = d * 32 + g * 8;
+      const int dim = d * 32 + (lane >> 4) * 8;
       typename frag<T>::type x{};
       if (in && dim < a.hd) {
         if constexpr (__is_same(T, float)) {
@@ -384,19 +404,40 @@ __device__ __forceinline__ void begin_job(const sg_attn_shared_args& a, state<T,
           x = *reinterpret_cast<const s16x8_t*>(q + dim);
         }
       }
+      if (a.negative) {
+        if constexpr (__is_same(T, float)) {
+          x.v[0] = -x.v[0];
+          x.v[1] = -x.v[1];
+        } else {
+          x ^= (short)0x8000;
+        }
+      }
       st.q[t][d] = x;
     }
-    const int4 seen = a.seen[row];
-    st.lo[t] = in ? (job.own ? seen.z : seen.x) : 0;
-    st.hi[t] = in ? (job.own ? seen.w : seen.y) : 0;
+    st.m[t] = -INFINITY;
+    st.l[t] = 0.0f;
+    st.sum[t] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int f = 0; f < D / 16; f++) st.o[t][f] = f32x4_t{0, 0, 0, 0};
+  }
+}
+
+// Which keys of the prefix (own 0) or of their own the wave's pairs see.
+template <typename T, bool Q8, int D, int QT>
+__device__ __forceinline__ void begin_keys(const sg_attn_shared_args& a, state<T, Q8, D, QT>& st, const sg_attn_job& job,
+                                           int pair0, int own, int lane) {
+  int all_lo = 0, all_hi = INT32_MAX;
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const int pair = pair0 + t * 16 + (lane & 15);
+    const bool in = pair < job.rows * a.group;
+    const int4 seen = a.seen[job.row0 + (in ? pair / a.group : 0)];
+    st.lo[t] = in ? (own ? seen.z : seen.x) : 0;
+    st.hi[t] = in ? (own ? seen.w : seen.y) : 0;
     if (in) {
       all_lo = max(all_lo, st.lo[t]);
       all_hi = min(all_hi, st.hi[t]);
     }
-    st.m[t] = -INFINITY;
-    st.l[t] = 0.0f;
-#pragma unroll
-    for (int f = 0; f < D / 16; f++) st.o[t][f] = f32x4_t{0, 0, 0, 0};
   }
 #pragma unroll
   for (int o = 8; o >= 1; o >>= 1) {  // (lanes 16 apart have the same pairs)
@@ -407,8 +448,9 @@ __device__ __forceinline__ void begin_job(const sg_attn_shared_args& a, state<T,
   st.all_hi = __builtin_amdgcn_readfirstlane(all_hi);
 }
 
-// What a wave has of a job to the workspace: the pairs' own place when the worker did the whole
-// job, the worker's first or last piece otherwise.
+// What a wave has of a job.  A worker that did the whole of it writes the output, if the job has
+// all keys of its rows, or the pairs' own places; otherwise it is the worker's first piece
+// (`later`: of a job that another worker began) or its last.
 template <typename T, bool Q8, int D, int QT>
 __device__ __forceinline__ void end_job(const sg_attn_shared_args& a, const sg_attn_list& list, state<T, Q8, D, QT>& st,
                                         const sg_attn_job& job, int head, int pair0, int in_job, int64_t worker, bool whole,
@@ -416,21 +458,51 @@ __device__ __forceinline__ void end_job(const sg_attn_shared_args& a, const sg_a
   const int g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    const float l = pair_sum(st.l[t]);
-    const int64_t pair = (int64_t)pair0 + t * 16 + (lane & 15);
-    if (pair >= (int64_t)job.rows * a.group) continue;
-    int64_t at;
-    if (whole) {
-      const int r = (int)(pair / a.group);
-      at = ((int64_t)(job.own ? a.rows : 0) + job.row0 + r) * a.heads + head * a.group + (pair - (int64_t)r * a.group);
-    } else {
-      at = list.piece0 + (worker * 2 + (later ? 0 : 1)) * list.piece_pairs + in_job + t * 16 + (lane & 15);
+    const float l = kSumByProduct<T, Q8> ? st.sum[t][0] : pair_sum(st.l[t]);
+    const int pair = pair0 + t * 16 + (lane & 15);
+    if (pair >= job.rows * a.group) continue;
+    const int r = pair / a.group, h = head * a.group + pair - r * a.group;
+    if (whole && job.kind == kAllKeys) {
+      T* out = static_cast<T*>(a.out) + (int64_t)(job.row0 + r) * a.ldo + (int64_t)h * a.hd;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      struct alignas(4 * sizeof(T)) four {
+        T v[4];
+      };
+#pragma unroll
+      for (int f = 0; f < D / 16; f++) {
+        four y;
+#pragma unroll
+        for (int i = 0; i < 4; i++) y.v[i] = elem<T>::from(l == 0.0f ? 0.0f : st.o[t][f][i] * inv);
+        if (f * 16 + g * 4 < a.hd) *reinterpret_cast<four*>(out + f * 16 + g * 4) = y;
+      }
+      continue;
     }
+    const int64_t at = whole ? ((int64_t)(job.kind == kOwnKeys ? a.rows : 0) + job.row0 + r) * a.heads + h
+                             : list.piece0 + (worker * 2 + (later ? 0 : 1)) * list.piece_pairs + in_job + t * 16 + (lane & 15);
     float* o = a.part_o + at * D;
 #pragma unroll
     for (int f = 0; f < D / 16; f++) *reinterpret_cast<f32x4_t*>(o + f * 16 + g * 4) = st.o[t][f];
     if (g == 0) a.part_ml[at] = make_float2(st.m[t], l);
   }
+}
+
+// A worker's part of a job: units [from, to) of it, all of its tiles if whole.  The list's cost of
+// a job (in tiles: queries, first tile, results) stands before its tiles and is no work.
+struct part {
+  int64_t from, to, all;
+  bool whole, later;
+  bool work;  // a job that has all keys and no tiles has zeros for its rows
+};
+__device__ __forceinline__ part part_of(const sg_attn_list& list, const sg_attn_job& job, int64_t at, int64_t left, int64_t c0,
+                                        int64_t c1) {
+  part p;
+  p.all = (int64_t)job.tiles[0] + job.tiles[1];
+  p.from = max(at - c0 - list.job_cost, (int64_t)0);
+  p.to = max(min(at + left, c1) - c0 - list.job_cost, (int64_t)0);
+  p.whole = p.from == 0 && p.to == p.all;
+  p.later = p.from > 0;
+  p.work = p.from < p.to || (p.all == 0 && job.kind == kAllKeys);
+  return p;
 }
 
 // Few pairs: every wave is a worker and takes fragments from memory, no barrier anywhere.
@@ -439,67 +511,73 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
   typedef typename weight<T, Q8>::type M;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t worker = (int64_t)spread(blockIdx.x, gridDim.x) * 4 + wave;
-  share sh = first_share<D, 1>(list, worker, a.kv_heads, lane);
+  share sh = first_share(list, worker, a.kv_heads, lane);
   state<T, Q8, D, 1> st;
   while (sh.left > 0) {
-    const sg_attn_job job = list.jobs[sh.job];
-    const int64_t c0 = list.cum[sh.job], c1 = list.cum[sh.job + 1];
-    const int64_t skip = sh.at - c0, n = min(c1 - sh.at, sh.left);
+    const int64_t c0 = list.cum[sh.job], c1 = list.cum[sh.job + 1], n = min(c1 - sh.at, sh.left);
     if (n > 0) {
+      const sg_attn_job job = list.jobs[sh.job];
+      const part pt = part_of(list, job, sh.at, sh.left, c0, c1);
       const int pair0 = job.tile * 16;
-      begin_job(a, st, job, sh.head, pair0, lane);
-      int64_t tile = job.slot_tile + skip;
-      int first = (int)(tile * kTile - job.key0);
-      const char* at = a.cache + (int64_t)sh.head * a.head_bytes + tile * a.tile_bytes;
-      for (int64_t u = 0; u < n; u++, first += kTile, at += a.tile_bytes) {
-        const char* vals = at + (int64_t)kTile * D * sizeof(typename sgc::kept<T, Q8>::type);
-        const char* tail = at + a.tile_bytes - kTail;
-        f32x4_t s[2][1] = {};
-        float p[1][8];
-        typename frag<M>::type w[weight<T, Q8>::parts];
-        if constexpr (Q8) {
-          constexpr int NU = D / 32;  // kilobytes of the keys, and of the values
-          u32x4_t kc[NU], vc[NU];
+      if (pt.work) begin_job(a, st, job, sh.head, pair0, lane);
+#pragma unroll 1
+      for (int seg = 0; seg < 2; seg++) {
+        const int64_t t0 = seg ? job.tiles[0] : 0, u0 = max(pt.from, t0), u1 = min(pt.to, t0 + (seg ? job.tiles[1] : job.tiles[0]));
+        if (u0 >= u1) continue;
+        begin_keys(a, st, job, pair0, job.kind == kOwnKeys || seg, lane);
+        const int64_t tile = (seg ? job.slot_tile[1] : job.slot_tile[0]) + (u0 - t0);
+        int first = (int)(tile * kTile - (seg ? job.key0[1] : job.key0[0]));
+        const char* at = a.cache + (int64_t)sh.head * a.head_bytes + tile * a.tile_bytes;
+        for (int64_t u = u0; u < u1; u++, first += kTile, at += a.tile_bytes) {
+          const char* vals = at + (int64_t)kTile * D * sizeof(typename sgc::kept<T, Q8>::type);
+          const char* tail = at + a.tile_bytes - kTail;
+          f32x4_t s[2][1] = {};
+          float p[1][8];
+          typename frag<M>::type w[1][weight<T, Q8>::parts];
+          if constexpr (Q8) {
+            constexpr int NU = D / 32;  // kilobytes of the keys, and of the values
+            u32x4_t kc[NU], vc[NU];
 #pragma unroll
-          for (int i = 0; i < NU; i++) kc[i] = *reinterpret_cast<const u32x4_t*>(at + i * 1024 + lane * 16);
+            for (int i = 0; i < NU; i++) kc[i] = *reinterpret_cast<const u32x4_t*>(at + i * 1024 + lane * 16);
 #pragma unroll
-          for (int i = 0; i < NU; i++) vc[i] = *reinterpret_cast<const u32x4_t*>(vals + i * 1024 + lane * 16);
+            for (int i = 0; i < NU; i++) vc[i] = *reinterpret_cast<const u32x4_t*>(vals + i * 1024 + lane * 16);
 #pragma unroll
-          for (int i = 0; i < NU; i++)
+            for (int i = 0; i < NU; i++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-              const int f = i * 2 + e, half = f / (D / 32), d = f % (D / 32);
-              s[half][0] = mma(T{}, decode<T>(kc[i][e * 2], kc[i][e * 2 + 1]), st.q[0][d], s[half][0]);
+              for (int e = 0; e < 2; e++) {
+                const int f = i * 2 + e, half = f / (D / 32), d = f % (D / 32);
+                s[half][0] = mma(T{}, decode<T>(kc[i][e * 2], kc[i][e * 2 + 1]), st.q[0][d], s[half][0]);
+              }
+            weigh<T, Q8, D, 1>(a, st, s, first, reinterpret_cast<const float*>(tail), lane, p);
+            pack_weights<T, Q8>(p[0], w[0]);
+#pragma unroll
+            for (int i = 0; i < NU; i++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const typename frag<M>::type x = decode<M>(vc[i][e * 2], vc[i][e * 2 + 1]);
+#pragma unroll
+                for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[0][i * 2 + e] = mma(M{}, x, w[0][h], st.o[0][i * 2 + e]);
+              }
+          } else {
+            const bool bad = *reinterpret_cast<const uint32_t*>(tail) != 0;
+#pragma unroll
+            for (int half = 0; half < 2; half++)
+#pragma unroll
+              for (int d = 0; d < D / 32; d++)
+                s[half][0] = mma(T{}, load_frag<T>(at, half * (D / 32) + d, lane), st.q[0][d], s[half][0]);
+            weigh<T, Q8, D, 1>(a, st, s, first, nullptr, lane, p);
+            pack_weights<T, Q8>(p[0], w[0]);
+            if constexpr (kSumByProduct<T, Q8>) add_sums(st, w);
+            if (bad) {
+              values_bad<T, D, 1>(st, first, p, vals, lane);
+            } else {
+#pragma unroll
+              for (int f = 0; f < D / 16; f++) st.o[0][f] = mma(M{}, load_frag<T>(vals, f, lane), w[0][0], st.o[0][f]);
             }
-          weigh<T, Q8, D, 1>(a, st, s, first, reinterpret_cast<const float*>(tail), lane, p);
-          pack_weights<T, Q8>(p[0], w);
-#pragma unroll
-          for (int i = 0; i < NU; i++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              const typename frag<M>::type x = decode<M>(vc[i][e * 2], vc[i][e * 2 + 1]);
-#pragma unroll
-              for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[0][i * 2 + e] = mma(M{}, x, w[h], st.o[0][i * 2 + e]);
-            }
-        } else {
-          const uint32_t bad = *reinterpret_cast<const uint32_t*>(tail);
-#pragma unroll
-          for (int half = 0; half < 2; half++)
-#pragma unroll
-            for (int d = 0; d < D / 32; d++)
-              s[half][0] = mma(T{}, load_frag<T>(at, half * (D / 32) + d, lane), st.q[0][d], s[half][0]);
-          weigh<T, Q8, D, 1>(a, st, s, first, nullptr, lane, p);
-          pack_weights<T, Q8>(p[0], w);
-#pragma unroll
-          for (int f = 0; f < D / 16; f++) {
-            typename frag<T>::type x = load_frag<T>(vals, f, lane);
-            if (bad) drop_bad<T>(x, bad, lane);
-            st.o[0][f] = mma(M{}, x, w[0], st.o[0][f]);
           }
-          if (bad) add_bad(st, p, first, bad, vals, lane);
         }
       }
-      end_job(a, list, st, job, sh.head, pair0, 0, worker, n == c1 - c0, skip > 0, lane);
+      if (pt.work) end_job(a, list, st, job, sh.head, pair0, 0, worker, pt.whole, pt.later, lane);
       sh.left -= n;
       sh.at += n;
     }
@@ -515,33 +593,32 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
 // in LDS, two stages.  Types go there by direct copies; codes through registers, and lie there
 // as the type that multiplies them.
 template <typename T, bool Q8, int D, int QT>
-__global__ __launch_bounds__(256, __is_same(T, float) && D == 256 ? 1 : 2) void k_attn_wide(sg_attn_shared_args a,
+__global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void k_attn_wide(sg_attn_shared_args a,
                                                                                           sg_attn_list list) {
   typedef typename weight<T, Q8>::type M;
   constexpr int ES = sizeof(T), KB = kTile * D * ES, STAGE = 2 * KB + (Q8 ? kTail : 0);
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t worker = spread(blockIdx.x, gridDim.x);
-  share sh = first_share<D, QT>(list, worker, a.kv_heads, lane);
+  share sh = first_share(list, worker, a.kv_heads, lane);
   state<T, Q8, D, QT> st;
   while (sh.left > 0) {
-    const sg_attn_job job = list.jobs[sh.job];
-    const int64_t c0 = list.cum[sh.job], c1 = list.cum[sh.job + 1];
-    const int64_t skip = sh.at - c0, n = min(c1 - sh.at, sh.left);
+    const int64_t c0 = list.cum[sh.job], c1 = list.cum[sh.job + 1], n = min(c1 - sh.at, sh.left);
     if (n > 0) {
+      const sg_attn_job job = list.jobs[sh.job];
+      const part pt = part_of(list, job, sh.at, sh.left, c0, c1);
       const int in_job = wave * QT * 16, pair0 = job.tile * (64 * QT) + in_job;
-      const int64_t tile = job.slot_tile + skip;
-      int first = (int)(tile * kTile - job.key0);
-      const char* at = a.cache + (int64_t)sh.head * a.head_bytes + tile * a.tile_bytes;
       constexpr int NU = Q8 ? D / 16 / 4 : 2 * KB / 1024 / 4;  // kilobytes of a tile for each wave
       u32x4_t codes[Q8 ? NU : 1];
       float tail_of = 0.0f;
+      uint32_t bad_next = 0;
       auto fetch = [&](const char* from, int stage) {
         if constexpr (Q8) {
 #pragma unroll
           for (int i = 0; i < NU; i++) codes[i] = *reinterpret_cast<const u32x4_t*>(from + (wave * NU + i) * 1024 + lane * 16);
           if (wave == 0) tail_of = *reinterpret_cast<const float*>(from + a.tile_bytes - kTail + lane * 4);
         } else {
+          bad_next = *reinterpret_cast<const uint32_t*>(from + a.tile_bytes - kTail);
           const i32x4_t rsrc = sg_raw_rsrc(from);
 #pragma unroll
           for (int i = 0; i < NU; i++) {
@@ -564,59 +641,60 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D == 256 ? 1 : 2) void 
           if (wave == 0) *reinterpret_cast<float*>(to + 2 * KB + lane * 4) = tail_of;
         }
       };
-      __syncthreads();  // the last job's stages have been read
-      fetch(at, 0);
-      begin_job(a, st, job, sh.head, pair0, lane);
-      put(0);
-      for (int64_t u = 0; u < n; u++, first += kTile) {
-        const int stage = (int)(u & 1);
-        if constexpr (!Q8) sg_wait_vmcnt<0>();
-        __syncthreads();
-        const char* here = at;
-        at += a.tile_bytes;
-        if (u + 1 < n) fetch(at, stage ^ 1);
-        const char* keys = lds + stage * STAGE;
-        const char* vals = keys + KB;
-        f32x4_t s[2][QT] = {};
-        float p[QT][8];
+      if (pt.work) begin_job(a, st, job, sh.head, pair0, lane);
+#pragma unroll 1
+      for (int seg = 0; seg < 2; seg++) {
+        const int64_t t0 = seg ? job.tiles[0] : 0, u0 = max(pt.from, t0), u1 = min(pt.to, t0 + (seg ? job.tiles[1] : job.tiles[0]));
+        if (u0 >= u1) continue;
+        const int64_t tile = (seg ? job.slot_tile[1] : job.slot_tile[0]) + (u0 - t0);
+        int first = (int)(tile * kTile - (seg ? job.key0[1] : job.key0[0]));
+        const char* at = a.cache + (int64_t)sh.head * a.head_bytes + tile * a.tile_bytes;
+        __syncthreads();  // the stages have been read
+        fetch(at, 0);
+        begin_keys(a, st, job, pair0, job.kind == kOwnKeys || seg, lane);
+        put(0);
+        for (int64_t u = u0; u < u1; u++, first += kTile) {
+          const int stage = (int)((u - u0) & 1);
+          if constexpr (!Q8) sg_wait_vmcnt<0>();
+          __syncthreads();
+          // (Taken here, where nothing is in flight: waiting for it later would wait for the next tile.)
+          uint32_t bad = __builtin_amdgcn_readfirstlane(bad_next);
+          asm volatile("" : "+s"(bad));
+          at += a.tile_bytes;
+          if (u + 1 < u1) fetch(at, stage ^ 1);
+          const char* keys = lds + stage * STAGE;
+          const char* vals = keys + KB;
+          f32x4_t s[2][QT] = {};
+          float p[QT][8];
 #pragma unroll
-        for (int half = 0; half < 2; half++)
+          for (int half = 0; half < 2; half++)
 #pragma unroll
-          for (int d = 0; d < D / 32; d++) {
-            const typename frag<T>::type x = load_frag<T>(keys, half * (D / 32) + d, lane);
+            for (int d = 0; d < D / 32; d++) {
+              const typename frag<T>::type x = load_frag<T>(keys, half * (D / 32) + d, lane);
 #pragma unroll
-            for (int t = 0; t < QT; t++) s[half][t] = mma(T{}, x, st.q[t][d], s[half][t]);
-          }
-        weigh<T, Q8, D, QT>(a, st, s, first, Q8 ? reinterpret_cast<const float*>(keys + 2 * KB) : nullptr, lane, p);
-        typename frag<M>::type w[QT][weight<T, Q8>::parts];
-#pragma unroll
-        for (int t = 0; t < QT; t++) pack_weights<T, Q8>(p[t], w[t]);
-        uint32_t bad = 0;
-        if constexpr (!Q8) {
-          bad = *reinterpret_cast<const uint32_t*>(here + a.tile_bytes - kTail);
-          if (bad) {  // (alike for the workgroup)
-            char* own = lds + stage * STAGE + KB;
-            for (int f = wave; f < D / 16; f += 4) {
-              typename frag<T>::type x = load_frag<T>(own, f, lane);
-              drop_bad<T>(x, bad, lane);
-              store_frag<T>(own, f, lane, x);
+              for (int t = 0; t < QT; t++) s[half][t] = mma(T{}, x, st.q[t][d], s[half][t]);
             }
-            __syncthreads();
+          weigh<T, Q8, D, QT>(a, st, s, first, Q8 ? reinterpret_cast<const float*>(keys + 2 * KB) : nullptr, lane, p);
+          typename frag<M>::type w[QT][weight<T, Q8>::parts];
+#pragma unroll
+          for (int t = 0; t < QT; t++) pack_weights<T, Q8>(p[t], w[t]);
+          if constexpr (kSumByProduct<T, Q8>) add_sums(st, w);
+          if constexpr (!Q8)
+            if (bad) values_bad<T, D, QT>(st, first, p, vals, lane);
+          if (Q8 || !bad) {
+#pragma unroll
+            for (int f = 0; f < D / 16; f++) {
+              const typename frag<M>::type x = load_frag<M>(vals, f, lane);
+#pragma unroll
+              for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[t][f] = mma(M{}, x, w[t][h], st.o[t][f]);
+            }
           }
+          if (u + 1 < u1) put(stage ^ 1);
         }
-#pragma unroll
-        for (int f = 0; f < D / 16; f++) {
-          const typename frag<M>::type x = load_frag<M>(vals, f, lane);
-#pragma unroll
-          for (int t = 0; t < QT; t++)
-#pragma unroll
-            for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[t][f] = mma(M{}, x, w[t][h], st.o[t][f]);
-        }
-        if constexpr (!Q8)
-          if (bad) add_bad(st, p, first, bad, here + KB, lane);
-        if (u + 1 < n) put(stage ^ 1);
       }
-      end_job(a, list, st, job, sh.head, pair0, in_job, worker, n == c1 - c0, skip > 0, lane);
+      if (pt.work) end_job(a, list, st, job, sh.head, pair0, in_job, worker, pt.whole, pt.later, lane);
       sh.left -= n;
       sh.at += n;
     }

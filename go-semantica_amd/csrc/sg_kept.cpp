@@ -192,8 +192,10 @@ int sg_attention_shared(sg_ctx* ctx, void* out, int64_t ldo, const void* q, int6
   a.ldq = ldq;
   a.head_bytes = cache->head_bytes;
   a.tile_bytes = cache->tile_bytes;
-  a.scale = cap != 0.0f ? scale / cap : scale * kLog2e;
+  a.scale = cap != 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
   a.cap = cap * kLog2e;
+  a.to_cap = cap != 0.0f ? std::fabs(scale) / cap : 0.0f;
+  a.negative = scale < 0.0f;
   a.rows = rows;
   a.heads = n_heads;
   a.kv_heads = cache->heads;

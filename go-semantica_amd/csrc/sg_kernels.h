@@ -115,14 +115,17 @@ struct sg_attn_shared_args {
   const int4* where;  // [rows]: first job and first row of its prefix's group, of its sequence's
   float* part_o;      // [2 rows * heads, then pieces][D]
   float2* part_ml;
-  float scale, cap;   // in powers of two
+  float scale;        // of scores, in powers of two, not negative (1 / log2 e under a cap: 1)
+  float cap, to_cap;  // cap * log2 e (0: none), and what a product is multiplied by before tanh
+  int negative;       // queries are negated
   int rows, heads, kv_heads, group, hd;
 };
-// Consecutive pairs of a group over a range of tiles.
+// Consecutive pairs of a group over one or two ranges of tiles: a prefix's, a sequence's own
+// (alone in the first place), or a sequence's prefix and its own, which is all its rows see.
+constexpr int kPrefixKeys = 0, kOwnKeys = 1, kAllKeys = 2;
 struct sg_attn_job {
-  int row0, rows, tile;  // the group's rows; which M pairs of them
-  int key0, slot_tile;   // the slot of the first key; the first tile with a visible one
-  int own;               // 0: a prefix, 1: a sequence's own keys
+  int row0, rows, tile, kind;           // the group's rows; which M pairs of them
+  int key0[2], slot_tile[2], tiles[2];  // the slot of the first key; the first tile with a visible one
 };
 struct sg_attn_plan {
   int64_t units, per;  // units of a head, of a worker
@@ -134,7 +137,8 @@ struct sg_attn_list {
   sg_attn_job* jobs;
   int64_t piece0;  // first row of the list's pieces in part_o
   int m, piece_pairs;  // pairs of a job, of a piece of one
-  int blocks, workers, wide, cap, min_units;  // cap: jobs that fit
+  int blocks, workers, wide;
+  int cap, min_units, job_cost;  // jobs that fit; units of a worker at least; what a job costs beside its tiles
 };
 // What the plan is made from (device arrays as sg_shared_keys names them).
 struct sg_attn_batch {
@@ -147,7 +151,7 @@ struct sg_attn_batch {
   int32_t* seq_jobs;     // [n_seq + 1]
   int32_t* prefix_jobs;  // [n_prefix + 1]
   int64_t slots;
-  int n_seq, n_prefix, causal, window;
+  int n_seq, n_prefix, causal, window, all_keys;
 };
 
 // One sg_matmul_q4 call (k_q4.hip): packed weights, strides in elements.

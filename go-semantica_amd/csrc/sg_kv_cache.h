@@ -51,4 +51,17 @@ __device__ __forceinline__ int value_at(int D, int key, int dim) {
   return kTile * D * ES + place<ES>(dim >> 4, (dim & 15) + ((key >> 2) & 3) * 16, (key >> 4) * 4 + (key & 3));
 }
 
+// The largest i in [0, n) with at[i] <= x, for ascending at with at[0] <= x; called by a whole
+// wave with a uniform x: 64 candidates a step.
+__device__ __forceinline__ int last_at_most(const int64_t* at, int n, int64_t x, int lane) {
+  int lo = 0, len = n;
+  while (len > 1) {
+    const int step = (len + 63) >> 6, j = lane * step;
+    const int c = __popcll(__ballot(j < len && at[lo + j] <= x));
+    lo += (c - 1) * step;
+    len = min(step, len - (c - 1) * step);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
 }  // namespace sgc

@@ -386,6 +386,19 @@ def test_shared_few_behind_many_prefixes(gpu_ctx, dtype, bits):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_shared_many_rows(gpu_ctx, dtype, bits, hd):
+    """More (row, head) than are joined one by one: sequences that fill jobs of their own, whole
+    and cut; hundreds of short ones behind shared prefixes, few and many pairs of each."""
+    check_shared(gpu_ctx, 1, dtype, bits, 8, 2, hd, [300, 170, 0, 200], [340, 170, 9, 230], [333, 90], first=1, behind=2)
+    check_shared(gpu_ctx, 2, dtype, bits, 8, 2, hd, [2] * 170, [2 + i % 40 for i in range(170)], [300, 61, 0])
+    check_shared(gpu_ctx, 3, dtype, bits, 8, 2, hd, [1] * 300, [i % 70 for i in range(300)], window=33)
+    check_shared(gpu_ctx, 4, dtype, bits, 4, 2, hd, [30] * 20, [60] * 20, [130], causal=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
 def test_shared_long(gpu_ctx, dtype, bits):
     """A prefix split over the GPU for one query, and for a few; running maxima that rise late."""
     check_shared(gpu_ctx, 2, dtype, bits, 8, 2, 128, [1], [3], [20011], by=3.0)

@@ -303,8 +303,8 @@ __device__ __forceinline__ void add_sums(state<T, Q8, D, QT>& st, const s16x8_t 
 }
 
 // Values that are not finite, in a tile that may be hidden in part: a zero weight times one is a
-// NaN.  So they are zeros in the product, and which pairs see an infinity or a NaN of a dim is
-// counted by products of ones: exact, and no business of the weights'.
+// NaN.  So they are zeros in the product (clean), and which pairs see an infinity or a NaN of a
+// dim is counted by products of ones behind it (mark_bad): exact, and no business of the weights'.
 template <typename M>
 __device__ __forceinline__ void set_elem(typename frag<M>::type& x, int j, float v) {
   if constexpr (__is_same(M, float)) x.v[j >> 2][j & 3] = v;
@@ -315,28 +315,33 @@ __device__ __forceinline__ float get_elem(const typename frag<M>::type& x, int j
   if constexpr (__is_same(M, float)) return x.v[j >> 2][j & 3];
   else return elem<M>::to(__builtin_bit_cast(M, (short)x[j]));
 }
-template <typename T, int D, int QT>
-__device__ __forceinline__ void values_bad(state<T, false, D, QT>& st, int first, const float (&p)[QT][8], const char* vals,
-                                           int lane) {
-  typedef typename frag<T>::type X;
-  X sees[QT], w[QT][1];
+template <typename T>
+__device__ __forceinline__ typename frag<T>::type clean(typename frag<T>::type x) {
 #pragma unroll
-  for (int t = 0; t < QT; t++) {
-    pack_weights<T, false>(p[t], w[t]);
+  for (int j = 0; j < 8; j++) {
+    const float v = get_elem<T>(x, j);
+    set_elem<T>(x, j, fabsf(v) < INFINITY ? v : 0.0f);
+  }
+  return x;
+}
+template <typename T, bool Q8, int D, int QT>
+__device__ __forceinline__ void mark_bad(state<T, Q8, D, QT>& st, int first, const char* vals, int lane) {
+  typedef typename frag<T>::type X;
+  X sees[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++)
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const int key = first + (j >> 2) * 16 + (lane >> 4) * 4 + (j & 3);
       set_elem<T>(sees[t], j, key >= st.lo[t] && key < st.hi[t] ? 1.0f : 0.0f);
     }
-  }
 #pragma unroll
   for (int f = 0; f < D / 16; f++) {
     const X x = load_frag<T>(vals, f, lane);
-    X one[3], clean;
+    X one[3];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const float v = get_elem<T>(x, j);
-      set_elem<T>(clean, j, fabsf(v) < INFINITY ? v : 0.0f);
       set_elem<T>(one[0], j, v == INFINITY ? 1.0f : 0.0f);
       set_elem<T>(one[1], j, v == -INFINITY ? 1.0f : 0.0f);
       set_elem<T>(one[2], j, v != v ? 1.0f : 0.0f);
@@ -346,14 +351,13 @@ __device__ __forceinline__ void values_bad(state<T, false, D, QT>& st, int first
       const f32x4_t none = {0, 0, 0, 0};
       const f32x4_t up = mma(T{}, one[0], sees[t], none), down = mma(T{}, one[1], sees[t], none),
                     nan = mma(T{}, one[2], sees[t], none);
-      f32x4_t o = mma(T{}, clean, w[t][0], st.o[t][f]);
+      f32x4_t add;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        o[i] = up[i] != 0.0f ? o[i] + INFINITY : o[i];
-        o[i] = down[i] != 0.0f ? o[i] - INFINITY : o[i];
-        o[i] = nan[i] != 0.0f ? __builtin_nanf("") : o[i];
+        const float a = (up[i] != 0.0f ? INFINITY : 0.0f) - (down[i] != 0.0f ? INFINITY : 0.0f);
+        add[i] = nan[i] != 0.0f ? __builtin_nanf("") : a;
       }
-      st.o[t][f] = o;
+      st.o[t][f] += add;
     }
     asm volatile("" ::: "memory");  // (one fragment at a time: registers)
   }
@@ -568,12 +572,13 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
             weigh<T, Q8, D, 1>(a, st, s, first, nullptr, lane, p);
             pack_weights<T, Q8>(p[0], w[0]);
             if constexpr (kSumByProduct<T, Q8>) add_sums(st, w);
-            if (bad) {
-              values_bad<T, D, 1>(st, first, p, vals, lane);
-            } else {
 #pragma unroll
-              for (int f = 0; f < D / 16; f++) st.o[0][f] = mma(M{}, load_frag<T>(vals, f, lane), w[0][0], st.o[0][f]);
+            for (int f = 0; f < D / 16; f++) {
+              typename frag<T>::type x = load_frag<T>(vals, f, lane);
+              if (bad) x = clean<T>(x);
+              st.o[0][f] = mma(M{}, x, w[0][0], st.o[0][f]);
             }
+            if (bad) mark_bad(st, first, vals, lane);
           }
         }
       }
@@ -679,18 +684,23 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void 
 #pragma unroll
           for (int t = 0; t < QT; t++) pack_weights<T, Q8>(p[t], w[t]);
           if constexpr (kSumByProduct<T, Q8>) add_sums(st, w);
-          if constexpr (!Q8)
-            if (bad) values_bad<T, D, QT>(st, first, p, vals, lane);
-          if (Q8 || !bad) {
-#pragma unroll
-            for (int f = 0; f < D / 16; f++) {
-              const typename frag<M>::type x = load_frag<M>(vals, f, lane);
-#pragma unroll
-              for (int t = 0; t < QT; t++)
-#pragma unroll
-                for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[t][f] = mma(M{}, x, w[t][h], st.o[t][f]);
+          if constexpr (!Q8) {
+            if (bad) {  // (alike for the workgroup)
+              char* own = lds + stage * STAGE + KB;
+              for (int f = wave; f < D / 16; f += 4) store_frag<T>(own, f, lane, clean<T>(load_frag<T>(own, f, lane)));
+              __syncthreads();
             }
           }
+#pragma unroll
+          for (int f = 0; f < D / 16; f++) {
+            const typename frag<M>::type x = load_frag<M>(vals, f, lane);
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+              for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[t][f] = mma(M{}, x, w[t][h], st.o[t][f]);
+          }
+          if constexpr (!Q8)
+            if (bad) mark_bad(st, first, at - a.tile_bytes + KB, lane);
           if (u + 1 < u1) put(stage ^ 1);
         }
       }

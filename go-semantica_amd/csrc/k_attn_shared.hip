@@ -213,9 +213,22 @@ struct joined {
     o = o * by + oo * now;
     m = top;
   }
-  __device__ __forceinline__ void add(const sg_attn_shared_args& a, int64_t at, int lane) {
-    const float2 ml = a.part_ml[at];
-    add(ml.x, ml.y, *reinterpret_cast<const vec*>(a.part_o + at * D + lane * V));
+  // The pieces at `at` of workers w0, w0 + step, ... up to w1: four loads at a time.
+  template <typename F>
+  __device__ __forceinline__ void add(const sg_attn_shared_args& a, int64_t w0, int64_t w1, int step, int lane, F at) {
+    for (int64_t w = w0; w <= w1; w += 4 * step) {
+      float2 ml[4];
+      vec x[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int64_t p = at(min(w + i * step, w1));
+        ml[i] = a.part_ml[p];
+        x[i] = *reinterpret_cast<const vec*>(a.part_o + p * D + lane * V);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (w + i * step <= w1) add(ml[i].x, ml[i].y, x[i]);
+    }
   }
   // A query that sees nothing, or nothing but scores of -infinity, has zeros.
   template <typename T>
@@ -256,8 +269,9 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_attn_join(sg_attn_s
     if (all_keys && (!h.any || h.first == h.last)) return;  // written
     if (!h.any) continue;
     const int in_job = (int)(pair % list.m);
-    for (int64_t w = h.first + (NW == 1 ? 0 : wave); w <= h.last; w += NW)
-      x.add(a, h.first == h.last ? (int64_t)(own ? a.rows : 0) * a.heads + i : piece_of(list, w, w == h.first, in_job), lane);
+    x.add(a, h.first + (NW == 1 ? 0 : wave), h.last, NW, lane, [&](int64_t w) {
+      return h.first == h.last ? (int64_t)(own ? a.rows : 0) * a.heads + i : piece_of(list, w, w == h.first, in_job);
+    });
   }
   if constexpr (NW > 1) {
     __shared__ float ms[NW], ls[NW];
@@ -292,7 +306,7 @@ __global__ __launch_bounds__(256) void k_attn_join_split(sg_attn_shared_args a, 
     if (pair >= (int64_t)jb.rows * a.group) return;
     const int r = (int)(pair / a.group);
     joined<D> x;
-    for (int64_t w = h.first; w <= h.last; w++) x.add(a, piece_of(list, w, w == h.first, in_job), lane);
+    x.add(a, h.first, h.last, 1, lane, [&](int64_t w) { return piece_of(list, w, w == h.first, in_job); });
     x.template put<T>(a, jb.row0 + r, kv * a.group + (int)(pair - (int64_t)r * a.group), lane);
   }
 }
@@ -301,8 +315,7 @@ __global__ __launch_bounds__(256) void k_attn_join_split(sg_attn_shared_args a, 
 // themselves.
 constexpr int kNarrowPairs = 32;
 constexpr int kFullJobs = 4;
-constexpr int kJoinWaves = 16;
-constexpr int64_t kJoinFew = 2048;  // (row, head) up to here: so many waves each
+constexpr int64_t kJoinFew = 256, kJoinSome = 4096;  // (row, head) up to here: 16 waves each, four
 
 struct layout {
   size_t plan, cum[2], jobs[2], seq_jobs, prefix_jobs, seen, where, ml, o, total;
@@ -350,8 +363,8 @@ layout lay_out(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, i
 template <typename T, int D>
 hipError_t join(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, int all_keys, hipStream_t s) {
   const int64_t n = (int64_t)a.rows * a.heads;
-  if (n <= kJoinFew)
-    return sgp::run_kernel(k_attn_join<T, D, kJoinWaves>, dim3(n), dim3(64 * kJoinWaves), 0, s, a, la, lb, all_keys);
+  if (n <= kJoinFew) return sgp::run_kernel(k_attn_join<T, D, 16>, dim3(n), dim3(64 * 16), 0, s, a, la, lb, all_keys);
+  if (n <= kJoinSome) return sgp::run_kernel(k_attn_join<T, D, 4>, dim3(n), dim3(64 * 4), 0, s, a, la, lb, all_keys);
   if (all_keys) return sgp::run_kernel(k_attn_join_split<T, D>, dim3(lb.workers, lb.m / 16), dim3(256), 0, s, a, lb);
   return sgp::run_kernel(k_attn_join<T, D, 1>, dim3((n + 3) / 4), dim3(256), 0, s, a, la, lb, 0);
 }
@@ -395,8 +408,8 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
     l.blocks = i ? l.workers : l.workers / 4;
     l.wide = i;
     l.cap = y.cap;
-    l.min_units = i ? 4 : 2;
-    l.job_cost = i ? 4 : 2;
+    l.min_units = i ? 12 : dtype == SG_F32 && D == 256 ? 1 : 2;
+    l.job_cost = i ? 4 : dtype == SG_F32 && D == 256 ? 1 : 2;
   }
   const int64_t pairs = (int64_t)a.rows * a.group;
   // A job for each M pairs of a sequence, over prefix and own keys in one go, where no prefix is

@@ -38,9 +38,6 @@ using sgp::elem;
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.44269504088896340736f;
-// A pair's maximum is raised (its sums rescaled) when a score passes it by so many powers of
-// two, so most tiles rescale nothing; weights stay below 2^8.
-constexpr float kSlack = 8.0f;
 
 // Eight elements in a row of a matrix core operand.
 template <typename T>
@@ -166,10 +163,14 @@ struct weight<bf16_t, true> {
   typedef bf16_t type;
   static constexpr int parts = 1;
 };
-// fp16 weights are multiplied by 2^6, so that they keep their bits down to 2^-20 (and with
-// the slack stay below 2^14); sums and outputs alike, so it leaves by itself.
+// fp16 weights are multiplied by 2^6, so that they keep their bits down to 2^-20; sums and outputs
+// alike, so it leaves by itself.
 template <typename T, bool Q8>
 constexpr float kShift = __is_same(T, _Float16) && !Q8 ? 6.0f : 0.0f;
+// A tile's sum of weights from which on a pair's maximum is raised (and its sums rescaled): far
+// above 32 weights of 1, within the weights' type.
+template <typename T, bool Q8>
+constexpr float kMost = __is_same(T, _Float16) && !Q8 ? 0x1p14f : 0x1p20f;
 
 // Sums of weights by the matrix core: 16-bit types whose weights are multiplied as they are.
 template <typename T, bool Q8>
@@ -181,7 +182,7 @@ struct state {
   typename frag<T>::type q[QT][D / 32];
   f32x4_t o[QT][D / 16];
   float m[QT], l[QT];
-  f32x4_t sum[QT];  // in place of l where the matrix core adds up: each of the four is the sum
+  float base[QT], most[QT];  // what scores are taken against: m, shifted; the sum that raises it
   int lo[QT], hi[QT];  // visible keys of the lane's pairs, counted from the job's first
   int all_lo, all_hi;  // keys that every pair of the wave sees
 };
@@ -215,12 +216,15 @@ __device__ __forceinline__ void pack_weights(const float* p, typename frag<typen
 // A tile's products become weights.  first: the place of the tile's first slot among the keys
 // that lo and hi count (negative where the tile begins before them); tail: the tile's, in LDS or
 // memory.  Weights are 2^(s c - m) of scores s as they come: c > 0 holds the scale (queries are
-// negated for a negative one), so a maximum is taken before it and one fma does the rest.
+// negated for a negative one), so one fma does the rest.  m need not be the maximum: it is that of
+// the tile that a pair saw first, and raised when a tile's weights add up to kMost or more, which
+// the sum tells that is taken anyway.
 template <typename T, bool Q8, int D, int QT>
 __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8, D, QT>& st, f32x4_t (&s)[2][QT], int first,
-                                      const float* tail, int lane, float (&p)[QT][8]) {
+                                      const float* tail, int lane,
+                                      typename frag<typename weight<T, Q8>::type>::type (&w)[QT][weight<T, Q8>::parts]) {
   const int g = lane >> 4;
-  float vs[8];
+  float vs[8], p[QT][8];
   if constexpr (Q8) {
     f32x4_t ks[2], v[2];
 #pragma unroll
@@ -258,48 +262,46 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
   }
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    float top = fmaxf(fmaxf(fmaxf(p[t][0], p[t][1]), fmaxf(p[t][2], p[t][3])),
-                      fmaxf(fmaxf(p[t][4], p[t][5]), fmaxf(p[t][6], p[t][7]))) * a.scale;
-    if (__ballot(top > st.m[t] + kSlack)) {
+    float e[8], sum;
+    auto form = [&] {
+#pragma unroll
+      for (int j = 0; j < 8; j++) e[j] = exp2_of(__builtin_fmaf(p[t][j], a.scale, -st.base[t]));
+      if constexpr (kSumByProduct<T, Q8>) {
+        // The packed weights' sum by a product with ones: a sixteenth of the second product's work
+        // in place of eight additions a lane, and the sum of the weights as they are multiplied.
+        pack_weights<T, Q8>(e, w[t]);
+        const short one = __builtin_bit_cast(short, elem<T>::from(1.0f));
+        const s16x8_t ones = {one, one, one, one, one, one, one, one};
+        sum = mma(T{}, ones, w[t][0], f32x4_t{0, 0, 0, 0})[0];
+      } else {
+        sum = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+      }
+    };
+    form();
+    if (__ballot(sum > st.most[t])) {
+      float top = fmaxf(fmaxf(fmaxf(p[t][0], p[t][1]), fmaxf(p[t][2], p[t][3])),
+                        fmaxf(fmaxf(p[t][4], p[t][5]), fmaxf(p[t][6], p[t][7]))) * a.scale;
       top = fmaxf(pair_max(top), st.m[t]);
       const float by = top > st.m[t] ? exp2_of(st.m[t] - top) : 1.0f;  // (m may be -infinity: 0)
       st.m[t] = top;
-      if constexpr (kSumByProduct<T, Q8>) st.sum[t] *= by;
-      else st.l[t] *= by;
+      st.base[t] = (top == -INFINITY ? 0.0f : top) - kShift<T, Q8>;
+      st.most[t] = top == -INFINITY ? -1.0f : kMost<T, Q8>;
+      st.l[t] *= by;
 #pragma unroll
       for (int f = 0; f < D / 16; f++) st.o[t][f] *= by;
+      form();
     }
-    const float m = (st.m[t] == -INFINITY ? 0.0f : st.m[t]) - kShift<T, Q8>;
-#pragma unroll
-    for (int j = 0; j < 8; j++) p[t][j] = exp2_of(__builtin_fmaf(p[t][j], a.scale, -m));
-    if constexpr (!kSumByProduct<T, Q8>) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; j++) sum += p[t][j];
-      st.l[t] += sum;
-    }
+    st.l[t] += sum;
     if constexpr (Q8) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) p[t][j] *= vs[j];
+      for (int j = 0; j < 8; j++) e[j] *= vs[j];
       if (part) {  // a hidden key's scale may be NaN
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const int key = first + (j >> 2) * 16 + g * 4 + (j & 3);
-          p[t][j] = key >= st.lo[t] && key < st.hi[t] ? p[t][j] : 0.0f;
-        }
+        for (int j = 0; j < 8; j++) e[j] = p[t][j] == -INFINITY ? 0.0f : e[j];
       }
     }
+    if constexpr (!kSumByProduct<T, Q8>) pack_weights<T, Q8>(e, w[t]);
   }
-}
-
-// The packed weights' sums, by a product with ones: a sixteenth of the second product's work in
-// place of eight additions a lane, and the sum of the weights as they are multiplied.
-template <typename T, bool Q8, int D, int QT>
-__device__ __forceinline__ void add_sums(state<T, Q8, D, QT>& st, const s16x8_t (&w)[QT][1]) {
-  const short one = __builtin_bit_cast(short, elem<T>::from(1.0f));
-  const s16x8_t ones = {one, one, one, one, one, one, one, one};
-#pragma unroll
-  for (int t = 0; t < QT; t++) st.sum[t] = mma(T{}, ones, w[t][0], st.sum[t]);
 }
 
 // Values that are not finite, in a tile that may be hidden in part: a zero weight times one is a
@@ -420,7 +422,8 @@ __device__ __forceinline__ void begin_job(const sg_attn_shared_args& a, state<T,
     }
     st.m[t] = -INFINITY;
     st.l[t] = 0.0f;
-    st.sum[t] = f32x4_t{0, 0, 0, 0};
+    st.base[t] = -kShift<T, Q8>;
+    st.most[t] = -1.0f;  // (any sum)
 #pragma unroll
     for (int f = 0; f < D / 16; f++) st.o[t][f] = f32x4_t{0, 0, 0, 0};
   }
@@ -462,7 +465,7 @@ __device__ __forceinline__ void end_job(const sg_attn_shared_args& a, const sg_a
   const int g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    const float l = kSumByProduct<T, Q8> ? st.sum[t][0] : pair_sum(st.l[t]);
+    const float l = kSumByProduct<T, Q8> ? st.l[t] : pair_sum(st.l[t]);
     const int pair = pair0 + t * 16 + (lane & 15);
     if (pair >= job.rows * a.group) continue;
     const int r = pair / a.group, h = head * a.group + pair - r * a.group;
@@ -532,11 +535,10 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
         const int64_t tile = (seg ? job.slot_tile[1] : job.slot_tile[0]) + (u0 - t0);
         int first = (int)(tile * kTile - (seg ? job.key0[1] : job.key0[0]));
         const char* at = a.cache + (int64_t)sh.head * a.head_bytes + tile * a.tile_bytes;
-        for (int64_t u = u0; u < u1; u++, first += kTile, at += a.tile_bytes) {
+        for (int left = (int)(u1 - u0); left > 0; left--, first += kTile, at += a.tile_bytes) {
           const char* vals = at + (int64_t)kTile * D * sizeof(typename sgc::kept<T, Q8>::type);
           const char* tail = at + a.tile_bytes - kTail;
           f32x4_t s[2][1] = {};
-          float p[1][8];
           typename frag<M>::type w[1][weight<T, Q8>::parts];
           if constexpr (Q8) {
             constexpr int NU = D / 32;  // kilobytes of the keys, and of the values
@@ -552,8 +554,7 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
                 const int f = i * 2 + e, half = f / (D / 32), d = f % (D / 32);
                 s[half][0] = mma(T{}, decode<T>(kc[i][e * 2], kc[i][e * 2 + 1]), st.q[0][d], s[half][0]);
               }
-            weigh<T, Q8, D, 1>(a, st, s, first, reinterpret_cast<const float*>(tail), lane, p);
-            pack_weights<T, Q8>(p[0], w[0]);
+            weigh<T, Q8, D, 1>(a, st, s, first, reinterpret_cast<const float*>(tail), lane, w);
 #pragma unroll
             for (int i = 0; i < NU; i++)
 #pragma unroll
@@ -569,9 +570,7 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
 #pragma unroll
               for (int d = 0; d < D / 32; d++)
                 s[half][0] = mma(T{}, load_frag<T>(at, half * (D / 32) + d, lane), st.q[0][d], s[half][0]);
-            weigh<T, Q8, D, 1>(a, st, s, first, nullptr, lane, p);
-            pack_weights<T, Q8>(p[0], w[0]);
-            if constexpr (kSumByProduct<T, Q8>) add_sums(st, w);
+            weigh<T, Q8, D, 1>(a, st, s, first, nullptr, lane, w);
 #pragma unroll
             for (int f = 0; f < D / 16; f++) {
               typename frag<T>::type x = load_frag<T>(vals, f, lane);
@@ -596,12 +595,25 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
 
 // Many pairs: a workgroup is a worker, its four waves have QT * 16 pairs each and share the tiles
 // in LDS, two stages.  Types go there by direct copies; codes through registers, and lie there
-// as the type that multiplies them.
+// as the type that multiplies them.  16-bit types of up to 128 dims copy codes to LDS as they
+// are first, kRing tiles of them, each wave its own quarter (and the scales): a tile of codes is
+// 8 KB, and one or two a CU in flight reach half of the memory's rate.
+constexpr int kRing = 4;
+template <typename T, bool Q8, int D>
+struct wide_lds {
+  static constexpr int KB = kTile * D * (int)sizeof(T);  // keys of a tile
+  static constexpr bool ring = Q8 && sizeof(T) == 2 && D <= 128;
+  static constexpr int stage = 2 * KB + (Q8 && !ring ? kTail : 0);
+  static constexpr int quarter = D / 64 * 1024 + kTail;  // a wave's part of a tile of codes
+  static constexpr int bytes = 2 * stage + (ring ? kRing * 4 * quarter : 0);
+};
 template <typename T, bool Q8, int D, int QT>
 __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void k_attn_wide(sg_attn_shared_args a,
                                                                                           sg_attn_list list) {
   typedef typename weight<T, Q8>::type M;
-  constexpr int ES = sizeof(T), KB = kTile * D * ES, STAGE = 2 * KB + (Q8 ? kTail : 0);
+  typedef wide_lds<T, Q8, D> L;
+  constexpr int KB = L::KB, STAGE = L::stage;
+  constexpr bool RING = L::ring;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t worker = spread(blockIdx.x, gridDim.x);
@@ -617,8 +629,15 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void 
       u32x4_t codes[Q8 ? NU : 1];
       float tail_of = 0.0f;
       uint32_t bad_next = 0;
-      auto fetch = [&](const char* from, int stage) {
-        if constexpr (Q8) {
+      const int mine = 2 * STAGE + wave * L::quarter;  // the wave's part of a ring slot
+      auto ring_at = [&](int u) { return mine + u % kRing * (4 * L::quarter); };
+      auto fetch = [&](const char* from, int stage, int u) {
+        if constexpr (RING) {
+          const i32x4_t rsrc = sg_raw_rsrc(from);
+#pragma unroll
+          for (int i = 0; i < NU; i++) sg_lds_copy16((uint32_t)(ring_at(u) + i * 1024), lane * 16, rsrc, (wave * NU + i) * 1024);
+          sg_lds_copy4((uint32_t)(ring_at(u) + NU * 1024), lane * 4, rsrc, (uint32_t)(2 * kTile * D));
+        } else if constexpr (Q8) {
 #pragma unroll
           for (int i = 0; i < NU; i++) codes[i] = *reinterpret_cast<const u32x4_t*>(from + (wave * NU + i) * 1024 + lane * 16);
           if (wave == 0) tail_of = *reinterpret_cast<const float*>(from + a.tile_bytes - kTail + lane * 4);
@@ -632,18 +651,24 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void 
           }
         }
       };
-      auto put = [&](int stage) {
+      auto put = [&](int stage, int u, int n) {
+        if constexpr (RING) {  // (the two tiles behind it stay in flight)
+          if (u + 2 < n) sg_wait_vmcnt<2 * (NU + 1)>();
+          else sg_wait_vmcnt<0>();
+#pragma unroll
+          for (int i = 0; i < NU; i++) codes[i] = *reinterpret_cast<const u32x4_t*>(lds + ring_at(u) + i * 1024 + lane * 16);
+        }
         if constexpr (Q8) {
           char* to = lds + stage * STAGE;
 #pragma unroll
           for (int i = 0; i < NU; i++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const int u = wave * NU + i, f = u * 2 + e;  // fragment of keys, then of values
-              if (u < D / 32) store_frag<T>(to, f, lane, decode<T>(codes[i][e * 2], codes[i][e * 2 + 1]));
+              const int k = wave * NU + i, f = k * 2 + e;  // fragment of keys, then of values
+              if (k < D / 32) store_frag<T>(to, f, lane, decode<T>(codes[i][e * 2], codes[i][e * 2 + 1]));
               else store_frag<M>(to + KB, f - D / 16, lane, decode<M>(codes[i][e * 2], codes[i][e * 2 + 1]));
             }
-          if (wave == 0) *reinterpret_cast<float*>(to + 2 * KB + lane * 4) = tail_of;
+          if (!RING && wave == 0) *reinterpret_cast<float*>(to + 2 * KB + lane * 4) = tail_of;
         }
       };
       if (pt.work) begin_job(a, st, job, sh.head, pair0, lane);
@@ -654,23 +679,31 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void 
         const int64_t tile = (seg ? job.slot_tile[1] : job.slot_tile[0]) + (u0 - t0);
         int first = (int)(tile * kTile - (seg ? job.key0[1] : job.key0[0]));
         const char* at = a.cache + (int64_t)sh.head * a.head_bytes + tile * a.tile_bytes;
+        const int tiles = (int)(u1 - u0);
         __syncthreads();  // the stages have been read
-        fetch(at, 0);
+        fetch(at, 0, 0);
+        if constexpr (RING) {
+          if (1 < tiles) fetch(at + a.tile_bytes, 0, 1);
+          if (2 < tiles) fetch(at + 2 * a.tile_bytes, 0, 2);
+        }
         begin_keys(a, st, job, pair0, job.kind == kOwnKeys || seg, lane);
-        put(0);
-        for (int64_t u = u0; u < u1; u++, first += kTile) {
-          const int stage = (int)((u - u0) & 1);
+        put(0, 0, tiles);
+        for (int u = 0; u < tiles; u++, first += kTile) {
+          const int stage = u & 1;
           if constexpr (!Q8) sg_wait_vmcnt<0>();
           __syncthreads();
           // (Taken here, where nothing is in flight: waiting for it later would wait for the next tile.)
           uint32_t bad = __builtin_amdgcn_readfirstlane(bad_next);
           asm volatile("" : "+s"(bad));
           at += a.tile_bytes;
-          if (u + 1 < u1) fetch(at, stage ^ 1);
+          if constexpr (RING) {
+            if (u + 3 < tiles) fetch(at + 2 * a.tile_bytes, 0, u + 3);
+          } else {
+            if (u + 1 < tiles) fetch(at, stage ^ 1, u + 1);
+          }
           const char* keys = lds + stage * STAGE;
           const char* vals = keys + KB;
           f32x4_t s[2][QT] = {};
-          float p[QT][8];
 #pragma unroll
           for (int half = 0; half < 2; half++)
 #pragma unroll
@@ -679,11 +712,9 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void 
 #pragma unroll
               for (int t = 0; t < QT; t++) s[half][t] = mma(T{}, x, st.q[t][d], s[half][t]);
             }
-          weigh<T, Q8, D, QT>(a, st, s, first, Q8 ? reinterpret_cast<const float*>(keys + 2 * KB) : nullptr, lane, p);
           typename frag<M>::type w[QT][weight<T, Q8>::parts];
-#pragma unroll
-          for (int t = 0; t < QT; t++) pack_weights<T, Q8>(p[t], w[t]);
-          if constexpr (kSumByProduct<T, Q8>) add_sums(st, w);
+          weigh<T, Q8, D, QT>(a, st, s, first,
+                              reinterpret_cast<const float*>(RING ? lds + ring_at(u) + NU * 1024 : keys + 2 * KB), lane, w);
           if constexpr (!Q8) {
             if (bad) {  // (alike for the workgroup)
               char* own = lds + stage * STAGE + KB;
@@ -701,7 +732,7 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void 
           }
           if constexpr (!Q8)
             if (bad) mark_bad(st, first, at - a.tile_bytes + KB, lane);
-          if (u + 1 < u1) put(stage ^ 1);
+          if (u + 1 < tiles) put(stage ^ 1, u + 1, tiles);
         }
       }
       if (pt.work) end_job(a, list, st, job, sh.head, pair0, in_job, worker, pt.whole, pt.later, lane);
@@ -720,7 +751,7 @@ template <typename T, bool Q8, int D>
 hipError_t launch_list(const sg_attn_shared_args& a, const sg_attn_list& list, hipStream_t s) {
   if (!list.wide) return sgp::run_kernel(k_attn_narrow<T, Q8, D>, dim3(list.blocks), dim3(256), 0, s, a, list);
   constexpr int QT = sgk::attn_wide_pairs(D) / 64;
-  constexpr size_t lds = 2 * (2 * kTile * D * sizeof(T) + (Q8 ? kTail : 0));
+  constexpr size_t lds = wide_lds<T, Q8, D>::bytes;
   auto kernel = k_attn_wide<T, Q8, D, QT>;
   // More than 64 KB has to be asked for, on every device.
   static std::atomic<uint64_t> asked{0};

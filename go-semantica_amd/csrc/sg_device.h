@@ -48,6 +48,21 @@ __device__ __forceinline__ void sg_lds_copy16(uint32_t lds_addr, uint32_t voff, 
       : "memory");
 }
 
+// The same for four bytes a lane (256 bytes to LDS).
+__device__ __forceinline__ void sg_lds_copy4(uint32_t lds_addr, uint32_t voff, i32x4_t rsrc, uint32_t soff) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %2, %3, %4 offen lds\n\t"
+      "s_nop 0\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(lds_addr), "v"(voff), "s"(rsrc), "s"(soff)
+      : "memory");
+}
+
 // Raw buffer descriptor over [base, base + 2 GB): stride 0, the rest as
 // __builtin_amdgcn_make_buffer_rsrc builds it (word 3: gfx9 raw buffer).
 __device__ __forceinline__ i32x4_t sg_raw_rsrc(const void* base) {

@@ -599,19 +599,18 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
 // are first, kRing tiles of them, each wave its own quarter (and the scales): a tile of codes is
 // 8 KB, and one or two a CU in flight reach half of the memory's rate.
 constexpr int kRing = 4;
-template <typename T, bool Q8, int D>
+template <typename T, bool Q8, int D, int NW>
 struct wide_lds {
   static constexpr int KB = kTile * D * (int)sizeof(T);  // keys of a tile
-  static constexpr bool ring = Q8 && sizeof(T) == 2 && D <= 128;
+  static constexpr bool ring = Q8 && sizeof(T) == 2 && D <= 128 && D / 16 >= NW;
   static constexpr int stage = 2 * KB + (Q8 && !ring ? kTail : 0);
-  static constexpr int quarter = D / 64 * 1024 + kTail;  // a wave's part of a tile of codes
-  static constexpr int bytes = 2 * stage + (ring ? kRing * 4 * quarter : 0);
+  static constexpr int part = D / 16 * 1024 / NW + kTail;  // a wave's part of a tile of codes
+  static constexpr int bytes = 2 * stage + (ring ? kRing * NW * part : 0);
 };
-template <typename T, bool Q8, int D, int QT>
-__global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void k_attn_wide(sg_attn_shared_args a,
-                                                                                          sg_attn_list list) {
+template <typename T, bool Q8, int D, int QT, int NW, int PER_CU>
+__global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_shared_args a, sg_attn_list list) {
   typedef typename weight<T, Q8>::type M;
-  typedef wide_lds<T, Q8, D> L;
+  typedef wide_lds<T, Q8, D, NW> L;
   constexpr int KB = L::KB, STAGE = L::stage;
   constexpr bool RING = L::ring;
   extern __shared__ __align__(16) char lds[];
@@ -624,13 +623,13 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void 
     if (n > 0) {
       const sg_attn_job job = list.jobs[sh.job];
       const part pt = part_of(list, job, sh.at, sh.left, c0, c1);
-      const int in_job = wave * QT * 16, pair0 = job.tile * (64 * QT) + in_job;
-      constexpr int NU = Q8 ? D / 16 / 4 : 2 * KB / 1024 / 4;  // kilobytes of a tile for each wave
+      const int in_job = wave * QT * 16, pair0 = job.tile * (16 * NW * QT) + in_job;
+      constexpr int NU = Q8 ? D / 16 / NW : 2 * KB / 1024 / NW;  // kilobytes of a tile for each wave
       u32x4_t codes[Q8 ? NU : 1];
       float tail_of = 0.0f;
       uint32_t bad_next = 0;
-      const int mine = 2 * STAGE + wave * L::quarter;  // the wave's part of a ring slot
-      auto ring_at = [&](int u) { return mine + u % kRing * (4 * L::quarter); };
+      const int mine = 2 * STAGE + wave * L::part;  // the wave's part of a ring slot
+      auto ring_at = [&](int u) { return mine + u % kRing * (NW * L::part); };
       auto fetch = [&](const char* from, int stage, int u) {
         if constexpr (RING) {
           const i32x4_t rsrc = sg_raw_rsrc(from);
@@ -703,32 +702,56 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void 
           }
           const char* keys = lds + stage * STAGE;
           const char* vals = keys + KB;
-          f32x4_t s[2][QT] = {};
-#pragma unroll
-          for (int half = 0; half < 2; half++)
-#pragma unroll
-            for (int d = 0; d < D / 32; d++) {
-              const typename frag<T>::type x = load_frag<T>(keys, half * (D / 32) + d, lane);
-#pragma unroll
-              for (int t = 0; t < QT; t++) s[half][t] = mma(T{}, x, st.q[t][d], s[half][t]);
-            }
-          typename frag<M>::type w[QT][weight<T, Q8>::parts];
-          weigh<T, Q8, D, QT>(a, st, s, first,
-                              reinterpret_cast<const float*>(RING ? lds + ring_at(u) + NU * 1024 : keys + 2 * KB), lane, w);
           if constexpr (!Q8) {
             if (bad) {  // (alike for the workgroup)
               char* own = lds + stage * STAGE + KB;
-              for (int f = wave; f < D / 16; f += 4) store_frag<T>(own, f, lane, clean<T>(load_frag<T>(own, f, lane)));
+              for (int f = wave; f < D / 16; f += NW) store_frag<T>(own, f, lane, clean<T>(load_frag<T>(own, f, lane)));
               __syncthreads();
             }
           }
+          // Fragments come from LDS NB at a time, a batch ahead of its products (the first values
+          // ahead of the softmax): one by one they would cost their latency each.
+          constexpr int NF = D / 16, NB = sizeof(T) == 2 ? 8 : 2, NBATCH = (NF + NB - 1) / NB, N0 = NF < NB ? NF : NB;
+          typename frag<T>::type kx[2][N0];
+          typename frag<M>::type vx[2][N0];
+          auto load_keys = [&](int i) {
 #pragma unroll
-          for (int f = 0; f < D / 16; f++) {
-            const typename frag<M>::type x = load_frag<M>(vals, f, lane);
+            for (int e = 0; e < N0; e++) kx[i & 1][e] = load_frag<T>(keys, i * N0 + e, lane);
+          };
+          auto load_vals = [&](int i) {
 #pragma unroll
-            for (int t = 0; t < QT; t++)
+            for (int e = 0; e < N0; e++) vx[i & 1][e] = load_frag<M>(vals, i * N0 + e, lane);
+          };
+          f32x4_t s[2][QT] = {};
+          load_keys(0);
 #pragma unroll
-              for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[t][f] = mma(M{}, x, w[t][h], st.o[t][f]);
+          for (int i = 0; i < NBATCH; i++) {
+            if (i + 1 < NBATCH) load_keys(i + 1);
+            else load_vals(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < N0; e++) {
+              const int f = i * N0 + e, half = f / (D / 32), d = f % (D / 32);
+#pragma unroll
+              for (int t = 0; t < QT; t++) s[half][t] = mma(T{}, kx[i & 1][e], st.q[t][d], s[half][t]);
+            }
+          }
+          typename frag<M>::type w[QT][weight<T, Q8>::parts];
+          weigh<T, Q8, D, QT>(a, st, s, first,
+                              reinterpret_cast<const float*>(RING ? lds + ring_at(u) + NU * 1024 : keys + 2 * KB), lane, w);
+#pragma unroll
+          for (int i = 0; i < NBATCH; i++) {
+            if (i + 1 < NBATCH) {
+              load_vals(i + 1);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int e = 0; e < N0; e++)
+#pragma unroll
+              for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int h = 0; h < weight<T, Q8>::parts; h++)
+                  st.o[t][i * N0 + e] = mma(M{}, vx[i & 1][e], w[t][h], st.o[t][i * N0 + e]);
           }
           if constexpr (!Q8)
             if (bad) mark_bad(st, first, at - a.tile_bytes + KB, lane);
@@ -747,12 +770,20 @@ __global__ __launch_bounds__(256, __is_same(T, float) && D >= 128 ? 1 : 2) void 
   }
 }
 
+// Waves of a workgroup, pairs of each, workgroups of a CU.
+template <typename T, bool Q8, int D>
+struct wide_form {
+  static constexpr int NW = 4;
+  static constexpr int QT = sgk::attn_wide_pairs(D) / (16 * NW);
+  static constexpr int PER_CU = sizeof(T) == 4 && D >= 128 ? 1 : 2;
+};
+
 template <typename T, bool Q8, int D>
 hipError_t launch_list(const sg_attn_shared_args& a, const sg_attn_list& list, hipStream_t s) {
   if (!list.wide) return sgp::run_kernel(k_attn_narrow<T, Q8, D>, dim3(list.blocks), dim3(256), 0, s, a, list);
-  constexpr int QT = sgk::attn_wide_pairs(D) / 64;
-  constexpr size_t lds = wide_lds<T, Q8, D>::bytes;
-  auto kernel = k_attn_wide<T, Q8, D, QT>;
+  typedef wide_form<T, Q8, D> W;
+  constexpr size_t lds = wide_lds<T, Q8, D, W::NW>::bytes;
+  auto kernel = k_attn_wide<T, Q8, D, W::QT, W::NW, W::PER_CU>;
   // More than 64 KB has to be asked for, on every device.
   static std::atomic<uint64_t> asked{0};
   int device = 0;
@@ -766,7 +797,7 @@ hipError_t launch_list(const sg_attn_shared_args& a, const sg_attn_list& list, h
     }
     if (device < 64) asked.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
   }
-  return sgp::run_kernel(kernel, dim3(list.blocks), dim3(256), lds, s, a, list);
+  return sgp::run_kernel(kernel, dim3(list.blocks), dim3(64 * W::NW), lds, s, a, list);
 }
 
 template <typename T>

@@ -18,7 +18,7 @@ using sgp::clamp_row;
 using sgp::elem;
 
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanSeqs = 8192;  // offsets kept in LDS up to so many sequences
+constexpr int kPlanSeqs = 4096, kPlanPrefixes = 512;  // numbers of so many are kept in LDS
 
 // The largest i in [0, n) with at(i) <= x for ascending at, 0 if there is none.
 template <typename F>
@@ -32,13 +32,13 @@ __device__ __forceinline__ int last_at_most(int n, int x, F at) {
   return lo;
 }
 
-// Running totals over a workgroup: out[0] = base, out[i + 1] = out[i] + count(i), none above
+// Running totals over a workgroup: put(0, base), put(i + 1, before + count(i)), none above
 // `most`.  Returns the last.
-template <typename O, typename F>
-__device__ int64_t running(int n, int64_t base, int64_t most, O* out, F count) {
+template <typename P, typename F>
+__device__ int64_t running(int n, int64_t base, int64_t most, P put, F count) {
   __shared__ int64_t wave_sum[kPlanThreads / 64];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  if (t == 0) out[0] = (O)base;
+  if (t == 0) put(0, base);
   for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
     const int i = i0 + t;
     int64_t v = i < n ? count(i) : 0;
@@ -55,7 +55,7 @@ __device__ int64_t running(int n, int64_t base, int64_t most, O* out, F count) {
       if (w == wave) v += total;
       total += wave_sum[w];
     }
-    if (i < n) out[i + 1] = (O)min(v, most);
+    if (i < n) put(i + 1, min(v, most));
     base = min(total, most);
   }
   __syncthreads();
@@ -67,108 +67,114 @@ __device__ __forceinline__ int kept_length(int start, int length, int64_t slots)
   return start >= 0 && length > 0 && (int64_t)start + length <= slots ? length : 0;
 }
 
-__device__ __forceinline__ int clamp32(int64_t v, int64_t most) { return (int)min(max(v, (int64_t)0), most); }
-
 __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args a, sg_attn_batch b, sg_attn_list la,
-                                                            sg_attn_list lb, int one_list, int4* seen_out, int4* where_out) {
-  __shared__ int32_t off_lds[kPlanSeqs + 1];
+                                                            sg_attn_list lb, int one_list, int rows_wanted, int2* seen_out,
+                                                            int4* where_out) {
+  __shared__ int32_t off_lds[kPlanSeqs + 1], seq_jobs_lds[kPlanSeqs + 1];
+  __shared__ int32_t group_lds[kPlanPrefixes + 1], prefix_jobs_lds[kPlanPrefixes + 1];
   const int t = threadIdx.x;
-  const bool small = b.n_seq <= kPlanSeqs;
+  const bool small = b.n_seq <= kPlanSeqs, few = b.n_prefix <= kPlanPrefixes;
   if (small)
     for (int i = t; i <= b.n_seq; i += kPlanThreads) off_lds[i] = clamp_row(b.off[i], a.rows);
+  if (few && b.n_prefix > 0)
+    for (int i = t; i <= b.n_prefix; i += kPlanThreads) group_lds[i] = min(max(b.shared[i], 0), b.n_seq);
   __syncthreads();
   auto off = [&](int i) { return small ? off_lds[i] : clamp_row(b.off[i], a.rows); };
-  auto rows_of = [&](int i) { return max(off(i + 1) - off(i), 0); };
-  auto group_at = [&](int p) { return min(max(b.shared[p], 0), b.n_seq); };
+  auto group_at = [&](int p) { return few ? group_lds[p] : min(max(b.shared[p], 0), b.n_seq); };
+  auto seq_jobs = [&](int i) { return small ? seq_jobs_lds[i] : b.seq_jobs[i]; };
+  auto prefix_jobs = [&](int p) { return few ? prefix_jobs_lds[p] : b.prefix_jobs[p]; };
 
   // Jobs of each prefix and sequence: those of prefixes first where both stand in one list; with
   // all_keys there are only sequences'.
   const bool prefixes = b.n_prefix > 0 && !b.all_keys;
-  const int prefix_jobs =
-      prefixes ? (int)running(b.n_prefix, 0, la.cap, b.prefix_jobs,
-                              [&](int p) {
-                                const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
-                                return (rows * a.group + la.m - 1) / la.m;
-                              })
-               : 0;
-  const int own0 = one_list ? prefix_jobs : 0;
-  const int own_end = (int)running(b.n_seq, own0, lb.cap, b.seq_jobs,
-                                   [&](int i) { return ((int64_t)rows_of(i) * a.group + lb.m - 1) / lb.m; });
+  int n_prefix_jobs = 0;
+  if (prefixes)
+    n_prefix_jobs = (int)running(
+        b.n_prefix, 0, la.cap, [&](int p, int64_t v) { few ? prefix_jobs_lds[p] = (int)v : b.prefix_jobs[p] = (int)v; },
+        [&](int p) {
+          const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
+          return (rows * a.group + la.m - 1) / la.m;
+        });
+  const int own0 = one_list ? n_prefix_jobs : 0;
+  const int own_end = (int)running(
+      b.n_seq, own0, lb.cap, [&](int i, int64_t v) { small ? seq_jobs_lds[i] = (int)v : b.seq_jobs[i] = (int)v; },
+      [&](int i) { return ((int64_t)max(off(i + 1) - off(i), 0) * a.group + lb.m - 1) / lb.m; });
   auto prefix_of = [&](int i) {  // of a sequence; -1: none
     if (b.n_prefix == 0) return -1;
     const int p = last_at_most(b.n_prefix, i, group_at);
     return i >= group_at(p) && i < group_at(p + 1) ? p : -1;
   };
+  auto prefix_length = [&](int p) { return p < 0 ? 0 : kept_length(b.prefix_starts[p], b.prefix_lengths[p], b.slots); };
 
-  // What each row sees.
-  for (int row = t; row < a.rows; row += kPlanThreads) {
-    const int i = last_at_most(b.n_seq, row, off);
-    const int r0 = off(i), r1 = off(i + 1);
-    int4 seen = make_int4(0, 0, 0, 0), where = make_int4(-2, 0, -2, 0);
-    if (row >= r0 && row < r1) {
-      const int64_t len = kept_length(b.starts[i], b.lengths[i], b.slots);
-      int64_t plen = 0;
-      where = make_int4(-1, 0, b.seq_jobs[i], r0);
-      const int p = prefix_of(i);
-      if (p >= 0) {
-        plen = kept_length(b.prefix_starts[p], b.prefix_lengths[p], b.slots);
-        if (prefixes) {
-          where.x = b.prefix_jobs[p];
+  // What each row sees of a prefix that sequences share, and where the join finds it.
+  if (rows_wanted)
+    for (int row = t; row < a.rows; row += kPlanThreads) {
+      const int i = last_at_most(b.n_seq, row, off);
+      const int r0 = off(i), r1 = off(i + 1);
+      int4 seen = make_int4(0, 0, 0, 0), where = make_int4(-2, 0, -2, 0);
+      if (row >= r0 && row < r1) {
+        where = make_int4(-1, 0, seq_jobs(i), r0);
+        const int p = prefixes ? prefix_of(i) : -1;
+        if (p >= 0) {
+          where.x = prefix_jobs(p);
           where.y = off(group_at(p));
+          const int plen = prefix_length(p), len = kept_length(b.starts[i], b.lengths[i], b.slots);
+          seen = sgc::places_seen((int64_t)plen + len - (r1 - r0) + (row - r0), plen, len, a.causal, a.window);
         }
       }
-      const int64_t pos = plen + len - (r1 - r0) + (row - r0);
-      int64_t lo = 0, hi = plen + len;
-      if (b.causal) hi = min(hi, pos + 1);
-      if (b.window > 0) {
-        lo = max(lo, pos - b.window + 1);
-        hi = min(hi, pos + b.window);
-      }
-      seen = make_int4(clamp32(lo, plen), clamp32(hi, plen), clamp32(lo - plen, len), clamp32(hi - plen, len));
+      if (prefixes) seen_out[row] = make_int2(seen.x, seen.y);
+      where_out[row] = where;
     }
-    seen_out[row] = seen;
-    where_out[row] = where;
-  }
   __syncthreads();
 
   // The jobs, and the running total of their costs.
   auto fill = [&](const sg_attn_list& list, int j0, int n, int kind, int64_t base) {
-    const int32_t* jobs = kind == kPrefixKeys ? b.prefix_jobs : b.seq_jobs;
-    const int64_t units = running(n, base, INT64_MAX, list.cum + j0, [&](int j) {
-      const int i = last_at_most(kind == kPrefixKeys ? b.n_prefix : b.n_seq, j + j0, [&](int k) { return jobs[k]; });
-      const int r0 = off(kind == kPrefixKeys ? group_at(i) : i), r1 = off(kind == kPrefixKeys ? group_at(i + 1) : i + 1);
-      sg_attn_job job{r0, max(r1 - r0, 0), j + j0 - jobs[i], kind, {0, 0}, {0, 0}, {0, 0}};
-      const int from = r0 + (int)((int64_t)job.tile * list.m / a.group);
-      const int to = (int)min((int64_t)r1 - 1, r0 + ((int64_t)(job.tile + 1) * list.m - 1) / a.group);
-      int lo[2] = {INT32_MAX, INT32_MAX}, hi[2] = {0, 0};
-      for (int r = from; r <= to; r++) {
-        const int4 s = seen_out[r];
-        if (s.x < s.y) {
-          lo[0] = min(lo[0], s.x);
-          hi[0] = max(hi[0], s.y);
-        }
-        if (s.z < s.w) {
-          lo[1] = min(lo[1], s.z);
-          hi[1] = max(hi[1], s.w);
-        }
-      }
-      int64_t count = 0;
-      for (int own = 0; own < 2; own++) {
-        const int p = kind == kPrefixKeys ? i : kind == kAllKeys ? prefix_of(i) : -1;
-        if (own ? kind == kPrefixKeys : p < 0) continue;
-        const int64_t start = own ? b.starts[i] : b.prefix_starts[p];
-        // (Cut once more: where offsets do not ascend, a row's range is another sequence's.)
-        const int end = min(hi[own], kept_length((int)start, own ? b.lengths[i] : b.prefix_lengths[p], b.slots));
-        if (lo[own] >= end) continue;
-        const int at = kind == kAllKeys ? own : 0;
-        job.key0[at] = (int)start;
-        job.slot_tile[at] = (int)((start + lo[own]) / kTile);
-        job.tiles[at] = (int)((start + end - 1) / kTile) - job.slot_tile[at] + 1;
-        count += job.tiles[at];
-      }
-      list.jobs[j + j0] = job;
-      return count + (count > 0 || kind == kAllKeys ? list.job_cost : 0);
-    });
+    const int64_t units = running(
+        n, base, INT64_MAX, [&](int j, int64_t v) { list.cum[j0 + j] = v; },
+        [&](int j) {
+          const bool prefix = kind == kPrefixKeys;
+          const int i = prefix ? last_at_most(b.n_prefix, j + j0, prefix_jobs) : last_at_most(b.n_seq, j + j0, seq_jobs);
+          const int r0 = off(prefix ? group_at(i) : i), r1 = off(prefix ? group_at(i + 1) : i + 1), rows = max(r1 - r0, 0);
+          const int p = prefix ? i : prefix_of(i), plen = prefix_length(p);
+          const int len = prefix ? 0 : kept_length(b.starts[i], b.lengths[i], b.slots);
+          sg_attn_job job{r0, rows, j + j0 - (prefix ? prefix_jobs(i) : seq_jobs(i)), kind, {0, 0}, {0, 0}, {0, 0}, plen, len};
+          const int from = (int)((int64_t)job.tile * list.m / a.group);
+          const int to = (int)min((int64_t)rows, ((int64_t)(job.tile + 1) * list.m - 1) / a.group + 1);
+          int lo[2] = {INT32_MAX, INT32_MAX}, hi[2] = {0, 0};
+          auto see = [&](int own, int l, int h) {
+            lo[own] = min(lo[own], l < h ? l : INT32_MAX);
+            hi[own] = max(hi[own], l < h ? h : 0);
+          };
+          if (prefix) {
+#pragma unroll 8
+            for (int r = from; r < to; r++) {
+              const int2 s = seen_out[r0 + r];
+              see(0, s.x, s.y);
+            }
+          } else if (from < to) {
+            // Both ends of a range grow with the row, empty or not: the first row's begin, the last one's end.
+            const int64_t pos0 = (int64_t)plen + len - rows;
+            const int4 s0 = sgc::places_seen(pos0 + from, plen, len, a.causal, a.window);
+            const int4 s1 = sgc::places_seen(pos0 + to - 1, plen, len, a.causal, a.window);
+            see(0, s0.x, s1.y);
+            see(1, s0.z, s1.w);
+          }
+          int64_t count = 0;
+          for (int own = 0; own < 2; own++) {
+            if (own ? prefix : kind == kOwnKeys || p < 0) continue;
+            const int64_t start = own ? b.starts[i] : b.prefix_starts[p];
+            // (Cut once more: where offsets do not ascend, a row's range is another group's.)
+            const int end = min(hi[own], own ? len : plen);
+            if (lo[own] >= end) continue;
+            const int at = kind == kAllKeys ? own : 0;
+            job.key0[at] = (int)start;
+            job.slot_tile[at] = (int)((start + lo[own]) / kTile);
+            job.tiles[at] = (int)((start + end - 1) / kTile) - job.slot_tile[at] + 1;
+            count += job.tiles[at];
+          }
+          list.jobs[j + j0] = job;
+          return count + (count > 0 || kind == kAllKeys ? list.job_cost : 0);
+        });
     if (t == 0) {
       list.plan->units = units;
       list.plan->jobs = j0 + n;
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
     return units;
   };
   int64_t base = 0;
-  if (prefixes) base = fill(la, 0, prefix_jobs, kPrefixKeys, 0);
+  if (prefixes) base = fill(la, 0, n_prefix_jobs, kPrefixKeys, 0);
   if (!one_list) base = 0;
   fill(lb, own0, own_end - own0, b.all_keys ? kAllKeys : kOwnKeys, base);
 }
@@ -346,7 +352,7 @@ layout lay_out(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, i
   }
   y.seq_jobs = take(sizeof(int32_t) * ((size_t)n_seq + 1));
   y.prefix_jobs = take(sizeof(int32_t) * ((size_t)n_prefix + 1));
-  y.seen = take(sizeof(int4) * (size_t)rows);
+  y.seen = take(sizeof(int2) * (size_t)rows);
   y.where = take(sizeof(int4) * (size_t)rows);
   int64_t rows_of_o = 2 * (int64_t)rows * heads;
   for (int i = 0; i < 2; i++) {
@@ -387,7 +393,7 @@ size_t attn_shared_work_bytes(int dtype, int rows, int heads, int kv_heads, int 
 hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q8, int D, void* work, hipStream_t s) {
   const layout y = lay_out(dtype, a.rows, a.heads, a.kv_heads, D, b.n_seq, b.n_prefix);
   char* w = static_cast<char*>(work);
-  int4* seen = reinterpret_cast<int4*>(w + y.seen);
+  int2* seen = reinterpret_cast<int2*>(w + y.seen);
   int4* where = reinterpret_cast<int4*>(w + y.where);
   a.seen = seen;
   a.where = where;
@@ -420,7 +426,9 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
   const sg_attn_list& lb = lists[wide_own];
   const sg_attn_list& la = lists[wide_prefix];
   const int one_list = &la == &lb;
-  hipError_t e = sgp::run_kernel(k_attn_plan, dim3(1), dim3(kPlanThreads), 0, s, a, b, la, lb, one_list, seen, where);
+  const int rows_wanted = !b.all_keys || (int64_t)a.rows * a.heads <= kJoinSome;
+  hipError_t e =
+      sgp::run_kernel(k_attn_plan, dim3(1), dim3(kPlanThreads), 0, s, a, b, la, lb, one_list, rows_wanted, seen, where);
   auto run = [&](const sg_attn_list& l) {
     if (e != hipSuccess) return;
     e = dtype == SG_F32   ? attn_shared_f32(a, l, q8, D, s)

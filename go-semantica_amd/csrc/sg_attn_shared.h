@@ -438,9 +438,19 @@ __device__ __forceinline__ void begin_keys(const sg_attn_shared_args& a, state<T
   for (int t = 0; t < QT; t++) {
     const int pair = pair0 + t * 16 + (lane & 15);
     const bool in = pair < job.rows * a.group;
-    const int4 seen = a.seen[job.row0 + (in ? pair / a.group : 0)];
-    st.lo[t] = in ? (own ? seen.z : seen.x) : 0;
-    st.hi[t] = in ? (own ? seen.w : seen.y) : 0;
+    const int r = in ? pair / a.group : 0;
+    int lo, hi;
+    if (job.kind == kPrefixKeys) {
+      const int2 seen = a.seen[job.row0 + r];
+      lo = seen.x;
+      hi = seen.y;
+    } else {
+      const int4 seen = sgc::places_seen((int64_t)job.plen + job.len - job.rows + r, job.plen, job.len, a.causal, a.window);
+      lo = own ? seen.z : seen.x;
+      hi = own ? seen.w : seen.y;
+    }
+    st.lo[t] = in ? lo : 0;
+    st.hi[t] = in ? hi : 0;
     if (in) {
       all_lo = max(all_lo, st.lo[t]);
       all_hi = min(all_hi, st.hi[t]);
@@ -736,6 +746,7 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
               for (int t = 0; t < QT; t++) s[half][t] = mma(T{}, kx[i & 1][e], st.q[t][d], s[half][t]);
             }
           }
+          if (RING && u + 1 < tiles) put(stage ^ 1, u + 1, tiles);  // (while the scores come)
           typename frag<M>::type w[QT][weight<T, Q8>::parts];
           weigh<T, Q8, D, QT>(a, st, s, first,
                               reinterpret_cast<const float*>(RING ? lds + ring_at(u) + NU * 1024 : keys + 2 * KB), lane, w);
@@ -755,7 +766,7 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
           }
           if constexpr (!Q8)
             if (bad) mark_bad(st, first, at - a.tile_bytes + KB, lane);
-          if (u + 1 < tiles) put(stage ^ 1, u + 1, tiles);
+          if (!RING && u + 1 < tiles) put(stage ^ 1, u + 1, tiles);
         }
       }
       if (pt.work) end_job(a, list, st, job, sh.head, pair0, in_job, worker, pt.whole, pt.later, lane);

@@ -196,6 +196,8 @@ int sg_attention_shared(sg_ctx* ctx, void* out, int64_t ldo, const void* q, int6
   a.cap = cap * kLog2e;
   a.to_cap = cap != 0.0f ? std::fabs(scale) / cap : 0.0f;
   a.negative = scale < 0.0f;
+  a.causal = keys->causal != 0;
+  a.window = keys->window;
   a.rows = rows;
   a.heads = n_heads;
   a.kv_heads = cache->heads;
@@ -211,8 +213,6 @@ int sg_attention_shared(sg_ctx* ctx, void* out, int64_t ldo, const void* q, int6
   b.slots = cache->slots;
   b.n_seq = n_seq;
   b.n_prefix = keys->n_prefix;
-  b.causal = keys->causal != 0;
-  b.window = keys->window;
   SG_HIP(sgk::attn_shared(a, b, cache->dtype, cache->q8, cache->D, work, ctx_stream(ctx, stream)));
   return SG_OK;
 }

@@ -111,13 +111,14 @@ struct sg_attn_shared_args {
   const void* q;
   const char* cache;
   int64_t ldo, ldq, head_bytes, tile_bytes;
-  const int4* seen;   // [rows]: visible places of the prefix, of the own keys (begin, end)
+  const int2* seen;   // [rows]: visible places of the prefix (begin, end), for prefixes' jobs
   const int4* where;  // [rows]: first job and first row of its prefix's group, of its sequence's
   float* part_o;      // [2 rows * heads, then pieces][D]
   float2* part_ml;
   float scale;        // of scores, in powers of two, not negative (1 / log2 e under a cap: 1)
   float cap, to_cap;  // cap * log2 e (0: none), and what a product is multiplied by before tanh
   int negative;       // queries are negated
+  int causal, window;
   int rows, heads, kv_heads, group, hd;
 };
 // Consecutive pairs of a group over one or two ranges of tiles: a prefix's, a sequence's own
@@ -126,6 +127,7 @@ constexpr int kPrefixKeys = 0, kOwnKeys = 1, kAllKeys = 2;
 struct sg_attn_job {
   int row0, rows, tile, kind;           // the group's rows; which M pairs of them
   int key0[2], slot_tile[2], tiles[2];  // the slot of the first key; the first tile with a visible one
+  int plen, len;                        // a sequence's: keys of its prefix, its own
 };
 struct sg_attn_plan {
   int64_t units, per;  // units of a head, of a worker
@@ -151,7 +153,7 @@ struct sg_attn_batch {
   int32_t* seq_jobs;     // [n_seq + 1]
   int32_t* prefix_jobs;  // [n_prefix + 1]
   int64_t slots;
-  int n_seq, n_prefix, causal, window, all_keys;
+  int n_seq, n_prefix, all_keys;
 };
 
 // One sg_matmul_q4 call (k_q4.hip): packed weights, strides in elements.

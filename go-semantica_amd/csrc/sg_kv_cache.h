@@ -51,6 +51,19 @@ __device__ __forceinline__ int value_at(int D, int key, int dim) {
   return kTile * D * ES + place<ES>(dim >> 4, (dim & 15) + ((key >> 2) & 3) * 16, (key >> 4) * 4 + (key & 3));
 }
 
+// The places that the query at place pos sees of its prefix (x, y) and of its own keys (z, w,
+// counted from the first).
+__device__ __forceinline__ int4 places_seen(int64_t pos, int plen, int len, int causal, int window) {
+  int64_t lo = 0, hi = (int64_t)plen + len;
+  if (causal) hi = min(hi, pos + 1);
+  if (window > 0) {
+    lo = max(lo, pos - window + 1);
+    hi = min(hi, pos + window);
+  }
+  auto cut = [](int64_t v, int most) { return (int)min(max(v, (int64_t)0), (int64_t)most); };
+  return make_int4(cut(lo, plen), cut(hi, plen), cut(lo - plen, len), cut(hi - plen, len));
+}
+
 // The largest i in [0, n) with at[i] <= x, for ascending at with at[0] <= x; called by a whole
 // wave with a uniform x: 64 candidates a step.
 __device__ __forceinline__ int last_at_most(const int64_t* at, int n, int64_t x, int lane) {

@@ -414,7 +414,7 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
     l.blocks = i ? l.workers : l.workers / 4;
     l.wide = i;
     l.cap = y.cap;
-    l.min_units = i ? 12 : dtype == SG_F32 && D == 256 ? 1 : 2;
+    l.min_units = i ? 8 : dtype == SG_F32 && D == 256 ? 1 : 2;
     l.job_cost = i ? 4 : dtype == SG_F32 && D == 256 ? 1 : 2;
   }
   const int64_t pairs = (int64_t)a.rows * a.group;

@@ -422,6 +422,9 @@ hipError_t q4_pack(const uint8_t* codes, const void* scales, int scale_dtype, co
                    int group, uint32_t* w, void* packed_scales, uint8_t* packed_zeros, hipStream_t s);
 hipError_t q4_pack_q4_0(const uint8_t* raw, int out_dim, int in_dim, uint32_t* w, void* packed_scales, hipStream_t s);
 hipError_t matmul_q4(const sg_q4_args& a, int dtype, hipStream_t s);
+hipError_t matmul_q4_f32(const sg_q4_args& a, hipStream_t s);
+hipError_t matmul_q4_f16(const sg_q4_args& a, hipStream_t s);
+hipError_t matmul_q4_bf16(const sg_q4_args& a, hipStream_t s);
 
 // ---- brute-force search (k_search.hip) ----
 // Storage modes, the values of brute.QuantizationMode (search/brute/quant.go:8-15).

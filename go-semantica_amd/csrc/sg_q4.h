@@ -129,19 +129,18 @@ struct alignas(PER * 4 * sizeof(S) < 16 ? 8 : 16) four {
 };
 
 // What a wave loads of a block, as it lies in memory.
-template <typename T, typename S, int PER, int OT, int MT>
+template <typename S, int PER, int OT>
 struct loaded {
   u32x4_t w[OT];
   four<S, PER> scale[OT];
   uint32_t zero[OT];  // a byte for each group
-  raw8<T> x[MT][4];
 };
 
 template <typename T, typename S, bool ZEROS, int GROUP, int OT, int MT>
 __global__ __launch_bounds__(64 * kWaves) void k_q4(sg_q4_args a) {
   typedef typename mul<T>::type M;
   constexpr int PER = kBlockK / GROUP;  // groups of a block
-  typedef loaded<T, S, PER, OT, MT> L;
+  typedef loaded<S, PER, OT> L;
   __shared__ f32x4_t red[kWaves][OT * MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
   const int tiles = (a.out_dim + 15) / 16, kb = (a.in_dim + kBlockK - 1) / kBlockK;
@@ -170,19 +169,30 @@ __global__ __launch_bounds__(64 * kWaves) void k_q4(sg_q4_args a) {
         if constexpr (PER == 1) l.zero[o] = *z;
       }
     }
-    // (A lane of no row holds anything: its column of the product is no one's.)
+  };
+  raw8<T> r[MT][4];
+  // (A lane of no row holds anything: its column of the product is no one's.)
+  auto load_rows = [&](int b, int s) {
+    const int k = b * kBlockK + s * 32;
 #pragma unroll
     for (int m = 0; m < MT; m++)
       if (there[m])
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-          const int k = b * kBlockK + s * 32;
-#pragma unroll
-          for (int e = 0; e < (int)sizeof(T) / 2; e++)
-            l.x[m][s].v[e] = k < a.in_dim ? *reinterpret_cast<const u32x4_t*>(x[m] + k + e * (16 / (int)sizeof(T))) : u32x4_t{0, 0, 0, 0};
-        }
+        for (int e = 0; e < (int)sizeof(T) / 2; e++)
+          r[m][s].v[e] = k < a.in_dim ? *reinterpret_cast<const u32x4_t*>(x[m] + k + e * (16 / (int)sizeof(T))) : u32x4_t{0, 0, 0, 0};
   };
-  auto multiply = [&](const L& l) {
+  // The next block's weights are on their way while a block is multiplied, and its rows from the
+  // moment that a product has taken this one's.
+  L l, next;
+  if (wave < kb) {
+    load(wave, l);
+#pragma unroll
+    for (int s = 0; s < 4; s++) load_rows(wave, s);
+  }
+  for (int b = wave; b < kb; b += kWaves) {
+    const bool more = b + kWaves < kb;
+    if (more) load(b + kWaves, next);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int s0 = 0; s0 < PER; s0++) {
       f32x4_t sum[OT][MT] = {};
@@ -191,7 +201,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_q4(sg_q4_args a) {
         const int s = s0 * (4 / PER) + i;
         s16x8_t p[MT][mul<T>::parts];
 #pragma unroll
-        for (int m = 0; m < MT; m++) split<T>(l.x[m][s], p[m]);
+        for (int m = 0; m < MT; m++) split<T>(r[m][s], p[m]);
 #pragma unroll
         for (int o = 0; o < OT; o++) {
           const s16x8_t c = decode(l.w[o][s], offset<M>(ZEROS ? (int)(l.zero[o] >> s0 * 8 & 0xff) : 8));
@@ -200,6 +210,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_q4(sg_q4_args a) {
 #pragma unroll
             for (int e = 0; e < mul<T>::parts; e++) sum[o][m] = mma(M{}, c, p[m][e], sum[o][m]);
         }
+        if (more) load_rows(b + kWaves, s);
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int o = 0; o < OT; o++)
@@ -207,29 +219,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_q4(sg_q4_args a) {
         for (int m = 0; m < MT; m++)
 #pragma unroll
           for (int i = 0; i < 4; i++) acc[o][m][i] = __builtin_fmaf((float)l.scale[o].v[s0][i], sum[o][m][i], acc[o][m][i]);
-    }
-  };
-  // A block is on its way while the one before it is multiplied.
-  if (wave < kb) {
-    L l[2];
-    load(wave, l[0]);
-    int b = wave + kWaves;
-    for (; b + kWaves < kb; b += 2 * kWaves) {
-      load(b, l[1]);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(l[0]);
-      load(b + kWaves, l[0]);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(l[1]);
     }
-    if (b < kb) {
-      load(b, l[1]);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(l[0]);
-      multiply(l[1]);
-    } else {
-      multiply(l[0]);
-    }
+    l = next;
   }
 #pragma unroll
   for (int o = 0; o < OT; o++)
@@ -260,9 +252,16 @@ hipError_t launch(const sg_q4_args& a, hipStream_t s) {
 template <typename T, typename S, bool ZEROS, int GROUP>
 hipError_t by_rows(const sg_q4_args& a, hipStream_t s) {
   const int tiles = (a.out_dim + 15) / 16;
-  if (a.rows > 32) return launch<T, S, ZEROS, GROUP, 2, 4>(a, s);
-  if (a.rows > 16) return launch<T, S, ZEROS, GROUP, 2, 2>(a, s);
-  if (a.rows > 2 && tiles >= 1024) return launch<T, S, ZEROS, GROUP, 4, 1>(a, s);
+  if constexpr (sizeof(T) == 2) {
+    if (a.rows > 32) return launch<T, S, ZEROS, GROUP, 1, 4>(a, s);
+    if (a.rows > 16) return launch<T, S, ZEROS, GROUP, 1, 2>(a, s);
+    if (a.rows > 2 && tiles >= 1024) return launch<T, S, ZEROS, GROUP, 4, 1>(a, s);
+    if (a.rows > 2 && tiles >= 512) return launch<T, S, ZEROS, GROUP, 2, 1>(a, s);
+  } else {
+    if (a.rows > 16) return launch<T, S, ZEROS, GROUP, 2, 2>(a, s);
+    if (a.rows > 2 && tiles >= 1024) return launch<T, S, ZEROS, GROUP, 4, 1>(a, s);
+    if (tiles >= 512) return launch<T, S, ZEROS, GROUP, 2, 1>(a, s);
+  }
   return launch<T, S, ZEROS, GROUP, 1, 1>(a, s);
 }
 

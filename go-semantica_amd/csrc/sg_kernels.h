@@ -404,7 +404,7 @@ size_t adapters_work_bytes(int dtype, int rows, int in_dim, int rank_pad);
 hipError_t adapters_apply(const sg_adapters_args& a, int dtype, hipStream_t s);
 
 // ---- kept keys and values (k_kv_cache.hip, k_attn_shared*.hip) ----
-int64_t kv_rows_threads(int rows);
+int64_t kv_rows_threads(int rows, int heads);
 hipError_t kv_write(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
 hipError_t kv_read(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
 constexpr int attn_wide_pairs(int D) { return D == 256 ? 64 : 128; }  // of a job of the wide form

@@ -17,8 +17,7 @@ using sgc::kTile;
 using sgp::clamp_row;
 using sgp::elem;
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanSeqs = 4096, kPlanPrefixes = 512;  // numbers of so many are kept in LDS
+constexpr int kPlanSeqs = 2048, kPlanPrefixes = 512;  // numbers of so many are kept in LDS
 
 // The largest i in [0, n) with at(i) <= x for ascending at, 0 if there is none.
 template <typename F>
@@ -34,12 +33,12 @@ __device__ __forceinline__ int last_at_most(int n, int x, F at) {
 
 // Running totals over a workgroup: put(0, base), put(i + 1, before + count(i)), none above
 // `most`.  Returns the last.
-template <typename P, typename F>
+template <int THREADS, typename P, typename F>
 __device__ int64_t running(int n, int64_t base, int64_t most, P put, F count) {
-  __shared__ int64_t wave_sum[kPlanThreads / 64];
+  __shared__ int64_t wave_sum[THREADS / 64];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   if (t == 0) put(0, base);
-  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+  for (int i0 = 0; i0 < n; i0 += THREADS) {
     const int i = i0 + t;
     int64_t v = i < n ? count(i) : 0;
 #pragma unroll
@@ -51,7 +50,7 @@ __device__ int64_t running(int n, int64_t base, int64_t most, P put, F count) {
     if (lane == 63) wave_sum[wave] = v;
     __syncthreads();
     int64_t total = base;
-    for (int w = 0; w < kPlanThreads / 64; w++) {
+    for (int w = 0; w < THREADS / 64; w++) {
       if (w == wave) v += total;
       total += wave_sum[w];
     }
@@ -67,36 +66,50 @@ __device__ __forceinline__ int kept_length(int start, int length, int64_t slots)
   return start >= 0 && length > 0 && (int64_t)start + length <= slots ? length : 0;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args a, sg_attn_batch b, sg_attn_list la,
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg_attn_batch b, sg_attn_list la,
                                                             sg_attn_list lb, int one_list, int rows_wanted, int2* seen_out,
                                                             int4* where_out) {
   __shared__ int32_t off_lds[kPlanSeqs + 1], seq_jobs_lds[kPlanSeqs + 1];
   __shared__ int32_t group_lds[kPlanPrefixes + 1], prefix_jobs_lds[kPlanPrefixes + 1];
+  __shared__ int2 keys_lds[kPlanSeqs], prefix_lds[kPlanPrefixes];  // start, length (0 outside the cache)
   const int t = threadIdx.x;
   const bool small = b.n_seq <= kPlanSeqs, few = b.n_prefix <= kPlanPrefixes;
+  auto range = [&](int start, int length) { return make_int2(start, kept_length(start, length, b.slots)); };
   if (small)
-    for (int i = t; i <= b.n_seq; i += kPlanThreads) off_lds[i] = clamp_row(b.off[i], a.rows);
+    for (int i = t; i <= b.n_seq; i += THREADS) {
+      off_lds[i] = clamp_row(b.off[i], a.rows);
+      if (i < b.n_seq) keys_lds[i] = range(b.starts[i], b.lengths[i]);
+    }
   if (few && b.n_prefix > 0)
-    for (int i = t; i <= b.n_prefix; i += kPlanThreads) group_lds[i] = min(max(b.shared[i], 0), b.n_seq);
+    for (int i = t; i <= b.n_prefix; i += THREADS) {
+      group_lds[i] = min(max(b.shared[i], 0), b.n_seq);
+      if (i < b.n_prefix) prefix_lds[i] = range(b.prefix_starts[i], b.prefix_lengths[i]);
+    }
   __syncthreads();
   auto off = [&](int i) { return small ? off_lds[i] : clamp_row(b.off[i], a.rows); };
   auto group_at = [&](int p) { return few ? group_lds[p] : min(max(b.shared[p], 0), b.n_seq); };
   auto seq_jobs = [&](int i) { return small ? seq_jobs_lds[i] : b.seq_jobs[i]; };
   auto prefix_jobs = [&](int p) { return few ? prefix_jobs_lds[p] : b.prefix_jobs[p]; };
+  auto own_keys = [&](int i) { return small ? keys_lds[i] : range(b.starts[i], b.lengths[i]); };
+  auto prefix_keys = [&](int p) {
+    if (p < 0) return make_int2(0, 0);
+    return few ? prefix_lds[p] : range(b.prefix_starts[p], b.prefix_lengths[p]);
+  };
 
   // Jobs of each prefix and sequence: those of prefixes first where both stand in one list; with
   // all_keys there are only sequences'.
   const bool prefixes = b.n_prefix > 0 && !b.all_keys;
   int n_prefix_jobs = 0;
   if (prefixes)
-    n_prefix_jobs = (int)running(
+    n_prefix_jobs = (int)running<THREADS>(
         b.n_prefix, 0, la.cap, [&](int p, int64_t v) { few ? prefix_jobs_lds[p] = (int)v : b.prefix_jobs[p] = (int)v; },
         [&](int p) {
           const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
           return (rows * a.group + la.m - 1) / la.m;
         });
   const int own0 = one_list ? n_prefix_jobs : 0;
-  const int own_end = (int)running(
+  const int own_end = (int)running<THREADS>(
       b.n_seq, own0, lb.cap, [&](int i, int64_t v) { small ? seq_jobs_lds[i] = (int)v : b.seq_jobs[i] = (int)v; },
       [&](int i) { return ((int64_t)max(off(i + 1) - off(i), 0) * a.group + lb.m - 1) / lb.m; });
   auto prefix_of = [&](int i) {  // of a sequence; -1: none
@@ -104,11 +117,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
     const int p = last_at_most(b.n_prefix, i, group_at);
     return i >= group_at(p) && i < group_at(p + 1) ? p : -1;
   };
-  auto prefix_length = [&](int p) { return p < 0 ? 0 : kept_length(b.prefix_starts[p], b.prefix_lengths[p], b.slots); };
 
   // What each row sees of a prefix that sequences share, and where the join finds it.
   if (rows_wanted)
-    for (int row = t; row < a.rows; row += kPlanThreads) {
+    for (int row = t; row < a.rows; row += THREADS) {
       const int i = last_at_most(b.n_seq, row, off);
       const int r0 = off(i), r1 = off(i + 1);
       int4 seen = make_int4(0, 0, 0, 0), where = make_int4(-2, 0, -2, 0);
@@ -118,7 +130,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
         if (p >= 0) {
           where.x = prefix_jobs(p);
           where.y = off(group_at(p));
-          const int plen = prefix_length(p), len = kept_length(b.starts[i], b.lengths[i], b.slots);
+          const int plen = prefix_keys(p).y, len = own_keys(i).y;
           seen = sgc::places_seen((int64_t)plen + len - (r1 - r0) + (row - r0), plen, len, a.causal, a.window);
         }
       }
@@ -129,14 +141,14 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
 
   // The jobs, and the running total of their costs.
   auto fill = [&](const sg_attn_list& list, int j0, int n, int kind, int64_t base) {
-    const int64_t units = running(
+    const int64_t units = running<THREADS>(
         n, base, INT64_MAX, [&](int j, int64_t v) { list.cum[j0 + j] = v; },
         [&](int j) {
           const bool prefix = kind == kPrefixKeys;
           const int i = prefix ? last_at_most(b.n_prefix, j + j0, prefix_jobs) : last_at_most(b.n_seq, j + j0, seq_jobs);
           const int r0 = off(prefix ? group_at(i) : i), r1 = off(prefix ? group_at(i + 1) : i + 1), rows = max(r1 - r0, 0);
-          const int p = prefix ? i : prefix_of(i), plen = prefix_length(p);
-          const int len = prefix ? 0 : kept_length(b.starts[i], b.lengths[i], b.slots);
+          const int2 pk = prefix_keys(prefix ? i : prefix_of(i)), ok = prefix ? make_int2(0, 0) : own_keys(i);
+          const int plen = pk.y, len = ok.y;
           sg_attn_job job{r0, rows, j + j0 - (prefix ? prefix_jobs(i) : seq_jobs(i)), kind, {0, 0}, {0, 0}, {0, 0}, plen, len};
           const int from = (int)((int64_t)job.tile * list.m / a.group);
           const int to = (int)min((int64_t)rows, ((int64_t)(job.tile + 1) * list.m - 1) / a.group + 1);
@@ -145,7 +157,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
             lo[own] = min(lo[own], l < h ? l : INT32_MAX);
             hi[own] = max(hi[own], l < h ? h : 0);
           };
-          if (prefix) {
+          if (prefix && a.window == 0) {
+            see(0, 0, plen);  // (some row sees it all, as a rule, and a wave that does not looks at each key)
+          } else if (prefix) {
 #pragma unroll 8
             for (int r = from; r < to; r++) {
               const int2 s = seen_out[r0 + r];
@@ -161,8 +175,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_attn_plan(sg_attn_shared_args 
           }
           int64_t count = 0;
           for (int own = 0; own < 2; own++) {
-            if (own ? prefix : kind == kOwnKeys || p < 0) continue;
-            const int64_t start = own ? b.starts[i] : b.prefix_starts[p];
+            if (own ? prefix : kind == kOwnKeys) continue;
+            const int64_t start = own ? ok.x : pk.x;
             // (Cut once more: where offsets do not ascend, a row's range is another group's.)
             const int end = min(hi[own], own ? len : plen);
             if (lo[own] >= end) continue;
@@ -427,8 +441,11 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
   const sg_attn_list& la = lists[wide_prefix];
   const int one_list = &la == &lb;
   const int rows_wanted = !b.all_keys || (int64_t)a.rows * a.heads <= kJoinSome;
+  // Few rows and sequences: four waves, which meet sooner than sixteen.
+  const int threads = a.rows > 512 || b.n_seq > 512 || b.n_prefix > 512 ? 1024 : 256;
   hipError_t e =
-      sgp::run_kernel(k_attn_plan, dim3(1), dim3(kPlanThreads), 0, s, a, b, la, lb, one_list, rows_wanted, seen, where);
+      sgp::run_kernel(threads == 1024 ? k_attn_plan<1024> : k_attn_plan<256>, dim3(1), dim3(threads), 0, s, a, b, la, lb, one_list,
+                      rows_wanted, seen, where);
   auto run = [&](const sg_attn_list& l) {
     if (e != hipSuccess) return;
     e = dtype == SG_F32   ? attn_shared_f32(a, l, q8, D, s)

@@ -20,7 +20,9 @@
 // score, the values' the weight.  With fp16 queries that product would leave fp16's range,
 // so weights are split into two bf16 halves (2^-17 of each, exponents of float32) and the
 // codes taken as bf16; with bf16 queries one rounding to bf16 is what the plain form of the
-// type has as well.  float32 goes through float32 matrix products.
+// type has as well.  float32 queries and weights go over codes as three bf16 parts, 24 bits (48
+// cycles of 32 products of 16 and 16 where float32's own take 256); over float32 keys and
+// values it goes through float32 matrix products.
 #pragma once
 #include <atomic>
 
@@ -63,6 +65,13 @@ __device__ __forceinline__ f32x4_t mma(float, const f32x8_t& a, const f32x8_t& b
 #pragma unroll
   for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j >> 2][j & 3], b.v[j >> 2][j & 3], c, 0, 0, 0);
   return c;
+}
+// A part of a score.  (float32: 32 products by themselves, then added: shorter sums are nearer, and
+// do not wait for each other, which few waves gain by; many lose 7 %.)
+template <typename K, typename F>
+__device__ __forceinline__ f32x4_t add_score(const F& a, const F& b, f32x4_t c) {
+  if constexpr (__is_same(K, float)) return c + mma(K{}, a, b, f32x4_t{0, 0, 0, 0});
+  else return mma(K{}, a, b, c);
 }
 
 // Eight codes (two words) as M.
@@ -163,6 +172,22 @@ struct weight<bf16_t, true> {
   typedef bf16_t type;
   static constexpr int parts = 1;
 };
+template <>
+struct weight<float, true> {
+  typedef bf16_t type;
+  static constexpr int parts = 3;
+};
+// The same of keys and queries.
+template <typename T, bool Q8>
+struct query {
+  typedef T type;
+  static constexpr int parts = 1;
+};
+template <>
+struct query<float, true> {
+  typedef bf16_t type;
+  static constexpr int parts = 3;
+};
 // fp16 weights are multiplied by 2^6, so that they keep their bits down to 2^-20; sums and outputs
 // alike, so it leaves by itself.
 template <typename T, bool Q8>
@@ -170,7 +195,7 @@ constexpr float kShift = __is_same(T, _Float16) && !Q8 ? 6.0f : 0.0f;
 // A tile's sum of weights from which on a pair's maximum is raised (and its sums rescaled): far
 // above 32 weights of 1, within the weights' type.
 template <typename T, bool Q8>
-constexpr float kMost = __is_same(T, _Float16) && !Q8 ? 0x1p14f : 0x1p20f;
+constexpr float kMost = __is_same(T, _Float16) && !Q8 ? 0x1p14f : 0x1p10f;
 
 // Sums of weights by the matrix core: 16-bit types whose weights are multiplied as they are.
 template <typename T, bool Q8>
@@ -179,7 +204,7 @@ constexpr bool kSumByProduct = !Q8 && sizeof(T) == 2;
 // What a wave has of its QT * 16 pairs: queries, running maxima and sums, outputs.
 template <typename T, bool Q8, int D, int QT>
 struct state {
-  typename frag<T>::type q[QT][D / 32];
+  typename frag<typename query<T, Q8>::type>::type q[QT][D / 32][query<T, Q8>::parts];
   f32x4_t o[QT][D / 16];
   float m[QT], l[QT];
   float base[QT], most[QT];  // what scores are taken against: m, shifted; the sum that raises it
@@ -190,6 +215,7 @@ struct state {
 // Eight weights as operands of the second product.
 template <typename T, bool Q8>
 __device__ __forceinline__ void pack_weights(const float* p, typename frag<typename weight<T, Q8>::type>::type* w) {
+  typedef typename query<T, Q8>::type K;
   typedef typename weight<T, Q8>::type M;
   if constexpr (__is_same(M, float)) {
 #pragma unroll
@@ -204,11 +230,16 @@ __device__ __forceinline__ void pack_weights(const float* p, typename frag<typen
 #pragma unroll
     for (int j = 0; j < 8; j++) x[j] = (__bf16)p[j];
     w[0] = __builtin_bit_cast(s16x8_t, x);
-    if constexpr (weight<T, Q8>::parts == 2) {
-      sgp::bf16x8_t y;
+    if constexpr (weight<T, Q8>::parts >= 2) {
+      sgp::bf16x8_t y, z;
 #pragma unroll
-      for (int j = 0; j < 8; j++) y[j] = (__bf16)(p[j] - (float)x[j]);
+      for (int j = 0; j < 8; j++) {
+        const float rest = p[j] - (float)x[j];
+        y[j] = (__bf16)rest;
+        z[j] = (__bf16)(rest - (float)y[j]);
+      }
       w[1] = __builtin_bit_cast(s16x8_t, y);
+      if constexpr (weight<T, Q8>::parts == 3) w[2] = __builtin_bit_cast(s16x8_t, z);
     }
   }
 }
@@ -418,7 +449,24 @@ __device__ __forceinline__ void begin_job(const sg_attn_shared_args& a, state<T,
           x ^= (short)0x8000;
         }
       }
-      st.q[t][d] = x;
+      if constexpr (query<T, Q8>::parts == 3) {
+        // Cut off, not rounded: eight bits each, and their sum is the query.
+        s16x8_t part[3];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const uint32_t u = __float_as_uint(x.v[j >> 2][j & 3]), hi = u & 0xffff0000u;
+          // (An infinity less itself would be a NaN: it has no further parts.)
+          const float rest = (u & 0x7f800000u) == 0x7f800000u ? 0.0f : __uint_as_float(u) - __uint_as_float(hi);
+          const uint32_t mid = __float_as_uint(rest) & 0xffff0000u;
+          part[0][j] = (short)(hi >> 16);
+          part[1][j] = (short)(mid >> 16);
+          part[2][j] = (short)(__float_as_uint(rest - __uint_as_float(mid)) >> 16);
+        }
+#pragma unroll
+        for (int h = 0; h < 3; h++) st.q[t][d][h] = part[h];
+      } else {
+        st.q[t][d][0] = x;
+      }
     }
     st.m[t] = -INFINITY;
     st.l[t] = 0.0f;
@@ -525,6 +573,7 @@ __device__ __forceinline__ part part_of(const sg_attn_list& list, const sg_attn_
 // Few pairs: every wave is a worker and takes fragments from memory, no barrier anywhere.
 template <typename T, bool Q8, int D>
 __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narrow(sg_attn_shared_args a, sg_attn_list list) {
+  typedef typename query<T, Q8>::type K;
   typedef typename weight<T, Q8>::type M;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t worker = (int64_t)spread(blockIdx.x, gridDim.x) * 4 + wave;
@@ -562,7 +611,9 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
 #pragma unroll
               for (int e = 0; e < 2; e++) {
                 const int f = i * 2 + e, half = f / (D / 32), d = f % (D / 32);
-                s[half][0] = mma(T{}, decode<T>(kc[i][e * 2], kc[i][e * 2 + 1]), st.q[0][d], s[half][0]);
+                const typename frag<K>::type x = decode<K>(kc[i][e * 2], kc[i][e * 2 + 1]);
+#pragma unroll
+                for (int h = query<T, Q8>::parts - 1; h >= 0; h--) s[half][0] = add_score<K>(x, st.q[0][d][h], s[half][0]);
               }
             weigh<T, Q8, D, 1>(a, st, s, first, reinterpret_cast<const float*>(tail), lane, w);
 #pragma unroll
@@ -571,7 +622,7 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
               for (int e = 0; e < 2; e++) {
                 const typename frag<M>::type x = decode<M>(vc[i][e * 2], vc[i][e * 2 + 1]);
 #pragma unroll
-                for (int h = 0; h < weight<T, Q8>::parts; h++) st.o[0][i * 2 + e] = mma(M{}, x, w[0][h], st.o[0][i * 2 + e]);
+                for (int h = weight<T, Q8>::parts - 1; h >= 0; h--) st.o[0][i * 2 + e] = mma(M{}, x, w[0][h], st.o[0][i * 2 + e]);
               }
           } else {
             const bool bad = *reinterpret_cast<const uint32_t*>(tail) != 0;
@@ -579,7 +630,7 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
             for (int half = 0; half < 2; half++)
 #pragma unroll
               for (int d = 0; d < D / 32; d++)
-                s[half][0] = mma(T{}, load_frag<T>(at, half * (D / 32) + d, lane), st.q[0][d], s[half][0]);
+                s[half][0] = add_score<T>(load_frag<T>(at, half * (D / 32) + d, lane), st.q[0][d][0], s[half][0]);
             weigh<T, Q8, D, 1>(a, st, s, first, nullptr, lane, w);
 #pragma unroll
             for (int f = 0; f < D / 16; f++) {
@@ -605,20 +656,21 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
 
 // Many pairs: a workgroup is a worker, its four waves have QT * 16 pairs each and share the tiles
 // in LDS, two stages.  Types go there by direct copies; codes through registers, and lie there
-// as the type that multiplies them.  16-bit types of up to 128 dims copy codes to LDS as they
+// as the type that multiplies them.  Codes of up to 128 dims go to LDS as they
 // are first, kRing tiles of them, each wave its own quarter (and the scales): a tile of codes is
 // 8 KB, and one or two a CU in flight reach half of the memory's rate.
 constexpr int kRing = 4;
 template <typename T, bool Q8, int D, int NW>
 struct wide_lds {
-  static constexpr int KB = kTile * D * (int)sizeof(T);  // keys of a tile
-  static constexpr bool ring = Q8 && sizeof(T) == 2 && D <= 128 && D / 16 >= NW;
+  static constexpr int KB = kTile * D * (int)sizeof(typename query<T, Q8>::type);  // keys of a tile
+  static constexpr bool ring = Q8 && D <= 128 && D / 16 >= NW;
   static constexpr int stage = 2 * KB + (Q8 && !ring ? kTail : 0);
   static constexpr int part = D / 16 * 1024 / NW + kTail;  // a wave's part of a tile of codes
   static constexpr int bytes = 2 * stage + (ring ? kRing * NW * part : 0);
 };
 template <typename T, bool Q8, int D, int QT, int NW, int PER_CU>
 __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_shared_args a, sg_attn_list list) {
+  typedef typename query<T, Q8>::type K;
   typedef typename weight<T, Q8>::type M;
   typedef wide_lds<T, Q8, D, NW> L;
   constexpr int KB = L::KB, STAGE = L::stage;
@@ -674,7 +726,7 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               const int k = wave * NU + i, f = k * 2 + e;  // fragment of keys, then of values
-              if (k < D / 32) store_frag<T>(to, f, lane, decode<T>(codes[i][e * 2], codes[i][e * 2 + 1]));
+              if (k < D / 32) store_frag<K>(to, f, lane, decode<K>(codes[i][e * 2], codes[i][e * 2 + 1]));
               else store_frag<M>(to + KB, f - D / 16, lane, decode<M>(codes[i][e * 2], codes[i][e * 2 + 1]));
             }
           if (!RING && wave == 0) *reinterpret_cast<float*>(to + 2 * KB + lane * 4) = tail_of;
@@ -721,12 +773,12 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
           }
           // Fragments come from LDS NB at a time, a batch ahead of its products (the first values
           // ahead of the softmax): one by one they would cost their latency each.
-          constexpr int NF = D / 16, NB = sizeof(T) == 2 ? 8 : 2, NBATCH = (NF + NB - 1) / NB, N0 = NF < NB ? NF : NB;
-          typename frag<T>::type kx[2][N0];
+          constexpr int NF = D / 16, NB = sizeof(K) == 2 ? 8 : 2, NBATCH = (NF + NB - 1) / NB, N0 = NF < NB ? NF : NB;
+          typename frag<K>::type kx[2][N0];
           typename frag<M>::type vx[2][N0];
           auto load_keys = [&](int i) {
 #pragma unroll
-            for (int e = 0; e < N0; e++) kx[i & 1][e] = load_frag<T>(keys, i * N0 + e, lane);
+            for (int e = 0; e < N0; e++) kx[i & 1][e] = load_frag<K>(keys, i * N0 + e, lane);
           };
           auto load_vals = [&](int i) {
 #pragma unroll
@@ -743,7 +795,9 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
             for (int e = 0; e < N0; e++) {
               const int f = i * N0 + e, half = f / (D / 32), d = f % (D / 32);
 #pragma unroll
-              for (int t = 0; t < QT; t++) s[half][t] = mma(T{}, kx[i & 1][e], st.q[t][d], s[half][t]);
+              for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int h = query<T, Q8>::parts - 1; h >= 0; h--) s[half][t] = mma(K{}, kx[i & 1][e], st.q[t][d][h], s[half][t]);
             }
           }
           if (RING && u + 1 < tiles) put(stage ^ 1, u + 1, tiles);  // (while the scores come)
@@ -761,7 +815,7 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
 #pragma unroll
               for (int t = 0; t < QT; t++)
 #pragma unroll
-                for (int h = 0; h < weight<T, Q8>::parts; h++)
+                for (int h = weight<T, Q8>::parts - 1; h >= 0; h--)
                   st.o[t][i * N0 + e] = mma(M{}, vx[i & 1][e], w[t][h], st.o[t][i * N0 + e]);
           }
           if constexpr (!Q8)
@@ -784,7 +838,7 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
 // Waves of a workgroup, pairs of each, workgroups of a CU.
 template <typename T, bool Q8, int D>
 struct wide_form {
-  static constexpr int NW = 4;
+  static constexpr int NW = __is_same(T, float) && Q8 && D == 128 ? 8 : 4;
   static constexpr int QT = sgk::attn_wide_pairs(D) / (16 * NW);
   static constexpr int PER_CU = sizeof(T) == 4 && D >= 128 ? 1 : 2;
 };

@@ -321,13 +321,29 @@ __global__ __launch_bounds__(256) void k_attn_join_split(sg_attn_shared_args a, 
   const holders h = holders_of(list, kv, job);
   if (!h.any || h.first != worker || h.last == worker) return;
   const sg_attn_job jb = list.jobs[job];
-  for (int in_job = blockIdx.y * 16 + wave; in_job < min((int)blockIdx.y * 16 + 16, list.m); in_job += 4) {
-    const int64_t pair = (int64_t)jb.tile * list.m + in_job;
-    if (pair >= (int64_t)jb.rows * a.group) return;
+  // Four pairs a wave, a piece of each at a time.
+  const int in_job = blockIdx.y * 16 + wave * 4;
+  const int64_t pair0 = (int64_t)jb.tile * list.m + in_job, pairs = (int64_t)jb.rows * a.group;
+  if (pair0 >= pairs) return;
+  joined<D> x[4];
+  for (int64_t w = h.first; w <= h.last; w++) {
+    float2 ml[4];
+    typename joined<D>::vec o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t at = piece_of(list, w, w == h.first, in_job + (int)min((int64_t)i, pairs - 1 - pair0));
+      ml[i] = a.part_ml[at];
+      o[i] = *reinterpret_cast<const typename joined<D>::vec*>(a.part_o + at * D + lane * joined<D>::V);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i].add(ml[i].x, ml[i].y, o[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int64_t pair = pair0 + i;
+    if (pair >= pairs) return;
     const int r = (int)(pair / a.group);
-    joined<D> x;
-    x.add(a, h.first, h.last, 1, lane, [&](int64_t w) { return piece_of(list, w, w == h.first, in_job); });
-    x.template put<T>(a, jb.row0 + r, kv * a.group + (int)(pair - (int64_t)r * a.group), lane);
+    x[i].template put<T>(a, jb.row0 + r, kv * a.group + (int)(pair - (int64_t)r * a.group), lane);
   }
 }
 
@@ -344,7 +360,7 @@ struct layout {
 };
 
 // Lists: 0 narrow, 1 wide.  All sizes grow with each of the arguments.
-layout lay_out(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix) {
+layout lay_out(int dtype, bool q8, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix) {
   layout y{};
   const int64_t pairs = (int64_t)rows * (heads / kv_heads);
   y.cap = (int)std::min<int64_t>(2 * (pairs / 16) + n_seq + n_prefix + 2, INT32_MAX);
@@ -352,7 +368,7 @@ layout lay_out(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, i
   y.workers[0] = cus * 4 * (dtype == SG_F32 ? 1 : 2);
   y.workers[1] = cus * (dtype == SG_F32 && D >= 128 ? 1 : 2);
   y.m[0] = 16;
-  y.m[1] = sgk::attn_wide_pairs(D);
+  y.m[1] = sgk::attn_wide_pairs(D, dtype == SG_F32, q8);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -400,12 +416,12 @@ hipError_t join_dims(const sg_attn_shared_args& a, const sg_attn_list& la, const
 
 namespace sgk {
 
-size_t attn_shared_work_bytes(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix) {
-  return lay_out(dtype, rows, heads, kv_heads, D, n_seq, n_prefix).total;
+size_t attn_shared_work_bytes(int dtype, bool q8, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix) {
+  return lay_out(dtype, q8, rows, heads, kv_heads, D, n_seq, n_prefix).total;
 }
 
 hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q8, int D, void* work, hipStream_t s) {
-  const layout y = lay_out(dtype, a.rows, a.heads, a.kv_heads, D, b.n_seq, b.n_prefix);
+  const layout y = lay_out(dtype, q8, a.rows, a.heads, a.kv_heads, D, b.n_seq, b.n_prefix);
   char* w = static_cast<char*>(work);
   int2* seen = reinterpret_cast<int2*>(w + y.seen);
   int4* where = reinterpret_cast<int4*>(w + y.where);

@@ -83,8 +83,8 @@ __device__ __forceinline__ void row_slots(const sg_kv_rows_args& a, int row0, in
     sgp::row_seq(a.off, a.n_seq, base, last, min(row, last), lane, i, s0, s1);
     const bool there = row <= last && row >= s0 && row < s1;
     const int start = a.starts[i];
-    const int64_t s = (int64_t)start + (row - s0);
-    const bool in = there && start >= 0 && s < a.slots;
+    const int64_t s = (int64_t)start + row - s0;
+    const bool in = there && start >= 0 && s >= 0 && s < a.slots;
     if (wave * 64 + lane < count) slot[wave * 64 + lane] = in ? (int)s : there ? kNone : kNoRow;
     if (in) {
       lo = hi = (int)s;

@@ -838,9 +838,10 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
 // Waves of a workgroup, pairs of each, workgroups of a CU.
 template <typename T, bool Q8, int D>
 struct wide_form {
-  static constexpr int NW = __is_same(T, float) && Q8 && D == 128 ? 8 : 4;
-  static constexpr int QT = sgk::attn_wide_pairs(D) / (16 * NW);
-  static constexpr int PER_CU = sizeof(T) == 4 && D >= 128 ? 1 : 2;
+  static constexpr bool F32 = __is_same(T, float);
+  static constexpr int NW = F32 && D == (Q8 ? 128 : 256) ? 8 : 4;
+  static constexpr int QT = sgk::attn_wide_pairs(D, F32, Q8) / (16 * NW);
+  static constexpr int PER_CU = F32 && D >= 128 ? 1 : 2;
 };
 
 template <typename T, bool Q8, int D>

@@ -151,7 +151,7 @@ int sg_attention_shared_work_bytes(const sg_kv_cache* cache, int32_t n_heads, in
                                    int32_t n_prefix, size_t* bytes) {
   if (!cache || !bytes) return fail(SG_ERR_INVALID, "NULL argument");
   SG_TRY(check_attention(cache, n_heads, rows, n_seq, n_prefix));
-  *bytes = sgk::attn_shared_work_bytes(cache->dtype, rows, n_heads, cache->heads, cache->D, n_seq, n_prefix);
+  *bytes = sgk::attn_shared_work_bytes(cache->dtype, cache->q8, rows, n_heads, cache->heads, cache->D, n_seq, n_prefix);
   return SG_OK;
 }
 
@@ -176,7 +176,7 @@ int sg_attention_shared(sg_ctx* ctx, void* out, int64_t ldo, const void* q, int6
   SG_TRY(check_pieces("out", so));
   SG_TRY(check_pieces("q", sq));
   if (so.overlaps(sq)) return fail(SG_ERR_INVALID, "out overlaps q");
-  const size_t need = sgk::attn_shared_work_bytes(cache->dtype, rows, n_heads, cache->heads, cache->D, n_seq, keys->n_prefix);
+  const size_t need = sgk::attn_shared_work_bytes(cache->dtype, cache->q8, rows, n_heads, cache->heads, cache->D, n_seq, keys->n_prefix);
   if (!work || work_bytes < need || reinterpret_cast<uintptr_t>(work) % 16)
     return fail(SG_ERR_INVALID, "work: %zu bytes, 16-byte aligned, are needed (%zu given)", need, work ? work_bytes : 0);
   const uintptr_t w0 = reinterpret_cast<uintptr_t>(work), w1 = w0 + need;

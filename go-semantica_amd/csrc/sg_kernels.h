@@ -407,8 +407,9 @@ hipError_t adapters_apply(const sg_adapters_args& a, int dtype, hipStream_t s);
 int64_t kv_rows_threads(int rows, int heads);
 hipError_t kv_write(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
 hipError_t kv_read(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
-constexpr int attn_wide_pairs(int D) { return D == 256 ? 64 : 128; }  // of a job of the wide form
-size_t attn_shared_work_bytes(int dtype, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix);
+// Pairs of a job of the wide form.
+constexpr int attn_wide_pairs(int D, bool f32, bool q8) { return D == 256 && !(f32 && !q8) ? 64 : 128; }
+size_t attn_shared_work_bytes(int dtype, bool q8, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix);
 // a's workspace pointers, seen and where, and the batch's arrays, are placed in work.
 hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q8, int D, void* work, hipStream_t s);
 hipError_t attn_shared_f32(const sg_attn_shared_args& a, const sg_attn_list& list, bool q8, int D, hipStream_t s);

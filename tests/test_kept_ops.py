@@ -702,3 +702,345 @@ def test_refusals_without_a_gpu():
     assert lib.sg_q4_weight_create_q4_0(None, None, 1, 32, ctypes.byref(out)) == bad
     assert lib.sg_matmul_q4(None, None, 0, None, None, 0, 0, 1, None) == bad
     lib.sg_q4_weight_free(None)
+
+
+def refused(call, *words):
+    from semantica_gpu import _lib
+    with pytest.raises((ValueError, _lib.SemanticaError)) as e:
+        call()
+    assert all(w in str(e.value) for w in words), str(e.value)
+
+
+@pytest.mark.gpu
+def test_refusals(gpu_ctx):
+    """What a call cannot do it says, and it leaves the outputs alone."""
+    from semantica_gpu import kernels
+    bf16, f32 = torch.bfloat16, torch.float32
+    refused(lambda: kernels.KVCache(gpu_ctx, 10, 1, 64, torch.int8), "float32")
+    refused(lambda: kernels.KVCache(gpu_ctx, 10, 1, 64, bf16, bits=4), "bits 4")
+    refused(lambda: kernels.KVCache(gpu_ctx, 0, 1, 64, bf16), "slots 0")
+    refused(lambda: kernels.KVCache(gpu_ctx, 10, 0, 64, bf16), "0 key heads")
+    for hd in (0, 12, 264):
+        refused(lambda: kernels.KVCache(gpu_ctx, 10, 1, hd, bf16), "head_dim")
+    cache = kernels.KVCache(gpu_ctx, 40, 2, 64, bf16)
+    assert cache.nbytes == 2 * 2 * (2 * 32 * 64 + 256)
+    off, starts = offsets([3]).cuda(), ints([0]).cuda()
+    k = torch.zeros(3, 128, dtype=bf16, device="cuda")
+    refused(lambda: kernels.kv_cache_write(gpu_ctx, cache, k.float(), k, off, starts), "k")
+    refused(lambda: kernels.kv_cache_write(gpu_ctx, cache, k[:, :64], k, off, starts), "shape")
+    refused(lambda: kernels.kv_cache_write(gpu_ctx, cache, k, k.cpu(), off, starts), "device")
+    refused(lambda: kernels.kv_cache_write(gpu_ctx, cache, k, k, off.long(), starts), "offsets")
+    refused(lambda: kernels.kv_cache_write(gpu_ctx, cache, k, k, off, ints([0, 1]).cuda()), "starts")
+    refused(lambda: kernels.kv_cache_read(gpu_ctx, k, k, cache, off, starts), "overlaps")
+    odd = torch.zeros(3, 140, dtype=bf16, device="cuda")
+    refused(lambda: kernels.kv_cache_write(gpu_ctx, cache, odd[:, 1:129], k, off, starts), "16")
+    q, out = torch.zeros(3, 256, dtype=bf16, device="cuda"), torch.full((3, 256), 7.0, dtype=bf16, device="cuda")
+    lengths = ints([3]).cuda()
+
+    def attend(o=out, x=q, heads=4, **kw):
+        kernels.attention_shared(gpu_ctx, o, x, cache, heads, off, starts, lengths, **kw)
+
+    refused(lambda: attend(heads=3), "q: shape")
+    refused(lambda: attend(o=q), "overlaps")
+    refused(lambda: attend(x=q.float()), "q")
+    refused(lambda: attend(window=-1), "window")
+    refused(lambda: attend(softcap=-1.0), "softcap")
+    refused(lambda: attend(scale=math.nan), "scale")
+    refused(lambda: attend(scale=1e30), "scale")
+    refused(lambda: attend(shared=ints([0, 1]).cuda()), "shared")
+    refused(lambda: attend(shared=ints([0, 1]).cuda(), prefix_starts=ints([0, 1]).cuda(), prefix_lengths=ints([1]).cuda()), "prefix_starts")
+    size = cache.work_bytes(4, 3, 1, 0)
+    refused(lambda: attend(work=torch.empty(size - 1, dtype=torch.uint8, device="cuda")), "work")
+    refused(lambda: attend(work=torch.empty(size + 8, dtype=torch.uint8, device="cuda")[8:]), "work")
+    refused(lambda: cache.work_bytes(3, 3, 1, 0), "heads")
+    refused(lambda: cache.work_bytes(4, -1, 1, 0), "rows")
+    for more in ((4, 4, 1, 0), (4, 3, 2, 0), (4, 3, 1, 5)):
+        assert cache.work_bytes(*more) >= size
+    assert bool((out == 7).all())
+    three = kernels.KVCache(gpu_ctx, 40, 3, 64, bf16)
+    refused(lambda: kernels.attention_shared(gpu_ctx, out, q, three, 4, off, starts, lengths), "heads")
+    three.close()
+    cache.close()
+    codes, scales = torch.zeros(8, 64, dtype=torch.uint8, device="cuda"), torch.ones(8, 4, dtype=torch.float16, device="cuda")
+    refused(lambda: kernels.Q4Weight(gpu_ctx, codes, scales[:, :3]), "scales")
+    refused(lambda: kernels.Q4Weight(gpu_ctx, codes, torch.ones(8, 8, device="cuda")), "group 16")
+    refused(lambda: kernels.Q4Weight(gpu_ctx, codes.int(), scales), "codes")
+    refused(lambda: kernels.Q4Weight(gpu_ctx, codes, scales.double()), "float")
+    refused(lambda: kernels.Q4Weight(gpu_ctx, codes, scales, codes), "zeros")
+    refused(lambda: kernels.Q4Weight.from_q4_0(gpu_ctx, np.zeros(17, np.uint8), 1, 32), "Q4_0")
+    w = kernels.Q4Weight(gpu_ctx, codes, scales)
+    x, dst = torch.zeros(2, 128, device="cuda"), torch.zeros(2, 8, device="cuda")
+    refused(lambda: kernels.matmul_q4(gpu_ctx, dst, w, x[:, :64]), "x: shape")
+    refused(lambda: kernels.matmul_q4(gpu_ctx, dst.half(), w, x), "dst")
+    refused(lambda: kernels.matmul_q4(gpu_ctx, x[:, :8], w, x), "overlaps")
+    wide = torch.zeros(2, 132, device="cuda")
+    refused(lambda: kernels.matmul_q4(gpu_ctx, dst, w, wide[:, 1:129]), "16")
+    w.close()
+    del f32
+
+
+@pytest.mark.gpu
+def test_nothing_to_do(gpu_ctx):
+    """Calls without rows, and sequences without rows."""
+    from semantica_gpu import kernels
+    cache = make_cache(gpu_ctx, 40, 1, 64, "bf16", 8)
+    none = torch.zeros(0, 64, dtype=torch.bfloat16, device="cuda")
+    off, starts = offsets([0, 0]).cuda(), ints([0, 5]).cuda()
+    kernels.kv_cache_write(gpu_ctx, cache, none, none, off, starts)
+    kernels.kv_cache_read(gpu_ctx, none, none.clone(), cache, off, starts)
+    kernels.attention_shared(gpu_ctx, none, none.clone(), cache, 1, off, starts, ints([3, 3]).cuda())
+    some = torch.full((4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    kernels.attention_shared(gpu_ctx, some, some.clone(), cache, 1, off, starts, ints([3, 3]).cuda())
+    kernels.kv_cache_read(gpu_ctx, some, some.clone(), cache, off, starts)
+    assert bool((some == 7).all())
+    w = kernels.Q4Weight(gpu_ctx, torch.zeros(8, 16, dtype=torch.uint8, device="cuda"), torch.ones(8, 1, device="cuda"))
+    kernels.matmul_q4(gpu_ctx, torch.zeros(0, 8, device="cuda"), w, torch.zeros(0, 32, device="cuda"))
+    w.close()
+    cache.close()
+
+
+# ---- together, and as programs run them -------------------------------------------------------
+
+
+class Served:
+    """A document kept once, and sequences that grow behind it a token at a time."""
+
+    def __init__(self, ctx, dtype, bits, seed, n=5, heads=8, kv_heads=2, hd=64, wide=256, doc=77, room=9):
+        from semantica_gpu import kernels
+        self.ctx, self.dtype, self.bits, self.n, self.heads, self.kv_heads, self.hd = ctx, dtype, bits, n, heads, kv_heads, hd
+        self.g, self.wide, self.doc, self.room = gen(seed), wide, doc, room
+        made = {m: q4_make(self.g, c, k, 64, "f16", True)
+                for m, (c, k) in {"qkv": ((heads + 2 * kv_heads) * hd, wide), "o": (wide, heads * hd)}.items()}
+        self.dense = {m: q4_dense(*v) for m, v in made.items()}
+        self.w = {m: kernels.Q4Weight(ctx, *(t.cuda() for t in v)) for m, v in made.items()}
+        self.slots = doc + n * room
+        self.cache = make_cache(ctx, self.slots, kv_heads, hd, dtype, bits)
+        self.kept = torch.zeros(2, self.slots, kv_heads * hd, dtype=dt(dtype))
+        self.off, self.starts = offsets([1] * n).cuda(), ints([doc + i * room for i in range(n)]).cuda()
+        self.lengths, self.slot = ints([0] * n).cuda(), self.starts.clone()
+        self.shared = [ints([0, n]).cuda(), ints([0]).cuda(), ints([doc]).cuda()]
+        d = dt(dtype)
+        self.x = torch.empty(n, wide, dtype=d, device="cuda")
+        self.qkv = torch.empty(n, (heads + 2 * kv_heads) * hd, dtype=d, device="cuda")
+        self.att = torch.empty(n, heads * hd, dtype=d, device="cuda")
+        self.y = torch.empty(n, wide, dtype=d, device="cuda")
+        self.work = torch.empty(self.cache.work_bytes(heads, n, n, 1), dtype=torch.uint8, device="cuda")
+
+    def parts(self, qkv):
+        a, b = self.heads * self.hd, (self.heads + self.kv_heads) * self.hd
+        return qkv[:, :a], qkv[:, a:b], qkv[:, b:]
+
+    def document(self):
+        from semantica_gpu import kernels
+        x = rand(self.g, self.doc, self.wide, dtype=self.dtype)
+        qkv = torch.empty(self.doc, self.qkv.shape[1], dtype=self.x.dtype, device="cuda")
+        kernels.matmul_q4(self.ctx, qkv, self.w["qkv"], x.cuda())
+        _, k, v = self.parts(qkv)
+        kernels.kv_cache_write(self.ctx, self.cache, k, v, offsets([self.doc]).cuda(), ints([0]).cuda())
+        self.kept[0, :self.doc], self.kept[1, :self.doc] = k.cpu(), v.cpu()
+
+    def step(self):
+        """One token of each sequence, in the tensors of the object."""
+        from semantica_gpu import kernels
+        kernels.matmul_q4(self.ctx, self.qkv, self.w["qkv"], self.x)
+        q, k, v = self.parts(self.qkv)
+        kernels.kv_cache_write(self.ctx, self.cache, k, v, self.off, self.slot)
+        self.lengths += 1
+        self.slot += 1
+        kernels.attention_shared(self.ctx, self.att, q, self.cache, self.heads, self.off, self.starts, self.lengths,
+                                 *self.shared, work=self.work)
+        kernels.matmul_q4(self.ctx, self.y, self.w["o"], self.att)
+
+    def check(self, t):
+        """What step t left, each part from the values that it was given."""
+        x, qkv, att, y = (a.cpu() for a in (self.x, self.qkv, self.att, self.y))
+        want = x.double() @ self.dense["qkv"].t()
+        close(qkv, want, q4_tol(self.dtype, x, self.dense["qkv"], want), "projection")
+        q, k, v = self.parts(qkv)
+        for i in range(self.n):
+            at = self.doc + i * self.room + t
+            self.kept[0, at], self.kept[1, at] = k[i], v[i]
+        kr, vr = (kept_ref(a, self.kv_heads, self.bits)[0] for a in self.kept)
+        lengths = ints([t + 1] * self.n)
+        want, mean, size = shared_ref(q, kr, vr, self.off.cpu(), self.heads, self.kv_heads, self.starts.cpu(), lengths,
+                                      *(a.cpu() for a in self.shared))
+        close(att, want, shared_tol(self.dtype, self.bits, self.hd, self.doc + t + 1, want, mean, size), "attention")
+        want = att.double() @ self.dense["o"].t()
+        close(y, want, q4_tol(self.dtype, att, self.dense["o"], want), "output")
+
+    def close(self):
+        self.cache.close()
+        for w in self.w.values():
+            w.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+def test_served_tokens(gpu_ctx, dtype, bits):
+    """Projection, cache, attention behind a kept document and output, token by token."""
+    s = Served(gpu_ctx, dtype, bits, 21)
+    s.document()
+    for t in range(4):
+        s.x.copy_(rand(s.g, s.n, s.wide, dtype=dtype))
+        s.step()
+        s.check(t)
+    s.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [0, 8])
+def test_served_tokens_by_a_replayed_graph(gpu_ctx, bits):
+    """One captured step serves every token: lengths and slots are read on the device.  Eager work
+    and synchronizations lie between the replays, and a cache that is dropped meanwhile is kept
+    until the capture is over."""
+    from semantica_gpu import kernels
+    s = Served(gpu_ctx, "bf16", bits, 22)
+    s.document()
+    s.x.zero_()
+    s.step()  # (first calls ask for their LDS)
+    s.lengths.zero_()
+    s.slot.copy_(s.starts)
+    torch.cuda.synchronize()
+    dropped = kernels.KVCache(gpu_ctx, 10, 1, 64, torch.bfloat16)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        del dropped
+        s.step()
+    for t in range(6):
+        s.x.copy_(rand(s.g, s.n, s.wide, dtype="bf16"))
+        graph.replay()
+        torch.cuda.synchronize()
+        s.check(t)
+        got = s.att.clone()
+        q, _, _ = s.parts(s.qkv)
+        again = torch.empty_like(s.att)
+        kernels.attention_shared(gpu_ctx, again, q, s.cache, s.heads, s.off, s.starts, s.lengths, *s.shared)
+        same(again, got, "eager and replayed")
+    s.close()
+
+
+@pytest.mark.gpu
+def test_streams_and_threads(gpu_ctx):
+    """Calls on streams of their own at once, from threads, with the default workspace and one of
+    their own: the bits of a call by itself."""
+    import threading
+    from semantica_gpu import kernels
+    g = gen(31)
+    n, heads, kv_heads, hd, plen = 40, 8, 2, 128, 4000
+    k, v = rand(g, plen + n, kv_heads * hd, dtype="f16"), rand(g, plen + n, kv_heads * hd, dtype="f16")
+    cache = make_cache(gpu_ctx, plen + n, kv_heads, hd, "f16", 8)
+    fill_cache(gpu_ctx, cache, k, v)
+    qs = [rand(g, n, heads * hd, dtype="f16").cuda() for _ in range(4)]
+    off, starts, lengths = offsets([1] * n).cuda(), ints(range(plen, plen + n)).cuda(), ints([1] * n).cuda()
+    shared = [ints([0, n]).cuda(), ints([0]).cuda(), ints([plen]).cuda()]
+    want = []
+    for q in qs:
+        want.append(torch.empty_like(q))
+        kernels.attention_shared(gpu_ctx, want[-1], q, cache, heads, off, starts, lengths, *shared)
+    torch.cuda.synchronize()
+    got = [[torch.empty_like(q) for _ in range(5)] for q in qs]
+    errors = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            own = torch.empty(cache.work_bytes(heads, n, n, 1), dtype=torch.uint8, device="cuda")
+            torch.cuda.synchronize()
+            for j, out in enumerate(got[i]):
+                if j % 2:
+                    kernels.attention_shared(gpu_ctx, out, qs[i], cache, heads, off, starts, lengths, *shared, work=own,
+                                             stream=stream.cuda_stream)
+                else:
+                    kernels.attention_shared(gpu_ctx, out, qs[i], cache, heads, off, starts, lengths, *shared,
+                                             stream=stream.cuda_stream)
+            stream.synchronize()
+        except Exception as e:  # pragma: no cover
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for w, outs in zip(want, got):
+        for o in outs:
+            same(o, w, "beside other calls")
+    cache.close()
+
+
+@pytest.mark.gpu
+def test_numbers_that_make_no_sense(gpu_ctx):
+    """Offsets, starts and lengths of any value: nothing outside the tensors is touched."""
+    from semantica_gpu import kernels
+    r = np.random.RandomState(4)
+    rows, slots, heads, kv_heads, hd, n, n_prefix = 50, 100, 4, 2, 64, 12, 3
+    for bits in (0, 8):
+        cache = make_cache(gpu_ctx, slots, kv_heads, hd, "bf16", bits)
+        pool = torch.full((rows + 2, heads * hd), 7.0, dtype=torch.bfloat16, device="cuda")
+        k = torch.full((rows + 2, kv_heads * hd), 7.0, dtype=torch.bfloat16, device="cuda")
+        v = k.clone()
+        q = torch.randn(rows, heads * hd, device="cuda").bfloat16()
+        for trial in range(30):
+            def some(m):
+                lim = int(r.choice([60, 200, 2**31 - 1]))
+                return ints(r.randint(-lim, lim, m)).cuda()
+            say("trial", bits, trial)
+            off, starts, lengths, shared = some(n + 1), some(n), some(n), some(n_prefix + 1)
+            kernels.kv_cache_write(gpu_ctx, cache, q[:, :128], q[:, 128:], off, starts)
+            kernels.kv_cache_read(gpu_ctx, k[1:-1], v[1:-1], cache, off, starts)
+            kernels.attention_shared(gpu_ctx, pool[1:-1], q, cache, heads, off, starts, lengths, shared, some(n_prefix),
+                                     some(n_prefix), window=int(r.choice([0, 5])), causal=bool(r.randint(2)))
+            torch.cuda.synchronize()
+        for t in (pool, k, v):
+            assert bool((t[0] == 7).all()) and bool((t[-1] == 7).all())
+        cache.close()
+
+
+@pytest.mark.gpu
+def test_slots_past_32_bits(gpu_ctx):
+    """A cache of 20 GB: the last slots of the last head lie past every 32-bit offset."""
+    from semantica_gpu import kernels
+    slots, kv_heads, hd, n = 1_250_000, 8, 256, 70
+    cache = make_cache(gpu_ctx, slots, kv_heads, hd, "f32", 0)
+    assert cache.nbytes > 2**34
+    g = gen(41)
+    k, v, q = rand(g, n, kv_heads * hd), rand(g, n, kv_heads * hd), rand(g, n, kv_heads * hd)
+    off, starts = offsets([n]).cuda(), ints([slots - n]).cuda()
+    kernels.kv_cache_write(gpu_ctx, cache, k.cuda(), v.cuda(), off, starts)
+    ko, vo = torch.empty_like(k).cuda(), torch.empty_like(v).cuda()
+    kernels.kv_cache_read(gpu_ctx, ko, vo, cache, off, starts)
+    same(ko, k, "keys")
+    same(vo, v, "values")
+    for queries in ([n], [1]):
+        rows = sum(queries)
+        got = run_shared(gpu_ctx, q[:rows], cache, kv_heads, offsets(queries), starts=ints([slots - n]), lengths=ints([n]))
+        want, mean, size = shared_ref(q[:rows], k.double(), v.double(), offsets(queries), kv_heads, kv_heads, ints([0]), ints([n]))
+        close(got, want, shared_tol("f32", 0, hd, n, want, mean, size), "attention")
+    cache.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_shared_columns_of_wider_tensors(gpu_ctx, dtype):
+    """q as columns of a projection, out as columns of a wider tensor, rows far apart."""
+    from semantica_gpu import kernels
+    g = gen(6)
+    heads, kv_heads, hd = 3, 1, 72
+    for queries, lengths in (([2, 1], [20, 5]), ([50, 13], [50, 33])):
+        off = offsets(queries)
+        rows = int(off[-1])
+        wide = rand(g, rows, heads * hd + 40, dtype=dtype).cuda()
+        out = torch.full((rows, heads * hd + 16), 7.0, dtype=dt(dtype), device="cuda")
+        k, v = rand(g, 100, hd, dtype=dtype), rand(g, 100, hd, dtype=dtype)
+        cache = make_cache(gpu_ctx, 100, kv_heads, hd, dtype, 0)
+        fill_cache(gpu_ctx, cache, k, v)
+        keys = dict(starts=ints([3, 60]), lengths=ints(lengths))
+        kernels.attention_shared(gpu_ctx, out[:, 8:8 + heads * hd], wide[:, 32:32 + heads * hd], cache, heads, off.cuda(),
+                                 **{n: t.cuda() for n, t in keys.items()})
+        cache.close()
+        want, mean, size = shared_ref(wide[:, 32:32 + heads * hd].cpu(), k.double(), v.double(), off, heads, kv_heads, **keys)
+        close(out[:, 8:8 + heads * hd], want, shared_tol(dtype, 0, hd, 60, want, mean, size), "attention")
+        assert bool((out[:, :8] == 7).all()) and bool((out[:, 8 + heads * hd:] == 7).all())

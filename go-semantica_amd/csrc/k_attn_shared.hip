@@ -68,7 +68,7 @@ __device__ __forceinline__ int kept_length(int start, int length, int64_t slots)
 
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg_attn_batch b, sg_attn_list la,
-                                                            sg_attn_list lb, int one_list, int rows_wanted, int2* seen_out,
+                                                            sg_attn_list lb, int one_list, int join_rows, int2* seen_out,
                                                             int4* where_out) {
   __shared__ int32_t off_lds[kPlanSeqs + 1], seq_jobs_lds[kPlanSeqs + 1];
   __shared__ int32_t group_lds[kPlanPrefixes + 1], prefix_jobs_lds[kPlanPrefixes + 1];
@@ -97,29 +97,53 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
     return few ? prefix_lds[p] : range(b.prefix_starts[p], b.prefix_lengths[p]);
   };
 
+  auto prefix_of = [&](int i) {  // of a sequence; -1: none
+    if (b.n_prefix == 0) return -1;
+    const int p = last_at_most(b.n_prefix, i, group_at);
+    return i >= group_at(p) && i < group_at(p + 1) ? p : -1;
+  };
+  auto tiles_of = [&](int64_t rows, int m) { return (rows * a.group + m - 1) / m; };
+  auto rows_of = [&](int i) { return max(off(i + 1) - off(i), 0); };
+
+  // A prefix by itself, read once for all that share it, or again with every sequence's own keys:
+  // the first pays for results of two parts that go through memory (kTraffic a pair) and a launch
+  // more, the second for every job of a sequence that goes over the prefix.
+  constexpr int64_t kTraffic = 6, kLaunch = 100000;  // in sixteenths of a narrow unit, 1 ns or so
+  bool all_keys = b.all_keys != 0;
+  if (!all_keys) {
+    auto none = [](int, int64_t) {};
+    auto units_of = [&](int p) {
+      const int plen = prefix_keys(p).y;
+      return (int64_t)(a.window > 0 ? min(plen, a.window) : plen) / kTile + 1;
+    };
+    const int64_t apart = running<THREADS>(b.n_prefix, 0, INT64_MAX, none, [&](int p) {
+      const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
+      return (tiles_of(rows, la.m) * (units_of(p) + la.job_cost) * la.unit_cost + rows * a.group * kTraffic) * a.kv_heads;
+    });
+    const int64_t with = running<THREADS>(b.n_seq, 0, INT64_MAX, none, [&](int i) {
+      const int p = prefix_of(i);
+      return p < 0 ? 0 : tiles_of(rows_of(i), lb.m) * units_of(p) * lb.unit_cost * a.kv_heads;
+    });
+    all_keys = with <= apart + (one_list ? 0 : kLaunch);
+  }
+
   // Jobs of each prefix and sequence: those of prefixes first where both stand in one list; with
   // all_keys there are only sequences'.
-  const bool prefixes = b.n_prefix > 0 && !b.all_keys;
+  const bool prefixes = !all_keys;
   int n_prefix_jobs = 0;
   if (prefixes)
     n_prefix_jobs = (int)running<THREADS>(
         b.n_prefix, 0, la.cap, [&](int p, int64_t v) { few ? prefix_jobs_lds[p] = (int)v : b.prefix_jobs[p] = (int)v; },
         [&](int p) {
           const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
-          return (rows * a.group + la.m - 1) / la.m;
+          return tiles_of(rows, la.m);
         });
   const int own0 = one_list ? n_prefix_jobs : 0;
   const int own_end = (int)running<THREADS>(
       b.n_seq, own0, lb.cap, [&](int i, int64_t v) { small ? seq_jobs_lds[i] = (int)v : b.seq_jobs[i] = (int)v; },
-      [&](int i) { return ((int64_t)max(off(i + 1) - off(i), 0) * a.group + lb.m - 1) / lb.m; });
-  auto prefix_of = [&](int i) {  // of a sequence; -1: none
-    if (b.n_prefix == 0) return -1;
-    const int p = last_at_most(b.n_prefix, i, group_at);
-    return i >= group_at(p) && i < group_at(p + 1) ? p : -1;
-  };
-
+      [&](int i) { return tiles_of(rows_of(i), lb.m); });
   // What each row sees of a prefix that sequences share, and where the join finds it.
-  if (rows_wanted)
+  if (join_rows || !all_keys)
     for (int row = t; row < a.rows; row += THREADS) {
       const int i = last_at_most(b.n_seq, row, off);
       const int r0 = off(i), r1 = off(i + 1);
@@ -192,14 +216,15 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
     if (t == 0) {
       list.plan->units = units;
       list.plan->jobs = j0 + n;
+      list.plan->all_keys = all_keys;
       list.plan->per = max((units * a.kv_heads + list.workers - 1) / list.workers, (int64_t)list.min_units);
     }
     return units;
   };
   int64_t base = 0;
-  if (prefixes) base = fill(la, 0, n_prefix_jobs, kPrefixKeys, 0);
+  if (prefixes || !one_list) base = fill(la, 0, n_prefix_jobs, kPrefixKeys, 0);
   if (!one_list) base = 0;
-  fill(lb, own0, own_end - own0, b.all_keys ? kAllKeys : kOwnKeys, base);
+  fill(lb, own0, own_end - own0, all_keys ? kAllKeys : kOwnKeys, base);
 }
 
 // The workers that have tiles of a job: [first, last], as of a whole list.
@@ -268,11 +293,9 @@ __device__ __forceinline__ int64_t piece_of(const sg_attn_list& list, int64_t wo
 // One (row, head) for NW waves: what there is of its prefix's job and of its own keys', or of
 // the job that has both.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_attn_join(sg_attn_shared_args a, sg_attn_list la, sg_attn_list lb,
-                                                                       int all_keys) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t i = NW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-  if (i >= (int64_t)a.rows * a.heads) return;
+__device__ __forceinline__ void join_one(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, int64_t i,
+                                         int wave, int lane) {
+  const bool all_keys = lb.plan->all_keys != 0;
   const int row = (int)(i / a.heads), head = (int)(i - (int64_t)row * a.heads);
   const int4 where = a.where[row];
   if (where.z == -2) return;  // a row of no sequence
@@ -307,6 +330,17 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_attn_join(sg_attn_s
   }
   x.template put<T>(a, row, head, lane);
 }
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void k_attn_join(sg_attn_shared_args a, sg_attn_list la, sg_attn_list lb) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if constexpr (NW > 1) {
+    join_one<T, D, NW>(a, la, lb, blockIdx.x, wave, lane);
+  } else {
+    if (lb.plan->all_keys) return;  // k_attn_join_split's
+    for (int64_t i = (int64_t)blockIdx.x * 4 + wave; i < (int64_t)a.rows * a.heads; i += (int64_t)gridDim.x * 4)
+      join_one<T, D, 1>(a, la, lb, i, wave, lane);
+  }
+}
 
 // The jobs with all keys that lie across workers, for many rows: a block column for each
 // worker that ends inside a job and began it.
@@ -314,6 +348,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void k_attn_join_split(sg_attn_shared_args a, sg_attn_list list) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t units = list.plan->units, per = list.plan->per, worker = blockIdx.x, end = (worker + 1) * per;
+  if (!list.plan->all_keys) return;
   if (end >= units * a.kv_heads) return;
   const int kv = (int)(end / units);
   const int64_t at = end - kv * units;
@@ -352,6 +387,7 @@ __global__ __launch_bounds__(256) void k_attn_join_split(sg_attn_shared_args a, 
 constexpr int kNarrowPairs = 32;
 constexpr int kFullJobs = 4;
 constexpr int64_t kJoinFew = 256, kJoinSome = 4096;  // (row, head) up to here: 16 waves each, four
+constexpr int64_t kJoinBlocks = 8192;                // beyond: one, in turn
 
 struct layout {
   size_t plan, cum[2], jobs[2], seq_jobs, prefix_jobs, seen, where, ml, o, total;
@@ -399,10 +435,11 @@ layout lay_out(int dtype, bool q8, int rows, int heads, int kv_heads, int D, int
 template <typename T, int D>
 hipError_t join(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, int all_keys, hipStream_t s) {
   const int64_t n = (int64_t)a.rows * a.heads;
-  if (n <= kJoinFew) return sgp::run_kernel(k_attn_join<T, D, 16>, dim3(n), dim3(64 * 16), 0, s, a, la, lb, all_keys);
-  if (n <= kJoinSome) return sgp::run_kernel(k_attn_join<T, D, 4>, dim3(n), dim3(64 * 4), 0, s, a, la, lb, all_keys);
-  if (all_keys) return sgp::run_kernel(k_attn_join_split<T, D>, dim3(lb.workers, lb.m / 16), dim3(256), 0, s, a, lb);
-  return sgp::run_kernel(k_attn_join<T, D, 1>, dim3((n + 3) / 4), dim3(256), 0, s, a, la, lb, 0);
+  if (n <= kJoinFew) return sgp::run_kernel(k_attn_join<T, D, 16>, dim3(n), dim3(64 * 16), 0, s, a, la, lb);
+  if (n <= kJoinSome) return sgp::run_kernel(k_attn_join<T, D, 4>, dim3(n), dim3(64 * 4), 0, s, a, la, lb);
+  hipError_t e = sgp::run_kernel(k_attn_join_split<T, D>, dim3(lb.workers, lb.m / 16), dim3(256), 0, s, a, lb);
+  if (e != hipSuccess || all_keys) return e;
+  return sgp::run_kernel(k_attn_join<T, D, 1>, dim3(std::min<int64_t>((n + 3) / 4, kJoinBlocks)), dim3(256), 0, s, a, la, lb);
 }
 template <typename T>
 hipError_t join_dims(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, int all_keys, int D,
@@ -444,24 +481,27 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
     l.blocks = i ? l.workers : l.workers / 4;
     l.wide = i;
     l.cap = y.cap;
-    l.min_units = i ? 8 : dtype == SG_F32 && D == 256 ? 1 : 2;
+    // Measured at 128 dims, us a unit and workers: bf16 and codes 1.5 (512 wide), 2 (2048 narrow);
+    // float32 4.9 (256), 3 (1024).
+    l.unit_cost = i ? (dtype == SG_F32 && !q8 ? 96 : 48) : 16;
+    l.min_units = i ? (dtype == SG_F32 && !q8 ? 3 : 8) : dtype == SG_F32 && D == 256 ? 1 : 2;
     l.job_cost = i ? 4 : dtype == SG_F32 && D == 256 ? 1 : 2;
   }
   const int64_t pairs = (int64_t)a.rows * a.group;
   // A job for each M pairs of a sequence, over prefix and own keys in one go, where no prefix is
-  // shared or sequences fill several jobs themselves; otherwise prefixes and own keys by themselves.
+  // shared or sequences fill several jobs themselves; otherwise the plan weighs it by the lengths.
   b.all_keys = b.n_seq <= b.n_prefix || b.n_prefix == 0 || pairs >= (int64_t)kFullJobs * y.m[1] * b.n_seq;
   const int wide_own = pairs > (int64_t)kNarrowPairs * b.n_seq;
   const int wide_prefix = b.all_keys ? wide_own : pairs > (int64_t)kNarrowPairs * b.n_prefix;
   const sg_attn_list& lb = lists[wide_own];
   const sg_attn_list& la = lists[wide_prefix];
   const int one_list = &la == &lb;
-  const int rows_wanted = !b.all_keys || (int64_t)a.rows * a.heads <= kJoinSome;
+  const int join_rows = (int64_t)a.rows * a.heads <= kJoinSome;  // one by one
   // Few rows and sequences: four waves, which meet sooner than sixteen.
   const int threads = a.rows > 512 || b.n_seq > 512 || b.n_prefix > 512 ? 1024 : 256;
   hipError_t e =
       sgp::run_kernel(threads == 1024 ? k_attn_plan<1024> : k_attn_plan<256>, dim3(1), dim3(threads), 0, s, a, b, la, lb, one_list,
-                      rows_wanted, seen, where);
+                      join_rows, seen, where);
   auto run = [&](const sg_attn_list& l) {
     if (e != hipSuccess) return;
     e = dtype == SG_F32   ? attn_shared_f32(a, l, q8, D, s)

@@ -131,7 +131,7 @@ struct sg_attn_job {
 };
 struct sg_attn_plan {
   int64_t units, per;  // units of a head, of a worker
-  int32_t jobs;
+  int32_t jobs, all_keys;
 };
 struct sg_attn_list {
   sg_attn_plan* plan;
@@ -141,6 +141,7 @@ struct sg_attn_list {
   int m, piece_pairs;  // pairs of a job, of a piece of one
   int blocks, workers, wide;
   int cap, min_units, job_cost;  // jobs that fit; units of a worker at least; what a job costs beside its tiles
+  int unit_cost;                 // time of a unit on the whole GPU, in sixteenths of a narrow one's
 };
 // What the plan is made from (device arrays as sg_shared_keys names them).
 struct sg_attn_batch {
@@ -153,7 +154,8 @@ struct sg_attn_batch {
   int32_t* seq_jobs;     // [n_seq + 1]
   int32_t* prefix_jobs;  // [n_prefix + 1]
   int64_t slots;
-  int n_seq, n_prefix, all_keys;
+  int n_seq, n_prefix;
+  int all_keys;  // jobs have all keys of their rows: 1 yes, 0 as the plan finds
 };
 
 // One sg_matmul_q4 call (k_q4.hip): packed weights, strides in elements.

@@ -402,7 +402,7 @@ layout lay_out(int dtype, bool q8, int rows, int heads, int kv_heads, int D, int
   y.cap = (int)std::min<int64_t>(2 * (pairs / 16) + n_seq + n_prefix + 2, INT32_MAX);
   const int cus = 256;
   y.workers[0] = cus * 4 * (dtype == SG_F32 ? 1 : 2);
-  y.workers[1] = cus * (dtype == SG_F32 && D >= 128 ? 1 : 2);
+  y.workers[1] = cus * (D == 256 || (dtype == SG_F32 && D == 128) ? 1 : 2);
   y.m[0] = 16;
   y.m[1] = sgk::attn_wide_pairs(D, dtype == SG_F32, q8);
   size_t at = 0;

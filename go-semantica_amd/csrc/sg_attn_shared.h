@@ -663,7 +663,7 @@ constexpr int kRing = 4;
 template <typename T, bool Q8, int D, int NW>
 struct wide_lds {
   static constexpr int KB = kTile * D * (int)sizeof(typename query<T, Q8>::type);  // keys of a tile
-  static constexpr bool ring = Q8 && D <= 128 && D / 16 >= NW;
+  static constexpr bool ring = Q8 && D <= 128;
   static constexpr int stage = 2 * KB + (Q8 && !ring ? kTail : 0);
   static constexpr int part = D / 16 * 1024 / NW + kTail;  // a wave's part of a tile of codes
   static constexpr int bytes = 2 * stage + (ring ? kRing * NW * part : 0);
@@ -839,9 +839,9 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
 template <typename T, bool Q8, int D>
 struct wide_form {
   static constexpr bool F32 = __is_same(T, float);
-  static constexpr int NW = F32 && D == (Q8 ? 128 : 256) ? 8 : 4;
+  static constexpr int NW = (F32 && Q8 ? D == 128 : D == 256) ? 8 : 4;
   static constexpr int QT = sgk::attn_wide_pairs(D, F32, Q8) / (16 * NW);
-  static constexpr int PER_CU = F32 && D >= 128 ? 1 : 2;
+  static constexpr int PER_CU = D == 256 || (F32 && D == 128) ? 1 : 2;
 };
 
 template <typename T, bool Q8, int D>

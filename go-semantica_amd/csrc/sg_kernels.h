@@ -410,7 +410,7 @@ int64_t kv_rows_threads(int rows, int heads);
 hipError_t kv_write(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
 hipError_t kv_read(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
 // Pairs of a job of the wide form.
-constexpr int attn_wide_pairs(int D, bool f32, bool q8) { return D == 256 && !(f32 && !q8) ? 64 : 128; }
+constexpr int attn_wide_pairs(int D, bool f32, bool q8) { return D == 256 && f32 && q8 ? 64 : 128; }
 size_t attn_shared_work_bytes(int dtype, bool q8, int rows, int heads, int kv_heads, int D, int n_seq, int n_prefix);
 // a's workspace pointers, seen and where, and the batch's arrays, are placed in work.
 hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q8, int D, void* work, hipStream_t s);

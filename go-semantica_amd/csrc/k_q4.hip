@@ -79,9 +79,9 @@ namespace sgk {
 int64_t q4_blocks(int out_dim, int in_dim) { return (int64_t)((out_dim + 15) / 16) * ((in_dim + kBlockK - 1) / kBlockK); }
 
 int64_t q4_threads(int rows, int out_dim) {
-  // The most that any form launches: 16 outputs and 16 rows to a workgroup up to 16 rows, 32 and 32 or 64 above.
+  // No form has workgroups of less than 16 outputs and, above 16 rows, 32 rows.
   const int64_t tiles = (out_dim + 15) / 16;
-  return (rows > 16 ? (tiles + 1) / 2 * (((int64_t)rows + 31) / 32) : tiles) * 64 * kWaves;
+  return tiles * (((int64_t)rows + 31) / 32) * 64 * kWaves;
 }
 
 hipError_t q4_pack(const uint8_t* codes, const void* scales, int scale_dtype, const uint8_t* zeros, int out_dim, int in_dim,

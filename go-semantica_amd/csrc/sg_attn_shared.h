@@ -294,9 +294,10 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
 #pragma unroll
   for (int t = 0; t < QT; t++) {
     float e[8], sum;
-    auto form = [&] {
+    auto form = [&](bool far) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) e[j] = exp2_of(__builtin_fmaf(p[t][j], a.scale, -st.base[t]));
+      for (int j = 0; j < 8; j++)
+        e[j] = exp2_of(far ? p[t][j] * a.scale - st.m[t] + kShift<T, Q8> : __builtin_fmaf(p[t][j], a.scale, -st.base[t]));
       if constexpr (kSumByProduct<T, Q8>) {
         // The packed weights' sum by a product with ones: a sixteenth of the second product's work
         // in place of eight additions a lane, and the sum of the weights as they are multiplied.
@@ -308,7 +309,7 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
         sum = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
       }
     };
-    form();
+    form(false);
     if (__ballot(sum > st.most[t])) {
       float top = fmaxf(fmaxf(fmaxf(p[t][0], p[t][1]), fmaxf(p[t][2], p[t][3])),
                         fmaxf(fmaxf(p[t][4], p[t][5]), fmaxf(p[t][6], p[t][7]))) * a.scale;
@@ -316,11 +317,14 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
       const float by = top > st.m[t] ? exp2_of(st.m[t] - top) : 1.0f;  // (m may be -infinity: 0)
       st.m[t] = top;
       st.base[t] = (top == -INFINITY ? 0.0f : top) - kShift<T, Q8>;
-      st.most[t] = top == -INFINITY ? -1.0f : kMost<T, Q8>;
+      // (A maximum of 2^24 or more is rounded by one or more: there the products are rounded as it was,
+      // tile by tile, so that the largest weight is 1 and not two to that rounding.)
+      const bool far = fabsf(top) >= 0x1p24f && top != -INFINITY;
+      st.most[t] = top == -INFINITY || far ? -1.0f : kMost<T, Q8>;
       st.l[t] *= by;
 #pragma unroll
       for (int f = 0; f < D / 16; f++) st.o[t][f] *= by;
-      form();
+      form(far);
     }
     st.l[t] += sum;
     if constexpr (Q8) {

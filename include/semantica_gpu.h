@@ -498,7 +498,9 @@ int sg_attention_shared_work_bytes(const sg_kv_cache *cache, int32_t n_heads, in
  * that share it.  The n queries of a sequence are the last n places of its prefix and
  * own keys together (a query before the first place has none, and sees under causal nothing);
  * a row that sees no key, or only scores of -infinity, is zeros, rows of no sequence stay as
- * they were.  What hidden slots hold does not matter.  q, out [rows][n_heads * head_dim] of
+ * they were.  What hidden slots hold does not matter.  Sums are float32 and up to 2^10 times the
+ * number of keys larger than the result: values beyond 2^90 may leave its range; float32 queries
+ * and values behind codes keep their bits down to 2^-100.  q, out [rows][n_heads * head_dim] of
  * the cache's type with row strides in elements, pointers 16-byte aligned, strides whole 16
  * bytes, apart from each other (other columns of one tensor are); n_heads is a multiple of the
  * cache's heads, head h reads key head h * n_kv_heads / n_heads.  rows * n_heads up to 2^25.
@@ -529,12 +531,13 @@ int sg_q4_weight_create(sg_ctx *ctx, const uint8_t *d_codes, const void *d_scale
 int sg_q4_weight_create_q4_0(sg_ctx *ctx, const void *raw, int32_t out_dim, int32_t in_dim, sg_q4_weight **out);
 void sg_q4_weight_free(sg_q4_weight *weight);
 
-/* dst[m][n] = sum over k of w[n][k] x[m][k] for a few rows (64 or fewer share one pass over the
- * weights, more take one for every 64).  x [rows][in_dim], dst [rows][out_dim] of type dtype with
+/* dst[m][n] = sum over k of w[n][k] x[m][k] for a few rows (64 or fewer, 32 of float32, share one
+ * pass over the weights, more take one for every so many).  x [rows][in_dim], dst [rows][out_dim] of type dtype with
  * row strides in elements; x 16-byte aligned, its stride whole 16 bytes; dst does not overlap
  * x (other columns of one tensor, with the same stride, do not).  Weights are not rounded, sums
  * are float32 and in the same order every time; float32 rows keep their bits down to 2^-102 (what
- * lies below 2^-126 is lost of smaller values).  Asynchronous on `stream`, allocates nothing,
+ * lies below 2^-126 is lost of smaller values), and values beyond 2^116 may leave float32's range in a
+ * group's sum, which is formed before its scale.  Asynchronous on `stream`, allocates nothing,
  * may be captured. */
 int sg_matmul_q4(sg_ctx *ctx, void *dst, int64_t ldd, const sg_q4_weight *weight, const void *x, int64_t ldx,
                  int32_t dtype, int32_t rows, void *stream);

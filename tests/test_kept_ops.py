@@ -548,6 +548,48 @@ def test_shared_far_apart_scales(gpu_ctx):
             close(got, want, shared_tol(dtype, bits, hd, n, want, mean, size), "attention")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("scale", [3e5, 1e9, -1e15])
+def test_shared_large_scores(gpu_ctx, dtype, bits, scale):
+    """Scores so large that one step of float32 is more than any weight: the keys of the largest share the answer.
+
+    Products of -1, 0 and 1 are whole numbers (times a scale of codes that is the same for all keys), so
+    keys tie exactly, their weights are 1, and all others' zero.  What is left is the values' weights'
+    rounding (bf16 over codes: half a step, fp16: two halves of bf16), the sums' and the result's."""
+    g = gen(17)
+    heads, kv_heads, hd, plen = 4, 2, 64, 300
+    for queries, lengths in (([1, 2, 1], [40, 3, 70]), ([70, 40], [70, 90])):
+        rows, slots = sum(queries), plen + sum(lengths)
+        q = torch.randint(-1, 2, (rows, heads * hd), generator=g).to(dt(dtype))
+        k = torch.randint(-1, 2, (slots, kv_heads * hd), generator=g).to(dt(dtype))
+        v = rand(g, slots, kv_heads * hd, dtype=dtype)
+        cache = make_cache(gpu_ctx, slots, kv_heads, hd, dtype, bits)
+        fill_cache(gpu_ctx, cache, k, v)
+        off = offsets(queries)
+        keys = dict(starts=ints(plen + np.concatenate([[0], np.cumsum(lengths)[:-1]])), lengths=ints(lengths),
+                    shared=ints([0, len(queries)]), prefix_starts=ints([0]), prefix_lengths=ints([plen]), scale=scale)
+        got = run_shared(gpu_ctx, q, cache, heads, off, **keys)
+        cache.close()
+        kr, vr = kept_ref(k, kv_heads, bits)[0], kept_ref(v, kv_heads, bits)[0]
+        want, mean, _ = shared_ref(q, kr, vr, off, heads, kv_heads, **keys)
+        own = 0.0 if bits == 0 else {"f32": 0.0, "f16": 2.0 ** -16, "bf16": U["bf16"]}[dtype]
+        close(got, want, 1.01 * U[dtype] * want.abs() + (1.01 * own + 400 * F) * mean, "attention")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,bits", [("f32", 0), ("bf16", 8)])
+def test_shared_many_sequences(gpu_ctx, dtype, bits):
+    """Thousands of sequences and hundreds of prefixes: more than a plan keeps at hand."""
+    n = 2100
+    check_shared(gpu_ctx, 1, dtype, bits, 2, 1, 64, [1] * n, [i % 7 for i in range(n)], [700])
+    check_shared(gpu_ctx, 2, dtype, bits, 2, 1, 64, [i % 3 for i in range(n)], [i % 9 for i in range(n)],
+                 [p * 13 % 70 for p in range(520)], first=2, behind=3)
+    check_shared(gpu_ctx, 3, dtype, bits, 2, 2, 64, [2] * 30, [5] * 30, [40] * 600, shared=[min(p // 15, 30) for p in range(601)],
+                 window=20)
+
+
 # ---- 4-bit weights -------------------------------------------------------------------------
 
 
@@ -598,6 +640,14 @@ def test_q4(gpu_ctx, dtype, group, zeros):
     for rows, out_dim, groups in ((1, 1, 1), (1, 100, 3), (2, 33, 24), (16, 130, 5), (17, 64, 9), (33, 70, 40),
                                   (64, 16, 2), (130, 49, 7), (5, 16401, 2)):
         check_q4(gpu_ctx, rows, dtype, rows, out_dim, groups * group, group, ("f16", "f32", "bf16")[rows % 3], zeros)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_q4_many_outputs(gpu_ctx, dtype):
+    """Two and four tiles of outputs to a workgroup, the last one's in part."""
+    for rows, out_dim in ((1, 8200), (3, 8200), (16, 8217), (3, 16390), (17, 8200), (40, 8200)):
+        check_q4(gpu_ctx, rows, dtype, rows, out_dim, 192, 32, "f16", rows == 3)
 
 
 @pytest.mark.gpu

@@ -106,9 +106,11 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
   auto rows_of = [&](int i) { return max(off(i + 1) - off(i), 0); };
 
   // A prefix by itself, read once for all that share it, or again with every sequence's own keys:
-  // the first pays for results of two parts that go through memory (kTraffic a pair) and a launch
-  // more, the second for every job of a sequence that goes over the prefix.
-  constexpr int64_t kTraffic = 6, kLaunch = 100000;  // in sixteenths of a narrow unit, 1 ns or so
+  // the first pays for results of two parts that go through memory, for a plan and a join of both
+  // and for a launch more, the second for every job of a sequence that goes over the prefix.
+  // (bf16 and codes, 8 heads over 2 of 128 dims, apart and again: 4 tokens behind 16384 37 and 30 us,
+  // 64 behind 4096 49 and 34; float32 of 256 dims: 4 behind 16384 57 and 82, 64 behind 4096 80 and 213.)
+  constexpr int64_t kTraffic = 6, kApart = 96000, kLaunch = 160000;  // in sixteenths of a nanosecond
   bool all_keys = b.all_keys != 0;
   if (!all_keys) {
     auto none = [](int, int64_t) {};
@@ -116,15 +118,20 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
       const int plen = prefix_keys(p).y;
       return (int64_t)(a.window > 0 ? min(plen, a.window) : plen) / kTile + 1;
     };
-    const int64_t apart = running<THREADS>(b.n_prefix, 0, INT64_MAX, none, [&](int p) {
+    // Units of a list one after another over the GPU, a worker's least at the least.
+    auto time = [&](const sg_attn_list& l, int64_t units) {
+      return max(units * a.kv_heads, (int64_t)l.min_units * l.workers) * l.unit_cost;
+    };
+    const int64_t pairs = (int64_t)a.rows * a.heads;
+    const int64_t prefix_units = running<THREADS>(b.n_prefix, 0, INT64_MAX, none, [&](int p) {
       const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
-      return (tiles_of(rows, la.m) * (units_of(p) + la.job_cost) * la.unit_cost + rows * a.group * kTraffic) * a.kv_heads;
+      return tiles_of(rows, la.m) * (units_of(p) + la.job_cost);
     });
-    const int64_t with = running<THREADS>(b.n_seq, 0, INT64_MAX, none, [&](int i) {
+    const int64_t again = running<THREADS>(b.n_seq, 0, INT64_MAX, none, [&](int i) {
       const int p = prefix_of(i);
-      return p < 0 ? 0 : tiles_of(rows_of(i), lb.m) * units_of(p) * lb.unit_cost * a.kv_heads;
+      return p < 0 ? 0 : tiles_of(rows_of(i), lb.m) * units_of(p);
     });
-    all_keys = with <= apart + (one_list ? 0 : kLaunch);
+    all_keys = time(lb, again) <= time(la, prefix_units) + pairs * kTraffic + kApart + (one_list ? 0 : kLaunch);
   }
 
   // Jobs of each prefix and sequence: those of prefixes first where both stand in one list; with
@@ -382,11 +389,20 @@ __global__ __launch_bounds__(256) void k_attn_join_split(sg_attn_shared_args a, 
   }
 }
 
+// Time of a unit with all workers busy, in sixteenths of a nanosecond.  Measured at 128 dims: 16-bit
+// types and codes 1 ns narrow, 3 wide; float32 over codes 1.6 and 7, over float32 3 and 19; at 256
+// dims 11 and 49 (a wave or two a SIMD, which wait for memory), the others in proportion.
+int unit_cost(int dtype, bool q8, int D, bool wide) {
+  if (dtype != SG_F32) return wide ? 3 * D / 8 : D / 8;
+  if (q8) return wide ? 7 * D / 8 : D / 5;
+  return D == 256 ? (wide ? 790 : 176) : wide ? 5 * D / 2 : 3 * D / 8;
+}
+
 // The form of each kind of job.  Up to so many pairs of a group on average, waves work for
 // themselves.
 constexpr int kNarrowPairs = 32;
 constexpr int kFullJobs = 4;
-constexpr int64_t kJoinFew = 256, kJoinSome = 4096;  // (row, head) up to here: 16 waves each, four
+constexpr int64_t kJoinFew = 256, kJoinSome = 1024;  // (row, head) up to here: 16 waves each, four
 constexpr int64_t kJoinBlocks = 8192;                // beyond: one, in turn
 
 struct layout {
@@ -481,9 +497,7 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
     l.blocks = i ? l.workers : l.workers / 4;
     l.wide = i;
     l.cap = y.cap;
-    // Measured at 128 dims, us a unit and workers: bf16 and codes 1.5 (512 wide), 2 (2048 narrow);
-    // float32 4.9 (256), 3 (1024).
-    l.unit_cost = i ? (dtype == SG_F32 && !q8 ? 96 : 48) : 16;
+    l.unit_cost = unit_cost(dtype, q8, D, i);
     l.min_units = i ? (dtype == SG_F32 && !q8 ? 3 : 8) : dtype == SG_F32 && D == 256 ? 1 : 2;
     l.job_cost = i ? 4 : dtype == SG_F32 && D == 256 ? 1 : 2;
   }

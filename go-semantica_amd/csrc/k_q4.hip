@@ -79,9 +79,8 @@ namespace sgk {
 int64_t q4_blocks(int out_dim, int in_dim) { return (int64_t)((out_dim + 15) / 16) * ((in_dim + kBlockK - 1) / kBlockK); }
 
 int64_t q4_threads(int rows, int out_dim) {
-  // No form has workgroups of less than 16 outputs and, above 16 rows, 32 rows.
-  const int64_t tiles = (out_dim + 15) / 16;
-  return tiles * (((int64_t)rows + 31) / 32) * 64 * kWaves;
+  // No form has workgroups of less than 16 outputs and 16 rows.
+  return (int64_t)((out_dim + 15) / 16) * (((int64_t)rows + 15) / 16) * 64 * kWaves;
 }
 
 hipError_t q4_pack(const uint8_t* codes, const void* scales, int scale_dtype, const uint8_t* zeros, int out_dim, int in_dim,

@@ -141,7 +141,7 @@ struct sg_attn_list {
   int m, piece_pairs;  // pairs of a job, of a piece of one
   int blocks, workers, wide;
   int cap, min_units, job_cost;  // jobs that fit; units of a worker at least; what a job costs beside its tiles
-  int unit_cost;                 // time of a unit on the whole GPU, in sixteenths of a narrow one's
+  int unit_cost;                 // time of a unit with all workers busy, in sixteenths of a nanosecond
 };
 // What the plan is made from (device arrays as sg_shared_keys names them).
 struct sg_attn_batch {

@@ -249,27 +249,41 @@ hipError_t launch(const sg_q4_args& a, hipStream_t s) {
   return sgp::run_kernel(k_q4<T, S, ZEROS, GROUP, OT, MT>, dim3((unsigned)blocks), dim3(64 * kWaves), 0, s, a);
 }
 
+// More outputs and rows to a workgroup as there are more blocks of 16 and 16 than fill the GPU: what
+// is loaded or decoded once then serves several products.  Measured with 4096 inputs (us; OT x MT, fp16
+// scales; * is taken):
+//   bf16, group 64    512 blocks   1x1 11.4  2x1 9.4*            (16 rows; 1 row 8.4* and 8.9)
+//                    1024, 16 rows 1x1 19.9  2x1 14.7  4x1 14.5*  (1 row, group 32: 15.2  14.3*  15.0)
+//                    1024, 64 rows           2x1 13.8  4x1 12.9  2x2 11.5*  4x2 15.2
+//                    2048, 64 rows 1x1 35    2x1 24    4x1 24    2x2 21     4x2 15.8*
+//   group 32, 2048, 64 rows 1x1 37  2x1 26  4x1 26  2x2 23.5*  4x2 31
+//   float32, group 64, 512 blocks  1x1 20.4  2x1 13.9*
+//                    2048, 64 rows 1x1 64    2x1 39    4x1 33*   2x2 40     4x2 34
+//   float32, group 128, 2048, 64 rows        2x1 40    4x1 34    2x2 40     4x2 26*
 template <typename T, typename S, bool ZEROS, int GROUP>
-hipError_t by_rows(const sg_q4_args& a, hipStream_t s) {
-  const int tiles = (a.out_dim + 15) / 16;
-  if constexpr (sizeof(T) == 2) {
-    if (a.rows > 32) return launch<T, S, ZEROS, GROUP, 1, 4>(a, s);
-    if (a.rows > 16) return launch<T, S, ZEROS, GROUP, 1, 2>(a, s);
-    if (a.rows > 2 && tiles >= 1024) return launch<T, S, ZEROS, GROUP, 4, 1>(a, s);
-    if (a.rows > 2 && tiles >= 512) return launch<T, S, ZEROS, GROUP, 2, 1>(a, s);
-  } else {
-    if (a.rows > 16) return launch<T, S, ZEROS, GROUP, 2, 2>(a, s);
-    if (a.rows > 2 && tiles >= 1024) return launch<T, S, ZEROS, GROUP, 4, 1>(a, s);
-    if (tiles >= 512) return launch<T, S, ZEROS, GROUP, 2, 1>(a, s);
+hipError_t by_size(const sg_q4_args& a, hipStream_t s) {
+  const int64_t tiles = (a.out_dim + 15) / 16, blocks = tiles * ((a.rows + 15) / 16);
+  if (tiles >= 16) {  // (a workgroup's last outputs may be none)
+    // (With shorter groups its scales and sums are more than registers hold.)
+    if constexpr (GROUP > (sizeof(T) == 2 ? 32 : 64))
+      if (a.rows > 16 && blocks >= 2048) return launch<T, S, ZEROS, GROUP, 4, 2>(a, s);
+    if constexpr (sizeof(T) == 2) {
+      if (a.rows > 16 && blocks >= 1024) return launch<T, S, ZEROS, GROUP, 2, 2>(a, s);
+      if (a.rows > 2 && blocks >= 1024) return launch<T, S, ZEROS, GROUP, 4, 1>(a, s);
+      if (blocks >= (a.rows > 2 ? 512 : 1024)) return launch<T, S, ZEROS, GROUP, 2, 1>(a, s);
+    } else {
+      if (blocks >= 1024) return launch<T, S, ZEROS, GROUP, 4, 1>(a, s);
+      if (blocks >= 512) return launch<T, S, ZEROS, GROUP, 2, 1>(a, s);
+    }
   }
   return launch<T, S, ZEROS, GROUP, 1, 1>(a, s);
 }
 
 template <typename T, typename S, bool ZEROS>
 hipError_t by_group(const sg_q4_args& a, hipStream_t s) {
-  if (a.group == 32) return by_rows<T, S, ZEROS, 32>(a, s);
-  if (a.group == 64) return by_rows<T, S, ZEROS, 64>(a, s);
-  return by_rows<T, S, ZEROS, 128>(a, s);
+  if (a.group == 32) return by_size<T, S, ZEROS, 32>(a, s);
+  if (a.group == 64) return by_size<T, S, ZEROS, 64>(a, s);
+  return by_size<T, S, ZEROS, 128>(a, s);
 }
 
 template <typename T>

@@ -531,7 +531,7 @@ int sg_q4_weight_create(sg_ctx *ctx, const uint8_t *d_codes, const void *d_scale
 int sg_q4_weight_create_q4_0(sg_ctx *ctx, const void *raw, int32_t out_dim, int32_t in_dim, sg_q4_weight **out);
 void sg_q4_weight_free(sg_q4_weight *weight);
 
-/* dst[m][n] = sum over k of w[n][k] x[m][k] for a few rows (64 or fewer, 32 of float32, share one
+/* dst[m][n] = sum over k of w[n][k] x[m][k] for a few rows (16 or 32 of them share one
  * pass over the weights, more take one for every so many).  x [rows][in_dim], dst [rows][out_dim] of type dtype with
  * row strides in elements; x 16-byte aligned, its stride whole 16 bytes; dst does not overlap
  * x (other columns of one tensor, with the same stride, do not).  Weights are not rounded, sums

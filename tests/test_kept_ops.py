@@ -646,8 +646,9 @@ def test_q4(gpu_ctx, dtype, group, zeros):
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_q4_many_outputs(gpu_ctx, dtype):
     """Two and four tiles of outputs to a workgroup, the last one's in part."""
-    for rows, out_dim in ((1, 8200), (3, 8200), (16, 8217), (3, 16390), (17, 8200), (40, 8200)):
-        check_q4(gpu_ctx, rows, dtype, rows, out_dim, 192, 32, "f16", rows == 3)
+    for rows, out_dim in ((1, 8200), (3, 8200), (16, 8217), (1, 16390), (3, 16390), (17, 8200), (40, 12000), (700, 770), (530, 250)):
+        for group in (32, 64, 128):
+            check_q4(gpu_ctx, rows, dtype, rows, out_dim, 384, group, "f16" if rows < 40 else "f32", rows in (3, 40))
 
 
 @pytest.mark.gpu

@@ -105,50 +105,74 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
   auto tiles_of = [&](int64_t rows, int m) { return (rows * a.group + m - 1) / m; };
   auto rows_of = [&](int i) { return max(off(i + 1) - off(i), 0); };
 
-  // A prefix by itself, read once for all that share it, or again with every sequence's own keys:
-  // the first pays for results of two parts that go through memory, for a plan and a join of both
-  // and for a launch more, the second for every job of a sequence that goes over the prefix.
-  // (bf16 and codes, 8 heads over 2 of 128 dims, apart and again: 4 tokens behind 16384 37 and 30 us,
-  // 64 behind 4096 49 and 34; float32 of 256 dims: 4 behind 16384 57 and 82, 64 behind 4096 80 and 213.)
-  constexpr int64_t kTraffic = 6, kApart = 96000, kLaunch = 160000;  // in sixteenths of a nanosecond
-  bool all_keys = b.all_keys != 0;
+  // Where jobs go.  Again: prefixes with every sequence's own keys, read again for each; or apart,
+  // which pays for results of two parts that go through memory (kTraffic a pair) and for a plan and
+  // a join of both (kApart): prefixes in the wide list and own keys in the narrow, one after the
+  // other (kLaunch), or both in one of the two, if what that list does worse is little.
+  // us (32 heads over 8 of 128 dims, 64 tokens with 40 own keys; again, two lists, narrow, wide):
+  //   bf16, codes   behind 512  34 47 32 37    2048  50 51 38 39    8192  120 58 57 53
+  //   float32       behind 512  55 59 44 77    2048 199 70 83 91    8192  695 117 221 141
+  bool all_keys = b.all_keys != 0, together = false, wide = false;
   if (!all_keys) {
-    auto none = [](int, int64_t) {};
-    auto units_of = [&](int p) {
-      const int plen = prefix_keys(p).y;
-      return (int64_t)(a.window > 0 ? min(plen, a.window) : plen) / kTile + 1;
-    };
+    constexpr int64_t kTraffic = 6, kApart = 96000, kLaunch = 160000;  // in sixteenths of a nanosecond
+    __shared__ int64_t sums[5][THREADS / 64];
+    auto tiles = [&](int keys) { return (int64_t)(a.window > 0 ? min(keys, a.window) : keys) / kTile + 1; };
+    int64_t sum[5] = {0, 0, 0, 0, 0};  // prefixes' units by la and lb, own keys' by la and lb, again by lb
+    for (int p = t; p < b.n_prefix; p += THREADS) {
+      const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0), n = tiles(prefix_keys(p).y);
+      sum[0] += tiles_of(rows, la.m) * (n + la.job_cost);
+      sum[1] += tiles_of(rows, lb.m) * (n + lb.job_cost);
+    }
+    for (int i = t; i < b.n_seq; i += THREADS) {
+      const int rows = rows_of(i), p = prefix_of(i);
+      const int64_t n = tiles(own_keys(i).y);
+      sum[2] += tiles_of(rows, la.m) * (n + la.job_cost);
+      sum[3] += tiles_of(rows, lb.m) * (n + lb.job_cost);
+      sum[4] += tiles_of(rows, lb.m) * (n + lb.job_cost + (p < 0 ? 0 : tiles(prefix_keys(p).y)));
+    }
+#pragma unroll
+    for (int k = 0; k < 5; k++) {
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) sum[k] += __shfl_xor(sum[k], o);
+      if ((t & 63) == 0) sums[k][t >> 6] = sum[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 5; k++) {
+      sum[k] = 0;
+      for (int w = 0; w < THREADS / 64; w++) sum[k] += sums[k][w];
+    }
     // Units of a list one after another over the GPU, a worker's least at the least.
     auto time = [&](const sg_attn_list& l, int64_t units) {
       return max(units * a.kv_heads, (int64_t)l.min_units * l.workers) * l.unit_cost;
     };
-    const int64_t pairs = (int64_t)a.rows * a.heads;
-    const int64_t prefix_units = running<THREADS>(b.n_prefix, 0, INT64_MAX, none, [&](int p) {
-      const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
-      return tiles_of(rows, la.m) * (units_of(p) + la.job_cost);
-    });
-    const int64_t again = running<THREADS>(b.n_seq, 0, INT64_MAX, none, [&](int i) {
-      const int p = prefix_of(i);
-      return p < 0 ? 0 : tiles_of(rows_of(i), lb.m) * units_of(p);
-    });
-    all_keys = time(lb, again) <= time(la, prefix_units) + pairs * kTraffic + kApart + (one_list ? 0 : kLaunch);
+    const int64_t apart = (int64_t)a.rows * a.heads * kTraffic + kApart;
+    const int64_t again = time(lb, sum[4]), narrow = time(lb, sum[1] + sum[3]) + apart;
+    const int64_t other = one_list ? INT64_MAX : time(la, sum[0] + sum[2]) + apart;
+    const int64_t two = one_list ? INT64_MAX : time(la, sum[0]) + time(lb, sum[3]) + apart + kLaunch;
+    all_keys = again <= min(min(narrow, other), two);
+    together = min(narrow, other) <= two;
+    wide = other < narrow;
   }
+  const bool prefixes = !all_keys;
+  const bool one = one_list || (prefixes && together);
+  // (One list: what stands in it is found by the jobs' kinds, the other is empty.)
+  const sg_attn_list pl = prefixes && together && !wide ? lb : la, ol = prefixes && together && wide ? la : lb;
 
   // Jobs of each prefix and sequence: those of prefixes first where both stand in one list; with
   // all_keys there are only sequences'.
-  const bool prefixes = !all_keys;
   int n_prefix_jobs = 0;
   if (prefixes)
     n_prefix_jobs = (int)running<THREADS>(
-        b.n_prefix, 0, la.cap, [&](int p, int64_t v) { few ? prefix_jobs_lds[p] = (int)v : b.prefix_jobs[p] = (int)v; },
+        b.n_prefix, 0, pl.cap, [&](int p, int64_t v) { few ? prefix_jobs_lds[p] = (int)v : b.prefix_jobs[p] = (int)v; },
         [&](int p) {
           const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
-          return tiles_of(rows, la.m);
+          return tiles_of(rows, pl.m);
         });
-  const int own0 = one_list ? n_prefix_jobs : 0;
+  const int own0 = one ? n_prefix_jobs : 0;
   const int own_end = (int)running<THREADS>(
-      b.n_seq, own0, lb.cap, [&](int i, int64_t v) { small ? seq_jobs_lds[i] = (int)v : b.seq_jobs[i] = (int)v; },
-      [&](int i) { return tiles_of(rows_of(i), lb.m); });
+      b.n_seq, own0, ol.cap, [&](int i, int64_t v) { small ? seq_jobs_lds[i] = (int)v : b.seq_jobs[i] = (int)v; },
+      [&](int i) { return tiles_of(rows_of(i), ol.m); });
   // What each row sees of a prefix that sequences share, and where the join finds it.
   if (join_rows || !all_keys)
     for (int row = t; row < a.rows; row += THREADS) {
@@ -224,14 +248,18 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
       list.plan->units = units;
       list.plan->jobs = j0 + n;
       list.plan->all_keys = all_keys;
+      list.plan->prefixes = list.plan->own = 0;
       list.plan->per = max((units * a.kv_heads + list.workers - 1) / list.workers, (int64_t)list.min_units);
     }
     return units;
   };
-  int64_t base = 0;
-  if (prefixes || !one_list) base = fill(la, 0, n_prefix_jobs, kPrefixKeys, 0);
-  if (!one_list) base = 0;
-  fill(lb, own0, own_end - own0, all_keys ? kAllKeys : kOwnKeys, base);
+  if (!one_list && (all_keys || together)) fill(ol.plan == la.plan ? lb : la, 0, 0, kPrefixKeys, 0);  // the empty one
+  const int64_t base = prefixes ? fill(pl, 0, n_prefix_jobs, kPrefixKeys, 0) : 0;
+  fill(ol, own0, own_end - own0, all_keys ? kAllKeys : kOwnKeys, one ? base : 0);
+  if (t == 0) {
+    la.plan->prefixes = pl.plan != la.plan;  // whose lists are the other's
+    lb.plan->own = ol.plan != lb.plan;
+  }
 }
 
 // The workers that have tiles of a job: [first, last], as of a whole list.
@@ -303,6 +331,7 @@ template <typename T, int D, int NW>
 __device__ __forceinline__ void join_one(const sg_attn_shared_args& a, const sg_attn_list& la, const sg_attn_list& lb, int64_t i,
                                          int wave, int lane) {
   const bool all_keys = lb.plan->all_keys != 0;
+  const bool prefixes_in_lb = la.plan->prefixes != 0, own_in_la = lb.plan->own != 0;
   const int row = (int)(i / a.heads), head = (int)(i - (int64_t)row * a.heads);
   const int4 where = a.where[row];
   if (where.z == -2) return;  // a row of no sequence
@@ -310,7 +339,7 @@ __device__ __forceinline__ void join_one(const sg_attn_shared_args& a, const sg_
   joined<D> x;
 #pragma unroll
   for (int own = 0; own < 2; own++) {
-    const sg_attn_list& list = own ? lb : la;
+    const sg_attn_list list = (own ? !own_in_la : prefixes_in_lb) ? lb : la;
     const int job0 = own ? where.z : where.x;
     if (job0 < 0) continue;
     const int64_t pair = (int64_t)(row - (own ? where.w : where.y)) * a.group + hg, job = job0 + pair / list.m;
@@ -389,13 +418,11 @@ __global__ __launch_bounds__(256) void k_attn_join_split(sg_attn_shared_args a, 
   }
 }
 
-// Time of a unit with all workers busy, in sixteenths of a nanosecond.  Measured at 128 dims: 16-bit
-// types and codes 1 ns narrow, 3 wide; float32 over codes 1.6 and 7, over float32 3 and 19; at 256
-// dims 11 and 49 (a wave or two a SIMD, which wait for memory), the others in proportion.
+// Time of a unit with all workers busy, in sixteenths of a nanosecond.  Measured at 128 dims (at 256 twice
+// that): bf16 2 ns narrow, 3 wide, over codes 1 and 3; float32 6 and 14, over codes 1.6 and 4.
 int unit_cost(int dtype, bool q8, int D, bool wide) {
-  if (dtype != SG_F32) return wide ? 3 * D / 8 : D / 8;
-  if (q8) return wide ? 7 * D / 8 : D / 5;
-  return D == 256 ? (wide ? 790 : 176) : wide ? 5 * D / 2 : 3 * D / 8;
+  if (dtype != SG_F32) return wide ? 3 * D / 8 : q8 ? D / 8 : D / 4;
+  return q8 ? (wide ? D / 2 : D / 5) : wide ? 7 * D / 4 : 3 * D / 4;
 }
 
 // The form of each kind of job.  Up to so many pairs of a group on average, waves work for
@@ -506,7 +533,8 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
   // shared or sequences fill several jobs themselves; otherwise the plan weighs it by the lengths.
   b.all_keys = b.n_seq <= b.n_prefix || b.n_prefix == 0 || pairs >= (int64_t)kFullJobs * y.m[1] * b.n_seq;
   const int wide_own = pairs > (int64_t)kNarrowPairs * b.n_seq;
-  const int wide_prefix = b.all_keys ? wide_own : pairs > (int64_t)kNarrowPairs * b.n_prefix;
+  const int64_t narrow_pairs = dtype != SG_F32 && !q8 ? kNarrowPairs / 2 : kNarrowPairs;
+  const int wide_prefix = b.all_keys ? wide_own : pairs > narrow_pairs * b.n_prefix;
   const sg_attn_list& lb = lists[wide_own];
   const sg_attn_list& la = lists[wide_prefix];
   const int one_list = &la == &lb;

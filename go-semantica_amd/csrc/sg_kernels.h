@@ -132,6 +132,7 @@ struct sg_attn_job {
 struct sg_attn_plan {
   int64_t units, per;  // units of a head, of a worker
   int32_t jobs, all_keys;
+  int32_t prefixes, own;  // 1: prefixes' jobs stand in the own keys' list, own keys' in the prefixes'
 };
 struct sg_attn_list {
   sg_attn_plan* plan;

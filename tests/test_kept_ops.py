@@ -579,6 +579,16 @@ def test_shared_large_scores(gpu_ctx, dtype, bits, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,bits", [("f32", 0), ("f16", 8), ("bf16", 0)])
+def test_shared_lists(gpu_ctx, dtype, bits):
+    """A hundred tokens behind one prefix, longer and longer, then with many own keys: the prefix read again
+    with every sequence, by itself beside the own keys in narrow jobs and in wide ones, and each in its own."""
+    for plen, own in ((300, 40), (3000, 40), (12000, 40), (8000, 1500)):
+        check_shared(gpu_ctx, plen, dtype, bits, 4, 1, 64, [1] * 100, [own - i % 30 for i in range(100)], [plen])
+    check_shared(gpu_ctx, 5, dtype, bits, 8, 2, 64, [1, 2, 0, 1] * 20, [9, 70, 3, 2] * 20, [2500, 40, 0, 3000], window=1500)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,bits", [("f32", 0), ("bf16", 8)])
 def test_shared_many_sequences(gpu_ctx, dtype, bits):
     """Thousands of sequences and hundreds of prefixes: more than a plan keeps at hand."""

@@ -4,7 +4,11 @@
 // The plan is one workgroup's work: for every row which places it sees, for every job its tiles,
 // and the running total of those, from which workers find their shares.  Offsets, ranges and
 // lengths come from device memory, so everything that is addressed later is cut here to the
-// tensors and the cache.
+// tensors and the cache.  It is a chain of loads, searches and barriers: 5 us for one query, 13 for 64
+// behind one prefix, 10 for 10476 and 16384 rows (sixteen waves).
+//
+// The join reads a float32 output for each piece of each (row, head): 27 rows of 32 heads whose
+// prefix is split over the GPU 13 us, 16384 rows of which the jobs of 512 workers were cut 21.
 #include <algorithm>
 
 #include "semantica_gpu.h"
@@ -87,14 +91,19 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
       if (i < b.n_prefix) prefix_lds[i] = range(b.prefix_starts[i], b.prefix_lengths[i]);
     }
   __syncthreads();
-  auto off = [&](int i) { return small ? off_lds[i] : clamp_row(b.off[i], a.rows); };
-  auto group_at = [&](int p) { return few ? group_lds[p] : min(max(b.shared[p], 0), b.n_seq); };
-  auto seq_jobs = [&](int i) { return small ? seq_jobs_lds[i] : b.seq_jobs[i]; };
-  auto prefix_jobs = [&](int p) { return few ? prefix_jobs_lds[p] : b.prefix_jobs[p]; };
-  auto own_keys = [&](int i) { return small ? keys_lds[i] : range(b.starts[i], b.lengths[i]); };
+  // (Loads from LDS and from memory stay two instructions, not one by a pointer that may be either.)
+  auto lds = [](int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  auto off = [&](int i) { return small ? lds(off_lds[i]) : clamp_row(b.off[i], a.rows); };
+  auto group_at = [&](int p) { return few ? lds(group_lds[p]) : min(max(b.shared[p], 0), b.n_seq); };
+  auto seq_jobs = [&](int i) { return small ? lds(seq_jobs_lds[i]) : b.seq_jobs[i]; };
+  auto prefix_jobs = [&](int p) { return few ? lds(prefix_jobs_lds[p]) : b.prefix_jobs[p]; };
+  auto own_keys = [&](int i) { return small ? make_int2(lds(keys_lds[i].x), lds(keys_lds[i].y)) : range(b.starts[i], b.lengths[i]); };
   auto prefix_keys = [&](int p) {
     if (p < 0) return make_int2(0, 0);
-    return few ? prefix_lds[p] : range(b.prefix_starts[p], b.prefix_lengths[p]);
+    return few ? make_int2(lds(prefix_lds[p].x), lds(prefix_lds[p].y)) : range(b.prefix_starts[p], b.prefix_lengths[p]);
   };
 
   auto prefix_of = [&](int i) {  // of a sequence; -1: none
@@ -102,8 +111,10 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
     const int p = last_at_most(b.n_prefix, i, group_at);
     return i >= group_at(p) && i < group_at(p + 1) ? p : -1;
   };
-  auto tiles_of = [&](int64_t rows, int m) { return (rows * a.group + m - 1) / m; };
+  // (m is a power of two; rows * group stay below 2^26.)
+  auto tiles_of = [&](int rows, int m) { return (rows * a.group + m - 1) >> (31 - __clz(m)); };
   auto rows_of = [&](int i) { return max(off(i + 1) - off(i), 0); };
+  auto rows_behind = [&](int p) { return max(off(group_at(p + 1)) - off(group_at(p)), 0); };
 
   // Where jobs go.  Again: prefixes with every sequence's own keys, read again for each; or apart,
   // which pays for results of two parts that go through memory (kTraffic a pair) and for a plan and
@@ -119,7 +130,8 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
     auto tiles = [&](int keys) { return (int64_t)(a.window > 0 ? min(keys, a.window) : keys) / kTile + 1; };
     int64_t sum[5] = {0, 0, 0, 0, 0};  // prefixes' units by la and lb, own keys' by la and lb, again by lb
     for (int p = t; p < b.n_prefix; p += THREADS) {
-      const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0), n = tiles(prefix_keys(p).y);
+      const int rows = rows_behind(p);
+      const int64_t n = tiles(prefix_keys(p).y);
       sum[0] += tiles_of(rows, la.m) * (n + la.job_cost);
       sum[1] += tiles_of(rows, lb.m) * (n + lb.job_cost);
     }
@@ -155,24 +167,31 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
     wide = other < narrow;
   }
   const bool prefixes = !all_keys;
+  auto plan_of = [&](const sg_attn_list& l, int64_t units, int jobs) {  // (workers are a power of two)
+    const int64_t per = (units * a.kv_heads + l.workers - 1) >> (31 - __clz(l.workers));
+    return sg_attn_plan{units, max(per, (int64_t)l.min_units), jobs, all_keys, 0, 0};
+  };
   const bool one = one_list || (prefixes && together);
   // (One list: what stands in it is found by the jobs' kinds, the other is empty.)
   const sg_attn_list pl = prefixes && together && !wide ? lb : la, ol = prefixes && together && wide ? la : lb;
 
   // Jobs of each prefix and sequence: those of prefixes first where both stand in one list; with
   // all_keys there are only sequences'.
-  int n_prefix_jobs = 0;
-  if (prefixes)
-    n_prefix_jobs = (int)running<THREADS>(
-        b.n_prefix, 0, pl.cap, [&](int p, int64_t v) { few ? prefix_jobs_lds[p] = (int)v : b.prefix_jobs[p] = (int)v; },
-        [&](int p) {
-          const int64_t rows = max(off(group_at(p + 1)) - off(group_at(p)), 0);
-          return tiles_of(rows, pl.m);
-        });
-  const int own0 = one ? n_prefix_jobs : 0;
-  const int own_end = (int)running<THREADS>(
-      b.n_seq, own0, ol.cap, [&](int i, int64_t v) { small ? seq_jobs_lds[i] = (int)v : b.seq_jobs[i] = (int)v; },
-      [&](int i) { return tiles_of(rows_of(i), ol.m); });
+  int end[2] = {0, 0}, own0 = 0;
+#pragma unroll 1
+  for (int own = prefixes ? 0 : 1; own < 2; own++) {
+    if (own) own0 = one ? end[0] : 0;
+    const int m = own ? ol.m : pl.m;
+    const int last = (int)running<THREADS>(
+        own ? b.n_seq : b.n_prefix, own0, own ? ol.cap : pl.cap,
+        [&](int i, int64_t v) {
+          (own ? b.seq_jobs : b.prefix_jobs)[i] = (int)v;
+          if (own ? small : few) (own ? seq_jobs_lds : prefix_jobs_lds)[i] = (int)v;
+        },
+        [&](int i) { return tiles_of(own ? rows_of(i) : rows_behind(i), m); });
+    if (own) end[1] = last;
+    else end[0] = last;
+  }
   // What each row sees of a prefix that sequences share, and where the join finds it.
   if (join_rows || !all_keys)
     for (int row = t; row < a.rows; row += THREADS) {
@@ -195,68 +214,65 @@ __global__ __launch_bounds__(THREADS) void k_attn_plan(sg_attn_shared_args a, sg
   __syncthreads();
 
   // The jobs, and the running total of their costs.
-  auto fill = [&](const sg_attn_list& list, int j0, int n, int kind, int64_t base) {
-    const int64_t units = running<THREADS>(
-        n, base, INT64_MAX, [&](int j, int64_t v) { list.cum[j0 + j] = v; },
+  int64_t base = 0;
+#pragma unroll 1
+  for (int pass = prefixes ? 0 : 1; pass < 2; pass++) {
+    const bool prefix = pass == 0;
+    const sg_attn_list list = prefix ? pl : ol;
+    const int j0 = prefix ? 0 : own0, n = (prefix ? end[0] : end[1]) - j0;
+    const int kind = prefix ? kPrefixKeys : all_keys ? kAllKeys : kOwnKeys;
+    base = running<THREADS>(
+        n, prefix || one ? base : 0, INT64_MAX, [&](int j, int64_t v) { list.cum[j0 + j] = v; },
         [&](int j) {
-          const bool prefix = kind == kPrefixKeys;
           const int i = prefix ? last_at_most(b.n_prefix, j + j0, prefix_jobs) : last_at_most(b.n_seq, j + j0, seq_jobs);
           const int r0 = off(prefix ? group_at(i) : i), r1 = off(prefix ? group_at(i + 1) : i + 1), rows = max(r1 - r0, 0);
           const int2 pk = prefix_keys(prefix ? i : prefix_of(i)), ok = prefix ? make_int2(0, 0) : own_keys(i);
           const int plen = pk.y, len = ok.y;
-          sg_attn_job job{r0, rows, j + j0 - (prefix ? prefix_jobs(i) : seq_jobs(i)), kind, {0, 0}, {0, 0}, {0, 0}, plen, len};
-          const int from = (int)((int64_t)job.tile * list.m / a.group);
-          const int to = (int)min((int64_t)rows, ((int64_t)(job.tile + 1) * list.m - 1) / a.group + 1);
-          int lo[2] = {INT32_MAX, INT32_MAX}, hi[2] = {0, 0};
-          auto see = [&](int own, int l, int h) {
-            lo[own] = min(lo[own], l < h ? l : INT32_MAX);
-            hi[own] = max(hi[own], l < h ? h : 0);
-          };
+          const int tile = j + j0 - (prefix ? prefix_jobs(i) : seq_jobs(i));
+          const int from = (int)((uint32_t)(tile * list.m) / (uint32_t)a.group);
+          const int to = min(rows, (int)((uint32_t)((tile + 1) * list.m - 1) / (uint32_t)a.group) + 1);
+          int2 see[2] = {make_int2(0, 0), make_int2(0, 0)};  // of the prefix, of their own
           if (prefix && a.window == 0) {
-            see(0, 0, plen);  // (some row sees it all, as a rule, and a wave that does not looks at each key)
+            see[0] = make_int2(0, plen);  // (some row sees it all, as a rule, and a wave that does not looks at each key)
           } else if (prefix) {
-#pragma unroll 8
+            see[0].x = INT32_MAX;
             for (int r = from; r < to; r++) {
               const int2 s = seen_out[r0 + r];
-              see(0, s.x, s.y);
+              see[0].x = min(see[0].x, s.x < s.y ? s.x : INT32_MAX);
+              see[0].y = max(see[0].y, s.x < s.y ? s.y : 0);
             }
           } else if (from < to) {
             // Both ends of a range grow with the row, empty or not: the first row's begin, the last one's end.
             const int64_t pos0 = (int64_t)plen + len - rows;
             const int4 s0 = sgc::places_seen(pos0 + from, plen, len, a.causal, a.window);
             const int4 s1 = sgc::places_seen(pos0 + to - 1, plen, len, a.causal, a.window);
-            see(0, s0.x, s1.y);
-            see(1, s0.z, s1.w);
+            see[0] = make_int2(s0.x, s1.y);
+            see[1] = make_int2(s0.z, s1.w);
           }
-          int64_t count = 0;
+          // (Cut once more: where offsets do not ascend, a row's range is another group's.)
+          int slot_tile[2], tiles[2];
+#pragma unroll
           for (int own = 0; own < 2; own++) {
-            if (own ? prefix : kind == kOwnKeys) continue;
-            const int64_t start = own ? ok.x : pk.x;
-            // (Cut once more: where offsets do not ascend, a row's range is another group's.)
-            const int end = min(hi[own], own ? len : plen);
-            if (lo[own] >= end) continue;
-            const int at = kind == kAllKeys ? own : 0;
-            job.key0[at] = (int)start;
-            job.slot_tile[at] = (int)((start + lo[own]) / kTile);
-            job.tiles[at] = (int)((start + end - 1) / kTile) - job.slot_tile[at] + 1;
-            count += job.tiles[at];
+            const int start = own ? ok.x : pk.x, stop = min(see[own].y, own ? len : plen);
+            const bool any = see[own].x < stop && !(own ? prefix : kind == kOwnKeys);
+            slot_tile[own] = any ? (int)((uint32_t)(start + see[own].x) / kTile) : 0;
+            tiles[own] = any ? (int)((uint32_t)(start + stop - 1) / kTile) - slot_tile[own] + 1 : 0;
           }
-          list.jobs[j + j0] = job;
+          // (Own keys alone stand in the first place.)
+          const bool alone = kind == kOwnKeys;
+          list.jobs[j + j0] = sg_attn_job{r0, rows, tile, kind, {alone ? ok.x : pk.x, ok.x},
+                                          {alone ? slot_tile[1] : slot_tile[0], slot_tile[1]},
+                                          {alone ? tiles[1] : tiles[0], alone ? 0 : tiles[1]}, plen, len};
+          const int64_t count = (int64_t)tiles[0] + tiles[1];
           return count + (count > 0 || kind == kAllKeys ? list.job_cost : 0);
         });
-    if (t == 0) {
-      list.plan->units = units;
-      list.plan->jobs = j0 + n;
-      list.plan->all_keys = all_keys;
-      list.plan->prefixes = list.plan->own = 0;
-      list.plan->per = max((units * a.kv_heads + list.workers - 1) / list.workers, (int64_t)list.min_units);
-    }
-    return units;
-  };
-  if (!one_list && (all_keys || together)) fill(ol.plan == la.plan ? lb : la, 0, 0, kPrefixKeys, 0);  // the empty one
-  const int64_t base = prefixes ? fill(pl, 0, n_prefix_jobs, kPrefixKeys, 0) : 0;
-  fill(ol, own0, own_end - own0, all_keys ? kAllKeys : kOwnKeys, one ? base : 0);
+    if (t == 0) *list.plan = plan_of(list, base, j0 + n);
+  }
   if (t == 0) {
+    if (!one_list && (all_keys || together)) {  // the empty one
+      const sg_attn_list none = ol.plan == la.plan ? lb : la;
+      *none.plan = plan_of(none, 0, 0);
+    }
     la.plan->prefixes = pl.plan != la.plan;  // whose lists are the other's
     lb.plan->own = ol.plan != lb.plan;
   }
@@ -271,8 +287,8 @@ __device__ __forceinline__ holders holders_of(const sg_attn_list& list, int kv, 
   const int64_t c0 = list.cum[job], c1 = list.cum[job + 1], head = kv * list.plan->units, per = list.plan->per;
   holders h{0, 0, c1 - c0 > list.job_cost};
   if (h.any) {
-    h.first = (head + c0 + list.job_cost) / per;
-    h.last = (head + c1 - 1) / per;
+    h.first = sgc::quotient(head + c0 + list.job_cost, per);
+    h.last = sgc::quotient(head + c1 - 1, per);
   }
   return h;
 }
@@ -332,7 +348,7 @@ __device__ __forceinline__ void join_one(const sg_attn_shared_args& a, const sg_
                                          int wave, int lane) {
   const bool all_keys = lb.plan->all_keys != 0;
   const bool prefixes_in_lb = la.plan->prefixes != 0, own_in_la = lb.plan->own != 0;
-  const int row = (int)(i / a.heads), head = (int)(i - (int64_t)row * a.heads);
+  const int row = (int)((uint32_t)i / (uint32_t)a.heads), head = (int)(i - (int64_t)row * a.heads);
   const int4 where = a.where[row];
   if (where.z == -2) return;  // a row of no sequence
   const int kv = head / a.group, hg = head - kv * a.group;
@@ -342,12 +358,12 @@ __device__ __forceinline__ void join_one(const sg_attn_shared_args& a, const sg_
     const sg_attn_list list = (own ? !own_in_la : prefixes_in_lb) ? lb : la;
     const int job0 = own ? where.z : where.x;
     if (job0 < 0) continue;
-    const int64_t pair = (int64_t)(row - (own ? where.w : where.y)) * a.group + hg, job = job0 + pair / list.m;
+    const int64_t pair = (int64_t)(row - (own ? where.w : where.y)) * a.group + hg, job = job0 + (pair >> (31 - __clz(list.m)));
     if (pair < 0 || job >= list.plan->jobs) continue;  // (offsets that do not ascend)
     const holders h = holders_of(list, kv, job);
     if (all_keys && (!h.any || h.first == h.last)) return;  // written
     if (!h.any) continue;
-    const int in_job = (int)(pair % list.m);
+    const int in_job = (int)pair & (list.m - 1);
     x.add(a, h.first + (NW == 1 ? 0 : wave), h.last, NW, lane, [&](int64_t w) {
       return h.first == h.last ? (int64_t)(own ? a.rows : 0) * a.heads + i : piece_of(list, w, w == h.first, in_job);
     });
@@ -386,7 +402,7 @@ __global__ __launch_bounds__(256) void k_attn_join_split(sg_attn_shared_args a, 
   const int64_t units = list.plan->units, per = list.plan->per, worker = blockIdx.x, end = (worker + 1) * per;
   if (!list.plan->all_keys) return;
   if (end >= units * a.kv_heads) return;
-  const int kv = (int)(end / units);
+  const int kv = (int)sgc::quotient(end, units);
   const int64_t at = end - kv * units;
   const int job = sgc::last_at_most(list.cum, list.plan->jobs, at, lane);
   const holders h = holders_of(list, kv, job);
@@ -427,10 +443,17 @@ int unit_cost(int dtype, bool q8, int D, bool wide) {
 
 // The form of each kind of job.  Up to so many pairs of a group on average, waves work for
 // themselves.
+// (Prefix of 16384 behind one key head, us, narrow and wide: float32 of 256 dims 16 pairs 53 and 54, 32 57
+// and 55, 64 69 and 58; bf16 over codes 128 pairs 37 and 41, where the plan takes either, but with 8 key
+// heads and 131072 places 136 pairs 301 and 128.)
 constexpr int kNarrowPairs = 32;
+// So many full jobs a sequence, and it takes a prefix again rather than in two parts (64 sequences of
+// 512 bf16 tokens of 4 heads behind 2048: 247 us, in two parts 405).
 constexpr int kFullJobs = 4;
-constexpr int64_t kJoinFew = 256, kJoinSome = 1024;  // (row, head) up to here: 16 waves each, four
-constexpr int64_t kJoinBlocks = 8192;                // beyond: one, in turn
+// (row, head) up to here: 16 waves each, four; beyond: one, in turn.  64: 29 us with 16, 32 with four, 38
+// with one; 512: 53, 49, 51; 2048: 81, 59, 56; 8192: 180, 103, 91.
+constexpr int64_t kJoinFew = 256, kJoinSome = 2048;
+constexpr int64_t kJoinBlocks = 8192;
 
 struct layout {
   size_t plan, cum[2], jobs[2], seq_jobs, prefix_jobs, seen, where, ml, o, total;
@@ -525,6 +548,9 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
     l.wide = i;
     l.cap = y.cap;
     l.unit_cost = unit_cost(dtype, q8, D, i);
+    // A worker's least, so that the join has fewer pieces (one query behind 1536 places of float32, 256 dims:
+    // 23 us with 1, 28 with 2, 40 with 4; a wide list with 16: 64 tokens of codes 72 for 64); and what a
+    // job costs beside its tiles (40 passages of float32 with 0: 214 for 206).
     l.min_units = i ? (dtype == SG_F32 && !q8 ? 3 : 8) : dtype == SG_F32 && D == 256 ? 1 : 2;
     l.job_cost = i ? 4 : dtype == SG_F32 && D == 256 ? 1 : 2;
   }
@@ -539,7 +565,8 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
   const sg_attn_list& la = lists[wide_prefix];
   const int one_list = &la == &lb;
   const int join_rows = (int64_t)a.rows * a.heads <= kJoinSome;  // one by one
-  // Few rows and sequences: four waves, which meet sooner than sixteen.
+  // Few rows and sequences: four waves, which meet sooner than sixteen (64 tokens: 49 and 54 us a call; 300
+  // and more alike).
   const int threads = a.rows > 512 || b.n_seq > 512 || b.n_prefix > 512 ? 1024 : 256;
   hipError_t e =
       sgp::run_kernel(threads == 1024 ? k_attn_plan<1024> : k_attn_plan<256>, dim3(1), dim3(threads), 0, s, a, b, la, lb, one_list,

@@ -1,6 +1,6 @@
 // sg_attn_shared.h -- attention of a batch's queries over kept keys and values
 // (sg_attention_shared): the kernels, shared by the files that instantiate them.
-// k_attn_shared.hip has the plan, the join and what was measured.
+// k_attn_shared.hip has the plan and the join.
 //
 // A query's keys are places 0 .. plen - 1, its prefix, and plen .. plen + len - 1, its
 // sequence's own.  Query rows times the query heads of a key head are pairs; a job is M
@@ -23,6 +23,18 @@
 // type has as well.  float32 queries and weights go over codes as three bf16 parts, 24 bits (48
 // cycles of 32 products of 16 and 16 where float32's own take 256); over float32 keys and
 // values it goes through float32 matrix products.
+//
+// What bounds them (MI355X): a wide workgroup of bf16 takes each fragment of a tile from LDS for two
+// products, and a pair and lane has eight exponentials of 16 cycles; vector and matrix
+// instructions of a SIMD overlap little, and two waves a SIMD hide the rest.
+//   bf16, 16384 rows of 32 heads over 8 of 128 dims behind 8192 places: 2.2 ms, 1040 TFLOP/s of the 1214
+//   that a large product reaches.
+//   bf16 over codes, 27 rows of 32 heads over 8 behind 131072 places: 110 us, 2.5 TB/s: decoding and
+//   the softmax of a tile stand between its load and the next barrier.
+//   float32, 10476 rows of 3 heads over 1 of 256 dims, window 512: 195 us, 85 of 152 TFLOP/s: two
+//   waves a SIMD, products that wait for fragments.
+//   one float32 query of 3 heads over 1 of 256 dims behind 1536 places (narrow): 11 us, one tile a
+//   wave, its loads' latency and 256 products in a row.
 #pragma once
 #include <atomic>
 
@@ -416,7 +428,7 @@ __device__ __forceinline__ share first_share(const sg_attn_list& list, int64_t w
   const int64_t begin = worker * per;
   if (begin >= total) return s;
   s.left = min(per, total - begin);
-  s.head = (int)(begin / units);
+  s.head = (int)sgc::quotient(begin, units);
   s.at = begin - s.head * units;
   // The last job that begins at or before the unit: it is not empty.
   s.job = sgc::last_at_most(list.cum, list.plan->jobs, s.at, lane);
@@ -658,11 +670,12 @@ __global__ __launch_bounds__(256, __is_same(T, float) ? 1 : 2) void k_attn_narro
   }
 }
 
-// Many pairs: a workgroup is a worker, its four waves have QT * 16 pairs each and share the tiles
+// Many pairs: a workgroup is a worker, its NW waves have QT * 16 pairs each and share the tiles
 // in LDS, two stages.  Types go there by direct copies; codes through registers, and lie there
 // as the type that multiplies them.  Codes of up to 128 dims go to LDS as they
-// are first, kRing tiles of them, each wave its own quarter (and the scales): a tile of codes is
-// 8 KB, and one or two a CU in flight reach half of the memory's rate.
+// are first, kRing tiles of them, each wave its own part (and the scales): a tile of codes is
+// 8 KB, and one or two a CU in flight reach half of the memory's rate (27 rows behind 131072 places: 133 us
+// without the ring, 110 with it).  At 256 dims the stages leave no room for it.
 constexpr int kRing = 4;
 template <typename T, bool Q8, int D, int NW>
 struct wide_lds {
@@ -839,7 +852,10 @@ __global__ __launch_bounds__(64 * NW, PER_CU * NW / 4) void k_attn_wide(sg_attn_
   }
 }
 
-// Waves of a workgroup, pairs of each, workgroups of a CU.
+// Waves of a workgroup, pairs of each, workgroups of a CU.  Outputs, queries and two batches of fragments
+// fill the registers: 32 pairs a wave up to 128 dims, 16 at 256 or in three parts.  (bf16 over codes at
+// 128 dims with eight waves of 16 pairs: 110 us for 107.  256 dims with four waves of 32 pairs, one to a
+// SIMD: 40 passages of float32 257 us, with eight of 16 190.)
 template <typename T, bool Q8, int D>
 struct wide_form {
   static constexpr bool F32 = __is_same(T, float);

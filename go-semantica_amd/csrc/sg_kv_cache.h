@@ -64,6 +64,12 @@ __device__ __forceinline__ int4 places_seen(int64_t pos, int plen, int len, int 
   return make_int4(cut(lo, plen), cut(hi, plen), cut(lo - plen, len), cut(hi - plen, len));
 }
 
+// a / b of numbers that are not negative; short where both are (64-bit division is a hundred instructions).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
+
 // The largest i in [0, n) with at[i] <= x, for ascending at with at[0] <= x; called by a whole
 // wave with a uniform x: 64 candidates a step.
 __device__ __forceinline__ int last_at_most(const int64_t* at, int n, int64_t x, int lane) {

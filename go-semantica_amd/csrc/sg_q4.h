@@ -111,8 +111,9 @@ __device__ __forceinline__ void split(const raw8<T>& r, s16x8_t (&p)[mul<T>::par
       for (int e = 0; e < 2; e++) {
         const uint32_t x = r.v[(2 * i + e) >> 2][(2 * i + e) & 3];
         hi[e] = x & 0xffff0000u;
-        // (An infinity less itself would be a NaN: it has no further parts.)
-        const float rest = (x & 0x7f800000u) == 0x7f800000u ? 0.0f : __uint_as_float(x) - __uint_as_float(hi[e]);
+        // (An infinity less itself would be a NaN: it has no further parts.  A NaN whose first part is cut to
+        // an infinity has a quiet one for its second, as any difference with it is.)
+        const float rest = (x & 0x7fffffffu) == 0x7f800000u ? 0.0f : __uint_as_float(x) - __uint_as_float(hi[e]);
         mid[e] = __float_as_uint(rest) & 0xffff0000u;
         lo[e] = __float_as_uint(rest - __uint_as_float(mid[e]));
       }

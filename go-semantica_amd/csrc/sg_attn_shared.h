@@ -471,8 +471,9 @@ __device__ __forceinline__ void begin_job(const sg_attn_shared_args& a, state<T,
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           const uint32_t u = __float_as_uint(x.v[j >> 2][j & 3]), hi = u & 0xffff0000u;
-          // (An infinity less itself would be a NaN: it has no further parts.)
-          const float rest = (u & 0x7f800000u) == 0x7f800000u ? 0.0f : __uint_as_float(u) - __uint_as_float(hi);
+          // (An infinity less itself would be a NaN: it has no further parts.  A NaN whose first part is cut to
+          // an infinity has a quiet one for its second, as any difference with it is.)
+          const float rest = (u & 0x7fffffffu) == 0x7f800000u ? 0.0f : __uint_as_float(u) - __uint_as_float(hi);
           const uint32_t mid = __float_as_uint(rest) & 0xffff0000u;
           part[0][j] = (short)(hi >> 16);
           part[1][j] = (short)(mid >> 16);

@@ -47,3 +47,28 @@ def test_q4_nan_of_any_payload(gpu_ctx):
         w = q4_dense(codes, scales, None)
         want = x[len(NANS):].double() @ w.t()
         close(dst[len(NANS):], want, q4_tol("f32", x[len(NANS):], w, want), "products")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_shared_query_nan_of_any_payload(gpu_ctx, bits, sign):
+    """A NaN in a query makes its row of that head NaN, whichever sign the keys have there, and no other row."""
+    g = gen(6)
+    for hd, queries, n in ((64, 9, 70), (128, 150, 300), (256, 9, 40), (256, 100, 150)):
+        q, k, v = rand(g, queries, 2 * hd), rand(g, n, hd), rand(g, n, hd)
+        for i, b in enumerate(NANS):
+            q.view(torch.int32)[i, 5 * i + 3] = nan_of(b).view(torch.int32)
+            k[:, 5 * i + 3] = sign * (0.5 + k[:, 5 * i + 3].abs())
+        cache = make_cache(gpu_ctx, n, 1, hd, "f32", bits)
+        fill_cache(gpu_ctx, cache, k, v)
+        off, keys = offsets([queries]), dict(starts=ints([0]), lengths=ints([n]))
+        got = run_shared(gpu_ctx, q, cache, 2, off, **keys)
+        cache.close()
+        m = len(NANS)
+        assert bool(torch.isnan(got[:m, :hd]).all()), "a NaN was lost"
+        kr, vr = kept_ref(k, 1, bits)[0], kept_ref(v, 1, bits)[0]
+        want, mean, size = shared_ref(q.nan_to_num(0.0), kr, vr, off, 2, 1, **keys)
+        tol = shared_tol("f32", bits, hd, n, want, mean, size)
+        close(got[m:], want[m:], tol[m:], "other rows")
+        close(got[:m, hd:], want[:m, hd:], tol[:m, hd:], "other heads")

@@ -302,11 +302,15 @@ struct joined {
   vec o = 0.0f;
   __device__ __forceinline__ void add(float om, float ol, vec oo) {
     const float top = fmaxf(m, om);  // (maxima are no NaN)
-    if (top == -INFINITY && ol == 0.0f) return;
     const float base = top == -INFINITY ? 0.0f : top;
     const float by = __builtin_amdgcn_exp2f(m - base), now = __builtin_amdgcn_exp2f(om - base);
     l = l * by + ol * now;
-    o = o * by + oo * now;
+    if (by != 0.0f && now != 0.0f) {
+      o = o * by + oo * now;
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; v++) o[v] = sgc::faded(o[v], by) + sgc::faded(oo[v], now);
+    }
     m = top;
   }
   // The pieces at `at` of workers w0, w0 + step, ... up to w1: four loads at a time.

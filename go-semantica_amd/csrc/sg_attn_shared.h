@@ -335,7 +335,14 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
       st.most[t] = top == -INFINITY || far ? -1.0f : kMost<T, Q8>;
       st.l[t] *= by;
 #pragma unroll
-      for (int f = 0; f < D / 16; f++) st.o[t][f] *= by;
+      for (int f = 0; f < D / 16; f++) {
+        if constexpr (Q8) {
+          st.o[t][f] *= by;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++) st.o[t][f][i] = sgc::faded(st.o[t][f][i], by);
+        }
+      }
       form(far);
     }
     st.l[t] += sum;
@@ -353,7 +360,8 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
 
 // Values that are not finite, in a tile that may be hidden in part: a zero weight times one is a
 // NaN.  So they are zeros in the product (clean), and which pairs see an infinity or a NaN of a
-// dim is counted by products of ones behind it (mark_bad): exact, and no business of the weights'.
+// dim is counted by products of ones behind it (mark_bad): exact, and no business of the weights',
+// not of later ones either (sgc::faded).
 template <typename M>
 __device__ __forceinline__ void set_elem(typename frag<M>::type& x, int j, float v) {
   if constexpr (__is_same(M, float)) x.v[j >> 2][j & 3] = v;

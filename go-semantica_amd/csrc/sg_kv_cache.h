@@ -64,6 +64,10 @@ __device__ __forceinline__ int4 places_seen(int64_t pos, int plen, int len, int 
   return make_int4(cut(lo, plen), cut(hi, plen), cut(lo - plen, len), cut(hi - plen, len));
 }
 
+// An output under a maximum that has risen by so much.  An infinity is a value's that was seen, and
+// stays one where the factor underflows: its key's weight is small, not zero.
+__device__ __forceinline__ float faded(float o, float by) { return fabsf(o) == INFINITY ? o : o * by; }
+
 // a / b of numbers that are not negative; short where both are (64-bit division is a hundred instructions).
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;

@@ -72,3 +72,85 @@ def test_shared_query_nan_of_any_payload(gpu_ctx, bits, sign):
         tol = shared_tol("f32", bits, hd, n, want, mean, size)
         close(got[m:], want[m:], tol[m:], "other rows")
         close(got[:m, hd:], want[:m, hd:], tol[:m, hd:], "other heads")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rise", [20.0, 200.0])
+def test_shared_infinite_values_anywhere(gpu_ctx, dtype, rise):
+    """An infinity in a value that is seen is the dim's result, wherever the large scores lie: before it,
+    behind it, in another piece; a NaN where both infinities are seen.
+
+    Scores are 0 but for two keys of `rise` in powers of e: their weights are 2^29 or 2^288 times the
+    infinite value's, which falls below float32 and, as a number of 64 bits, not below zero."""
+    g = gen(23)
+    hd, heads = 64, 2
+    for queries, plen, n in (([3], 0, 200), ([1, 2], 9000, 70), ([100], 0, 700), ([90, 70], 1500, 130)):
+        slots = plen + n * len(queries)
+        rows = sum(queries)
+        q = torch.zeros(rows, heads * hd, dtype=dt(dtype))
+        q[:, ::hd] = 1.0
+        k, v = torch.zeros(slots, hd, dtype=dt(dtype)), rand(g, slots, hd, dtype=dtype)
+        keys = dict(starts=ints([plen + i * n for i in range(len(queries))]), lengths=ints([n] * len(queries)), causal=False,
+                    scale=1.0)
+        if plen:
+            keys.update(shared=ints([0, len(queries)]), prefix_starts=ints([0]), prefix_lengths=ints([plen]))
+        first = [plen + i * n for i in range(len(queries))]
+        last = [plen + i * n + n - 1 for i in range(len(queries))]
+        for name, large, plus, minus in (
+                ("before", [0] + first, last, []), ("behind", last, [0] + first, []),
+                ("between", [slots // 2] + [f + n // 2 for f in first], [0] + first + last, []),
+                ("both", [slots // 2] + [f + n // 2 for f in first], [0] + first, last)):
+            kk, vv = k.clone(), v.clone()
+            kk[large, 0] = rise
+            vv[plus, 3], vv[minus, 3] = math.inf, -math.inf
+            cache = make_cache(gpu_ctx, slots, 1, hd, dtype, 0)
+            fill_cache(gpu_ctx, cache, kk, vv)
+            off = offsets(queries)
+            say("infinite", name, dtype, rise, queries, plen, n)
+            got = run_shared(gpu_ctx, q, cache, heads, off, **keys)
+            cache.close()
+            dim = got.reshape(rows, heads, hd)[:, :, 3].float()
+            if name == "both":
+                assert bool(torch.isnan(dim).all())
+            else:
+                assert bool((dim == math.inf).all()), f"{name}: {dim.flatten()[:8]}"
+            vv[plus, 3], vv[minus, 3] = 0.0, 0.0
+            want, mean, size = shared_ref(q, kk.double(), vv.double(), off, heads, 1, **keys)
+            rest = torch.ones(heads * hd, dtype=torch.bool)
+            rest[3::hd] = False
+            tol = shared_tol(dtype, 0, hd, plen + n, want, mean, size)
+            if dtype == "f16":
+                # A weight of fp16 is a multiple of 2^-24 after its factor of 2^6: off by 2^-31 of the largest, in
+                # the sum of the weights as in that of the values.
+                tol = tol + (plen + n) * 2.0 ** -31 * (vv.double().abs().max() + want.abs())
+            close(got[:, rest], want[:, rest], tol[:, rest], "other dims")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_shared_infinite_values_of_hopeless_keys(gpu_ctx, dtype):
+    """A value counts if its key is seen, though its score be -infinity: the infinity is the dim's
+    result in every cut of the work, unless no score is above -infinity (zeros)."""
+    g = gen(24)
+    hd = 64
+    for queries, n in ((1, 5), (1, 3000), (60, 500)):
+        q = torch.zeros(queries, hd, dtype=dt(dtype))
+        q[:, 0] = 1.0
+        for at in (0, 1, n // 2, n - 1):
+            k, v = torch.zeros(n, hd, dtype=dt(dtype)), rand(g, n, hd, dtype=dtype)
+            low = slice(at // 32 * 32, min(n - 1, at // 32 * 32 + 32)) if n > 32 else slice(at, at + 1)
+            k[low, 0] = -math.inf
+            v[at, 3] = math.inf
+            cache = make_cache(gpu_ctx, n, 1, hd, dtype, 0)
+            fill_cache(gpu_ctx, cache, k, v)
+            keys = dict(starts=ints([0]), lengths=ints([n]), causal=False)
+            got = run_shared(gpu_ctx, q, cache, 1, offsets([queries]), **keys).float()
+            assert bool((got[:, 3] == math.inf).all()), (n, at, got[:, 3])
+            got[:, 3] = 0
+            assert bool(torch.isfinite(got).all())
+            k[:, 0] = -math.inf
+            fill_cache(gpu_ctx, cache, k, v)
+            got = run_shared(gpu_ctx, q, cache, 1, offsets([queries]), **keys)
+            cache.close()
+            assert bool((got == 0).all()), "only scores of -infinity"

@@ -303,6 +303,12 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
         p[t][j] = key >= st.lo[t] && key < st.hi[t] ? p[t][j] : -INFINITY;
       }
   }
+  // A hidden key's scale may be NaN, and one's whose score is -infinity: it has no weight.
+  bool skip = part;
+  if constexpr (Q8) {
+    const float any = ((vs[0] + vs[1]) + (vs[2] + vs[3])) + ((vs[4] + vs[5]) + (vs[6] + vs[7]));
+    skip |= __ballot(any != any) != 0;
+  }
 #pragma unroll
   for (int t = 0; t < QT; t++) {
     float e[8], sum;
@@ -349,7 +355,7 @@ __device__ __forceinline__ void weigh(const sg_attn_shared_args& a, state<T, Q8,
     if constexpr (Q8) {
 #pragma unroll
       for (int j = 0; j < 8; j++) e[j] *= vs[j];
-      if (part) {  // a hidden key's scale may be NaN
+      if (skip) {
 #pragma unroll
         for (int j = 0; j < 8; j++) e[j] = p[t][j] == -INFINITY ? 0.0f : e[j];
       }

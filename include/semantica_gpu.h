@@ -499,7 +499,8 @@ int sg_attention_shared_work_bytes(const sg_kv_cache *cache, int32_t n_heads, in
  * own keys together (a query before the first place has none, and sees under causal nothing);
  * a row that sees no key, or only scores of -infinity, is zeros, rows of no sequence stay as
  * they were.  What hidden slots hold does not matter.  An infinity or a NaN in a value that is
- * seen is that dim's result whatever its key's score (a NaN where infinities of both signs are seen).
+ * seen is that dim's result whatever its key's score (a NaN where infinities of both signs are seen; kept
+ * as codes it is a NaN in all dims, and none with a score of -infinity, which has no weight).
  * Sums are float32 and up to 2^10 times the
  * number of keys larger than the result: values beyond 2^90 may leave its range; float32 queries
  * and values behind codes keep their bits down to 2^-100.  q, out [rows][n_heads * head_dim] of

@@ -154,3 +154,31 @@ def test_shared_infinite_values_of_hopeless_keys(gpu_ctx, dtype):
             got = run_shared(gpu_ctx, q, cache, 1, offsets([queries]), **keys)
             cache.close()
             assert bool((got == 0).all()), "only scores of -infinity"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [1, 60])
+def test_shared_nan_values_of_hopeless_keys(gpu_ctx, queries):
+    """Codes: a key whose score is -infinity has no weight, whatever its value holds, in a tile that is seen
+    whole and in one that is seen in part; with any other score a value's NaN is the row's."""
+    g = gen(25)
+    hd = 64
+    q = torch.zeros(queries, hd)
+    q[:, 0] = 1e25
+    for n, at in ((32, 7), (64, 40), (5, 2), (45, 40), (90, 3)):
+        k, v = torch.zeros(n + 3, hd), rand(g, n + 3, hd)
+        v[at, 9] = math.nan
+        v[n + 1, 9] = math.nan  # behind what is seen
+        cache = make_cache(gpu_ctx, n + 3, 1, hd, "f32", 8)
+        fill_cache(gpu_ctx, cache, k, v)
+        off, keys = offsets([queries]), dict(starts=ints([0]), lengths=ints([n]), causal=False)
+        got = run_shared(gpu_ctx, q, cache, 1, off, **keys)
+        assert bool(torch.isnan(got).all()), (n, at)
+        k[at, 0] = -1e15  # a score of -1e40
+        fill_cache(gpu_ctx, cache, k, v)
+        got = run_shared(gpu_ctx, q, cache, 1, off, **keys)
+        cache.close()
+        assert bool(torch.isfinite(got).all()), (n, at)
+        v[at], v[n + 1] = 0.0, 0.0
+        want, mean, size = shared_ref(q, kept_ref(k, 1, 8)[0], kept_ref(v, 1, 8)[0], off, 1, 1, **keys)
+        close(got, want, shared_tol("f32", 8, hd, n, want, mean, size), "attention")

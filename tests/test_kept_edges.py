@@ -182,3 +182,78 @@ def test_shared_nan_values_of_hopeless_keys(gpu_ctx, queries):
         v[at], v[n + 1] = 0.0, 0.0
         want, mean, size = shared_ref(q, kept_ref(k, 1, 8)[0], kept_ref(v, 1, 8)[0], off, 1, 1, **keys)
         close(got, want, shared_tol("f32", 8, hd, n, want, mean, size), "attention")
+
+
+def check_many_rows(ctx, seed, dtype, bits, kv_heads, hd, lens, starts, slots, first=0, behind=0):
+    """Rows in and out, bit for bit; the later of two sequences keeps a slot."""
+    from semantica_gpu import kernels
+    say("many rows", dtype, bits, "heads", kv_heads, "hd", hd, "sequences", len(lens), "rows", int(np.sum(lens)), "slots", slots)
+    g = gen(seed)
+    off = offsets(lens, first)
+    rows = int(off[-1]) + behind
+    k, v = rand(g, rows, kv_heads * hd, by=3.0, dtype=dtype), rand(g, rows, kv_heads * hd, dtype=dtype)
+    kr, vr = kept_ref(k, kv_heads, bits)[1], kept_ref(v, kv_heads, bits)[1]
+    seq = np.repeat(np.arange(len(lens)), lens)
+    row = np.arange(first, int(off[-1]))
+    at = np.asarray(starts, np.int64)[seq] + row - off.numpy()[seq]
+    there = (np.asarray(starts)[seq] >= 0) & (at < slots)
+    owner = np.full(slots, -1)
+    np.maximum.at(owner, at[there], row[there])  # rows of later sequences are higher
+    owner = torch.from_numpy(owner)
+
+    def kept(x):
+        return torch.where((owner >= 0)[:, None], x[owner.clamp_min(0)], torch.zeros((), dtype=x.dtype))
+
+    def back(x):
+        y = torch.full_like(x, 7.0)
+        seen = kept(x)[torch.from_numpy(np.where(there, at, 0))]
+        y[first:int(off[-1])] = torch.where(torch.from_numpy(there)[:, None], seen, torch.zeros((), dtype=x.dtype))
+        return y
+
+    cache = make_cache(ctx, slots, kv_heads, hd, dtype, bits)
+    try:
+        kernels.kv_cache_write(ctx, cache, k.cuda(), v.cuda(), off.cuda(), ints(starts).cuda())
+        out_k, out_v = torch.full_like(k, 7.0).cuda(), torch.full_like(v, 7.0).cuda()
+        kernels.kv_cache_read(ctx, out_k, out_v, cache, off.cuda(), ints(starts).cuda())
+        got_k, got_v = read_cache(ctx, cache)
+    finally:
+        cache.close()
+    same(got_k, kept(kr), "keys")
+    same(got_v, kept(vr), "values")
+    same(out_k, back(kr), "keys read")
+    same(out_v, back(vr), "values read")
+
+
+def parts_of(r, rows, n):
+    """Lengths of n sequences of so many rows, some of them empty."""
+    cuts = np.sort(r.randint(0, rows + 1, n - 1))
+    return np.diff(np.concatenate([[0], cuts, [rows]]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bits", [0, 8])
+@pytest.mark.parametrize("kv_heads,hd,rows", [(8, 64, 17003), (3, 24, 45001), (9, 16, 44017), (1, 64, 140003), (1, 8, 530011)])
+def test_rows_of_several_blocks_and_heads_a_workgroup(gpu_ctx, dtype, bits, kv_heads, hd, rows):
+    """Workgroups that go over several heads, the last of them fewer, or over several blocks of rows:
+    ends inside a block, gaps, slots named twice, starts and ends outside the cache."""
+    r = np.random.RandomState(kv_heads * hd)
+    # One after another with odd gaps; the last sequences before the cache, past it and over earlier ones.
+    lens = parts_of(r, rows, 37)
+    starts = np.cumsum(lens) - lens + 5 * np.arange(37) + 3
+    slots = int(starts[-1] + lens[-1] + 40)
+    starts[30], starts[33] = -2, starts[33] + 41
+    starts[32] = slots - 5
+    starts[34:] = np.maximum(starts[[1, 9, 20]] + 7, 0)
+    check_many_rows(gpu_ctx, rows, dtype, bits, kv_heads, hd, lens, starts, slots, first=3, behind=29)
+    # In whole, from a slot within a run of four, to the cache's last one.
+    check_many_rows(gpu_ctx, rows + 1, dtype, bits, kv_heads, hd, [rows], [1], rows + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [0, 8])
+def test_many_single_rows(gpu_ctx, bits):
+    """Tens of thousands of tokens, each a sequence: slots in any order, some named by several."""
+    r = np.random.RandomState(3)
+    n = 17000
+    check_many_rows(gpu_ctx, 4, "bf16", bits, 8, 64, [1] * n, r.randint(-3, 20000, n), 19990)

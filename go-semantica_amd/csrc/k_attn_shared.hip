@@ -461,7 +461,7 @@ constexpr int64_t kJoinBlocks = 8192;
 
 struct layout {
   size_t plan, cum[2], jobs[2], seq_jobs, prefix_jobs, seen, where, ml, o, total;
-  int64_t full, pieces[2];
+  int64_t pieces[2];
   int cap, workers[2], m[2], piece_pairs[2];
 };
 
@@ -490,7 +490,11 @@ layout lay_out(int dtype, bool q8, int rows, int heads, int kv_heads, int D, int
   y.prefix_jobs = take(sizeof(int32_t) * ((size_t)n_prefix + 1));
   y.seen = take(sizeof(int2) * (size_t)rows);
   y.where = take(sizeof(int4) * (size_t)rows);
-  int64_t rows_of_o = 2 * (int64_t)rows * heads;
+  // Rows whose jobs may lie in two lists, each with a place of its own for a (row, head): none where
+  // nothing is shared or sequences fill several jobs themselves (all_keys), so no more than those that
+  // such sequences may have.
+  const int64_t apart = n_prefix == 0 ? 0 : std::min<int64_t>(rows, (int64_t)kFullJobs * y.m[1] * n_seq / (heads / kv_heads));
+  int64_t rows_of_o = 2 * apart * heads;
   for (int i = 0; i < 2; i++) {
     y.pieces[i] = rows_of_o;
     y.piece_pairs[i] = (int)std::min<int64_t>(y.m[i], pairs);
@@ -561,6 +565,7 @@ hipError_t attn_shared(sg_attn_shared_args a, sg_attn_batch b, int dtype, bool q
   const int64_t pairs = (int64_t)a.rows * a.group;
   // A job for each M pairs of a sequence, over prefix and own keys in one go, where no prefix is
   // shared or sequences fill several jobs themselves; otherwise the plan weighs it by the lengths.
+  // (lay_out counts on it.)
   b.all_keys = b.n_seq <= b.n_prefix || b.n_prefix == 0 || pairs >= (int64_t)kFullJobs * y.m[1] * b.n_seq;
   const int wide_own = pairs > (int64_t)kNarrowPairs * b.n_seq;
   const int64_t narrow_pairs = dtype != SG_F32 && !q8 ? kNarrowPairs / 2 : kNarrowPairs;

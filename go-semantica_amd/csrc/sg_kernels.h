@@ -113,7 +113,7 @@ struct sg_attn_shared_args {
   int64_t ldo, ldq, head_bytes, tile_bytes;
   const int2* seen;   // [rows]: visible places of the prefix (begin, end), for prefixes' jobs
   const int4* where;  // [rows]: first job and first row of its prefix's group, of its sequence's
-  float* part_o;      // [2 rows * heads, then pieces][D]
+  float* part_o;      // [2 rows * heads (where a list may have a part of a row's keys), then pieces][D]
   float2* part_ml;
   float scale;        // of scores, in powers of two, not negative (1 / log2 e under a cap: 1)
   float cap, to_cap;  // cap * log2 e (0: none), and what a product is multiplied by before tanh

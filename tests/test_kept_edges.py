@@ -257,3 +257,54 @@ def test_many_single_rows(gpu_ctx, bits):
     r = np.random.RandomState(3)
     n = 17000
     check_many_rows(gpu_ctx, 4, "bf16", bits, 8, 64, [1] * n, r.randint(-3, 20000, n), 19990)
+
+
+@pytest.mark.gpu
+def test_workspace_to_the_byte(gpu_ctx):
+    """Calls stay inside the bytes that they ask for, also those of a larger batch's workspace or of a smaller
+    call in it, whatever the plan takes; without prefixes no (row, head) has a place of its own there."""
+    from semantica_gpu import kernels
+    g = gen(30)
+    for dtype, bits, hd, heads, kv_heads in (("bf16", 8, 128, 4, 2), ("f32", 0, 64, 3, 1), ("f16", 0, 256, 8, 1), ("f32", 8, 256, 4, 2)):
+        slots = 4000
+        cache = make_cache(gpu_ctx, slots, kv_heads, hd, dtype, bits)
+        fill_cache(gpu_ctx, cache, rand(g, slots, kv_heads * hd, dtype=dtype), rand(g, slots, kv_heads * hd, dtype=dtype))
+        for queries, prefixes in (([1], 0), ([1], 1), ([1] * 60, 1), ([1] * 60, 3), ([300], 1), ([300, 1, 40], 1), ([40] * 20, 1),
+                                  ([700, 300], 0), ([2] * 400, 2), ([129] * 9, 4)):
+            rows, n = sum(queries), len(queries)
+            keys = dict(starts=ints([i * 3 for i in range(n)]).cuda(), lengths=ints([m + 5 for m in queries]).cuda())
+            if prefixes:
+                keys.update(shared=ints([n * p // prefixes for p in range(prefixes + 1)]).cuda(),
+                            prefix_starts=ints([1500 + 13 * p for p in range(prefixes)]).cuda(),
+                            prefix_lengths=ints([2000 >> (p % 3 * 3) for p in range(prefixes)]).cuda())
+            q, off = rand(g, rows, heads * hd, dtype=dtype).cuda(), offsets(queries).cuda()
+            need = cache.work_bytes(heads, rows, n, prefixes)
+            assert need <= cache.work_bytes(heads, rows + 1, n, prefixes) and need <= cache.work_bytes(heads, rows, n + 1, prefixes)
+            assert need <= cache.work_bytes(heads, rows, n, prefixes + 1)
+            say("workspace", dtype, bits, hd, "queries", queries[:3], n, "prefixes", prefixes, need)
+            outs = []
+            for size in (need, cache.work_bytes(heads, rows + 999, n + 7, prefixes + 1)):
+                buf = torch.full((size + 512,), 0xa5, dtype=torch.uint8, device="cuda")
+                out = torch.empty_like(q)
+                kernels.attention_shared(gpu_ctx, out, q, cache, heads, off, work=buf[256:256 + size], **keys)
+                assert bool((buf[:256] == 0xa5).all()) and bool((buf[256 + need:] == 0xa5).all()), "bytes around the workspace"
+                outs.append(out)
+            same(outs[1], outs[0], "in a larger workspace")
+        cache.close()
+
+
+@pytest.mark.gpu
+def test_workspace_of_large_batches(gpu_ctx):
+    """It grows with the rows that a plan may leave apart: none without prefixes, and so many of each
+    sequence behind one, not with every row of long prompts."""
+    cache = make_cache(gpu_ctx, 64, 8, 128, "bf16", 0)
+    own = 16384 * 32 * 128 * 4  # a float32 output of every (row, head)
+    beside = cache.work_bytes(32, 16384, 32, 0)
+    behind = cache.work_bytes(32, 16384, 32, 1)
+    short = cache.work_bytes(32, 16384, 16384, 1)
+    cache.close()
+    assert beside < 110e6
+    assert beside < behind < beside + 2.1 * own / 4
+    assert short > 2 * own
+
+

@@ -466,9 +466,11 @@ launch_shape shape(int rows, int heads, bool wide) {
   return s;
 }
 
+constexpr bool is_wide(bool f32, bool q8) { return f32 && !q8; }
+
 template <typename T, bool Q8, bool WRITE>
 hipError_t run_rows(const sg_kv_rows_args& a, hipStream_t s) {
-  constexpr int MANY = sizeof(T) == 4 && !Q8 ? 16 : 32;
+  constexpr int MANY = is_wide(sizeof(T) == 4, Q8) ? 16 : 32;
   const launch_shape f = shape(a.rows, a.heads, MANY == 16);
   const dim3 grid((unsigned)f.groups);
   if (f.rows == kFewRows)
@@ -487,7 +489,9 @@ hipError_t by_type(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s) 
 
 namespace sgk {
 
-int64_t kv_rows_threads(int rows, int heads) { return shape(rows, heads, true).groups * kThreads; }
+int64_t kv_rows_threads(int rows, int heads, int dtype, bool q8) {
+  return shape(rows, heads, is_wide(dtype == SG_F32, q8)).groups * kThreads;
+}
 
 hipError_t kv_write(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s) { return by_type<true>(a, dtype, q8, s); }
 hipError_t kv_read(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s) { return by_type<false>(a, dtype, q8, s); }

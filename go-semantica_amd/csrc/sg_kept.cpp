@@ -29,7 +29,7 @@ int rows_call(sg_ctx* ctx, const sg_kv_cache* c, void* k, int64_t ldk, void* v, 
   SG_TRY(check_batch(d_off, rows, n_seq));
   if (c->device != ctx_device(ctx)) return fail(SG_ERR_INVALID, "the cache lies on another device");
   if (rows == 0) return SG_OK;
-  if (sgk::kv_rows_threads(rows, c->heads) > sgk::kMostThreads)
+  if (sgk::kv_rows_threads(rows, c->heads, c->dtype, c->q8) > sgk::kMostThreads)
     return fail(SG_ERR_INVALID, "%d rows of %d heads are more than one launch takes", rows, c->heads);
   const int cols = c->heads * c->hd;
   const Span sk{k, ldk, rows, cols, c->dtype}, sv{v, ldv, rows, cols, c->dtype};

@@ -407,7 +407,7 @@ size_t adapters_work_bytes(int dtype, int rows, int in_dim, int rank_pad);
 hipError_t adapters_apply(const sg_adapters_args& a, int dtype, hipStream_t s);
 
 // ---- kept keys and values (k_kv_cache.hip, k_attn_shared*.hip) ----
-int64_t kv_rows_threads(int rows, int heads);
+int64_t kv_rows_threads(int rows, int heads, int dtype, bool q8);
 hipError_t kv_write(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
 hipError_t kv_read(const sg_kv_rows_args& a, int dtype, bool q8, hipStream_t s);
 // Pairs of a job of the wide form.

@@ -465,7 +465,7 @@ int sg_kv_cache_bytes(const sg_kv_cache *cache, size_t *bytes);
  * overlap (columns of one tensor, with the same stride, do not).  Rows of no sequence are
  * neither written nor read.  A slot outside the cache (every slot of a negative start)
  * is not written, and reads as zeros.  Where two sequences of a write name the same slot, the
- * later one's row is kept.  rows * n_kv_heads: up to 2^29 or a little less. */
+ * later one's row is kept.  rows * n_kv_heads: up to 2^30, or somewhat more. */
 int sg_kv_cache_write(sg_ctx *ctx, sg_kv_cache *cache, const void *k, int64_t ldk, const void *v, int64_t ldv,
                       int32_t rows, const int32_t *d_seq_offsets, int32_t n_seq, const int32_t *d_starts, void *stream);
 int sg_kv_cache_read(sg_ctx *ctx, const sg_kv_cache *cache, void *k, int64_t ldk, void *v, int64_t ldv, int32_t rows,

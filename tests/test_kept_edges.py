@@ -308,3 +308,36 @@ def test_workspace_of_large_batches(gpu_ctx):
     assert short > 2 * own
 
 
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads", [1, 2, 3, 5, 8, 9, 17, 1000])
+def test_rows_up_to_the_launch(gpu_ctx, kv_heads):
+    """rows * n_kv_heads up to 2^30 is no reason to refuse a call, and what one launch does not take is.  (Rows that
+    are not aligned are refused behind that check and before anything is done.)"""
+    from semantica_gpu import _lib
+    lib = gpu_ctx.lib
+    k = torch.zeros(64, device="cuda")
+    off, starts = ints([0, 1]).cuda(), ints([0]).cuda()
+
+    def says(cache, rows):
+        r = lib.sg_kv_cache_write(gpu_ctx.handle, cache.handle, ctypes.c_void_p(k.data_ptr() + 8), 16 * kv_heads,
+                                  ctypes.c_void_p(k.data_ptr()), 16 * kv_heads, rows, ctypes.c_void_p(off.data_ptr()), 1,
+                                  ctypes.c_void_p(starts.data_ptr()), None)
+        assert r == _lib.SG_ERR_INVALID
+        return lib.sg_last_error().decode()
+
+    for dtype in ("f32", "bf16"):
+        for bits in (0, 8):
+            cache = make_cache(gpu_ctx, 8, kv_heads, 8, dtype, bits)
+            try:
+                # Workgroups of 256 threads take 16 rows of float32 as it is and 32 of others, of up to eight heads.
+                assert "16-byte aligned" in says(cache, 2**30 // kv_heads)
+                blocks = 16 if dtype == "f32" and bits == 0 else 32
+                if kv_heads >= 8:
+                    most = (2**24 - 1) // -(-kv_heads // 8) * blocks
+                    if most < 2**31 - 2**16:
+                        assert "16-byte aligned" in says(cache, most)
+                        assert "launch" in says(cache, most + 1)
+            finally:
+                cache.close()

@@ -341,3 +341,62 @@ def test_rows_up_to_the_launch(gpu_ctx, kv_heads):
                         assert "launch" in says(cache, most + 1)
             finally:
                 cache.close()
+
+
+FIRST_CALLS = r"""
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from semantica_gpu import Context, kernels
+ctx = Context(0)
+dev = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+torch.manual_seed(1)
+for dtype in (torch.float32, torch.float16, torch.bfloat16):
+    for hd in (64, 128, 256):
+        for bits in (0, 8):
+            for queries in (2, 150):  # narrow jobs, wide ones
+                n = queries + 200
+                cache = kernels.KVCache(ctx, n, 1, hd, dtype, bits=bits)
+                w = kernels.Q4Weight(ctx, torch.randint(0, 256, (hd, hd // 2), dtype=torch.uint8, device="cuda"),
+                                     torch.rand(hd, hd // 32, device="cuda").half())
+                k, v, q = (torch.randn(m, hd, device="cuda").to(dtype) for m in (n, n, queries))
+                o, y, kb, vb = (torch.zeros_like(t) for t in (q, q, k, v))
+                work = torch.empty(cache.work_bytes(1, queries, 1, 0), dtype=torch.uint8, device="cuda")
+                every, some, zero, length = dev(0, n), dev(0, queries), dev(0), dev(n)
+
+                def step():
+                    kernels.kv_cache_write(ctx, cache, k, v, every, zero)
+                    kernels.kv_cache_read(ctx, kb, vb, cache, every, zero)
+                    kernels.attention_shared(ctx, o, q, cache, 1, some, zero, length, work=work)
+                    kernels.matmul_q4(ctx, y, w, o)
+
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    step()
+                for t in range(3):
+                    k.normal_(), v.normal_(), q.normal_()
+                    graph.replay()
+                    torch.cuda.synchronize()
+                    got = [x.clone() for x in (o, y, kb, vb)]
+                    for x in (o, y, kb, vb):
+                        x.zero_()
+                    step()
+                    torch.cuda.synchronize()
+                    for x, a in zip((o, y, kb, vb), got):
+                        assert bool((x == a).all()) and bool(torch.isfinite(a).all()) and bool((a != 0).any())
+                cache.close()
+                w.close()
+            print(dtype, hd, bits, flush=True)
+ctx.close()
+print("first calls captured", flush=True)
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_inside_a_capture():
+    """A program's first call of each kernel may be the one that it captures: in a process of its own."""
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "go-semantica_amd")
+    r = subprocess.run([sys.executable, "-u", "-c", FIRST_CALLS, at], capture_output=True, text=True, timeout=110)
+    say(r.stdout[-2000:], r.stderr[-2000:])
+    assert r.returncode == 0 and "first calls captured" in r.stdout

@@ -8,7 +8,7 @@
 // behind one prefix, 10 for 10476 and 16384 rows (sixteen waves).
 //
 // The join reads a float32 output for each piece of each (row, head): 27 rows of 32 heads whose
-// prefix is split over the GPU 13 us, 16384 rows of which the jobs of 512 workers were cut 21.
+// prefix is split over the GPU 12 us, 16384 rows of which the jobs of 512 workers were cut 21.
 #include <algorithm>
 
 #include "semantica_gpu.h"

@@ -15,8 +15,10 @@
 // stored as one, others element by element.
 //
 // Memory bounds them where there are many rows (131072 bf16 rows of 8 heads of 128 from codes: 170 us,
-// 4.8 TB/s; 32768 float32 rows of one head of 256 to codes and back: 23 and 17 us, 3.6 and 4.8 TB/s), three dependent loads and a round through LDS where there are few
-// (64 tokens 6 us in, 4.7 out).  Rows that stand alone in their run of four slots cost four times
+// 4.8 TB/s, as they are in and out 255 and 220; 32768 float32 rows of one head of 256 to codes and back: 23
+// and 17 us, 3.6 and 4.8 TB/s, as they are 31 and 29, 4.3 and 4.6: a workgroup of these has one block of
+// rows, which it loads whole before it stores), three dependent loads and a round through LDS where there
+// are few (64 tokens 6 us in, 4.7 out).  Rows that stand alone in their run of four slots cost four times
 // their bytes in values: 32768 single tokens 145 us out.
 //
 // Two sequences may name the same slots: the later one's rows are kept, whole (each

@@ -17,23 +17,30 @@
 // B operand of O^T += V^T P^T, for values are kept in that order (sg_kv_cache.h).
 //
 // Codes of 8 bits are whole numbers, exact in the type: the keys' scale multiplies the
-// score, the values' the weight.  With fp16 queries that product would leave fp16's range,
-// so weights are split into two bf16 halves (2^-17 of each, exponents of float32) and the
-// codes taken as bf16; with bf16 queries one rounding to bf16 is what the plain form of the
-// type has as well.  float32 queries and weights go over codes as three bf16 parts, 24 bits (48
-// cycles of 32 products of 16 and 16 where float32's own take 256); over float32 keys and
+// score, the values' the weight.  float32 queries and weights go over codes as three bf16 parts, 24
+// bits (48 cycles of 32 products of 16 and 16 where float32's own take 256); over float32 keys and
 // values it goes through float32 matrix products.
+//
+// 16-bit types round the weights once, for the second product: to the type itself over keys
+// and values as they are (their sum is taken of the rounded ones), and over codes, with the value's
+// scale in them, to bf16 with bf16 queries; with fp16 queries that product would leave fp16's range, so
+// they are split into two bf16 halves (2^-17 of each, exponents of float32) and the codes taken
+// as bf16.  This is as large as the rounding of the result: the error against 64 bits is 2.3e-3 in
+// bf16 for 1.66e-3 with weights of float32's precision, in fp16 2.8e-4 for 2.1e-4.  Two halves everywhere
+// would give that, for another second product (us, rounded and in halves): 32 x 512 bf16 behind 8192 2250
+// and 3140, 600 bf16 rows of 256 dims behind 20000 146 and 177, over codes 64 tokens behind 8192 68 and
+// 72, 27 rows behind 131072 133 and 154.
 //
 // What bounds them (MI355X): a wide workgroup of bf16 takes each fragment of a tile from LDS for two
 // products, and a pair and lane has eight exponentials of 16 cycles; vector and matrix
 // instructions of a SIMD overlap little, and two waves a SIMD hide the rest.
-//   bf16, 16384 rows of 32 heads over 8 of 128 dims behind 8192 places: 2.2 ms, 1040 TFLOP/s of the 1214
+//   bf16, 16384 rows of 32 heads over 8 of 128 dims behind 8192 places: 2.2 ms, 1020 TFLOP/s of the 1214
 //   that a large product reaches.
-//   bf16 over codes, 27 rows of 32 heads over 8 behind 131072 places: 110 us, 2.5 TB/s: decoding and
+//   bf16 over codes, 27 rows of 32 heads over 8 behind 131072 places: 112 us, 2.5 TB/s: decoding and
 //   the softmax of a tile stand between its load and the next barrier.
-//   float32, 10476 rows of 3 heads over 1 of 256 dims, window 512: 195 us, 85 of 152 TFLOP/s: two
+//   float32, 10476 rows of 3 heads over 1 of 256 dims, window 512: 198 us, 83 of 152 TFLOP/s: two
 //   waves a SIMD, products that wait for fragments.
-//   one float32 query of 3 heads over 1 of 256 dims behind 1536 places (narrow): 11 us, one tile a
+//   one float32 query of 3 heads over 1 of 256 dims behind 1536 places (narrow): 12 us, one tile a
 //   wave, its loads' latency and 256 products in a row.
 #pragma once
 #include <atomic>

@@ -440,7 +440,8 @@ int sg_adapters_apply(sg_ctx *ctx, void *dst, int64_t ldd, const void *base, int
  * kept, and every request runs only its own tokens.  No counterpart in the reference.
  * The calls are asynchronous on `stream` (NULL: the context's), allocate nothing and may
  * be captured; the order of calls that write slots and calls that read them is the
- * caller's, by streams, as with any memory. */
+ * caller's, by streams, as with any memory (a row with an infinity or a NaN, written to a cache
+ * of bits 0, counts as written to all 32 slots of its s / 32). */
 
 /* A cache of `slots` tokens' keys and values, n_kv_heads heads of head_dim (a multiple of
  * 8 up to 256; kept as 64, 128 or 256).  dtype: the type of rows in and out, and of
@@ -501,9 +502,12 @@ int sg_attention_shared_work_bytes(const sg_kv_cache *cache, int32_t n_heads, in
  * they were.  What hidden slots hold does not matter.  An infinity or a NaN in a value that is
  * seen is that dim's result whatever its key's score (a NaN where infinities of both signs are seen; kept
  * as codes it is a NaN in all dims, and none with a score of -infinity, which has no weight).
- * Sums are float32 and up to 2^10 times the
- * number of keys larger than the result: values beyond 2^90 may leave its range; float32 queries
- * and values behind codes keep their bits down to 2^-100.  q, out [rows][n_heads * head_dim] of
+ * Sums are float32 and up to 2^10 times the number of keys larger than the result: values beyond
+ * 2^90 may leave its range, and queries beyond 2^112 over codes, whose scores are formed before the
+ * key's scale.  16-bit types round the weights to their type before they multiply values (fp16's to
+ * 2^-31 of the largest at worst; over codes, with the value's scale in them, bf16's to bf16 and fp16's
+ * within 2^-17); float32 keeps its bits, queries and values behind codes down to 2^-100, weights down to
+ * 2^-126.  q, out [rows][n_heads * head_dim] of
  * the cache's type with row strides in elements, pointers 16-byte aligned, strides whole 16
  * bytes, apart from each other (other columns of one tensor are); n_heads is a multiple of the
  * cache's heads, head h reads key head h * n_kv_heads / n_heads.  rows * n_heads up to 2^25.
@@ -535,7 +539,8 @@ int sg_q4_weight_create_q4_0(sg_ctx *ctx, const void *raw, int32_t out_dim, int3
 void sg_q4_weight_free(sg_q4_weight *weight);
 
 /* dst[m][n] = sum over k of w[n][k] x[m][k] for a few rows (16 or 32 of them share one
- * pass over the weights, more take one for every so many).  x [rows][in_dim], dst [rows][out_dim] of type dtype with
+ * pass over the weights, more take one for every so many: from some 64 rows on a dense product of
+ * 16-bit weights is faster, at 512 three to five times).  x [rows][in_dim], dst [rows][out_dim] of type dtype with
  * row strides in elements; x 16-byte aligned, its stride whole 16 bytes; dst does not overlap
  * x (other columns of one tensor, with the same stride, do not).  Weights are not rounded, sums
  * are float32 and in the same order every time; float32 rows keep their bits down to 2^-102 (what

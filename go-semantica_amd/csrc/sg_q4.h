@@ -18,7 +18,8 @@
 // both slower).  Few rows: the weights' bytes bound it, 8192 x 8192 and one fp16 row 14.4 us, 2.6 TB/s,
 // out of memory (16 such weights in turn; 10 us, 3.8 TB/s, where the 256 MB cache behind the L2s holds
 // them); 16 bf16 rows of 4096 to 16384 with zeros 14.9 and 12.9 us, 2.4 and 2.8 TB/s: two dozen vector
-// instructions decode a lane's eight codes of a product.  One float32 row of 768 to 2304: 4 us, a chain of two loads, the products and the join.
+// instructions decode a lane's eight codes of a product.  One float32 row of 768 to 2304: 4 us, a chain of
+// two loads, the products and the join.
 // Many rows: weights are decoded again for every 16 or 32 of them, so that a dense bf16 product of
 // the same size takes over (4096 to 8192, groups of 32, 128, dense: 32 rows 13.5, 12.6 and 15 us, 64 23.9,
 // 16.1 and 16.2, 512 171, 107 and 37).

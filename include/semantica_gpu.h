@@ -540,8 +540,8 @@ void sg_q4_weight_free(sg_q4_weight *weight);
 
 /* dst[m][n] = sum over k of w[n][k] x[m][k] for a few rows (16 or 32 of them share one
  * pass over the weights, more take one for every so many: from some 64 rows on a dense product of
- * 16-bit weights is faster, at 512 three to five times).  x [rows][in_dim], dst [rows][out_dim] of type dtype with
- * row strides in elements; x 16-byte aligned, its stride whole 16 bytes; dst does not overlap
+ * 16-bit weights is faster, at 512 three to five times).  x [rows][in_dim], dst [rows][out_dim] of
+ * type dtype with row strides in elements; x 16-byte aligned, its stride whole 16 bytes; dst does not overlap
  * x (other columns of one tensor, with the same stride, do not).  Weights are not rounded, sums
  * are float32 and in the same order every time; float32 rows keep their bits down to 2^-102 (what
  * lies below 2^-126 is lost of smaller values), and values beyond 2^116 may leave float32's range in a
